@@ -15,7 +15,9 @@ LIB = os.path.join(LIBDIR, 'libdig3d.so')
 SOURCES = ['abi.hip', 'graph.hip', 'geometry.hip', 'basis.hip', 'segment.hip', 'triplet.hip', 'triplet_wave.hip', 'basis_mfma.hip', 'dense.hip', 'chain.hip', 'wide.hip', 'diffgeom.hip', 'norm.hip',
            'readout.hip', 'radial.hip', 'sbf2.hip']
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-ffp-contract=off', '-fPIC',
-         '-fhip-fp32-correctly-rounded-divide-sqrt', '-Wno-unused-result']
+         '-fhip-fp32-correctly-rounded-divide-sqrt', '-Wno-unused-result',
+         # packed float32 arithmetic has given wrong results now and then on this chip: scalar instructions only
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 HEADER = os.path.join(os.path.dirname(HERE), 'include', 'dig3d.h')
