@@ -1,0 +1,1085 @@
+// dig3d — the trained output head: losses over the classes of logits z = x W^T + bias that are never kept.
+//
+//   classes:  loss_n = lse(z_n) - z_n[y_n]                                     e_n = c_n (softmax(z_n) - onehot(y_n))
+//   teacher:  loss_n = tau^2 sum_k q_k (log q_k - log p_n[i_k]), p = softmax(z / tau)   e_n = c_n (p_n - scatter(q_n))
+//   gx = S e W,  gW = S e^T x,  gb = S sum_n e_n          (c_n S: the gradient that reaches row n, |c_n| <= 1)
+//
+// Four products of 2 N V D operations: the logits, the logits again in the backward (the price of not keeping them), e W and
+// e^T x.  Bound: the matrix cores.  All four run on ONE product kernel (k_head_gemm): out[j, i] = sum_k Q[j, k] P[i, k], each
+// operand either contiguous along k or along its own index, staged through LDS by 16-byte direct loads and read as matrix
+// operands (the second kind by the transposing LDS read), so nothing is transposed in memory.  Its epilogues: the softmax
+// statistics of a tile of logits (forward), the gradient e of a piece of the vocabulary (backward), or the stored product.
+//
+// Types.  bf16 / f16: the inputs as they are, sums in f32; e is rounded once to the same type (2^-9 / 2^-12 of each entry at
+// random sign, below the rounding of the gradients it leads to).  f32: every value is two f16 numbers, v s = h + l with
+// s = 2^k chosen so that the largest |v| of the tensor lies in [2^14, 2^15): 22 bits of every v down to 2^-29 of that
+// largest one, and an absolute error of 2^-40 of it below; three products h h, h l, l h with f32 sums (l l is below 2^-22 of
+// the term).  Three f16 matrix products have 5x the rate of one in f32 on this chip, at the error of an f32 product.
+#include <string.h>
+
+#include "half16.h"
+
+#define HD_BK 64           // the k step of the product kernel: row pitches are multiples of it
+#define L2E 1.44269504088896340736f
+#define LN2 0.69314718055994530942f
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+
+template <class T>
+__device__ __forceinline__ f32x4 hd_mfma(s16x8 a, s16x8 b, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 hd_mfma<bf16_t>(s16x8 a, s16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 hd_mfma<f16_t>(s16x8 a, s16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// One operand: `planes` matrices of `rows` rows with pitch `ld` (elements, a multiple of 8; base 16-byte aligned).
+//   not TR: row = the operand's own index, columns = k (k extent a multiple of HD_BK inside the pitch)
+//   TR:     row = k, columns = the operand's own index (`cols` of them are readable, a multiple of 8)
+// Rows beyond the last are read as the last one: for the own index their results are not used, for k the other operand
+// holds zeros there.
+struct HdOperand {
+  const short* p;
+  int64_t ld, plane;
+  int rows, cols;
+};
+
+enum { EPI_STATS = 0, EPI_GRAD = 1, EPI_OUT = 2 };
+
+struct HdArgs {
+  HdOperand P, Q;
+  int ni, nj;                // extents of the own indices of P and Q
+  int ktiles;                // k steps of one product
+  int nseg;                  // 1, or 3 products of planes (h h, h l, l h)
+  int ti, tj;                // tiles along i and j
+  int splits;                // the k steps are dealt to gridDim.z workgroups
+  // logits epilogues: i = class v0 + i, j = row
+  const void* bias;
+  int dt;                    // type of bias / of the stored output
+  const float* scal;         // device scalars of the call (SC_*)
+  float inv_tau;
+  int64_t v0;                // first class of the piece
+  int64_t V;
+  const int64_t* target;     // null: no class is kept apart
+  float2* part;              // EPI_STATS [nj][ti_all]: (max, sum of exp) of the tile
+  int part_ld, part_c0;
+  float* zt;                 // EPI_STATS: the target's logit
+  const float* lse;          // EPI_GRAD
+  const float* loss;
+  const float* coef;
+  short* E;                  // EPI_GRAD [planes][rowsE][ldE]
+  int64_t ldE, planeE;
+  int rowsE;
+  // EPI_OUT
+  float* acc;                // f32 partial slots [splits][nj][ni], written or added to
+  int add;
+  void* out;                 // or the finished result, row pitch ldo
+  int64_t ldo;
+  int other;                 // scale of the operand beside e (SC_X / SC_W with f32 inputs, else -1)
+};
+
+// device scalars: the power-of-two scales of x and W (f32 inputs) and the common factor S of the gradients
+enum { SC_X = 0, SC_W = 1, SC_S = 2, SC_COUNT = 4 };
+
+#define E_SCALE 32768.0f   // e in f16 (|e| <= 1) is stored times this: small entries stay normal numbers
+
+// what a product with e is multiplied by: S over the scales of its operands
+template <class T>
+__device__ __forceinline__ float hd_factor(const float* scal, int other) {
+  const float s = __is_same(T, f16_t) ? scal[SC_S] * (1.f / E_SCALE) : scal[SC_S];
+  return other >= 0 ? s / scal[other] : s;
+}
+
+// LDS of one stage: P tile then Q tile, HD_BK deep
+template <int B>
+constexpr int hd_tile_shorts() {
+  return B * HD_BK;
+}
+
+// lane l of load `q` of a wave fetches 16 bytes to LDS offset 1024 q + 16 l of its tile.
+// not TR: LDS row r holds 8 chunks of 8 k; chunk s of it is source chunk s ^ (r & 7) (reads of 16 rows hit all banks)
+// TR:     LDS row k holds B / 8 chunks; chunk s of it is source chunk s ^ (2 g(k) mod B / 8), g(k) = (k & 3) | (k >> 3 & 3) << 2
+template <int B, bool TR, int NW>
+__device__ __forceinline__ void hd_load(const HdOperand& o, const short* __restrict__ base, int own0, int k0, short* lds, int wave,
+                                        int lane) {
+  constexpr int NL = B * HD_BK * 2 / 1024 / NW;
+#pragma unroll
+  for (int q = 0; q < NL; ++q) {
+    const int blk = q * NW + wave;
+    const short* src;
+    if constexpr (!TR) {
+      const int r = blk * 8 + (lane >> 3);
+      const int row = min(own0 + r, o.rows - 1);
+      const int ch = (lane & 7) ^ (r & 7);
+      src = base + (int64_t)row * o.ld + k0 + ch * 8;
+    } else {
+      constexpr int CH = B / 8, RPL = 64 / CH;       // chunks per row, rows per load
+      const int k = blk * RPL + lane / CH;
+      const int row = min(k0 + k, o.rows - 1);
+      const int g = (k & 3) | (((k >> 3) & 3) << 2);
+      const int ch = (lane % CH) ^ ((2 * g) & (CH - 1));
+      const int col = min(own0 + ch * 8, o.cols - 8);
+      src = base + (int64_t)row * o.ld + col;
+    }
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)(lds + blk * 512), 16, 0, 0);
+  }
+}
+
+// the matrix operand of 16 own indices from o0 and k half kk (32 of the 64) of a staged tile
+template <int B, bool TR>
+__device__ __forceinline__ s16x8 hd_frag(const short* lds, int o0, int kk, int lane) {
+  if constexpr (!TR) {
+    const int r = o0 + (lane & 15);
+    return *(const s16x8*)(lds + r * 64 + (((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 8));
+  } else {
+    constexpr int CH = B / 8;
+    const int k = kk * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2);
+    const int ch = ((o0 >> 3) + ((lane & 3) >> 1)) ^ ((2 * (lane >> 2)) & (CH - 1));
+    const short* a = lds + k * B + ch * 8 + (lane & 1) * 4;
+    typedef __attribute__((address_space(3))) s16x4* lp;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(short*)a);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(short*)(a + 4 * B));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void hd_store4(void* out, int64_t at, f32x4 v, int n) {
+  T* o = (T*)out + at;
+  if (n == 4 && ((uintptr_t)o & (4 * sizeof(T) - 1)) == 0) {
+    struct alignas(4 * sizeof(T)) { T t[4]; } u;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) u.t[r] = to_t<T>(v[r]);
+    *(decltype(u)*)o = u;
+  } else {
+    for (int r = 0; r < n; ++r) o[r] = to_t<T>(v[r]);
+  }
+}
+
+// out[j, i] = sum_k Q[j, k] P[i, k] on tiles of BI x BJ, WI x WJ waves; the lanes of a matrix result hold 4 consecutive i of
+// one j, so rows of the output are written in pieces of 4.
+template <class T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
+__global__ void __launch_bounds__(WI* WJ * 64) k_head_gemm(HdArgs a) {
+  constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
+  __shared__ __attribute__((aligned(1024))) short sm0[hd_tile_shorts<BI>() + hd_tile_shorts<BJ>()];
+  __shared__ __attribute__((aligned(1024))) short sm1[hd_tile_shorts<BI>() + hd_tile_shorts<BJ>()];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // tile of this workgroup: an XCD takes a contiguous range of tiles, ordered in bands of 4 tiles along j so that the
+  // tiles in flight on one L2 share operand panels along both indices
+  const int n = a.ti * a.tj, per = gridDim.x >> 3;
+  const int id = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+  if (id >= n) return;
+  const int band = id / (4 * a.ti), j0b = band * 4, bw = min(4, a.tj - j0b), rem = id - band * 4 * a.ti;
+  const int tj = j0b + rem % bw, ti = rem / bw;
+  const int i0 = ti * BI, j0 = tj * BJ;
+  const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
+
+  f32x4 acc[MI][MJ];
+#pragma unroll
+  for (int x = 0; x < MI; ++x)
+#pragma unroll
+    for (int y = 0; y < MJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int total = a.ktiles * a.nseg;
+  const int t0 = (int)((int64_t)total * blockIdx.z / a.splits), t1 = (int)((int64_t)total * (blockIdx.z + 1) / a.splits);
+
+  auto load = [&](int t, short* sm) {
+    const int seg = t / a.ktiles, k0 = (t - seg * a.ktiles) * HD_BK;    // planes (h, h), (h, l), (l, h)
+    hd_load<BI, PT, NW>(a.P, a.P.p + (seg == 2 ? a.P.plane : 0), i0, k0, sm, wave, lane);
+    hd_load<BJ, QT, NW>(a.Q, a.Q.p + (seg == 1 ? a.Q.plane : 0), j0, k0, sm + hd_tile_shorts<BI>(), wave, lane);
+  };
+  auto mul = [&](const short* sm) {
+    const short* sp = sm;
+    const short* sq = sm + hd_tile_shorts<BI>();
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      s16x8 fq[MJ];
+#pragma unroll
+      for (int y = 0; y < MJ; ++y) fq[y] = hd_frag<BJ, QT>(sq, wj + y * 16, kk, lane);
+#pragma unroll
+      for (int x = 0; x < MI; ++x) {
+        const s16x8 fp = hd_frag<BI, PT>(sp, wi + x * 16, kk, lane);
+#pragma unroll
+        for (int y = 0; y < MJ; ++y) acc[x][y] = hd_mfma<T>(fp, fq[y], acc[x][y]);
+      }
+    }
+  };
+  if (t0 < t1) load(t0, sm0);
+  for (int t = t0; t < t1; t += 2) {
+    __syncthreads();                       // stage 0 has arrived; stage 1 has been read
+    if (t + 1 < t1) load(t + 1, sm1);
+    mul(sm0);
+    __syncthreads();
+    if (t + 1 < t1) {
+      if (t + 2 < t1) load(t + 2, sm0);
+      mul(sm1);
+    }
+  }
+
+  const int q4 = 4 * (lane >> 4), l15 = lane & 15;
+  if constexpr (EPI == EPI_OUT) {
+    const float s = a.out ? hd_factor<T>(a.scal, a.other) : 1.f;
+#pragma unroll
+    for (int y = 0; y < MJ; ++y) {
+      const int j = j0 + wj + y * 16 + l15;
+      if (j >= a.nj) continue;
+#pragma unroll
+      for (int x = 0; x < MI; ++x) {
+        const int i = i0 + wi + x * 16 + q4;
+        const int left = min(4, a.ni - i);
+        if (left <= 0) continue;
+        f32x4 v = acc[x][y];
+        if (a.out) {
+          v *= s;
+          if (a.dt == DT_F32) hd_store4<float>(a.out, (int64_t)j * a.ldo + i, v, left);
+          else if (a.dt == DT_BF16) hd_store4<bf16_t>(a.out, (int64_t)j * a.ldo + i, v, left);
+          else hd_store4<f16_t>(a.out, (int64_t)j * a.ldo + i, v, left);
+        } else {
+          float* o = a.acc + ((int64_t)blockIdx.z * a.nj + j) * a.ni + i;
+          for (int r = 0; r < left; ++r) o[r] = a.add ? o[r] + v[r] : v[r];
+        }
+      }
+    }
+  } else {
+    const float dsc = a.nseg > 1 ? a.inv_tau / (a.scal[SC_X] * a.scal[SC_W]) : a.inv_tau;   // powers of two, and 1 / tau
+    // z = (product + bias) / tau
+#pragma unroll
+    for (int x = 0; x < MI; ++x) {
+      float b[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = i0 + wi + x * 16 + q4 + r;
+        b[r] = a.bias && i < a.ni ? load_as(a.bias, a.dt, a.v0 + i) * a.inv_tau : 0.f;
+      }
+#pragma unroll
+      for (int y = 0; y < MJ; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[x][y][r] = __fmaf_rn(acc[x][y][r], dsc, b[r]);
+    }
+    if constexpr (EPI == EPI_STATS) {
+      // (max, sum of exp) over this tile's classes without the target, per row; a row's classes lie in the 4 lane groups of
+      // WI waves
+      float* sh = (float*)sm0;             // [WI][BJ][2]; the last products have read the stages
+      __syncthreads();
+#pragma unroll
+      for (int y = 0; y < MJ; ++y) {
+        const int jl = wj + y * 16 + l15, j = j0 + jl;
+        int64_t tg = -1;
+        if (a.target && j < a.nj) tg = a.target[j] - a.v0;
+        float m = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int x = 0; x < MI; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = i0 + wi + x * 16 + q4 + r;
+            if (i < a.ni && i == tg) a.zt[j] = acc[x][y][r];
+            if (i >= a.ni || i == tg) acc[x][y][r] = -INFINITY;
+            m = fmaxf(m, acc[x][y][r]);
+          }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int x = 0; x < MI; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[x][y][r] - ms) * L2E);
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (lane < 16) {
+          sh[((wave % WI) * BJ + jl) * 2] = m;
+          sh[((wave % WI) * BJ + jl) * 2 + 1] = s;
+        }
+      }
+      __syncthreads();
+      for (int jl = tid; jl < BJ; jl += NW * 64) {
+        const int j = j0 + jl;
+        if (j >= a.nj) continue;
+        float m = sh[jl * 2], s = sh[jl * 2 + 1];
+        for (int w = 1; w < WI; ++w) {
+          const float m2 = sh[(w * BJ + jl) * 2], s2 = sh[(w * BJ + jl) * 2 + 1];
+          const float mm = fmaxf(m, m2), ms = mm == -INFINITY ? 0.f : mm;
+          s = s * __builtin_amdgcn_exp2f((m - ms) * L2E) + s2 * __builtin_amdgcn_exp2f((m2 - ms) * L2E);
+          m = mm;
+        }
+        a.part[(int64_t)j * a.part_ld + a.part_c0 + ti] = make_float2(m, s);
+      }
+    } else {
+      // e = c (exp(z - lse) - [target]); zeros in the padding that the next products read
+#pragma unroll
+      for (int y = 0; y < MJ; ++y) {
+        const int j = j0 + wj + y * 16 + l15;
+        if (j >= a.rowsE) continue;
+        const bool in = j < a.nj;
+        const float lse = in ? a.lse[j] : 0.f, c = in ? a.coef[j] : 0.f;
+        int64_t tg = -1;
+        float et = 0.f;
+        if (a.target && in) {
+          tg = a.target[j] - a.v0;
+          et = c * expm1f(-a.loss[j]);     // p - 1 of the target: what the other classes hold, not a difference near 1
+        }
+#pragma unroll
+        for (int x = 0; x < MI; ++x) {
+          const int i = i0 + wi + x * 16 + q4;
+          if (i >= a.ldE) continue;
+          float e[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = c * __builtin_amdgcn_exp2f((acc[x][y][r] - lse) * L2E);
+            e[r] = i + r >= a.ni || c == 0.f ? 0.f : i + r == tg ? et : p;   // a row without a loss gives nothing, whatever it holds
+          }
+          struct alignas(8) { T t[4]; } h, l;
+          if (a.nseg > 1) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float v = e[r] * E_SCALE;
+              h.t[r] = to_t<T>(v);
+              l.t[r] = to_t<T>(v - (float)h.t[r]);
+            }
+            *(decltype(l)*)(a.E + a.planeE + (int64_t)j * a.ldE + i) = l;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) h.t[r] = to_t<T>(__is_same(T, f16_t) ? e[r] * E_SCALE : e[r]);
+          }
+          *(decltype(h)*)(a.E + (int64_t)j * a.ldE + i) = h;
+        }
+      }
+    }
+  }
+}
+
+// ---- small kernels ---------------------------------------------------------------------------------------------------------
+// partial max |v| over the finite entries of x (blocks [0, HD_AMAX)) and W (the rest): amax[2 HD_AMAX]
+#define HD_AMAX 256
+__global__ void __launch_bounds__(256) k_head_amax(const float* __restrict__ x, int64_t ldx, int64_t R, const float* __restrict__ w,
+                                                    int64_t ldw, int64_t V, int D, float* __restrict__ amax) {
+  __shared__ float sh[4];
+  const bool second = blockIdx.x >= HD_AMAX;
+  const float* p = second ? w : x;
+  const int64_t ld = second ? ldw : ldx, rows = second ? V : R;
+  const int b = second ? blockIdx.x - HD_AMAX : blockIdx.x;
+  float m = 0.f;
+  auto see = [&](float v) {
+    v = fabsf(v);
+    m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
+  };
+  if (ld == D && D % 4 == 0 && ((uintptr_t)p & 15) == 0) {
+    const float4* q = (const float4*)p;
+    const int64_t n = rows * D / 4;
+    for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n; i += HD_AMAX * 256) {
+      const float4 v = q[i];
+      see(v.x); see(v.y); see(v.z); see(v.w);
+    }
+  } else {
+    for (int64_t r = b * 4 + (threadIdx.x >> 6); r < rows; r += HD_AMAX * 4)
+      for (int d = threadIdx.x & 63; d < D; d += 64) see(p[r * ld + d]);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) amax[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+}
+
+// 2^k with 2^k m in [2^14, 2^15); 1 for an all-zero tensor.  k is kept in the range where 2^k and 2^-k are normal.
+__device__ __forceinline__ float hd_scale(float m) {
+  if (!(m > 0.f)) return 1.f;
+  int e;
+  frexpf(m, &e);
+  const int k = min(max(15 - e, -100), 100);
+  return ldexpf(1.f, k);
+}
+
+// out [planes][orows][ocols] <- rows [0, R) of src (type dt, pitch ld, D columns), zeros elsewhere; `coef`: a row with
+// coefficient 0 is written as zeros (its contents, whatever they are, take no part in any sum).  f32: two planes, and block
+// 0 leaves the scale in scal[slot].
+__global__ void __launch_bounds__(256) k_head_pack(const void* __restrict__ src, int dt, int64_t ld, int64_t R, int D,
+                                                    const float* __restrict__ coef, const float* __restrict__ amax, int slot,
+                                                    float* __restrict__ scal, short* __restrict__ out, int64_t orows, int ocols,
+                                                    int64_t plane) {
+  __shared__ float sh[4];
+  float s = 1.f;
+  if (dt == DT_F32) {
+    float m = amax[slot * HD_AMAX + threadIdx.x];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+    __syncthreads();
+    s = hd_scale(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
+    if (blockIdx.x == 0 && threadIdx.x == 0) scal[slot] = s;
+  }
+  const int oc8 = ocols >> 3;
+  const int64_t n = orows * oc8;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < n; u += (int64_t)gridDim.x * 256) {
+    const int64_t r = u / oc8;
+    const int c = (int)(u - r * oc8) * 8;
+    const bool live = r < R && (!coef || coef[r] != 0.f);
+    const int left = live ? min(8, D - c) : 0;
+    s16x8 h = {0, 0, 0, 0, 0, 0, 0, 0}, l = h;
+    if (dt == DT_F32) {
+      float f[8];
+      const float* p = (const float*)src + r * ld + c;
+      if (left == 8) {
+        const RowVec<float, 8> v = *(const RowVec<float, 8>*)p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = v.v[i] * s;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < left ? p[i] * s : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const f16_t hi = (f16_t)f[i];
+        const float d = f[i] - (float)hi;
+        const f16_t lo = (f16_t)(fabsf(d) <= 65504.f ? d : 0.f);    // an infinity or NaN is its first plane's alone
+        h[i] = __builtin_bit_cast(short, hi);
+        l[i] = __builtin_bit_cast(short, lo);
+      }
+      *(s16x8*)(out + plane + r * ocols + c) = l;
+    } else {
+      const short* p = (const short*)src + r * ld + c;
+      if (left == 8) {
+        const RowVec<short, 8> v = *(const RowVec<short, 8>*)p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = v.v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = i < left ? p[i] : (short)0;
+      }
+    }
+    *(s16x8*)(out + r * ocols + c) = h;
+  }
+}
+
+__device__ __forceinline__ float hd_wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// the tiles' statistics of a row joined, a wave per row.  With targets: lse[n] and loss[n] (0 where the target is
+// `ignore`, NaN where it is no class); without: lse[n].
+__global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ part, int tiles, int N, int64_t V,
+                                                    const int64_t* __restrict__ target, int64_t ignore,
+                                                    const float* __restrict__ zt, float* __restrict__ lse,
+                                                    float* __restrict__ loss) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N) return;
+  const float2* p = part + n * tiles;
+  float m = -INFINITY, s = 0.f;
+  for (int t = lane; t < tiles; t += 64) m = fmaxf(m, p[t].x);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float ms = m == -INFINITY ? 0.f : m;
+  for (int t = lane; t < tiles; t += 64) s += p[t].y * __builtin_amdgcn_exp2f((p[t].x - ms) * L2E);
+  s = hd_wave_sum(s);
+  if (lane != 0) return;
+  if (!target) {
+    lse[n] = m == -INFINITY && s == 0.f ? -INFINITY : ms + logf(s);
+    return;
+  }
+  const int64_t tg = target[n];
+  if (tg == ignore) {
+    lse[n] = 0.f;
+    loss[n] = 0.f;
+    return;
+  }
+  if (tg < 0 || tg >= V) {
+    lse[n] = loss[n] = NAN;
+    return;
+  }
+  // s exp(m) over the other classes, z the target's logit.  The loss from the others' share, not from a difference of
+  // two near numbers, where the target holds almost everything
+  const float z = zt[n];
+  const float M = fmaxf(m, z), Ms = M == -INFINITY ? 0.f : M;
+  const float so = s * expf(ms - Ms), st = expf(z - Ms);
+  lse[n] = Ms + logf(so + st);
+  loss[n] = z >= m ? log1pf(so) : (Ms - z) + logf(so + st);
+}
+
+// teacher: a workgroup per row.  q [N, K] = softmax over the row's listed classes of t / tau (0 where the index is negative
+// or the logit -inf), z [N, K] = their own logits / tau, loss[n], count via live[n]
+__global__ void __launch_bounds__(256) k_head_teacher(const void* __restrict__ x, const void* __restrict__ w,
+                                                       const void* __restrict__ bias, int dt, int64_t ldx, int64_t ldw, int D,
+                                                       int64_t V, const int64_t* __restrict__ index, const void* __restrict__ tl,
+                                                       int tdt, int K, float inv_tau, float tau, const float* __restrict__ lse,
+                                                       float* __restrict__ q, float* __restrict__ z, float* __restrict__ loss,
+                                                       float* __restrict__ live) {
+  __shared__ float sh[8];
+  const int64_t n = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  index += n * K;
+  q += n * K;
+  z += n * K;
+  auto teacher = [&](int k) {              // t / tau, -inf for an entry that is not there
+    return index[k] < 0 ? -INFINITY : load_as(tl, tdt, n * K + k) * inv_tau;
+  };
+  float m = -INFINITY;
+  for (int k = tid; k < K; k += 256) m = fmaxf(m, teacher(k));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if (lane == 0) sh[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+  const float ms = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  for (int k = tid; k < K; k += 256) s += expf(teacher(k) - ms);
+  s = hd_wave_sum(s);
+  if (lane == 0) sh[4 + wave] = s;
+  __syncthreads();
+  s = (sh[4] + sh[5]) + (sh[6] + sh[7]);
+  const bool any = s > 0.f || s != s;      // a NaN among the listed logits is not an empty row
+  const float ls = any ? logf(s) : 0.f;
+  const float L = lse[n];
+  // the student's logits of the listed classes: a wave per entry
+  float part = 0.f;
+  for (int k = wave; k < K; k += 4) {
+    const int64_t v = index[k];
+    const float t = teacher(k);
+    const bool there = any && v >= 0 && t != -INFINITY;
+    float d = 0.f;
+    if (there && v < V)
+      for (int c = lane; c < D; c += 64) d = __fmaf_rn(load_as(x, dt, n * ldx + c), load_as(w, dt, v * ldw + c), d);
+    d = hd_wave_sum(d);
+    if (lane == 0) {
+      float zk = 0.f, qk = 0.f;
+      if (there) {
+        zk = v < V ? (bias ? d + load_as(bias, dt, v) : d) * inv_tau : NAN;      // no such class: the row says so
+        const float lq = t - ms - ls;
+        qk = expf(lq);
+        part += qk * (lq - (zk - L));
+      }
+      z[k] = zk;
+      q[k] = qk;
+    }
+  }
+  __syncthreads();
+  if (lane == 0) sh[wave] = part;
+  __syncthreads();
+  if (tid == 0) {
+    const float v = tau * tau * ((sh[0] + sh[1]) + (sh[2] + sh[3]));
+    loss[n] = any ? v : 0.f;
+    live[n] = !any ? 0.f : v == v ? 1.f : v;
+  }
+}
+
+// out = sum or mean of the rows' losses, count = how many rows have one (at least 1); a fixed tree of additions
+__global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ loss, const int64_t* __restrict__ target,
+                                                      int64_t ignore, const float* __restrict__ live, int N, int mean,
+                                                      float* __restrict__ out, float* __restrict__ count) {
+  __shared__ float sh[32];
+  float s = 0.f, c = 0.f;
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    s += loss[n];
+    c += target ? (target[n] != ignore ? 1.f : 0.f) : live[n];
+  }
+  s = hd_wave_sum(s);
+  c = hd_wave_sum(c);
+  if ((threadIdx.x & 63) == 0) {
+    sh[threadIdx.x >> 6] = s;
+    sh[16 + (threadIdx.x >> 6)] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = c = 0.f;
+    for (int w = 0; w < 16; ++w) {
+      s += sh[w];
+      c += sh[16 + w];
+    }
+    c = fmaxf(c, 1.f);
+    *out = mean ? s / c : s;
+    *count = c;
+  }
+}
+
+// coef[n] (|.| <= 1, 0 for a row without a loss) and the scalar S with coef[n] S = the gradient of row n's logits' loss:
+// reductions: coef = 1 or 0, S = g f / count;  none: S = a power of two over max |g f|.  f: tau for the teacher's loss.
+__global__ void __launch_bounds__(1024) k_head_coef(const float* __restrict__ g, int per_row, const float* __restrict__ count,
+                                                     float f, const int64_t* __restrict__ target, int64_t ignore,
+                                                     const float* __restrict__ live, int N, float* __restrict__ coef,
+                                                     float* __restrict__ scal) {
+  __shared__ float sh[16];
+  float S = 1.f;
+  auto has = [&](int n) { return target ? target[n] != ignore : live[n] != 0.f; };
+  if (per_row) {
+    float m = 0.f;
+    for (int n = threadIdx.x; n < N; n += 1024)
+      if (has(n)) {
+        const float v = fabsf(g[n] * f);
+        m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
+      }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = 0.f;
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, sh[w]);
+    if (m > 0.f) {
+      int e;
+      frexpf(m, &e);
+      S = ldexpf(1.f, min(max(e, -100), 100));
+    }
+  } else {
+    S = g[0] * f / (count ? *count : 1.f);
+  }
+  // live is NaN for a row that lists a class that does not exist: its gradient says so too
+  for (int n = threadIdx.x; n < N; n += 1024) coef[n] = has(n) ? (per_row ? g[n] * f / S : 1.f) * (live ? live[n] : 1.f) : 0.f;
+  if (threadIdx.x == 0) scal[SC_S] = S;
+}
+
+// teacher: the listed classes of this piece get e = c (exp(z_k - lse) - sum of q over the entries of the same class), from
+// the entry's own logit, over what the product's epilogue wrote there.  Equal indices write the same value.
+template <class T>
+__global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __restrict__ index, const float* __restrict__ q,
+                                                            const float* __restrict__ z, const float* __restrict__ lse,
+                                                            const float* __restrict__ coef, int64_t N, int K, int64_t v0,
+                                                            int64_t nv, int planes, short* __restrict__ E, int64_t ldE,
+                                                            int64_t planeE) {
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= N * K) return;
+  const int64_t n = u / K;
+  const float c = coef[n];
+  const int64_t v = index[u];
+  if (v < v0 || v >= v0 + nv || c == 0.f) return;
+  float sum = 0.f;
+  float zz = z[u];
+  bool here = false;                       // at least one of the class's entries is there
+  for (int k = 0; k < K; ++k)
+    if (index[n * K + k] == v && q[n * K + k] != 0.f) {
+      sum += q[n * K + k];
+      if (!here) zz = z[n * K + k];
+      here = true;
+    }
+  if (!here) return;
+  const float e = c * (__builtin_amdgcn_exp2f((zz - lse[n]) * L2E) - sum);
+  T* o = (T*)E + n * ldE + (v - v0);
+  if (planes == 2) {
+    const float s = e * E_SCALE;
+    const T h = to_t<T>(s);
+    *o = h;
+    o[planeE] = to_t<T>(s - (float)h);
+  } else {
+    *o = to_t<T>(__is_same(T, f16_t) ? e * E_SCALE : e);
+  }
+}
+
+// column sums of e over slices of 256 rows: part[slice][ldE]
+template <class T>
+__global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E, int64_t ldE, int64_t planeE, int planes, int rows,
+                                                      float* __restrict__ part) {
+  const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4, sl = threadIdx.x >> 6;
+  __shared__ float sh[4][64][4];
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < ldE) {
+    const int r0 = blockIdx.y * 256, r1 = min(rows, r0 + 256);
+    for (int r = r0 + sl; r < r1; r += 4)
+      for (int p = 0; p < planes; ++p) {
+        const T* e = (const T*)E + p * planeE + (int64_t)r * ldE + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += (float)e[i];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sh[sl][threadIdx.x & 63][i] = s[i];
+  __syncthreads();
+  if (sl == 0 && c < ldE)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      part[(int64_t)blockIdx.y * ldE + c + i] = (sh[0][threadIdx.x][i] + sh[1][threadIdx.x][i]) + (sh[2][threadIdx.x][i] + sh[3][threadIdx.x][i]);
+}
+
+// out[at0 + i] = factor * sum_s part[s][i] over `slots` partials, in order
+template <class T>
+__global__ void __launch_bounds__(256) k_head_sum(const float* __restrict__ part, int slots, int64_t stride, int64_t n,
+                                                   const float* __restrict__ scal, int other, void* __restrict__ out, int dt,
+                                                   int64_t at0) {
+  const float f = hd_factor<T>(scal, other);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = part[i];
+    for (int k = 1; k < slots; ++k) s += part[(int64_t)k * stride + i];
+    store_as(out, dt, at0 + i, s * f);
+  }
+}
+
+// ---- host: tile shapes, pieces and workspace ---------------------------------------------------------------------------------
+struct HdShape {
+  int b, splits;             // tile edge 64 / 128 / 256
+};
+
+// The tile edge and the number of k ranges with the smallest estimated time: rounds of tiles over the CUs at the measured
+// rate of each tile edge, no k step under its latency, and the partial results of a split product written and read once.
+static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) {
+  static const int edge[3] = {64, 128, 256};
+  static const double step_us[3] = {0.60, 0.75, 1.60};       // one k step of a tile (measured, all CUs busy)
+  const int cus = dig3d_num_cus();
+  HdShape best = {64, 1};
+  double tb = 1e30;
+  for (int e = 0; e < 3; ++e) {
+    const int64_t tiles = ((ni + edge[e] - 1) / edge[e]) * ((nj + edge[e] - 1) / edge[e]);
+    const int slots = cus * (edge[e] == 256 ? 1 : edge[e] == 128 ? 2 : 4);
+    const double us = edge[e] == 256 ? step_us[e] : step_us[e] * (edge[e] == 128 ? 1.0 : 1.0);
+    for (int s = 1; s <= max_splits; s *= 2) {
+      if (s > 1 && (ksteps / s < 4 || (double)s * ni * nj * 4 > 512e6)) break;
+      const int64_t rounds = (tiles * s + slots - 1) / slots;
+      double t = (double)rounds * ((ksteps + s - 1) / s) * us;
+      if (s > 1) t += 3.0 + (double)s * ni * nj * 8 / 4e6;     // 4 TB/s = 4e6 bytes a us
+      if (t < tb) {
+        tb = t;
+        best = {edge[e], s};
+      }
+    }
+  }
+  return best;
+}
+
+static inline int64_t up64(int64_t v) { return (v + 63) & ~63ll; }
+static inline int64_t al256(int64_t v) { return (v + 255) & ~255ll; }
+
+struct HdPlan {
+  int planes, Dp;
+  bool dx, dw;               // x / W are read where they are
+  int64_t Np, vp, np, ldE;
+  HdShape lg, gx, gw;
+  int tiles_all;
+  // byte offsets into the workspace
+  int64_t o_x, o_w, o_part, o_zt, o_coef, o_E, o_gx, o_gw, o_col, total;
+};
+
+// 16-bit rows are used in place when their pitch keeps 16-byte loads aligned and D is whole k steps
+static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
+  return dt != DT_F32 && D % HD_BK == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0;
+}
+
+#define HD_PIECE_BYTES (512ll << 20)   // e of one piece, per plane; a piece also bounds the packed part of W
+
+// needs: bit 0 gx, bit 1 gw, bit 2 gb; backward = 0: the forward's plan
+static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int backward, int needs) {
+  HdPlan p;
+  memset(&p, 0, sizeof p);
+  p.planes = dt == DT_F32 ? 2 : 1;
+  p.Dp = (int)up64(D);
+  p.dx = dx && !backward;    // the backward masks rows while it copies x (N D elements: nothing beside its products)
+  p.dw = dw;
+  p.Np = up64(N);
+  int64_t most = V;
+  if (backward) most = min(most, HD_PIECE_BYTES / (p.Np * 2));
+  if (!p.dw) most = min(most, HD_PIECE_BYTES / ((int64_t)p.Dp * 2 * p.planes));
+  most = max((int64_t)256, most & ~255ll);
+  p.np = (V + most - 1) / most;
+  p.vp = p.np == 1 ? V : ((V + p.np - 1) / p.np + 255) & ~255ll;
+  p.np = (V + p.vp - 1) / p.vp;
+  p.ldE = up64(p.vp);
+  const int nseg = p.planes == 2 ? 3 : 1;
+  p.lg = hd_shape(p.vp, N, (int64_t)p.Dp / HD_BK * nseg, 1);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += al256(bytes);
+    return o;
+  };
+  if (!p.dx) p.o_x = take(p.Np * p.Dp * 2 * p.planes);
+  if (!p.dw) p.o_w = take(min(p.vp, V) * p.Dp * 2 * p.planes);
+  if (!backward) {
+    p.tiles_all = 0;
+    for (int64_t v0 = 0; v0 < V; v0 += p.vp) p.tiles_all += (int)((min(p.vp, V - v0) + p.lg.b - 1) / p.lg.b);
+    p.o_part = take(N * p.tiles_all * 8);
+    p.o_zt = take(N * 4);
+  } else {
+    p.o_coef = take(N * 4);
+    p.o_E = take(p.Np * p.ldE * 2 * p.planes);
+    if (needs & 1) {
+      p.gx = hd_shape(D, N, p.ldE / HD_BK * nseg, 64);
+      if (p.np > 1 || p.gx.splits > 1) p.o_gx = take((int64_t)p.gx.splits * N * D * 4);
+    }
+    if (needs & 2) {
+      p.gw = hd_shape(D, p.vp, p.Np / HD_BK * nseg, 64);
+      if (p.gw.splits > 1) p.o_gw = take((int64_t)p.gw.splits * p.vp * D * 4);
+    }
+    if (needs & 4) p.o_col = take((N + 255) / 256 * p.ldE * 4);
+  }
+  p.total = at;
+  return p;
+}
+
+template <class T, bool PT, bool QT, int EPI>
+static void hd_gemm(const HdArgs& a0, const HdShape& sh, hipStream_t st) {
+  HdArgs a = a0;
+  a.ti = (a.ni + sh.b - 1) / sh.b;
+  a.tj = (a.nj + sh.b - 1) / sh.b;
+  a.splits = sh.splits;
+  const dim3 grid((unsigned)dig3d_xcd_grid(a.ti * a.tj), 1, (unsigned)sh.splits);
+  if (sh.b == 256) hipLaunchKernelGGL((k_head_gemm<T, 256, 256, 2, 4, PT, QT, EPI>), grid, dim3(512), 0, st, a);
+  else if (sh.b == 128) hipLaunchKernelGGL((k_head_gemm<T, 128, 128, 2, 2, PT, QT, EPI>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_head_gemm<T, 64, 64, 2, 2, PT, QT, EPI>), grid, dim3(256), 0, st, a);
+}
+
+static inline unsigned hd_grid(int64_t items, int per) {
+  const int64_t b = (items + per - 1) / per, cap = 16ll * dig3d_num_cus();
+  return (unsigned)(b < 1 ? 1 : b < cap ? b : cap);
+}
+
+static void hd_pack(const void* src, int dt, int64_t ld, int64_t R, int D, const float* coef, const float* amax, int slot,
+                    float* scal, short* out, int64_t orows, int ocols, int64_t plane, hipStream_t st) {
+  hipLaunchKernelGGL(k_head_pack, dim3(hd_grid(orows * (ocols >> 3), 256)), dim3(256), 0, st, src, dt, ld, R, D, coef, amax,
+                     slot, scal, out, orows, ocols, plane);
+}
+
+static bool hd_bad(int dt, int N, int D, int V, int64_t ldx, int64_t ldw) {
+  // tile counts and row offsets of the small index type stay far inside 32 bits
+  return dt < 0 || dt > 2 || N <= 0 || D <= 0 || V <= 0 || ldx < D || ldw < D ||
+         ((int64_t)N + 63) / 64 * (((int64_t)V + 63) / 64) > (1ll << 30) || N > (1 << 28) || V > (1 << 28) || D > (1 << 20);
+}
+
+static const short* at_bytes(const void* p, int64_t o) { return (const short*)((const char*)p + o); }
+
+template <class T>
+static int hd_lse(int dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
+                  int64_t ignore, float inv_tau, int N, int D, int V, float* scal, float* lse, float* loss, char* ws,
+                  const HdPlan& p, hipStream_t st) {
+  float* amax = scal + SC_COUNT;
+  if (dt == DT_F32) {
+    hipLaunchKernelGGL(k_head_amax, dim3(2 * HD_AMAX), dim3(256), 0, st, (const float*)x, ldx, (int64_t)N, (const float*)w, ldw,
+                       (int64_t)V, D, amax);
+    DIG3D_CHECK_LAUNCH();
+  }
+  HdArgs a;
+  memset(&a, 0, sizeof a);
+  const int64_t xplane = p.Np * p.Dp;
+  if (p.dx) a.Q = {(const short*)x, ldx, 0, N, D};
+  else {
+    hd_pack(x, dt, ldx, N, D, nullptr, amax, SC_X, scal, (short*)(ws + p.o_x), p.Np, p.Dp, xplane, st);
+    DIG3D_CHECK_LAUNCH();
+    a.Q = {at_bytes(ws, p.o_x), p.Dp, xplane, N, p.Dp};
+  }
+  a.nj = N;
+  a.ktiles = p.Dp / HD_BK;
+  a.nseg = p.planes == 2 ? 3 : 1;
+  a.bias = bias;
+  a.dt = dt;
+  a.scal = scal;
+  a.inv_tau = inv_tau;
+  a.V = V;
+  a.target = target;
+  a.part = (float2*)(ws + p.o_part);
+  a.part_ld = p.tiles_all;
+  a.zt = (float*)(ws + p.o_zt);
+  const int esz = dt == DT_F32 ? 4 : 2;
+  for (int64_t v0 = 0; v0 < V; v0 += p.vp) {
+    const int nv = (int)min(p.vp, V - v0);
+    const char* wp = (const char*)w + v0 * ldw * esz;
+    if (p.dw) a.P = {(const short*)wp, ldw, 0, nv, D};
+    else {
+      const int64_t plane = (int64_t)nv * p.Dp;
+      hd_pack(wp, dt, ldw, nv, D, nullptr, amax, SC_W, scal, (short*)(ws + p.o_w), nv, p.Dp, plane, st);
+      DIG3D_CHECK_LAUNCH();
+      a.P = {at_bytes(ws, p.o_w), p.Dp, plane, nv, p.Dp};
+    }
+    a.ni = nv;
+    a.v0 = v0;
+    a.part_c0 = (int)(v0 / p.lg.b);
+    hd_gemm<T, false, false, EPI_STATS>(a, p.lg, st);
+    DIG3D_CHECK_LAUNCH();
+  }
+  hipLaunchKernelGGL(k_head_join, dim3((N + 3) / 4), dim3(256), 0, st, a.part, p.tiles_all, N, (int64_t)V, target, ignore, a.zt,
+                     lse, loss);
+  DIG3D_CHECK_LAUNCH();
+  return DIG3D_OK;
+}
+
+struct HdTeacher {
+  const int64_t* index;
+  const float *q, *z, *live;
+  int K;
+};
+
+template <class T>
+static int hd_bwd(int dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
+                  int64_t ignore, const HdTeacher& th, float tau, int N, int D, int V, const float* g, int per_row,
+                  const float* count, float* scal, const float* lse, const float* loss, void* gx, void* gw, void* gb, char* ws,
+                  const HdPlan& p, hipStream_t st) {
+  float* amax = scal + SC_COUNT;
+  float* coef = (float*)(ws + p.o_coef);
+  hipLaunchKernelGGL(k_head_coef, dim3(1), dim3(1024), 0, st, g, per_row, count, tau, target, ignore, th.live, N, coef, scal);
+  DIG3D_CHECK_LAUNCH();
+  const int64_t xplane = p.Np * p.Dp;
+  const bool planes2 = p.planes == 2;
+  hd_pack(x, dt, ldx, N, D, coef, amax, SC_X, scal, (short*)(ws + p.o_x), p.Np, p.Dp, xplane, st);
+  DIG3D_CHECK_LAUNCH();
+  short* E = (short*)(ws + p.o_E);
+  const int64_t eplane = p.Np * p.ldE;
+  const int esz = dt == DT_F32 ? 4 : 2;
+  const bool gx_slots = gx && (p.np > 1 || p.gx.splits > 1);
+  for (int64_t v0 = 0; v0 < V; v0 += p.vp) {
+    const int nv = (int)min(p.vp, V - v0);
+    const char* wsrc = (const char*)w + v0 * ldw * esz;
+    HdOperand W;
+    if (p.dw) W = {(const short*)wsrc, ldw, 0, nv, D};
+    else {
+      const int64_t plane = (int64_t)nv * p.Dp;
+      hd_pack(wsrc, dt, ldw, nv, D, nullptr, amax, SC_W, scal, (short*)(ws + p.o_w), nv, p.Dp, plane, st);
+      DIG3D_CHECK_LAUNCH();
+      W = {at_bytes(ws, p.o_w), p.Dp, plane, nv, p.Dp};
+    }
+    HdArgs a;
+    memset(&a, 0, sizeof a);
+    a.P = W;
+    a.Q = {at_bytes(ws, p.o_x), p.Dp, xplane, (int)p.Np, p.Dp};
+    a.ni = nv;
+    a.nj = N;
+    a.ktiles = p.Dp / HD_BK;
+    a.nseg = planes2 ? 3 : 1;
+    a.bias = bias;
+    a.dt = dt;
+    a.scal = scal;
+    a.inv_tau = 1.0f / tau;
+    a.v0 = v0;
+    a.V = V;
+    a.target = target;
+    a.lse = lse;
+    a.loss = loss;
+    a.coef = coef;
+    a.E = E;
+    a.ldE = p.ldE;
+    a.planeE = eplane;
+    a.rowsE = (int)p.Np;
+    hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, st);
+    DIG3D_CHECK_LAUNCH();
+    if (th.index) {
+      hipLaunchKernelGGL((k_head_teacher_grad<T>), dim3((unsigned)(((int64_t)N * th.K + 255) / 256)), dim3(256), 0, st, th.index,
+                         th.q, th.z, lse, coef, (int64_t)N, th.K, v0, (int64_t)nv, p.planes, E, p.ldE, eplane);
+      DIG3D_CHECK_LAUNCH();
+    }
+    HdArgs o;
+    memset(&o, 0, sizeof o);
+    o.nseg = a.nseg;
+    o.scal = scal;
+    o.dt = dt;
+    if (gx) {                              // gx[n, d] += sum_v e[n, v] W[v, d]
+      o.P = W;
+      o.Q = {E, p.ldE, eplane, (int)p.Np, (int)p.ldE};
+      o.ni = D;
+      o.nj = N;
+      o.ktiles = (int)(up64(nv) / HD_BK);
+      o.acc = gx_slots ? (float*)(ws + p.o_gx) : nullptr;
+      o.add = v0 > 0;
+      o.out = gx_slots ? nullptr : gx;
+      o.ldo = D;
+      o.other = planes2 ? SC_W : -1;
+      hd_gemm<T, true, false, EPI_OUT>(o, p.gx, st);
+      DIG3D_CHECK_LAUNCH();
+    }
+    if (gw) {                              // gw[v, d] = sum_n e[n, v] x[n, d]
+      const bool slots = p.gw.splits > 1;
+      o.P = {at_bytes(ws, p.o_x), p.Dp, xplane, (int)p.Np, p.Dp};
+      o.Q = {E, p.ldE, eplane, (int)p.Np, (int)p.ldE};
+      o.ni = D;
+      o.nj = nv;
+      o.ktiles = (int)(p.Np / HD_BK);
+      o.acc = slots ? (float*)(ws + p.o_gw) : nullptr;
+      o.add = 0;
+      o.out = slots ? nullptr : (char*)gw + v0 * D * esz;
+      o.ldo = D;
+      o.other = planes2 ? SC_X : -1;
+      hd_gemm<T, true, true, EPI_OUT>(o, p.gw, st);
+      DIG3D_CHECK_LAUNCH();
+      if (slots) {
+        const int64_t n = (int64_t)nv * D;
+        hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(n, 256)), dim3(256), 0, st, (const float*)(ws + p.o_gw), p.gw.splits, n, n,
+                           scal, o.other, gw, dt, v0 * D);
+        DIG3D_CHECK_LAUNCH();
+      }
+    }
+    if (gb) {
+      float* part = (float*)(ws + p.o_col);
+      const int slices = (N + 255) / 256;
+      hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)((p.ldE + 255) / 256), (unsigned)slices), dim3(256), 0, st, E, p.ldE,
+                         eplane, p.planes, N, part);
+      DIG3D_CHECK_LAUNCH();
+      hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(nv, 256)), dim3(256), 0, st, part, slices, p.ldE, (int64_t)nv, scal, -1, gb,
+                         dt, v0);
+      DIG3D_CHECK_LAUNCH();
+    }
+  }
+  if (gx_slots) {
+    const int64_t n = (int64_t)N * D;
+    hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(n, 256)), dim3(256), 0, st, (const float*)(ws + p.o_gx), p.gx.splits, n, n, scal,
+                       planes2 ? SC_W : -1, gx, dt, (int64_t)0);
+    DIG3D_CHECK_LAUNCH();
+  }
+  return DIG3D_OK;
+}
+
+extern "C" {
+
+int dig3d_head_ws_kib(int dtype, int64_t ldx, const void* x, int64_t ldw, const void* w, int N, int D, int V, int backward, int needs) {
+  if (hd_bad(dtype, N, D, V, ldx, ldw)) return DIG3D_ERR_ARG;
+  const HdPlan p = hd_plan(dtype, N, D, V, hd_direct(dtype, x, ldx, D), hd_direct(dtype, w, ldw, D), backward, needs);
+  const int64_t kib = (p.total + 1023) / 1024;
+  return kib > 2147483647ll ? DIG3D_ERR_ARG : (int)kib;
+}
+
+int dig3d_head_lse(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
+                   int64_t ignore_index, float tau, int N, int D, int V, float* scal, float* lse, float* loss, void* ws, int ws_kib,
+                   void* stream) {
+  DIG3D_ENTER();
+  if (hd_bad(dtype, N, D, V, ldx, ldw) || !x || !w || !scal || !lse || (!target) != (!loss) || !(tau > 0.f)) return DIG3D_ERR_ARG;
+  const HdPlan p = hd_plan(dtype, N, D, V, hd_direct(dtype, x, ldx, D), hd_direct(dtype, w, ldw, D), 0, 0);
+  if (p.total > (int64_t)ws_kib * 1024 || (p.total && !ws)) return DIG3D_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DT_BF16)
+    return hd_lse<bf16_t>(dtype, x, ldx, w, ldw, bias, target, ignore_index, 1.0f / tau, N, D, V, scal, lse, loss, (char*)ws, p, st);
+  return hd_lse<f16_t>(dtype, x, ldx, w, ldw, bias, target, ignore_index, 1.0f / tau, N, D, V, scal, lse, loss, (char*)ws, p, st);
+}
+
+int dig3d_head_teacher(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* index,
+                       const void* teacher, int tdtype, int K, float tau, int N, int D, int V, const float* lse, float* q, float* z,
+                       float* loss, float* live, void* stream) {
+  DIG3D_ENTER();
+  if (hd_bad(dtype, N, D, V, ldx, ldw) || tdtype < 0 || tdtype > 2 || K <= 0 || K > (1 << 20) || !x || !w || !index || !teacher || !lse ||
+      !q || !z || !loss || !live || !(tau > 0.f))
+    return DIG3D_ERR_ARG;
+  hipLaunchKernelGGL(k_head_teacher, dim3((unsigned)N), dim3(256), 0, (hipStream_t)stream, x, w, bias, dtype, ldx, ldw, D, (int64_t)V,
+                     index, teacher, tdtype, K, 1.0f / tau, tau, lse, q, z, loss, live);
+  DIG3D_CHECK_LAUNCH();
+  return DIG3D_OK;
+}
+
+int dig3d_head_total(const float* loss, const int64_t* target, int64_t ignore_index, const float* live, int N, int mean, float* out,
+                     float* count, void* stream) {
+  DIG3D_ENTER();
+  if (!loss || !out || !count || N < 0 || (!target) == (!live)) return DIG3D_ERR_ARG;
+  hipLaunchKernelGGL(k_head_total, dim3(1), dim3(1024), 0, (hipStream_t)stream, loss, target, ignore_index, live, N, mean, out,
+                     count);
+  DIG3D_CHECK_LAUNCH();
+  return DIG3D_OK;
+}
+
+int dig3d_head_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
+                   int64_t ignore_index, const int64_t* index, const float* q, const float* z, const float* live, int K, float tau, int N,
+                   int D, int V, const float* g, int per_row, const float* count, float* scal, const float* lse, const float* loss,
+                   void* gx, void* gw, void* gb, void* ws, int ws_kib, void* stream) {
+  DIG3D_ENTER();
+  if (hd_bad(dtype, N, D, V, ldx, ldw) || !x || !w || !g || !scal || !lse || !(tau > 0.f)) return DIG3D_ERR_ARG;
+  if ((!target) == (!index) || (target && !loss) || (index && (!q || !z || !live || K <= 0 || K > (1 << 20)))) return DIG3D_ERR_ARG;
+  const int needs = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
+  if (!needs) return DIG3D_OK;
+  const HdPlan p = hd_plan(dtype, N, D, V, hd_direct(dtype, x, ldx, D), hd_direct(dtype, w, ldw, D), 1, needs);
+  if (p.total > (int64_t)ws_kib * 1024 || !ws) return DIG3D_ERR_ARG;
+  const HdTeacher th = {index, q, z, live, K};
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DT_BF16)
+    return hd_bwd<bf16_t>(dtype, x, ldx, w, ldw, bias, target, ignore_index, th, tau, N, D, V, g, per_row, count, scal, lse, loss, gx, gw,
+                          gb, (char*)ws, p, st);
+  return hd_bwd<f16_t>(dtype, x, ldx, w, ldw, bias, target, ignore_index, th, tau, N, D, V, g, per_row, count, scal, lse, loss, gx, gw, gb,
+                       (char*)ws, p, st);
+}
+
+}  // extern "C"

@@ -742,6 +742,51 @@ int dig3d_wide_dd(int G, int nl, int M, int K0, const void* const* H0, const voi
                   const void* const* G0, void* const* HZ, void* const* U, const int* act, const int* res, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------
+ * Layer norm over the C channels of a row (rownorm.hip).  No reference counterpart (its models normalise per graph,
+ * method/comenet/comenet.py:160): y = w (x - mean) rstd + b, the variance centred, statistics in f32.
+ * dtype of x / y / gy / gx and wdtype of w / b / gw / gb: 0 f32, 1 bf16, 2 f16; w, b may be NULL.  x: R rows of pitch ldx
+ * >= C elements, any alignment of the element type; y, gy, gx: pitch C.  mean / rstd [R]: kept for the backward (both NULL:
+ * not wanted).  Backward: gx, and gw / gb [C] from part = float[nb * 2 * C], nb = dig3d_rownorm_bwd_blocks(R, C, dtype);
+ * gx, gw, gb may be NULL; gw == gb == NULL with a part: the caller sums its nb rows (dig3d_reduce_many).
+ * ------------------------------------------------------------------------------------------------- */
+int dig3d_rownorm_fwd(int dtype, const void* x, int64_t ldx, int R, int C, const void* w, const void* b, int wdtype, float eps,
+                      void* y, float* mean, float* rstd, void* stream);
+int dig3d_rownorm_bwd_blocks(int R, int C, int dtype);
+int dig3d_rownorm_bwd(int dtype, const void* gy, const void* x, int64_t ldx, int R, int C, const void* w, int wdtype,
+                      const float* mean, const float* rstd, void* gx, float* part, int nb, void* gw, void* gb, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * Losses over the V classes of the logits z = x w^T + bias of an output head, the logits never kept (head.hip; the class
+ * heads of method/pronet/pronet.py:349-352 and of the generator's atom types).  dtype of x [N, D] (pitch ldx), w [V, D]
+ * (pitch ldw), bias [V] or NULL, and of the gradients gx [N, D], gw [V, D], gb [V] (pitch D; each may be NULL): 0 f32, 1
+ * bf16, 2 f16.  Statistics, losses and sums: f32.
+ *   dig3d_head_ws_kib   KiB of workspace for dig3d_head_lse (backward = 0) or dig3d_head_bwd (backward = 1; needs = 1 gx + 2 gw
+ *                       + 4 gb); x and w enter by their alignment.  Negative: refused sizes.
+ *   dig3d_head_lse      lse[N] of z / tau; with target [N] (int64) the loss of each row too: 0 where target == ignore_index,
+ *                       NaN where it is no class.  scal: float[516], kept for the backward.
+ *   dig3d_head_teacher  teacher's K largest logits (type tdtype) and their classes index [N, K] (int64; an entry with a negative
+ *                       index or the logit -inf is absent, equal indices add): q = softmax over a row's entries of t / tau, z = the
+ *                       student's own logits / tau there, loss = tau^2 sum q (log q - (z - lse)), live = 1, or 0 for a row
+ *                       without entries (loss 0), or NaN for a row with an index >= V.
+ *   dig3d_head_total    out = sum of loss[N] (mean: over the rows that have one, at least 1), count = that number
+ *   dig3d_head_bwd      exactly one of target / index says which loss; tau 1 with target.  g: the incoming gradient, a scalar, or
+ *                       [N] with per_row; count: the divisor of a mean, or NULL.
+ * ------------------------------------------------------------------------------------------------- */
+int dig3d_head_ws_kib(int dtype, int64_t ldx, const void* x, int64_t ldw, const void* w, int N, int D, int V, int backward, int needs);
+int dig3d_head_lse(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
+                   int64_t ignore_index, float tau, int N, int D, int V, float* scal, float* lse, float* loss, void* ws, int ws_kib,
+                   void* stream);
+int dig3d_head_teacher(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* index,
+                       const void* teacher, int tdtype, int K, float tau, int N, int D, int V, const float* lse, float* q, float* z,
+                       float* loss, float* live, void* stream);
+int dig3d_head_total(const float* loss, const int64_t* target, int64_t ignore_index, const float* live, int N, int mean, float* out,
+                     float* count, void* stream);
+int dig3d_head_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
+                   int64_t ignore_index, const int64_t* index, const float* q, const float* z, const float* live, int K, float tau, int N,
+                   int D, int V, const float* g, int per_row, const float* count, float* scal, const float* lse, const float* loss,
+                   void* gx, void* gw, void* gb, void* ws, int ws_kib, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------
  * Library identity (abi.hip).  No reference counterpart: the reference reaches its kernels through Python wheels
  * (torch_scatter / torch_cluster / torch_sparse, imported at method/spherenet/spherenet.py:1-20) whose version check is
  * pip's; a ctypes binding has none, so the host compares dig3d_abi_hash with the hash of the header it parsed.
