@@ -19,7 +19,7 @@
 
 #include "half16.h"
 
-#define HD_BK 64           // the k step of the product kernel: row pitches are multiples of it
+#define HD_BK 64           // the k step of the product kernel
 #define L2E 1.44269504088896340736f
 #define LN2 0.69314718055994530942f
 
@@ -103,42 +103,67 @@ constexpr int hd_tile_shorts() {
   return B * HD_BK;
 }
 
+// an address that is the same in every lane, in scalar registers
+__device__ __forceinline__ const char* hd_uniform(const char* p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const char*)((uint64_t)hi << 32 | lo);
+}
+
 // lane l of load `q` of a wave fetches 16 bytes to LDS offset 1024 q + 16 l of its tile.
 // not TR: LDS row r holds 8 chunks of 8 k; chunk s of it is source chunk s ^ (r & 7) (reads of 16 rows hit all banks)
 // TR:     LDS row k holds B / 8 chunks; chunk s of it is source chunk s ^ (2 g(k) mod B / 8), g(k) = (k & 3) | (k >> 3 & 3) << 2
-template <int B, bool TR, int NW>
-__device__ __forceinline__ void hd_load(const HdOperand& o, const short* __restrict__ base, int own0, int k0, short* lds, int wave,
-                                        int lane) {
-  constexpr int NL = B * HD_BK * 2 / 1024 / NW;
+// The lane's byte offsets from the tile's first element are formed once (32 bits: 256 rows of at most HD_MAX_PITCH elements);
+// a k step moves the uniform base.
+#define HD_MAX_PITCH (1 << 22)
+template <int B, bool TR, bool CLAMP, int NW>
+struct HdLoad {
+  static constexpr int NL = B * HD_BK * 2 / 1024 / NW;
+  static constexpr int CH = B / 8, RPL = TR ? 64 / CH : 8;      // TR: chunks per row, rows per load
+  uint32_t off[NL];
+  __device__ __forceinline__ void init(const HdOperand& o, int own0, int wave, int lane) {
 #pragma unroll
-  for (int q = 0; q < NL; ++q) {
-    const int blk = q * NW + wave;
-    const short* src;
-    if constexpr (!TR) {
-      const int r = blk * 8 + (lane >> 3);
-      const int row = min(own0 + r, o.rows - 1);
-      const int ch = (lane & 7) ^ (r & 7);
-      src = base + (int64_t)row * o.ld + k0 + ch * 8;
-    } else {
-      constexpr int CH = B / 8, RPL = 64 / CH;       // chunks per row, rows per load
-      const int k = blk * RPL + lane / CH;
-      const int row = min(k0 + k, o.rows - 1);
-      const int g = (k & 3) | (((k >> 3) & 3) << 2);
-      const int ch = (lane % CH) ^ ((2 * g) & (CH - 1));
-      const int col = min(own0 + ch * 8, o.cols - 8);
-      src = base + (int64_t)row * o.ld + col;
+    for (int q = 0; q < NL; ++q) {
+      const int blk = q * NW + wave;
+      if constexpr (!TR) {
+        const int r = blk * 8 + (lane >> 3);
+        const int ch = (lane & 7) ^ (r & 7);
+        off[q] = 2u * ((uint32_t)(min(own0 + r, o.rows - 1) - own0) * (uint32_t)o.ld + ch * 8);
+      } else {
+        const int k = blk * RPL + lane / CH;
+        const int g = (k & 3) | (((k >> 3) & 3) << 2);
+        const int ch = (lane % CH) ^ ((2 * g) & (CH - 1));
+        off[q] = 2u * ((uint32_t)k * (uint32_t)o.ld + min(own0 + ch * 8, o.cols - 8));
+      }
     }
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)(lds + blk * 512), 16, 0, 0);
   }
-}
+  // base: the operand plane's first element.  The load is written out so that the compiler's own waits do not count it: it
+  // has no register result, and the kernel waits for it by count (vmcnt) before the barrier that hands the stage over.
+  // s_nop: the wait states between a scalar register's writer (M0, or a base that came through a vector instruction) and
+  // its reader, which the compiler does not see here.
+  __device__ __forceinline__ void issue(const HdOperand& o, const short* __restrict__ base, int own0, int k0, uint32_t lds,
+                                        int wave, int lane) const {
+    const char* at = hd_uniform((const char*)(base + (TR ? (int64_t)k0 * o.ld : (int64_t)own0 * o.ld + k0)));
+#pragma unroll
+    for (int q = 0; q < NL; ++q) {
+      const int blk = q * NW + wave;
+      uint32_t v = off[q];
+      if constexpr (CLAMP) {               // rows of k beyond the last: the last one again
+        const int k = blk * RPL + lane / CH;
+        v -= 2u * (uint32_t)max(0, k - (o.rows - 1 - k0)) * (uint32_t)o.ld;
+      }
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + blk * 1024), "v"(v), "s"(at)
+                   : "memory");
+    }
+  }
+};
 
-// the matrix operand of 16 own indices from o0 and k half kk (32 of the 64) of a staged tile
+// the matrix operand of 16 own indices from o0 and k half kk of a staged tile
 template <int B, bool TR>
 __device__ __forceinline__ s16x8 hd_frag(const short* lds, int o0, int kk, int lane) {
   if constexpr (!TR) {
     const int r = o0 + (lane & 15);
-    return *(const s16x8*)(lds + r * 64 + (((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 8));
+    return *(const s16x8*)(lds + r * HD_BK + (((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 8));
   } else {
     constexpr int CH = B / 8;
     const int k = kk * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2);
@@ -169,8 +194,8 @@ __device__ __forceinline__ void hd_store4(void* out, int64_t at, f32x4 v, int n)
 template <class T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
 __global__ void __launch_bounds__(WI* WJ * 64) k_head_gemm(HdArgs a) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
-  __shared__ __attribute__((aligned(1024))) short sm0[hd_tile_shorts<BI>() + hd_tile_shorts<BJ>()];
-  __shared__ __attribute__((aligned(1024))) short sm1[hd_tile_shorts<BI>() + hd_tile_shorts<BJ>()];
+  constexpr int SZ = hd_tile_shorts<BI>() + hd_tile_shorts<BJ>();
+  __shared__ __attribute__((aligned(1024))) short sm[2 * SZ];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // tile of this workgroup: an XCD takes a contiguous range of tiles, ordered in bands of 4 tiles along j so that the
   // tiles in flight on one L2 share operand panels along both indices
@@ -191,38 +216,83 @@ __global__ void __launch_bounds__(WI* WJ * 64) k_head_gemm(HdArgs a) {
   const int total = a.ktiles * a.nseg;
   const int t0 = (int)((int64_t)total * blockIdx.z / a.splits), t1 = (int)((int64_t)total * (blockIdx.z + 1) / a.splits);
 
-  auto load = [&](int t, short* sm) {
+  // only W is read along k where it lies, with rows beyond its last (PT && !QT); e and the copied x are whole k steps
+  using LP = HdLoad<BI, PT, PT && !QT, NW>;
+  using LQ = HdLoad<BJ, QT, false, NW>;
+  LP lp;
+  LQ lq;
+  lp.init(a.P, i0, wave, lane);
+  lq.init(a.Q, j0, wave, lane);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) short*)sm;
+  auto load = [&](int t, int stage) {
     const int seg = t / a.ktiles, k0 = (t - seg * a.ktiles) * HD_BK;    // planes (h, h), (h, l), (l, h)
-    hd_load<BI, PT, NW>(a.P, a.P.p + (seg == 2 ? a.P.plane : 0), i0, k0, sm, wave, lane);
-    hd_load<BJ, QT, NW>(a.Q, a.Q.p + (seg == 1 ? a.Q.plane : 0), j0, k0, sm + hd_tile_shorts<BI>(), wave, lane);
+    lp.issue(a.P, a.P.p + (seg == 2 ? a.P.plane : 0), i0, k0, lds0 + stage * (SZ * 2), wave, lane);
+    lq.issue(a.Q, a.Q.p + (seg == 1 ? a.Q.plane : 0), j0, k0, lds0 + stage * (SZ * 2) + hd_tile_shorts<BI>() * 2, wave, lane);
   };
-  auto mul = [&](const short* sm) {
-    const short* sp = sm;
-    const short* sq = sm + hd_tile_shorts<BI>();
+  // Two stages.  A k step is four phases (two halves of k, two of the wave's i); the operands of a phase are read while the
+  // phase before it multiplies.  The barrier that ends a step stands before its last phase, whose operands are in registers
+  // by then: the loads of step t + 2 and the first reads of step t + 1 are issued under that phase's products.
+  constexpr int HX = MI / 2, NLD = LP::NL + LQ::NL;
+  s16x8 fp[2][HX], fq[2][MJ];
+  auto read_p = [&](int stage, int ph) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      s16x8 fq[MJ];
-#pragma unroll
-      for (int y = 0; y < MJ; ++y) fq[y] = hd_frag<BJ, QT>(sq, wj + y * 16, kk, lane);
-#pragma unroll
-      for (int x = 0; x < MI; ++x) {
-        const s16x8 fp = hd_frag<BI, PT>(sp, wi + x * 16, kk, lane);
-#pragma unroll
-        for (int y = 0; y < MJ; ++y) acc[x][y] = hd_mfma<T>(fp, fq[y], acc[x][y]);
-      }
-    }
+    for (int x = 0; x < HX; ++x) fp[ph & 1][x] = hd_frag<BI, PT>(sm + stage * SZ, wi + ((ph & 1) * HX + x) * 16, ph >> 1, lane);
   };
-  if (t0 < t1) load(t0, sm0);
-  for (int t = t0; t < t1; t += 2) {
-    __syncthreads();                       // stage 0 has arrived; stage 1 has been read
-    if (t + 1 < t1) load(t + 1, sm1);
-    mul(sm0);
-    __syncthreads();
-    if (t + 1 < t1) {
-      if (t + 2 < t1) load(t + 2, sm0);
-      mul(sm1);
+  auto read_q = [&](int stage, int kk) {
+#pragma unroll
+    for (int y = 0; y < MJ; ++y) fq[kk][y] = hd_frag<BJ, QT>(sm + stage * SZ + hd_tile_shorts<BI>(), wj + y * 16, kk, lane);
+  };
+  auto mul = [&](int ph) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int x = 0; x < HX; ++x)
+#pragma unroll
+      for (int y = 0; y < MJ; ++y) acc[(ph & 1) * HX + x][y] = hd_mfma<T>(fp[ph & 1][x], fq[ph >> 1][y], acc[(ph & 1) * HX + x][y]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // all loads of this wave have landed, its LDS reads are done, and every other wave's
+  auto meet = [&]() {
+    __builtin_amdgcn_s_waitcnt(7 << 4);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+  // Every step issues its loads: beyond the last step they fetch that one again, into a stage that is read no more, so that
+  // the count of loads in flight is the same everywhere
+  auto step = [&](int t, int cur) {
+    read_p(cur, 1);
+    mul(0);
+    read_q(cur, 1);
+    read_p(cur, 2);
+    mul(1);
+    read_p(cur, 3);
+    mul(2);
+    meet();                                // step t + 1 has arrived; step t has been read by all
+    load(min(t + 2, t1 - 1), cur);
+    read_q(cur ^ 1, 0);
+    read_p(cur ^ 1, 0);
+    mul(3);
+  };
+  if (t0 < t1) {
+    load(t0, 0);
+    load(min(t0 + 1, t1 - 1), 1);
+    constexpr int left = NLD;
+    __builtin_amdgcn_s_waitcnt((left & 15) | ((left >> 4) << 14) | (7 << 4) | (15 << 8));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    read_q(0, 0);
+    read_p(0, 0);
+    int t = t0;
+    for (; t + 2 <= t1; t += 2) {
+      step(t, 0);
+      step(t + 1, 1);
     }
+    if (t < t1) step(t, 0);
   }
+  __builtin_amdgcn_s_waitcnt(0);           // what was issued by hand has landed
+  __syncthreads();                         // nothing is in flight into LDS when it is used again, or given back
 
   const int q4 = 4 * (lane >> 4), l15 = lane & 15;
   if constexpr (EPI == EPI_OUT) {
@@ -267,8 +337,7 @@ __global__ void __launch_bounds__(WI* WJ * 64) k_head_gemm(HdArgs a) {
     if constexpr (EPI == EPI_STATS) {
       // (max, sum of exp) over this tile's classes without the target, per row; a row's classes lie in the 4 lane groups of
       // WI waves
-      float* sh = (float*)sm0;             // [WI][BJ][2]; the last products have read the stages
-      __syncthreads();
+      float* sh = (float*)sm;             // [WI][BJ][2]
 #pragma unroll
       for (int y = 0; y < MJ; ++y) {
         const int jl = wj + y * 16 + l15, j = j0 + jl;
@@ -714,26 +783,31 @@ struct HdShape {
   int b, splits;             // tile edge 64 / 128 / 256
 };
 
-// The tile edge and the number of k ranges with the smallest estimated time: rounds of tiles over the CUs at the measured
-// rate of each tile edge, no k step under its latency, and the partial results of a split product written and read once.
+// The tile edge and the number of k ranges with the smallest estimated time.  The estimate is fitted to measured launches of
+// the product kernel (bf16; us of one k step of 64 with c tiles on a CU, and us of a tile's first loads and epilogue):
+//   64: 0.5 alone, 1.1 with five on the CU;   128: 0.8 alone, 1.2 with two;   256: 1.9 (one to a CU)
+// e.g. 4096 x 2048 x 65536 (logits): 64 -> 1.9 ms, 128 -> 1.21, 256 -> 1.00;  2048 x 256 x 32768: 103, 83, 74 us;
+// 64 x 1024 x 16384: 11, 17, 35 us;  e W of 1024 x 128 x 65536 in 16 ranges: 51, 56, 113 us.
+// A split product writes its partial results and a second launch adds them (bytes at 4 TB/s and 4 us).
 static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) {
-  static const int edge[3] = {64, 128, 256};
-  static const double step_us[3] = {0.60, 0.75, 1.60};       // one k step of a tile (measured, all CUs busy)
   const int cus = dig3d_num_cus();
   HdShape best = {64, 1};
   double tb = 1e30;
   for (int e = 0; e < 3; ++e) {
-    const int64_t tiles = ((ni + edge[e] - 1) / edge[e]) * ((nj + edge[e] - 1) / edge[e]);
-    const int slots = cus * (edge[e] == 256 ? 1 : edge[e] == 128 ? 2 : 4);
-    const double us = edge[e] == 256 ? step_us[e] : step_us[e] * (edge[e] == 128 ? 1.0 : 1.0);
+    const int edge = 64 << e, occ = e == 0 ? 5 : e == 1 ? 2 : 1;
+    const int64_t tiles = ((ni + edge - 1) / edge) * ((nj + edge - 1) / edge);
     for (int s = 1; s <= max_splits; s *= 2) {
       if (s > 1 && (ksteps / s < 4 || (double)s * ni * nj * 4 > 512e6)) break;
-      const int64_t rounds = (tiles * s + slots - 1) / slots;
-      double t = (double)rounds * ((ksteps + s - 1) / s) * us;
-      if (s > 1) t += 3.0 + (double)s * ni * nj * 8 / 4e6;     // 4 TB/s = 4e6 bytes a us
+      const int64_t items = tiles * s, c0 = (items + cus - 1) / cus;
+      const int c = (int)(c0 < occ ? c0 : occ);
+      const int64_t rounds = (items + (int64_t)cus * c - 1) / ((int64_t)cus * c);
+      const double step = e == 0 ? 0.35 + 0.15 * c : e == 1 ? 0.42 + 0.38 * c : 1.9;
+      const double fixed = e == 0 ? 2.0 + 0.5 * c : e == 1 ? 3.0 + 1.3 * c : 10.0;
+      double t = (double)rounds * (fixed + (double)((ksteps + s - 1) / s) * step);
+      if (s > 1) t += 4.0 + (double)s * ni * nj * 8 / 4e6;
       if (t < tb) {
         tb = t;
-        best = {edge[e], s};
+        best = {edge, s};
       }
     }
   }
@@ -755,7 +829,7 @@ struct HdPlan {
 
 // 16-bit rows are used in place when their pitch keeps 16-byte loads aligned and D is whole k steps
 static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
-  return dt != DT_F32 && D % HD_BK == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0;
+  return dt != DT_F32 && D % HD_BK == 0 && ld % 8 == 0 && ld <= HD_MAX_PITCH && ((uintptr_t)p & 15) == 0;
 }
 
 #define HD_PIECE_BYTES (512ll << 20)   // e of one piece, per plane; a piece also bounds the packed part of W
@@ -967,7 +1041,7 @@ static int hd_bwd(int dt, const void* x, int64_t ldx, const void* w, int64_t ldw
       o.Q = {E, p.ldE, eplane, (int)p.Np, (int)p.ldE};
       o.ni = D;
       o.nj = N;
-      o.ktiles = (int)(up64(nv) / HD_BK);
+      o.ktiles = (int)(up64(nv) / HD_BK);  // no step starts beyond W's last row
       o.acc = gx_slots ? (float*)(ws + p.o_gx) : nullptr;
       o.add = v0 > 0;
       o.out = gx_slots ? nullptr : gx;
