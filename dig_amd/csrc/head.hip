@@ -424,7 +424,9 @@ __global__ void __launch_bounds__(WI* WJ * 64) k_head_gemm(HdArgs a) {
   }
 }
 
-// ---- small kernels ---------------------------------------------------------------------------------------------------------
+#include "head_small.h"
+
+// ---- kernels around the products ---------------------------------------------------------------------------------------------------------
 // partial max |v| over the finite entries of x (blocks [0, HD_AMAX)) and W (the rest): amax[2 HD_AMAX]
 #define HD_AMAX 256
 __global__ void __launch_bounds__(256) k_head_amax(const float* __restrict__ x, int64_t ldx, int64_t R, const float* __restrict__ w,
@@ -533,16 +535,10 @@ __device__ __forceinline__ float hd_wave_sum(float v) {
   return v;
 }
 
-// the tiles' statistics of a row joined, a wave per row.  With targets: lse[n] and loss[n] (0 where the target is
-// `ignore`, NaN where it is no class); without: lse[n].
-__global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ part, int tiles, int N, int64_t V,
-                                                    const int64_t* __restrict__ target, int64_t ignore,
-                                                    const float* __restrict__ zt, float* __restrict__ lse,
-                                                    float* __restrict__ loss) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= N) return;
-  const float2* p = part + n * tiles;
+// the tiles' statistics of one row joined by a wave (result in lane 0): lse, and with a target the row's loss (0 where the
+// target is `ignore`, NaN where it is no class)
+__device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int tiles, int64_t V, bool with_target, int64_t tg,
+                                            int64_t ignore, const float* zt, int lane, float& lse, float& loss) {
   float m = -INFINITY, s = 0.f;
   for (int t = lane; t < tiles; t += 64) m = fmaxf(m, p[t].x);
 #pragma unroll
@@ -550,106 +546,47 @@ __global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ pa
   const float ms = m == -INFINITY ? 0.f : m;
   for (int t = lane; t < tiles; t += 64) s += p[t].y * __builtin_amdgcn_exp2f((p[t].x - ms) * L2E);
   s = hd_wave_sum(s);
-  if (lane != 0) return;
-  if (!target) {
-    lse[n] = m == -INFINITY && s == 0.f ? -INFINITY : ms + logf(s);
+  lse = loss = 0.f;
+  if (!with_target) {
+    lse = ms + logf(s);
     return;
   }
-  const int64_t tg = target[n];
-  if (tg == ignore) {
-    lse[n] = 0.f;
-    loss[n] = 0.f;
-    return;
-  }
+  if (tg == ignore) return;
   if (tg < 0 || tg >= V) {
-    lse[n] = loss[n] = NAN;
+    lse = loss = NAN;
     return;
   }
   // s exp(m) over the other classes, z the target's logit.  The loss from the others' share, not from a difference of
   // two near numbers, where the target holds almost everything
-  const float z = zt[n];
+  const float z = *zt;
   const float M = fmaxf(m, z), Ms = M == -INFINITY ? 0.f : M;
   const float so = s * expf(ms - Ms), st = expf(z - Ms);
-  lse[n] = Ms + logf(so + st);
-  loss[n] = z >= m ? log1pf(so) : (Ms - z) + logf(so + st);
+  lse = Ms + logf(so + st);
+  loss = z >= m ? log1pf(so) : (Ms - z) + logf(so + st);
 }
 
-// teacher: a workgroup per row.  q [N, K] = softmax over the row's listed classes of t / tau (0 where the index is negative
-// or the logit -inf), z [N, K] = their own logits / tau, loss[n], count via live[n]
-__global__ void __launch_bounds__(256) k_head_teacher(const void* __restrict__ x, const void* __restrict__ w,
-                                                       const void* __restrict__ bias, int dt, int64_t ldx, int64_t ldw, int D,
-                                                       int64_t V, const int64_t* __restrict__ index, const void* __restrict__ tl,
-                                                       int tdt, int K, float inv_tau, float tau, const float* __restrict__ lse,
-                                                       float* __restrict__ q, float* __restrict__ z, float* __restrict__ loss,
-                                                       float* __restrict__ live) {
-  __shared__ float sh[8];
-  const int64_t n = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  index += n * K;
-  q += n * K;
-  z += n * K;
-  auto teacher = [&](int k) {              // t / tau, -inf for an entry that is not there
-    return index[k] < 0 ? -INFINITY : load_as(tl, tdt, n * K + k) * inv_tau;
-  };
-  float m = -INFINITY;
-  for (int k = tid; k < K; k += 256) m = fmaxf(m, teacher(k));
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (lane == 0) sh[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-  const float ms = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
-  for (int k = tid; k < K; k += 256) s += expf(teacher(k) - ms);
-  s = hd_wave_sum(s);
-  if (lane == 0) sh[4 + wave] = s;
-  __syncthreads();
-  s = (sh[4] + sh[5]) + (sh[6] + sh[7]);
-  const bool any = s > 0.f || s != s;      // a NaN among the listed logits is not an empty row
-  const float ls = any ? logf(s) : 0.f;
-  const float L = lse[n];
-  // the student's logits of the listed classes: a wave per entry
-  float part = 0.f;
-  for (int k = wave; k < K; k += 4) {
-    const int64_t v = index[k];
-    const float t = teacher(k);
-    const bool there = any && v >= 0 && t != -INFINITY;
-    float d = 0.f;
-    if (there && v < V)
-      for (int c = lane; c < D; c += 64) d = __fmaf_rn(load_as(x, dt, n * ldx + c), load_as(w, dt, v * ldw + c), d);
-    d = hd_wave_sum(d);
-    if (lane == 0) {
-      float zk = 0.f, qk = 0.f;
-      if (there) {
-        zk = v < V ? (bias ? d + load_as(bias, dt, v) : d) * inv_tau : NAN;      // no such class: the row says so
-        const float lq = t - ms - ls;
-        qk = expf(lq);
-        part += qk * (lq - (zk - L));
-      }
-      z[k] = zk;
-      q[k] = qk;
+// a wave per row
+__global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ part, int tiles, int N, int64_t V,
+                                                    const int64_t* __restrict__ target, int64_t ignore,
+                                                    const float* __restrict__ zt, float* __restrict__ lse,
+                                                    float* __restrict__ loss, float* __restrict__ rows_out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N) return;
+  float l, v;
+  hd_join_row(part + n * tiles, tiles, V, target != nullptr, target ? target[n] : 0, ignore, zt + n, lane, l, v);
+  if (lane == 0) {
+    lse[n] = l;
+    if (target) {
+      loss[n] = v;
+      if (rows_out) rows_out[n] = v;
     }
   }
-  __syncthreads();
-  if (lane == 0) sh[wave] = part;
-  __syncthreads();
-  if (tid == 0) {
-    const float v = tau * tau * ((sh[0] + sh[1]) + (sh[2] + sh[3]));
-    loss[n] = any ? v : 0.f;
-    live[n] = !any ? 0.f : v == v ? 1.f : v;
-  }
 }
 
-// out = sum or mean of the rows' losses, count = how many rows have one (at least 1); a fixed tree of additions
-__global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ loss, const int64_t* __restrict__ target,
-                                                      int64_t ignore, const float* __restrict__ live, int N, int mean,
-                                                      float* __restrict__ out, float* __restrict__ count) {
-  __shared__ float sh[32];
-  float s = 0.f, c = 0.f;
-  for (int n = threadIdx.x; n < N; n += 1024) {
-    s += loss[n];
-    c += target ? (target[n] != ignore ? 1.f : 0.f) : live[n];
-  }
+// out = sum or mean of the rows' losses, count = how many rows have one (at least 1): a fixed tree of additions over the
+// 1024 threads of one workgroup
+__device__ __forceinline__ void hd_total(float s, float c, int mean, float* out, float* count, float* sh) {
   s = hd_wave_sum(s);
   c = hd_wave_sum(c);
   if ((threadIdx.x & 63) == 0) {
@@ -666,6 +603,140 @@ __global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ l
     c = fmaxf(c, 1.f);
     *out = mean ? s / c : s;
     *count = c;
+  }
+}
+__global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ loss, const int64_t* __restrict__ target,
+                                                      int64_t ignore, const float* __restrict__ live, int N, int mean,
+                                                      float* __restrict__ out, float* __restrict__ count) {
+  __shared__ float sh[32];
+  float s = 0.f, c = 0.f;
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    s += loss[n];
+    c += target ? (target[n] != ignore ? 1.f : 0.f) : live[n];
+  }
+  hd_total(s, c, mean, out, count, sh);
+}
+// few rows: the join and the total in one workgroup
+__global__ void __launch_bounds__(1024) k_head_join_total(const float2* __restrict__ part, int tiles, int N, int64_t V,
+                                                           const int64_t* __restrict__ target, int64_t ignore,
+                                                           const float* __restrict__ zt, float* __restrict__ lse,
+                                                           float* __restrict__ loss, int mean, float* __restrict__ out,
+                                                           float* __restrict__ count) {
+  __shared__ float sh[32];
+  const int lane = threadIdx.x & 63;
+  float s = 0.f, c = 0.f;
+  for (int n = threadIdx.x >> 6; n < N; n += 16) {
+    float l, v;
+    hd_join_row(part + (int64_t)n * tiles, tiles, V, true, target[n], ignore, zt + n, lane, l, v);
+    if (lane == 0) {
+      lse[n] = l;
+      loss[n] = v;
+      s += v;
+      c += target[n] != ignore ? 1.f : 0.f;
+    }
+  }
+  hd_total(s, c, mean, out, count, sh);
+}
+
+#define TC_MAX 2048          // a teacher's entries per row (16 bytes of LDS each)
+
+// teacher: a workgroup per row.  q [N, K]: the softmax over the row's listed classes of t / tau, summed over the entries of
+// the same class, -1 for an absent entry (negative index, or logit -inf); z [N, K]: the student's own logits / tau there;
+// loss[n]; live[n] = 1, 0 without entries, NaN with an index that is no class.  A wave forms four logits at a time: the
+// row of x and four rows of W in 16-byte pieces (N K D elements of W are gathered: bound by the caches).
+template <class T>
+__global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, const T* __restrict__ w, const void* __restrict__ bias,
+                                                       int dt, int64_t ldx, int64_t ldw, int D, int64_t V,
+                                                       const int64_t* __restrict__ index, const void* __restrict__ tl, int tdt, int K,
+                                                       float inv_tau, float tau, const float* __restrict__ lse, float* __restrict__ q,
+                                                       float* __restrict__ z, float* __restrict__ loss, float* __restrict__ live,
+                                                       float* __restrict__ rows_out) {
+  constexpr int N8 = VecLen<T>::n;
+  extern __shared__ int64_t dyn[];         // index [K], then t / tau [K], then q [K]
+  float* st = (float*)(dyn + K);
+  float* sq = st + K;
+  __shared__ float sh[8];
+  const int64_t n = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float m = -INFINITY;
+  for (int k = tid; k < K; k += 256) {
+    const int64_t v = index[n * K + k];
+    const float t = v < 0 ? -INFINITY : load_as(tl, tdt, n * K + k) * inv_tau;
+    dyn[k] = v;
+    st[k] = t;
+    m = fmaxf(m, t);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if (lane == 0) sh[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+  const float ms = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  for (int k = tid; k < K; k += 256) s += expf(st[k] - ms);
+  s = hd_wave_sum(s);
+  if (lane == 0) sh[4 + wave] = s;
+  __syncthreads();
+  s = (sh[4] + sh[5]) + (sh[6] + sh[7]);
+  const bool any = s > 0.f || s != s;      // a NaN among the listed logits is not an empty row
+  const float ls = any ? logf(s) : 0.f;
+  const float L = lse[n];
+  for (int k = tid; k < K; k += 256) sq[k] = st[k] == -INFINITY ? 0.f : expf(st[k] - ms - ls);
+  __syncthreads();
+  const T* xr = x + n * ldx;
+  float part = 0.f;
+  for (int k0 = wave * 4; k0 < K; k0 += 16) {
+    const T* row[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t v = k0 + e < K ? dyn[k0 + e] : 0;
+      row[e] = w + (v >= 0 && v < V ? v : 0) * ldw;              // what is not there reads class 0, and is not used
+    }
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = lane * N8; c < D; c += 64 * N8) {
+      if (c + N8 <= D) {
+        const RowVec<T, N8> xv = *(const RowVec<T, N8>*)(xr + c);
+        RowVec<T, N8> wv[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wv[e] = *(const RowVec<T, N8>*)(row[e] + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < N8; ++i) d[e] = __fmaf_rn((float)xv.v[i], (float)wv[e].v[i], d[e]);
+      } else {
+        for (int i = c; i < D; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[e] = __fmaf_rn((float)xr[i], (float)row[e][i], d[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float dot = hd_wave_sum(d[e]);
+      const int k = k0 + e;
+      if (lane != 0 || k >= K) continue;
+      const int64_t v = dyn[k];
+      const float t = st[k];
+      float zk = 0.f;
+      if (any && t != -INFINITY) {
+        zk = v < V ? (bias ? dot + load_as(bias, dt, v) : dot) * inv_tau : NAN;     // no such class: the row says so
+        part += sq[k] * (t - ms - ls - (zk - L));
+      }
+      z[n * K + k] = zk;
+    }
+  }
+  if (lane == 0) sh[wave] = part;
+  for (int k = tid; k < K; k += 256) {     // entries of the same class add up
+    float sum = 0.f;
+    const int64_t v = dyn[k];
+    for (int e = 0; e < K; ++e) sum += dyn[e] == v ? sq[e] : 0.f;
+    q[n * K + k] = st[k] == -INFINITY ? -1.f : sum;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    const float v = tau * tau * ((sh[0] + sh[1]) + (sh[2] + sh[3]));
+    loss[n] = any ? v : 0.f;
+    live[n] = !any ? 0.f : v == v ? 1.f : v;
+    if (rows_out) rows_out[n] = any ? v : 0.f;
   }
 }
 
@@ -704,33 +775,25 @@ __global__ void __launch_bounds__(1024) k_head_coef(const float* __restrict__ g,
   if (threadIdx.x == 0) scal[SC_S] = S;
 }
 
-// teacher: the listed classes of this piece get e = c (exp(z_k - lse) - sum of q over the entries of the same class), from
-// the entry's own logit, over what the product's epilogue wrote there.  Equal indices write the same value.
+// teacher: the listed classes of this piece get e = c (exp(z_k - lse) - q_k), from the entry's own logit, over what the
+// product's epilogue wrote there.  Entries of the same class hold the same q and z and write the same value.
 template <class T>
 __global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __restrict__ index, const float* __restrict__ q,
                                                             const float* __restrict__ z, const float* __restrict__ lse,
                                                             const float* __restrict__ coef, int64_t N, int K, int64_t v0,
-                                                            int64_t nv, int planes, short* __restrict__ E, int64_t ldE,
+                                                            int64_t nv, int planes, void* __restrict__ E, int64_t ldE,
                                                             int64_t planeE) {
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (u >= N * K) return;
   const int64_t n = u / K;
-  const float c = coef[n];
+  const float qk = q[u], c = coef[n];
   const int64_t v = index[u];
-  if (v < v0 || v >= v0 + nv || c == 0.f) return;
-  float sum = 0.f;
-  float zz = z[u];
-  bool here = false;                       // at least one of the class's entries is there
-  for (int k = 0; k < K; ++k)
-    if (index[n * K + k] == v && q[n * K + k] != 0.f) {
-      sum += q[n * K + k];
-      if (!here) zz = z[n * K + k];
-      here = true;
-    }
-  if (!here) return;
-  const float e = c * (__builtin_amdgcn_exp2f((zz - lse[n]) * L2E) - sum);
+  if (v < v0 || v >= v0 + nv || c == 0.f || qk < 0.f) return;
+  const float e = c * (__builtin_amdgcn_exp2f((z[u] - lse[n]) * L2E) - qk);
   T* o = (T*)E + n * ldE + (v - v0);
-  if (planes == 2) {
+  if constexpr (sizeof(T) == 4) {
+    *o = e;
+  } else if (planes == 2) {
     const float s = e * E_SCALE;
     const T h = to_t<T>(s);
     *o = h;
@@ -740,7 +803,8 @@ __global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __rest
   }
 }
 
-// column sums of e over slices of 256 rows: part[slice][ldE]
+#define HD_SLICE 256
+// column sums of e over slices of HD_SLICE rows: part[slice][ldE]
 template <class T>
 __global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E, int64_t ldE, int64_t planeE, int planes, int rows,
                                                       float* __restrict__ part) {
@@ -748,7 +812,7 @@ __global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E
   __shared__ float sh[4][64][4];
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < ldE) {
-    const int r0 = blockIdx.y * 256, r1 = min(rows, r0 + 256);
+    const int r0 = blockIdx.y * HD_SLICE, r1 = min(rows, r0 + HD_SLICE);
     for (int r = r0 + sl; r < r1; r += 4)
       for (int p = 0; p < planes; ++p) {
         const T* e = (const T*)E + p * planeE + (int64_t)r * ldE + c;
@@ -770,7 +834,7 @@ template <class T>
 __global__ void __launch_bounds__(256) k_head_sum(const float* __restrict__ part, int slots, int64_t stride, int64_t n,
                                                    const float* __restrict__ scal, int other, void* __restrict__ out, int dt,
                                                    int64_t at0) {
-  const float f = hd_factor<T>(scal, other);
+  const float f = scal ? hd_factor<T>(scal, other) : 1.f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     float s = part[i];
     for (int k = 1; k < slots; ++k) s += part[(int64_t)k * stride + i];
@@ -818,6 +882,7 @@ static inline int64_t up64(int64_t v) { return (v + 63) & ~63ll; }
 static inline int64_t al256(int64_t v) { return (v + 255) & ~255ll; }
 
 struct HdPlan {
+  bool small;                // head_small.h
   int planes, Dp;
   bool dx, dw;               // x / W are read where they are
   int64_t Np, vp, np, ldE;
@@ -834,10 +899,41 @@ static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
 
 #define HD_PIECE_BYTES (512ll << 20)   // e of one piece, per plane; a piece also bounds the packed part of W
 
+// Float32 products in place (head_small.h) below this size: SMALL_RULE
+static bool hd_small(int64_t N, int64_t D, int64_t V) { return (double)N * D * V <= 33554432.0; }
+
 // needs: bit 0 gx, bit 1 gw, bit 2 gb; backward = 0: the forward's plan
 static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int backward, int needs) {
   HdPlan p;
   memset(&p, 0, sizeof p);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += al256(bytes);
+    return o;
+  };
+  p.small = hd_small(N, D, V);
+  if (p.small) {
+    p.vp = V;
+    p.np = 1;
+    p.ldE = (V + 3) & ~3ll;
+    p.tiles_all = (int)((V + 63) / 64);
+    if (!backward) {
+      p.o_part = take(N * p.tiles_all * 8);
+      p.o_zt = take(N * 4);
+    } else {
+      p.o_coef = take(2 * N * 4);
+      p.o_E = take(N * p.ldE * 4);
+      p.gx = {64, 1};
+      if (needs & 1) {       // about two workgroups per CU, at least four k steps each
+        const int64_t tiles = ((D + 63) / 64) * ((N + 63) / 64), steps = (V + SM_BK - 1) / SM_BK;
+        while (p.gx.splits < 32 && tiles * p.gx.splits < 2 * dig3d_num_cus() && steps / (2 * p.gx.splits) >= 2) p.gx.splits *= 2;
+        if (p.gx.splits > 1) p.o_gx = take(p.gx.splits * N * D * 4);
+      }
+    }
+    p.total = at;
+    return p;
+  }
   p.planes = dt == DT_F32 ? 2 : 1;
   p.Dp = (int)up64(D);
   p.dx = dx && !backward;    // the backward masks rows while it copies x (N D elements: nothing beside its products)
@@ -853,12 +949,6 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
   p.ldE = up64(p.vp);
   const int nseg = p.planes == 2 ? 3 : 1;
   p.lg = hd_shape(p.vp, N, (int64_t)p.Dp / HD_BK * nseg, 1);
-  int64_t at = 0;
-  auto take = [&](int64_t bytes) {
-    const int64_t o = at;
-    at += al256(bytes);
-    return o;
-  };
   if (!p.dx) p.o_x = take(p.Np * p.Dp * 2 * p.planes);
   if (!p.dw) p.o_w = take(min(p.vp, V) * p.Dp * 2 * p.planes);
   if (!backward) {
@@ -877,7 +967,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
       p.gw = hd_shape(D, p.vp, p.Np / HD_BK * nseg, 64);
       if (p.gw.splits > 1) p.o_gw = take((int64_t)p.gw.splits * p.vp * D * 4);
     }
-    if (needs & 4) p.o_col = take((N + 255) / 256 * p.ldE * 4);
+    if (needs & 4) p.o_col = take((N + HD_SLICE - 1) / HD_SLICE * p.ldE * 4);
   }
   p.total = at;
   return p;
@@ -914,91 +1004,214 @@ static bool hd_bad(int dt, int N, int D, int V, int64_t ldx, int64_t ldw) {
 
 static const short* at_bytes(const void* p, int64_t o) { return (const short*)((const char*)p + o); }
 
+// everything the entries share
+struct HdCall {
+  int dt;
+  const void *x, *w, *bias;
+  int64_t ldx, ldw;
+  int N, D, V;
+  const int64_t* target;
+  int64_t ignore;
+  const int64_t* index;
+  const void* teacher;
+  int tdt, K;
+  float tau;
+  int reduction;             // 0 one loss per row, 1 mean, 2 sum
+  // kept from the forward for the backward (float[HD_KEEP + 3 N + 2 N K])
+  float *scal, *amax, *count, *lse, *loss, *live, *q, *z;
+  hipStream_t st;
+};
+#define HD_KEEP 520
+
+static void hd_keep(HdCall& c, float* keep) {
+  c.scal = keep;
+  c.amax = keep + SC_COUNT;
+  c.count = keep + SC_COUNT + 2 * HD_AMAX;
+  c.lse = keep + HD_KEEP;
+  c.loss = c.lse + c.N;
+  c.live = c.loss + c.N;
+  c.q = c.live + c.N;
+  c.z = c.q + (int64_t)c.N * c.K;
+}
+
+static SmArgs sm_args(const HdCall& c, const HdPlan& p, char* ws) {
+  SmArgs a;
+  memset(&a, 0, sizeof a);
+  a.W = {c.w, c.dt, c.ldw, c.V, c.D, nullptr, -1};
+  a.x = {c.x, c.dt, c.ldx, c.N, c.D, nullptr, -1};
+  a.bias = c.bias;
+  a.dt = c.dt;
+  a.N = c.N;
+  a.D = c.D;
+  a.V = c.V;
+  a.inv_tau = 1.0f / c.tau;
+  a.f = c.index ? c.tau : 1.f;
+  a.target = c.target;
+  a.ignore = c.ignore;
+  a.live = c.live;
+  a.part = (float2*)(ws + p.o_part);
+  a.tiles = p.tiles_all;
+  a.zt = (float*)(ws + p.o_zt);
+  a.lse = c.lse;
+  a.loss = c.loss;
+  return a;
+}
+
+// the logits' statistics into a.part / a.zt
 template <class T>
-static int hd_lse(int dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
-                  int64_t ignore, float inv_tau, int N, int D, int V, float* scal, float* lse, float* loss, char* ws,
-                  const HdPlan& p, hipStream_t st) {
-  float* amax = scal + SC_COUNT;
-  if (dt == DT_F32) {
-    hipLaunchKernelGGL(k_head_amax, dim3(2 * HD_AMAX), dim3(256), 0, st, (const float*)x, ldx, (int64_t)N, (const float*)w, ldw,
-                       (int64_t)V, D, amax);
+static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
+  if (c.dt == DT_F32) {
+    hipLaunchKernelGGL(k_head_amax, dim3(2 * HD_AMAX), dim3(256), 0, c.st, (const float*)c.x, c.ldx, (int64_t)c.N, (const float*)c.w,
+                       c.ldw, (int64_t)c.V, c.D, c.amax);
     DIG3D_CHECK_LAUNCH();
   }
   HdArgs a;
   memset(&a, 0, sizeof a);
   const int64_t xplane = p.Np * p.Dp;
-  if (p.dx) a.Q = {(const short*)x, ldx, 0, N, D};
+  if (p.dx) a.Q = {(const short*)c.x, c.ldx, 0, c.N, c.D};
   else {
-    hd_pack(x, dt, ldx, N, D, nullptr, amax, SC_X, scal, (short*)(ws + p.o_x), p.Np, p.Dp, xplane, st);
+    hd_pack(c.x, c.dt, c.ldx, c.N, c.D, nullptr, c.amax, SC_X, c.scal, (short*)(ws + p.o_x), p.Np, p.Dp, xplane, c.st);
     DIG3D_CHECK_LAUNCH();
-    a.Q = {at_bytes(ws, p.o_x), p.Dp, xplane, N, p.Dp};
+    a.Q = {at_bytes(ws, p.o_x), p.Dp, xplane, c.N, p.Dp};
   }
-  a.nj = N;
+  a.nj = c.N;
   a.ktiles = p.Dp / HD_BK;
   a.nseg = p.planes == 2 ? 3 : 1;
-  a.bias = bias;
-  a.dt = dt;
-  a.scal = scal;
-  a.inv_tau = inv_tau;
-  a.V = V;
-  a.target = target;
+  a.bias = c.bias;
+  a.dt = c.dt;
+  a.scal = c.scal;
+  a.inv_tau = 1.0f / c.tau;
+  a.V = c.V;
+  a.target = c.target;
   a.part = (float2*)(ws + p.o_part);
   a.part_ld = p.tiles_all;
   a.zt = (float*)(ws + p.o_zt);
-  const int esz = dt == DT_F32 ? 4 : 2;
-  for (int64_t v0 = 0; v0 < V; v0 += p.vp) {
-    const int nv = (int)min(p.vp, V - v0);
-    const char* wp = (const char*)w + v0 * ldw * esz;
-    if (p.dw) a.P = {(const short*)wp, ldw, 0, nv, D};
+  const int esz = c.dt == DT_F32 ? 4 : 2;
+  for (int64_t v0 = 0; v0 < c.V; v0 += p.vp) {
+    const int nv = (int)min(p.vp, c.V - v0);
+    const char* wp = (const char*)c.w + v0 * c.ldw * esz;
+    if (p.dw) a.P = {(const short*)wp, c.ldw, 0, nv, c.D};
     else {
       const int64_t plane = (int64_t)nv * p.Dp;
-      hd_pack(wp, dt, ldw, nv, D, nullptr, amax, SC_W, scal, (short*)(ws + p.o_w), nv, p.Dp, plane, st);
+      hd_pack(wp, c.dt, c.ldw, nv, c.D, nullptr, c.amax, SC_W, c.scal, (short*)(ws + p.o_w), nv, p.Dp, plane, c.st);
       DIG3D_CHECK_LAUNCH();
       a.P = {at_bytes(ws, p.o_w), p.Dp, plane, nv, p.Dp};
     }
     a.ni = nv;
     a.v0 = v0;
     a.part_c0 = (int)(v0 / p.lg.b);
-    hd_gemm<T, false, false, EPI_STATS>(a, p.lg, st);
+    hd_gemm<T, false, false, EPI_STATS>(a, p.lg, c.st);
     DIG3D_CHECK_LAUNCH();
   }
-  hipLaunchKernelGGL(k_head_join, dim3((N + 3) / 4), dim3(256), 0, st, a.part, p.tiles_all, N, (int64_t)V, target, ignore, a.zt,
-                     lse, loss);
+  return DIG3D_OK;
+}
+
+static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
+  float2* part = (float2*)(ws + p.o_part);
+  float* zt = (float*)(ws + p.o_zt);
+  if (p.small) {
+    hipLaunchKernelGGL((k_head_small_logits<false>), dim3((unsigned)p.tiles_all, (unsigned)((c.N + 63) / 64)), dim3(256), 0, c.st,
+                       sm_args(c, p, ws));
+    DIG3D_CHECK_LAUNCH();
+  } else {
+    const int rc = c.dt == DT_BF16 ? hd_stats<bf16_t>(c, p, ws) : hd_stats<f16_t>(c, p, ws);
+    if (rc != DIG3D_OK) return rc;
+  }
+  // 64 rows: one workgroup joins them in the time of one more launch (2 us each)
+  if (c.target && c.reduction && c.N <= 64) {
+    hipLaunchKernelGGL(k_head_join_total, dim3(1), dim3(1024), 0, c.st, part, p.tiles_all, c.N, (int64_t)c.V, c.target, c.ignore, zt,
+                       c.lse, c.loss, c.reduction == 1, out, c.count);
+    DIG3D_CHECK_LAUNCH();
+    return DIG3D_OK;
+  }
+  float* rows_out = c.reduction ? nullptr : out;
+  hipLaunchKernelGGL(k_head_join, dim3((c.N + 3) / 4), dim3(256), 0, c.st, part, p.tiles_all, c.N, (int64_t)c.V, c.target, c.ignore, zt,
+                     c.lse, c.loss, rows_out);
+  DIG3D_CHECK_LAUNCH();
+  if (c.index) {
+    const dim3 g((unsigned)c.N), b(256);
+    const size_t lds = (size_t)c.K * 16;
+    const float it = 1.0f / c.tau;
+#define TC_GO(T)                                                                                                                       \
+  hipLaunchKernelGGL((k_head_teacher<T>), g, b, lds, c.st, (const T*)c.x, (const T*)c.w, c.bias, c.dt, c.ldx, c.ldw, c.D, (int64_t)c.V, \
+                     c.index, c.teacher, c.tdt, c.K, it, c.tau, c.lse, c.q, c.z, c.loss, c.live, rows_out)
+    if (c.dt == DT_F32) TC_GO(float);
+    else if (c.dt == DT_BF16) TC_GO(bf16_t);
+    else TC_GO(f16_t);
+#undef TC_GO
+    DIG3D_CHECK_LAUNCH();
+  }
+  if (c.reduction) {
+    hipLaunchKernelGGL(k_head_total, dim3(1), dim3(1024), 0, c.st, c.loss, c.target, c.ignore, c.live, c.N, c.reduction == 1, out,
+                       c.count);
+    DIG3D_CHECK_LAUNCH();
+  }
+  return DIG3D_OK;
+}
+
+template <class T>
+static int hd_teacher_grad(const HdCall& c, const float* coef, int64_t v0, int64_t nv, int planes, void* E, int64_t ldE,
+                           int64_t planeE) {
+  hipLaunchKernelGGL((k_head_teacher_grad<T>), dim3((unsigned)(((int64_t)c.N * c.K + 255) / 256)), dim3(256), 0, c.st, c.index, c.q,
+                     c.z, c.lse, coef, (int64_t)c.N, c.K, v0, nv, planes, E, ldE, planeE);
   DIG3D_CHECK_LAUNCH();
   return DIG3D_OK;
 }
 
-struct HdTeacher {
-  const int64_t* index;
-  const float *q, *z, *live;
-  int K;
-};
+static int hd_bwd_small(const HdCall& c, const HdPlan& p, const float* g, void* gx, void* gw, void* gb, char* ws) {
+  SmArgs a = sm_args(c, p, ws);
+  a.g = g;
+  a.count = c.reduction == 1 ? c.count : nullptr;
+  a.per_row = c.reduction == 0;
+  a.coef = (float*)(ws + p.o_coef);
+  a.E = (float*)(ws + p.o_E);
+  a.ldE = p.ldE;
+  hipLaunchKernelGGL((k_head_small_logits<true>), dim3((unsigned)p.tiles_all, (unsigned)((c.N + 63) / 64)), dim3(256), 0, c.st, a);
+  DIG3D_CHECK_LAUNCH();
+  if (c.index) {
+    const int rc = hd_teacher_grad<float>(c, a.coef + c.N, 0, c.V, 1, a.E, a.ldE, 0);
+    if (rc != DIG3D_OK) return rc;
+  }
+  a.gx = gx;
+  a.gw = gw;
+  a.gb = gb;
+  a.splits = p.gx.splits;
+  a.slots = gx && p.gx.splits > 1 ? (float*)(ws + p.o_gx) : nullptr;
+  a.gx_tiles = gx ? ((c.D + 63) / 64) * ((c.N + 63) / 64) : 0;
+  a.gw_tiles = gw || gb ? ((c.D + (gb ? 1 : 0) + 63) / 64) * ((c.V + 63) / 64) : 0;
+  hipLaunchKernelGGL(k_head_small_grads, dim3((unsigned)(a.gx_tiles * a.splits + a.gw_tiles)), dim3(256), 0, c.st, a);
+  DIG3D_CHECK_LAUNCH();
+  if (a.slots) {
+    const int64_t n = (int64_t)c.N * c.D;
+    hipLaunchKernelGGL((k_head_sum<bf16_t>), dim3(hd_grid(n, 256)), dim3(256), 0, c.st, a.slots, p.gx.splits, n, n, (const float*)nullptr, -1,
+                       gx, c.dt, (int64_t)0);
+    DIG3D_CHECK_LAUNCH();
+  }
+  return DIG3D_OK;
+}
 
 template <class T>
-static int hd_bwd(int dt, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
-                  int64_t ignore, const HdTeacher& th, float tau, int N, int D, int V, const float* g, int per_row,
-                  const float* count, float* scal, const float* lse, const float* loss, void* gx, void* gw, void* gb, char* ws,
-                  const HdPlan& p, hipStream_t st) {
-  float* amax = scal + SC_COUNT;
+static int hd_bwd(const HdCall& c, const HdPlan& p, const float* g, void* gx, void* gw, void* gb, char* ws) {
   float* coef = (float*)(ws + p.o_coef);
-  hipLaunchKernelGGL(k_head_coef, dim3(1), dim3(1024), 0, st, g, per_row, count, tau, target, ignore, th.live, N, coef, scal);
+  hipLaunchKernelGGL(k_head_coef, dim3(1), dim3(1024), 0, c.st, g, c.reduction == 0, c.reduction == 1 ? c.count : (const float*)nullptr,
+                     c.index ? c.tau : 1.f, c.target, c.ignore, c.index ? c.live : (const float*)nullptr, c.N, coef, c.scal);
   DIG3D_CHECK_LAUNCH();
   const int64_t xplane = p.Np * p.Dp;
   const bool planes2 = p.planes == 2;
-  hd_pack(x, dt, ldx, N, D, coef, amax, SC_X, scal, (short*)(ws + p.o_x), p.Np, p.Dp, xplane, st);
+  hd_pack(c.x, c.dt, c.ldx, c.N, c.D, coef, c.amax, SC_X, c.scal, (short*)(ws + p.o_x), p.Np, p.Dp, xplane, c.st);
   DIG3D_CHECK_LAUNCH();
   short* E = (short*)(ws + p.o_E);
   const int64_t eplane = p.Np * p.ldE;
-  const int esz = dt == DT_F32 ? 4 : 2;
+  const int esz = c.dt == DT_F32 ? 4 : 2;
   const bool gx_slots = gx && (p.np > 1 || p.gx.splits > 1);
-  for (int64_t v0 = 0; v0 < V; v0 += p.vp) {
-    const int nv = (int)min(p.vp, V - v0);
-    const char* wsrc = (const char*)w + v0 * ldw * esz;
+  for (int64_t v0 = 0; v0 < c.V; v0 += p.vp) {
+    const int nv = (int)min(p.vp, c.V - v0);
+    const char* wsrc = (const char*)c.w + v0 * c.ldw * esz;
     HdOperand W;
-    if (p.dw) W = {(const short*)wsrc, ldw, 0, nv, D};
+    if (p.dw) W = {(const short*)wsrc, c.ldw, 0, nv, c.D};
     else {
       const int64_t plane = (int64_t)nv * p.Dp;
-      hd_pack(wsrc, dt, ldw, nv, D, nullptr, amax, SC_W, scal, (short*)(ws + p.o_w), nv, p.Dp, plane, st);
+      hd_pack(wsrc, c.dt, c.ldw, nv, c.D, nullptr, c.amax, SC_W, c.scal, (short*)(ws + p.o_w), nv, p.Dp, plane, c.st);
       DIG3D_CHECK_LAUNCH();
       W = {at_bytes(ws, p.o_w), p.Dp, plane, nv, p.Dp};
     }
@@ -1007,153 +1220,137 @@ static int hd_bwd(int dt, const void* x, int64_t ldx, const void* w, int64_t ldw
     a.P = W;
     a.Q = {at_bytes(ws, p.o_x), p.Dp, xplane, (int)p.Np, p.Dp};
     a.ni = nv;
-    a.nj = N;
+    a.nj = c.N;
     a.ktiles = p.Dp / HD_BK;
     a.nseg = planes2 ? 3 : 1;
-    a.bias = bias;
-    a.dt = dt;
-    a.scal = scal;
-    a.inv_tau = 1.0f / tau;
+    a.bias = c.bias;
+    a.dt = c.dt;
+    a.scal = c.scal;
+    a.inv_tau = 1.0f / c.tau;
     a.v0 = v0;
-    a.V = V;
-    a.target = target;
-    a.lse = lse;
-    a.loss = loss;
+    a.V = c.V;
+    a.target = c.target;
+    a.lse = c.lse;
+    a.loss = c.loss;
     a.coef = coef;
     a.E = E;
     a.ldE = p.ldE;
     a.planeE = eplane;
     a.rowsE = (int)p.Np;
-    hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, st);
+    hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, c.st);
     DIG3D_CHECK_LAUNCH();
-    if (th.index) {
-      hipLaunchKernelGGL((k_head_teacher_grad<T>), dim3((unsigned)(((int64_t)N * th.K + 255) / 256)), dim3(256), 0, st, th.index,
-                         th.q, th.z, lse, coef, (int64_t)N, th.K, v0, (int64_t)nv, p.planes, E, p.ldE, eplane);
-      DIG3D_CHECK_LAUNCH();
+    if (c.index) {
+      const int rc = hd_teacher_grad<T>(c, coef, v0, nv, p.planes, E, p.ldE, eplane);
+      if (rc != DIG3D_OK) return rc;
     }
     HdArgs o;
     memset(&o, 0, sizeof o);
     o.nseg = a.nseg;
-    o.scal = scal;
-    o.dt = dt;
+    o.scal = c.scal;
+    o.dt = c.dt;
     if (gx) {                              // gx[n, d] += sum_v e[n, v] W[v, d]
       o.P = W;
       o.Q = {E, p.ldE, eplane, (int)p.Np, (int)p.ldE};
-      o.ni = D;
-      o.nj = N;
+      o.ni = c.D;
+      o.nj = c.N;
       o.ktiles = (int)(up64(nv) / HD_BK);  // no step starts beyond W's last row
       o.acc = gx_slots ? (float*)(ws + p.o_gx) : nullptr;
       o.add = v0 > 0;
       o.out = gx_slots ? nullptr : gx;
-      o.ldo = D;
+      o.ldo = c.D;
       o.other = planes2 ? SC_W : -1;
-      hd_gemm<T, true, false, EPI_OUT>(o, p.gx, st);
+      hd_gemm<T, true, false, EPI_OUT>(o, p.gx, c.st);
       DIG3D_CHECK_LAUNCH();
     }
     if (gw) {                              // gw[v, d] = sum_n e[n, v] x[n, d]
       const bool slots = p.gw.splits > 1;
       o.P = {at_bytes(ws, p.o_x), p.Dp, xplane, (int)p.Np, p.Dp};
       o.Q = {E, p.ldE, eplane, (int)p.Np, (int)p.ldE};
-      o.ni = D;
+      o.ni = c.D;
       o.nj = nv;
       o.ktiles = (int)(p.Np / HD_BK);
       o.acc = slots ? (float*)(ws + p.o_gw) : nullptr;
       o.add = 0;
-      o.out = slots ? nullptr : (char*)gw + v0 * D * esz;
-      o.ldo = D;
+      o.out = slots ? nullptr : (char*)gw + v0 * c.D * esz;
+      o.ldo = c.D;
       o.other = planes2 ? SC_X : -1;
-      hd_gemm<T, true, true, EPI_OUT>(o, p.gw, st);
+      hd_gemm<T, true, true, EPI_OUT>(o, p.gw, c.st);
       DIG3D_CHECK_LAUNCH();
       if (slots) {
-        const int64_t n = (int64_t)nv * D;
-        hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(n, 256)), dim3(256), 0, st, (const float*)(ws + p.o_gw), p.gw.splits, n, n,
-                           scal, o.other, gw, dt, v0 * D);
+        const int64_t n = (int64_t)nv * c.D;
+        hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(n, 256)), dim3(256), 0, c.st, (const float*)(ws + p.o_gw), p.gw.splits, n, n,
+                           c.scal, o.other, gw, c.dt, v0 * c.D);
         DIG3D_CHECK_LAUNCH();
       }
     }
     if (gb) {
       float* part = (float*)(ws + p.o_col);
-      const int slices = (N + 255) / 256;
-      hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)((p.ldE + 255) / 256), (unsigned)slices), dim3(256), 0, st, E, p.ldE,
-                         eplane, p.planes, N, part);
+      const int slices = (c.N + HD_SLICE - 1) / HD_SLICE;
+      hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)((p.ldE + 255) / 256), (unsigned)slices), dim3(256), 0, c.st, E, p.ldE,
+                         eplane, p.planes, c.N, part);
       DIG3D_CHECK_LAUNCH();
-      hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(nv, 256)), dim3(256), 0, st, part, slices, p.ldE, (int64_t)nv, scal, -1, gb,
-                         dt, v0);
+      hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(nv, 256)), dim3(256), 0, c.st, part, slices, p.ldE, (int64_t)nv, c.scal, -1, gb,
+                         c.dt, v0);
       DIG3D_CHECK_LAUNCH();
     }
   }
   if (gx_slots) {
-    const int64_t n = (int64_t)N * D;
-    hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(n, 256)), dim3(256), 0, st, (const float*)(ws + p.o_gx), p.gx.splits, n, n, scal,
-                       planes2 ? SC_W : -1, gx, dt, (int64_t)0);
+    const int64_t n = (int64_t)c.N * c.D;
+    hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(n, 256)), dim3(256), 0, c.st, (const float*)(ws + p.o_gx), p.gx.splits, n, n, c.scal,
+                       planes2 ? SC_W : -1, gx, c.dt, (int64_t)0);
     DIG3D_CHECK_LAUNCH();
   }
   return DIG3D_OK;
 }
 
+// the arguments that both entries take; false: refused
+static bool hd_call(HdCall& c, int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                    const int64_t* target, int64_t ignore, const int64_t* index, const void* teacher, int tdtype, int K, float tau,
+                    int N, int D, int V, int reduction, float* keep, void* stream) {
+  if (hd_bad(dtype, N, D, V, ldx, ldw) || !x || !w || !keep || reduction < 0 || reduction > 2 || !(tau > 0.f)) return false;
+  if ((!target) == (!index) || (target && (K != 0 || tau != 1.f))) return false;
+  if (index && (!teacher || tdtype < 0 || tdtype > 2 || K <= 0 || K > TC_MAX)) return false;
+  c = {dtype, x, w, bias, ldx, ldw, N, D, V, target, ignore, index, teacher, tdtype, K, tau, reduction};
+  c.st = (hipStream_t)stream;
+  hd_keep(c, keep);
+  return true;
+}
+
 extern "C" {
 
-int dig3d_head_ws_kib(int dtype, int64_t ldx, const void* x, int64_t ldw, const void* w, int N, int D, int V, int backward, int needs) {
+int dig3d_head_ws_kib(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int N, int D, int V, int backward, int needs) {
   if (hd_bad(dtype, N, D, V, ldx, ldw)) return DIG3D_ERR_ARG;
   const HdPlan p = hd_plan(dtype, N, D, V, hd_direct(dtype, x, ldx, D), hd_direct(dtype, w, ldw, D), backward, needs);
   const int64_t kib = (p.total + 1023) / 1024;
   return kib > 2147483647ll ? DIG3D_ERR_ARG : (int)kib;
 }
 
-int dig3d_head_lse(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
-                   int64_t ignore_index, float tau, int N, int D, int V, float* scal, float* lse, float* loss, void* ws, int ws_kib,
-                   void* stream) {
+int dig3d_head_fwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
+                   int64_t ignore_index, const int64_t* index, const void* teacher, int tdtype, int K, float tau, int N, int D, int V,
+                   int reduction, float* keep, float* out, void* ws, int ws_kib, void* stream) {
   DIG3D_ENTER();
-  if (hd_bad(dtype, N, D, V, ldx, ldw) || !x || !w || !scal || !lse || (!target) != (!loss) || !(tau > 0.f)) return DIG3D_ERR_ARG;
-  const HdPlan p = hd_plan(dtype, N, D, V, hd_direct(dtype, x, ldx, D), hd_direct(dtype, w, ldw, D), 0, 0);
-  if (p.total > (int64_t)ws_kib * 1024 || (p.total && !ws)) return DIG3D_ERR_ARG;
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == DT_BF16)
-    return hd_lse<bf16_t>(dtype, x, ldx, w, ldw, bias, target, ignore_index, 1.0f / tau, N, D, V, scal, lse, loss, (char*)ws, p, st);
-  return hd_lse<f16_t>(dtype, x, ldx, w, ldw, bias, target, ignore_index, 1.0f / tau, N, D, V, scal, lse, loss, (char*)ws, p, st);
-}
-
-int dig3d_head_teacher(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* index,
-                       const void* teacher, int tdtype, int K, float tau, int N, int D, int V, const float* lse, float* q, float* z,
-                       float* loss, float* live, void* stream) {
-  DIG3D_ENTER();
-  if (hd_bad(dtype, N, D, V, ldx, ldw) || tdtype < 0 || tdtype > 2 || K <= 0 || K > (1 << 20) || !x || !w || !index || !teacher || !lse ||
-      !q || !z || !loss || !live || !(tau > 0.f))
+  HdCall c;
+  if (!hd_call(c, dtype, x, ldx, w, ldw, bias, target, ignore_index, index, teacher, tdtype, K, tau, N, D, V, reduction, keep, stream) ||
+      !out)
     return DIG3D_ERR_ARG;
-  hipLaunchKernelGGL(k_head_teacher, dim3((unsigned)N), dim3(256), 0, (hipStream_t)stream, x, w, bias, dtype, ldx, ldw, D, (int64_t)V,
-                     index, teacher, tdtype, K, 1.0f / tau, tau, lse, q, z, loss, live);
-  DIG3D_CHECK_LAUNCH();
-  return DIG3D_OK;
-}
-
-int dig3d_head_total(const float* loss, const int64_t* target, int64_t ignore_index, const float* live, int N, int mean, float* out,
-                     float* count, void* stream) {
-  DIG3D_ENTER();
-  if (!loss || !out || !count || N < 0 || (!target) == (!live)) return DIG3D_ERR_ARG;
-  hipLaunchKernelGGL(k_head_total, dim3(1), dim3(1024), 0, (hipStream_t)stream, loss, target, ignore_index, live, N, mean, out,
-                     count);
-  DIG3D_CHECK_LAUNCH();
-  return DIG3D_OK;
+  const HdPlan p = hd_plan(dtype, N, D, V, hd_direct(dtype, x, ldx, D), hd_direct(dtype, w, ldw, D), 0, 0);
+  if (p.total > (int64_t)ws_kib * 1024 || !ws) return DIG3D_ERR_ARG;
+  return hd_fwd(c, p, (char*)ws, out);
 }
 
 int dig3d_head_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
-                   int64_t ignore_index, const int64_t* index, const float* q, const float* z, const float* live, int K, float tau, int N,
-                   int D, int V, const float* g, int per_row, const float* count, float* scal, const float* lse, const float* loss,
-                   void* gx, void* gw, void* gb, void* ws, int ws_kib, void* stream) {
+                   int64_t ignore_index, const int64_t* index, const void* teacher, int tdtype, int K, float tau, int N, int D, int V,
+                   int reduction, float* keep, const float* g, void* gx, void* gw, void* gb, void* ws, int ws_kib, void* stream) {
   DIG3D_ENTER();
-  if (hd_bad(dtype, N, D, V, ldx, ldw) || !x || !w || !g || !scal || !lse || !(tau > 0.f)) return DIG3D_ERR_ARG;
-  if ((!target) == (!index) || (target && !loss) || (index && (!q || !z || !live || K <= 0 || K > (1 << 20)))) return DIG3D_ERR_ARG;
+  HdCall c;
+  if (!hd_call(c, dtype, x, ldx, w, ldw, bias, target, ignore_index, index, teacher, tdtype, K, tau, N, D, V, reduction, keep, stream) || !g)
+    return DIG3D_ERR_ARG;
   const int needs = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
   if (!needs) return DIG3D_OK;
   const HdPlan p = hd_plan(dtype, N, D, V, hd_direct(dtype, x, ldx, D), hd_direct(dtype, w, ldw, D), 1, needs);
   if (p.total > (int64_t)ws_kib * 1024 || !ws) return DIG3D_ERR_ARG;
-  const HdTeacher th = {index, q, z, live, K};
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == DT_BF16)
-    return hd_bwd<bf16_t>(dtype, x, ldx, w, ldw, bias, target, ignore_index, th, tau, N, D, V, g, per_row, count, scal, lse, loss, gx, gw,
-                          gb, (char*)ws, p, st);
-  return hd_bwd<f16_t>(dtype, x, ldx, w, ldw, bias, target, ignore_index, th, tau, N, D, V, g, per_row, count, scal, lse, loss, gx, gw, gb,
-                       (char*)ws, p, st);
+  if (p.small) return hd_bwd_small(c, p, g, gx, gw, gb, (char*)ws);
+  return dtype == DT_BF16 ? hd_bwd<bf16_t>(c, p, g, gx, gw, gb, (char*)ws) : hd_bwd<f16_t>(c, p, g, gx, gw, gb, (char*)ws);
 }
 
 }  // extern "C"

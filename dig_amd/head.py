@@ -5,90 +5,70 @@ import torch
 from torch.autograd import Function
 
 from . import _hip, ops
-from ._hip import call, ptr
-from .graph import _stream
+from ._hip import ptr
 
-_REDUCTIONS = ('none', 'mean', 'sum')
-
-
-def _pitch(t):
-    return t.stride(0) if t.size(0) > 1 else t.size(1)
+_REDUCTIONS = {'none': 0, 'mean': 1, 'sum': 2}
+_TOP_MAX = 2048                                    # entries of a teacher's row (csrc/head.hip: TC_MAX)
 
 
-def _workspace(x, w, V, backward, needs):
-    N, D = x.shape
-    kib = _hip.query('dig3d_head_ws_kib', ops._DTYPES[x.dtype], _pitch(x), ptr(x), _pitch(w), ptr(w), N, D, V, backward, needs)
+def _call(name, dev, backward, needs, x, w, bias, target, index, teacher, keep, tau, ignore_index, reduction, *last):
+    """one C entry on these operands and a fresh workspace; ``last``: its arguments between ``keep`` and the workspace"""
+    (N, D), V, dt = x.shape, w.size(0), ops._DTYPES[x.dtype]
+    operands = (dt, x.data_ptr(), ops._pitch(x), w.data_ptr(), ops._pitch(w))
+    kib = _hip.query('dig3d_head_ws_kib', *operands, N, D, V, backward, needs)
     if kib < 0:
         raise _hip.Dig3dError(f'class head of {N} rows x {D} x {V} classes is beyond the supported sizes')
-    return torch.empty(max(kib, 1) * 1024, dtype=torch.uint8, device=x.device), kib
+    ws = torch.empty(max(kib, 1) * 1024, dtype=torch.uint8, device=x.device)
+    K, tdt = (0, 0) if index is None else (index.size(1), ops._DTYPES[teacher.dtype])
+    ops._on_device(dev, name, *operands, ptr(bias), ptr(target), ignore_index, ptr(index), ptr(teacher), tdt, K, tau, N, D, V, reduction,
+                   keep.data_ptr(), *last, ws.data_ptr(), kib)
 
 
 class _HeadLoss(Function):
-    """loss of the classes of x w^T + bias; ``teacher``: (index, logits) instead of targets."""
+    """The loss of the classes of x w^T + bias against targets, or against a teacher's entries (index, teacher)."""
 
     @staticmethod
     def forward(ctx, x, w, bias, target, index, teacher, tau, ignore_index, reduction):
-        (N, D), V, dev = x.shape, w.size(0), x.device
-        ctx.meta = (tau, ignore_index, reduction)
-        f32 = dict(dtype=torch.float32, device=dev)
-        dt = ops._DTYPES[x.dtype]
+        N, D = x.shape
+        f32 = dict(dtype=torch.float32, device=x.device)
+        out = torch.empty(N, **f32) if reduction == 0 else torch.empty((), **f32)
         if N == 0:
+            ctx.meta = None
             ctx.save_for_backward(x, w, bias)
-            return torch.zeros(N, **f32) if reduction == 'none' else torch.zeros((), **f32)
-        scal = torch.empty(516, **f32)
-        rows = torch.empty(3, N, **f32)                     # lse, loss, live
-        lse, loss, live = rows[0], rows[1], rows[2]
-        with torch.cuda.device(dev):
-            st = _stream()
-            ws, kib = _workspace(x, w, V, 0, 0)
-            call('dig3d_head_lse', dt, ptr(x), _pitch(x), ptr(w), _pitch(w), ptr(bias), ptr(target), ignore_index, tau, N, D, V,
-                 ptr(scal), ptr(lse), ptr(loss) if target is not None else None, ptr(ws), kib, st)
-            q = None
-            if index is not None:
-                K = index.size(1)
-                q = torch.empty(2, N, K, **f32)
-                call('dig3d_head_teacher', dt, ptr(x), _pitch(x), ptr(w), _pitch(w), ptr(bias), ptr(index), ptr(teacher),
-                     ops._DTYPES[teacher.dtype], K, tau, N, D, V, ptr(lse), ptr(q), q.data_ptr() + 4 * N * K, ptr(loss), ptr(live), st)
-            count = out = None
-            if reduction != 'none':
-                out, count = torch.empty((), **f32), torch.empty((), **f32)
-                call('dig3d_head_total', ptr(loss), ptr(target), ignore_index, ptr(live) if index is not None else None, N,
-                     int(reduction == 'mean'), ptr(out), ptr(count), st)
-        ctx.save_for_backward(x, w, bias, target, index, q, scal, rows, count)
-        return loss.clone() if reduction == 'none' else out
+            return out.zero_()
+        keep = torch.empty(520 + N * (3 + 2 * (0 if index is None else index.size(1))), **f32)
+        _call('dig3d_head_fwd', x.get_device(), 0, 0, x, w, bias, target, index, teacher, keep, tau, ignore_index, reduction, out.data_ptr())
+        ctx.meta = (tau, ignore_index, reduction)
+        ctx.save_for_backward(x, w, bias, target, index, teacher, keep)
+        return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops._once
     def backward(ctx, g):
-        tau, ignore_index, reduction = ctx.meta
-        none = (None,) * 6
         needs = ctx.needs_input_grad[:3]
-        if len(ctx.saved_tensors) == 3:
-            return tuple(torch.zeros_like(t) if n else None for t, n in zip(ctx.saved_tensors, needs)) + none
-        x, w, bias, target, index, q, scal, rows, count = ctx.saved_tensors
-        (N, D), V = x.shape, w.size(0)
-        new = lambda n, *shape: torch.empty(*shape, dtype=x.dtype, device=x.device) if n else None
-        gx, gw, gb = new(needs[0], N, D), new(needs[1], V, D), new(needs[2], V)
-        g = g.to(torch.float32).contiguous()
-        K = index.size(1) if index is not None else 0
-        with torch.cuda.device(x.device):
-            ws, kib = _workspace(x, w, V, 1, needs[0] + 2 * needs[1] + 4 * needs[2])
-            call('dig3d_head_bwd', ops._DTYPES[x.dtype], ptr(x), _pitch(x), ptr(w), _pitch(w), ptr(bias), ptr(target), ignore_index, ptr(index),
-                 ptr(q), q.data_ptr() + 4 * N * K if K else None, rows.data_ptr() + 8 * N if K else None, K, tau, N, D, V, ptr(g),
-                 int(reduction == 'none'), ptr(count) if reduction == 'mean' else None, ptr(scal), ptr(rows), rows.data_ptr() + 4 * N,
-                 ptr(gx), ptr(gw), ptr(gb), ptr(ws), kib, _stream())
-        return (gx, gw, gb) + none
+        saved = ctx.saved_tensors
+        x, w, bias = saved[:3]
+        if ctx.meta is None:
+            return tuple(torch.zeros_like(t) if n else None for t, n in zip((x, w, bias), needs)) + (None,) * 6
+        gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
+        gw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if needs[1] else None
+        gb = torch.empty(bias.shape, dtype=x.dtype, device=x.device) if needs[2] else None
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.to(torch.float32).contiguous()
+        _call('dig3d_head_bwd', x.get_device(), 1, needs[0] + 2 * needs[1] + 4 * needs[2], *saved, *ctx.meta, g.data_ptr(), ptr(gx), ptr(gw),
+              ptr(gb))
+        return gx, gw, gb, None, None, None, None, None, None
 
 
 def _check_head(name, x, weight, bias, reduction):
     if reduction not in _REDUCTIONS:
-        raise ValueError(f"{name}: reduction is one of {_REDUCTIONS}, got {reduction!r}")
-    x2, _ = ops._check_rows(name, x)
+        raise ValueError(f'{name}: reduction is one of {tuple(_REDUCTIONS)}, got {reduction!r}')
+    x2 = ops._check_rows(name, x)
     if not weight.is_cuda or weight.device != x2.device:
         raise _hip.Dig3dError(f'{name}: weight is on {weight.device}, the rows on {x2.device}')
     if weight.dim() != 2 or weight.size(1) != x2.size(1) or weight.size(0) < 1 or weight.dtype != x2.dtype:
         raise RuntimeError(f'{name}: expected weight [V, {x2.size(1)}] of {x2.dtype} with V >= 1, got {tuple(weight.shape)} {weight.dtype}')
-    weight, _ = ops._check_rows(name, weight)
+    weight = ops._check_rows(name, weight)
     if bias is not None:
         bias = ops._check_vector(name, 'bias', bias, weight.size(0), x2, (x2.dtype,))
     return x2, weight, bias
@@ -112,7 +92,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     gradients have the type of their inputs and the same bits every time."""
     x2, weight, bias = _check_head('linear_cross_entropy', x, weight, bias, reduction)
     _check_index('linear_cross_entropy', 'target', target, x.shape[:-1], x2)
-    loss = _HeadLoss.apply(x2, weight, bias, target.reshape(-1).contiguous(), None, None, 1.0, int(ignore_index), reduction)
+    loss = _HeadLoss.apply(x2, weight, bias, target.reshape(-1).contiguous(), None, None, 1.0, int(ignore_index), _REDUCTIONS[reduction])
     return loss.reshape(target.shape) if reduction == 'none' else loss
 
 
@@ -129,8 +109,8 @@ def linear_distillation(x, weight, teacher_index, teacher_logits, bias=None, tem
     x2, weight, bias = _check_head(name, x, weight, bias, reduction)
     if not (isinstance(temperature, (int, float)) and 0.0 < float(temperature) < float('inf')):
         raise ValueError(f'{name}: temperature is a positive number, got {temperature!r}')
-    if teacher_index.dim() != x.dim() or teacher_index.size(-1) < 1:
-        raise RuntimeError(f'{name}: expected teacher_index [..., K] with K >= 1 for rows {tuple(x.shape)}, got {tuple(teacher_index.shape)}')
+    if teacher_index.dim() != x.dim() or not 1 <= teacher_index.size(-1) <= _TOP_MAX:
+        raise RuntimeError(f'{name}: expected teacher_index [..., K] with 1 <= K <= {_TOP_MAX} for rows {tuple(x.shape)}, got {tuple(teacher_index.shape)}')
     K = teacher_index.size(-1)
     _check_index(name, 'teacher_index', teacher_index, tuple(x.shape[:-1]) + (K,), x2)
     if teacher_logits.shape != teacher_index.shape or teacher_logits.dtype not in ops._DTYPES or teacher_logits.device != x2.device:
@@ -138,5 +118,5 @@ def linear_distillation(x, weight, teacher_index, teacher_logits, bias=None, tem
                            f'{tuple(teacher_logits.shape)} {teacher_logits.dtype} on {teacher_logits.device}')
     index = teacher_index.reshape(-1, K).contiguous()
     teacher = teacher_logits.detach().reshape(-1, K).contiguous()
-    loss = _HeadLoss.apply(x2, weight, bias, None, index, teacher, float(temperature), 0, reduction)
+    loss = _HeadLoss.apply(x2, weight, bias, None, index, teacher, float(temperature), 0, _REDUCTIONS[reduction])
     return loss.reshape(x.shape[:-1]) if reduction == 'none' else loss

@@ -2123,27 +2123,50 @@ def graph_norm(x, weight, bias, mean_scale, gptr, B, eps=1e-5, padded=False):
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # csrc/half16.h
 
 
-def _check_rows(name, x, width=None):
+def _on_device(dev, name, *args):
+    """The C entry ``name`` on the current stream of device number ``dev``, whatever the current device is."""
+    if torch.cuda.current_device() == dev:
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _once(backward):
+    """``once_differentiable`` whose checks are only paid for where the backward itself is recorded (create_graph)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def wrapped(ctx, g):
+        return guarded(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+    return wrapped
+
+
+def _check_rows(name, x):
     """The row operand of layer_norm and of the class losses: a GPU tensor [..., C] of a supported type -> [R, C] with unit
-    stride along C and rows that do not overlap, and its row pitch."""
+    stride along C and rows that do not overlap."""
     if not x.is_cuda:
         raise _hip.Dig3dError(f'{name}: dig_amd op received a CPU tensor; the engine has no CPU fallback')
     if x.dtype not in _DTYPES:
         raise RuntimeError(f'{name}: expected float32, bfloat16 or float16 rows, got {x.dtype}')
-    if x.dim() < 1 or x.size(-1) < 1:
-        raise RuntimeError(f'{name}: expected [..., C] with C >= 1, got {tuple(x.shape)}')
-    C = x.size(-1)
     if x.dim() != 2:
-        x = x.reshape(-1, C)
-    if (C > 1 and x.stride(1) != 1) or (x.size(0) > 1 and x.stride(0) < C):
-        x = x.contiguous()
-    return x, (x.stride(0) if x.size(0) > 1 else C)
+        if x.dim() < 1 or x.size(-1) < 1:
+            raise RuntimeError(f'{name}: expected [..., C] with C >= 1, got {tuple(x.shape)}')
+        x = x.reshape(-1, x.size(-1))
+    if x.is_contiguous():
+        if x.size(1) < 1:
+            raise RuntimeError(f'{name}: expected [..., C] with C >= 1, got {tuple(x.shape)}')
+        return x
+    return x if x.stride(1) == 1 and x.stride(0) >= x.size(1) else x.contiguous()
+
+
+def _pitch(x):
+    return x.stride(0) if x.size(0) > 1 else x.size(1)
 
 
 def _check_vector(name, what, p, n, x, dtypes):
     if not p.is_cuda or p.device != x.device:
         raise _hip.Dig3dError(f'{name}: {what} is on {p.device}, the rows on {x.device}')
-    if p.dtype not in dtypes or tuple(p.shape) != (n,):
+    if p.dtype not in dtypes or p.dim() != 1 or p.size(0) != n:
         raise RuntimeError(f'{name}: expected {what} [{n}] of {" or ".join(str(d) for d in dtypes)}, got {tuple(p.shape)} {p.dtype}')
     return p.contiguous()
 
@@ -2154,64 +2177,68 @@ class _LayerNorm(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         R, C = x.shape
-        keep = any(ctx.needs_input_grad)
-        wd = _DTYPES[(weight if weight is not None else bias if bias is not None else x).dtype]
-        y = torch.empty(R, C, dtype=x.dtype, device=x.device)
-        stat = torch.empty(2, R, dtype=torch.float32, device=x.device) if keep else None
-        ld = x.stride(0) if R > 1 else C
-        with torch.cuda.device(x.device):
-            call('dig3d_rownorm_fwd', _DTYPES[x.dtype], ptr(x), ld, R, C, ptr(weight), ptr(bias), wd, float(eps), ptr(y), ptr(stat),
-                 stat.data_ptr() + 4 * R if keep else None, _stream())
-        ctx.wd, ctx.has_bias = wd, bias is not None
-        ctx.leaf = _all_leaf((weight, bias))
-        ctx.save_for_backward(x, weight, stat)
+        dt, dev = _DTYPES[x.dtype], x.get_device()
+        p = weight if weight is not None else bias
+        wd = dt if p is None else _DTYPES[p.dtype]
+        ld = _pitch(x)
+        y = torch.empty((R, C), dtype=x.dtype, device=x.device)
+        if any(ctx.needs_input_grad):
+            stat = torch.empty(2 * R, dtype=torch.float32, device=x.device)
+            m = stat.data_ptr()
+            _on_device(dev, 'dig3d_rownorm_fwd', dt, x.data_ptr(), ld, R, C, ptr(weight), ptr(bias), wd, eps, y.data_ptr(), m, m + 4 * R)
+            ctx.meta = (wd, None if p is None else p.dtype, _all_leaf((weight, bias)))
+            ctx.save_for_backward(x, weight, stat)
+        else:
+            _on_device(dev, 'dig3d_rownorm_fwd', dt, x.data_ptr(), ld, R, C, ptr(weight), ptr(bias), wd, eps, y.data_ptr(), None, None)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gy):
         x, weight, stat = ctx.saved_tensors
+        wd, pd, leaf = ctx.meta
         R, C = x.shape
-        dev = x.device
-        nx, nw, nb_ = ctx.needs_input_grad[:3]
-        gy = gy.contiguous()
-        pd = weight.dtype if weight is not None else list(_DTYPES)[ctx.wd]
-        if R == 0:
-            z = torch.zeros(C, dtype=pd, device=dev)
-            return (torch.empty_like(gy) if nx else None), (z if nw else None), (z.clone() if nb_ else None), None
         dt = _DTYPES[x.dtype]
-        ld = x.stride(0) if R > 1 else C
-        gx = torch.empty(R, C, dtype=x.dtype, device=dev) if nx else None
-        nb = _hip.query('dig3d_rownorm_bwd_blocks', R, C, dt)
-        part = gp = None
-        pw = pb = None
-        if nw or nb_:
-            part = torch.empty(nb * 2 * C, dtype=torch.float32, device=dev)
-            gp = torch.empty(2 * C, dtype=pd, device=dev)
-            # float32 parameters: the workgroups' partials join the deferred reductions of the pass when there is one
-            if pd != torch.float32 or _reduce_later(part, nb, 2 * C, gp, ctx.leaf):
-                pw = ptr(gp) if nw else None
-                pb = gp.data_ptr() + gp.element_size() * C if nb_ else None
-        with torch.cuda.device(dev):
-            call('dig3d_rownorm_bwd', dt, ptr(gy), ptr(x), ld, R, C, ptr(weight), ctx.wd, ptr(stat), stat.data_ptr() + 4 * R, ptr(gx),
-                 ptr(part), nb, pw, pb, _stream())
-        return gx, (gp[:C] if nw else None), (gp[C:] if nb_ else None), None
+        nx, nw, nb = ctx.needs_input_grad[:3]
+        gy = gy.contiguous()
+        gx = torch.empty_like(gy) if nx else None
+        gw = gb = part = later = None
+        blocks = _hip.query('dig3d_rownorm_bwd_blocks', R, C, dt)
+        if nw or nb:
+            if R == 0:
+                gw = torch.zeros(C, dtype=pd, device=x.device) if nw else None
+                gb = torch.zeros(C, dtype=pd, device=x.device) if nb else None
+                return gx, gw, gb, None
+            part = torch.empty(blocks * 2 * C, dtype=torch.float32, device=x.device)
+            if pd == torch.float32 and _deferred is not None and leaf:
+                # the workgroups' partials join the deferred reductions of the pass
+                later = torch.empty(2 * C, dtype=pd, device=x.device)
+                _reduce_later(part, blocks, 2 * C, later, leaf)
+            else:
+                gw = torch.empty(C, dtype=pd, device=x.device) if nw else None
+                gb = torch.empty(C, dtype=pd, device=x.device) if nb else None
+        if R:
+            m = stat.data_ptr()
+            _on_device(x.get_device(), 'dig3d_rownorm_bwd', dt, gy.data_ptr(), x.data_ptr(), _pitch(x), R, C, ptr(weight), wd, m, m + 4 * R, ptr(gx), ptr(part),
+                       blocks, ptr(gw), ptr(gb))
+        if later is not None:
+            gw, gb = (later[:C] if nw else None), (later[C:] if nb else None)
+        return gx, gw, gb, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """``weight * (x - mean) / sqrt(var + eps) + bias`` over the last dimension of ``x`` [..., C] (float32, bfloat16 or float16;
     statistics in float32, the variance centred); ``weight`` / ``bias`` [C] of x's type or float32, both of one type, each may be
     None.  Rows may be strided (a slice of a wider buffer is read in place).  Differentiable once, in x, weight and bias."""
-    x2, _ = _check_rows('layer_norm', x)
+    x2 = _check_rows('layer_norm', x)
     C = x2.size(1)
     if weight is not None:
-        weight = _check_vector('layer_norm', 'weight', weight, C, x2, (x2.dtype, torch.float32) if x2.dtype != torch.float32 else (x2.dtype,))
+        weight = _check_vector('layer_norm', 'weight', weight, C, x2, (x2.dtype, torch.float32))
     if bias is not None:
-        kinds = (weight.dtype,) if weight is not None else (x2.dtype, torch.float32) if x2.dtype != torch.float32 else (x2.dtype,)
-        bias = _check_vector('layer_norm', 'bias', bias, C, x2, kinds)
+        bias = _check_vector('layer_norm', 'bias', bias, C, x2, (x2.dtype, torch.float32) if weight is None else (weight.dtype,))
     if x2.size(0) >= 1 << 31 or C >= 1 << 30:
         raise RuntimeError(f'layer_norm: {tuple(x.shape)} is beyond 2^31 rows or 2^30 channels')
-    y = _LayerNorm.apply(x2, weight, bias, eps)
+    y = _LayerNorm.apply(x2, weight, bias, float(eps))
     return y if x.dim() == 2 else y.reshape(x.shape)
 
 

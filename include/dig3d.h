@@ -760,31 +760,25 @@ int dig3d_rownorm_bwd(int dtype, const void* gy, const void* x, int64_t ldx, int
  * heads of method/pronet/pronet.py:349-352 and of the generator's atom types).  dtype of x [N, D] (pitch ldx), w [V, D]
  * (pitch ldw), bias [V] or NULL, and of the gradients gx [N, D], gw [V, D], gb [V] (pitch D; each may be NULL): 0 f32, 1
  * bf16, 2 f16.  Statistics, losses and sums: f32.
- *   dig3d_head_ws_kib   KiB of workspace for dig3d_head_lse (backward = 0) or dig3d_head_bwd (backward = 1; needs = 1 gx + 2 gw
- *                       + 4 gb); x and w enter by their alignment.  Negative: refused sizes.
- *   dig3d_head_lse      lse[N] of z / tau; with target [N] (int64) the loss of each row too: 0 where target == ignore_index,
- *                       NaN where it is no class.  scal: float[516], kept for the backward.
- *   dig3d_head_teacher  teacher's K largest logits (type tdtype) and their classes index [N, K] (int64; an entry with a negative
- *                       index or the logit -inf is absent, equal indices add): q = softmax over a row's entries of t / tau, z = the
- *                       student's own logits / tau there, loss = tau^2 sum q (log q - (z - lse)), live = 1, or 0 for a row
- *                       without entries (loss 0), or NaN for a row with an index >= V.
- *   dig3d_head_total    out = sum of loss[N] (mean: over the rows that have one, at least 1), count = that number
- *   dig3d_head_bwd      exactly one of target / index says which loss; tau 1 with target.  g: the incoming gradient, a scalar, or
- *                       [N] with per_row; count: the divisor of a mean, or NULL.
+ *   exactly one of     target [N] (int64): loss = -log softmax(z)[target]; 0 where target == ignore_index, NaN where it is no
+ *                      class (K 0, tau 1)
+ *               and    index [N, K] (int64, K <= 2048) with the teacher's logits (type tdtype): loss = tau^2 sum_k q_k (log q_k - log
+ *                      softmax(z / tau)[index_k]), q the softmax over the row's entries of teacher / tau.  An entry with a negative
+ *                      index or the logit -inf is absent, equal indices add; a row without entries has the loss 0 and does not
+ *                      count, one with an index >= V has the loss NaN.
+ *   reduction          0: out [N]; 1: the mean over the rows that count (0 without any); 2: the sum
+ *   keep               float[520 + 3 N + 2 N K], from the forward to the backward
+ *   g                  the incoming gradient: [N] with reduction 0, else one value
+ *   dig3d_head_ws_kib  KiB of workspace of the forward, or of the backward (needs = 1 gx + 2 gw + 4 gb); x and w enter by
+ *                      their alignment.  Negative: sizes beyond the kernels.
  * ------------------------------------------------------------------------------------------------- */
-int dig3d_head_ws_kib(int dtype, int64_t ldx, const void* x, int64_t ldw, const void* w, int N, int D, int V, int backward, int needs);
-int dig3d_head_lse(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
-                   int64_t ignore_index, float tau, int N, int D, int V, float* scal, float* lse, float* loss, void* ws, int ws_kib,
-                   void* stream);
-int dig3d_head_teacher(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* index,
-                       const void* teacher, int tdtype, int K, float tau, int N, int D, int V, const float* lse, float* q, float* z,
-                       float* loss, float* live, void* stream);
-int dig3d_head_total(const float* loss, const int64_t* target, int64_t ignore_index, const float* live, int N, int mean, float* out,
-                     float* count, void* stream);
+int dig3d_head_ws_kib(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int N, int D, int V, int backward, int needs);
+int dig3d_head_fwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
+                   int64_t ignore_index, const int64_t* index, const void* teacher, int tdtype, int K, float tau, int N, int D, int V,
+                   int reduction, float* keep, float* out, void* ws, int ws_kib, void* stream);
 int dig3d_head_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
-                   int64_t ignore_index, const int64_t* index, const float* q, const float* z, const float* live, int K, float tau, int N,
-                   int D, int V, const float* g, int per_row, const float* count, float* scal, const float* lse, const float* loss,
-                   void* gx, void* gw, void* gb, void* ws, int ws_kib, void* stream);
+                   int64_t ignore_index, const int64_t* index, const void* teacher, int tdtype, int K, float tau, int N, int D, int V,
+                   int reduction, float* keep, const float* g, void* gx, void* gw, void* gb, void* ws, int ws_kib, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------
  * Library identity (abi.hip).  No reference counterpart: the reference reaches its kernels through Python wheels

@@ -26,14 +26,15 @@ def test_row_norm_partials():
 
 def test_head_workspace():
     from dig_amd import _hip
-    q = lambda dt, N, D, V, bwd, needs, ptr=0, ld=None: _hip.query('dig3d_head_ws_kib', dt, ld or D, ptr, ld or D, ptr, N, D, V, bwd, needs)
+    q = lambda dt, N, D, V, bwd, needs, ptr=0, ld=None: _hip.query('dig3d_head_ws_kib', dt, ptr, ld or D, ptr, ld or D, N, D, V, bwd, needs)
     for bad in ((3, 4, 64, 10), (0, 0, 64, 10), (0, 4, 0, 10), (0, 4, 64, 0)):
         assert q(*bad, 0, 0) < 0
     assert q(0, 4, 64, 10, 0, 0, ld=63) < 0                                   # a pitch below the width
     assert q(1, 1 << 20, 64, 1 << 27, 0, 0) < 0                               # more tiles than the kernels index
     # 16-bit rows of whole k steps are read in place; odd widths, odd pitches and odd addresses are copied
-    direct = q(1, 64, 128, 4096, 0, 0)
-    assert direct < q(1, 64, 127, 4096, 0, 0) and direct < q(1, 64, 128, 4096, 0, 0, ptr=2) and direct < q(1, 64, 128, 4096, 0, 0, ld=129)
+    direct = q(1, 64, 128, 40960, 0, 0)
+    assert direct < q(1, 64, 127, 40960, 0, 0) and direct < q(1, 64, 128, 40960, 0, 0, ptr=2) and direct < q(1, 64, 128, 40960, 0, 0, ld=129)
+    assert q(1, 64, 128, 4096, 0, 0) == q(1, 64, 128, 4096, 0, 0, ptr=2)      # small products read anything in place
     # the backward's workspace is bounded in the vocabulary: e in pieces of at most 512 MiB per plane
     big, bigger = q(1, 4096, 1024, 1 << 17, 1, 7), q(1, 4096, 1024, 1 << 20, 1, 7)
     assert bigger <= big + (64 << 10) and bigger < (1 << 21)
