@@ -837,6 +837,7 @@ __global__ void __launch_bounds__(256) k_head_sum(const float* __restrict__ part
   const float f = scal ? hd_factor<T>(scal, other) : 1.f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     float s = part[i];
+#pragma unroll 8
     for (int k = 1; k < slots; ++k) s += part[(int64_t)k * stride + i];
     store_as(out, dt, at0 + i, s * f);
   }

@@ -6,7 +6,7 @@
 // Bound: memory.  One read of x and one write of y; in the backward one read of x and gy and one write of gx.  A row stays
 // in the registers of its group of threads between the passes over it (mean, centred squares, output), so the variance is
 // the centred one, in 32 bits, at the traffic of a single pass.  Groups: 8 to 64 lanes of a wave for the widths that fit
-// them (several short rows per wave), 256 or 512 threads beyond; rows longer than 512 threads hold are read again.
+// them (several short rows per wave), 256 or 1024 threads beyond; rows longer than 1024 threads hold are read again.
 // The parameters' gradients are summed over the rows of a workgroup in registers, joined through LDS and written as one
 // partial row per workgroup; a second kernel adds the partials in a fixed order (no atomics: the same bits every time).
 #include "half16.h"
@@ -310,22 +310,24 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// out[c] = sum_b part[b][c] in the order of b within each of 16 slices, then over the slices; columns [0, C) go to gw and
-// [C, 2C) to gb (either may be null)
+// out[c] = sum_b part[b][c]: 64 slices of the partial rows, each in order, then the slices in order; 16 columns a workgroup
+// (64-byte pieces of a row, four of them in flight).  Columns [0, C) go to gw and [C, 2C) to gb (either may be null)
 __global__ void __launch_bounds__(1024) k_rownorm_params(const float* __restrict__ part, int nb, int C, void* __restrict__ gw,
                                                           void* __restrict__ gb, int wdt) {
-  __shared__ float sh[16][64];
-  const int lane = threadIdx.x & 63, sl = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane, C2 = 2 * (int64_t)C;
+  __shared__ float sh[64][17];
+  const int col = threadIdx.x & 15, sl = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + col, C2 = 2 * (int64_t)C;
   float s = 0.f;
-  if (c < C2)
-    for (int b = sl; b < nb; b += 16) s += part[(int64_t)b * C2 + c];
-  sh[sl][lane] = s;
+  if (c < C2) {
+#pragma unroll 4
+    for (int b = sl; b < nb; b += 64) s += part[(int64_t)b * C2 + c];
+  }
+  sh[sl][col] = s;
   __syncthreads();
   if (sl != 0 || c >= C2) return;
   s = 0.f;
 #pragma unroll
-  for (int q = 0; q < 16; ++q) s += sh[q][lane];
+  for (int q = 0; q < 64; ++q) s += sh[q][col];
   if (c < C) {
     if (gw) store_as(gw, wdt, c, s);
   } else if (gb) {
@@ -334,8 +336,8 @@ __global__ void __launch_bounds__(1024) k_rownorm_params(const float* __restrict
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-// the smallest group whose registers hold the row: two vectors per thread at most (the backward keeps five values of each
-// element of them: four vectors of eight spilled)
+// the smallest group whose registers hold the row: two vectors per thread at most, one at 1024 threads (the backward keeps
+// five values of each element: four vectors of eight spilled)
 static inline void rn_pick(int C, int n, int& tpr, int& nv) {
   const int v = (C + n - 1) / n;
   if (v <= 8) { tpr = 8; nv = 1; }
@@ -345,8 +347,23 @@ static inline void rn_pick(int C, int n, int& tpr, int& nv) {
   else if (v <= 128) { tpr = 64; nv = 2; }
   else if (v <= 256) { tpr = 256; nv = 1; }
   else if (v <= 512) { tpr = 256; nv = 2; }
-  else if (v <= 1024) { tpr = 512; nv = 2; }
+  else if (v <= 1024) { tpr = 1024; nv = 1; }
   else { tpr = 0; nv = 0; }
+}
+
+// Workgroups per CU, the rows dealt over them: enough bytes in flight, and no more rows at once than the caches and the
+// memory's pages like (TB/s, forward / backward):
+//   131072 x 1024 bf16 (a wave per row):   2: 3.5 / 3.7   3: 4.8 / 5.0   4: 5.2 / 5.4   6: 4.9 / 4.5   16: 4.1 / 4.4
+//   262144 x 256 f32 (a wave per row):     2: 3.2 / 5.2   3: 4.6 / 5.7   4: 5.4 / 5.3   6: 5.3 / 5.0
+//   65536 x 2048 bf16 (256 threads, 1):    3: 3.6 / 4.2   4: 4.4 / 4.8   6: 5.3 / 5.1   8: 5.1 / 4.3
+//   32768 x 4096 bf16 (256 threads, 2):    2: 3.1 / 3.3   3: 4.5 / 4.5   4: 5.0 / 3.2
+//   32768 x 2048 f32 (256 threads, 2):     2: 4.6 / 5.7   3: 5.8 / 5.4   4: 5.3 / 5.1
+//   16384 x 8192 bf16 (1024 threads):      1: 3.6 / 4.2   2: 5.0 / 4.1   4: 4.7 / 3.7
+static inline int rn_per_cu(int tpr, int nv, bool f32, bool backward) {
+  if (tpr <= 64 && tpr) return backward && f32 ? 3 : 4;
+  if (tpr == 256 && nv == 1) return backward ? (f32 ? 3 : 5) : 6;
+  if (tpr == 256) return backward ? (f32 ? 2 : 3) : (f32 ? 3 : 4);
+  return backward && !f32 ? 1 : 2;
 }
 
 static inline int64_t rn_groups_per_block(int tpr) { return tpr == 0 || tpr > RN_TPB ? 1 : RN_TPB / tpr; }
@@ -371,13 +388,13 @@ static void rn_fwd(const void* x, int64_t ldx, int R, int C, const void* w, cons
   rn_pick(C, VecLen<T>::n, tpr, nv);
   const int64_t per = rn_groups_per_block(tpr);
   int64_t g = (R + per - 1) / per;
-  const int64_t cap = 16ll * dig3d_num_cus();
+  const int64_t cap = (int64_t)rn_per_cu(tpr, nv, sizeof(T) == 4, false) * dig3d_num_cus();
   const int grid = (int)(g < cap ? g : cap);
 #define RN_CASE(TP, NVV)                                                                                       \
   if (tpr == TP && nv == NVV)                                                                                  \
     return rn_launch_fwd<T, TP, NVV>(x, ldx, R, C, w, b, wdt, eps, y, mean, rstd, grid, st);
   RN_CASE(8, 1) RN_CASE(16, 1) RN_CASE(32, 1) RN_CASE(64, 1) RN_CASE(64, 2)
-  RN_CASE(256, 1) RN_CASE(256, 2) RN_CASE(512, 2)
+  RN_CASE(256, 1) RN_CASE(256, 2) RN_CASE(1024, 1)
 #undef RN_CASE
   hipLaunchKernelGGL((k_rownorm_fwd_long<T>), dim3(grid), dim3(1024), 0, st, (const T*)x, ldx, R, C, w, b, wdt, eps, (T*)y,
                      mean, rstd);
@@ -392,7 +409,7 @@ static void rn_bwd(const void* gy, const void* x, int64_t ldx, int R, int C, con
   if (tpr == TP && nv == NVV)                                                                                  \
     return rn_launch_bwd<T, TP, NVV>(gy, x, ldx, R, C, w, wdt, mean, rstd, gx, part, grid, st);
   RN_CASE(8, 1) RN_CASE(16, 1) RN_CASE(32, 1) RN_CASE(64, 1) RN_CASE(64, 2)
-  RN_CASE(256, 1) RN_CASE(256, 2) RN_CASE(512, 2)
+  RN_CASE(256, 1) RN_CASE(256, 2) RN_CASE(1024, 1)
 #undef RN_CASE
   hipLaunchKernelGGL((k_rownorm_bwd_long<T>), dim3(grid), dim3(1024), 0, st, (const T*)gy, (const T*)x, ldx, R, C, w, wdt,
                      mean, rstd, (T*)gx, part);
@@ -406,7 +423,7 @@ int dig3d_rownorm_bwd_blocks(int R, int C, int dtype) {
   rn_pick(C, dtype == DT_F32 ? 4 : 8, tpr, nv);
   const int64_t per = rn_groups_per_block(tpr);
   const int64_t g = (R + per - 1) / per;
-  const int64_t cap = 2ll * dig3d_num_cus();
+  const int64_t cap = (int64_t)rn_per_cu(tpr, nv, dtype == DT_F32, true) * dig3d_num_cus();
   return (int)(g < cap ? g : cap);
 }
 
@@ -436,7 +453,7 @@ int dig3d_rownorm_bwd(int dtype, const void* gy, const void* x, int64_t ldx, int
   else rn_bwd<f16_t>(gy, x, ldx, R, C, w, wdtype, mean, rstd, gx, part, nb, st);
   DIG3D_CHECK_LAUNCH();
   if (gw || gb) {
-    hipLaunchKernelGGL(k_rownorm_params, dim3((unsigned)((2 * (int64_t)C + 63) / 64)), dim3(1024), 0, st, part, nb, C, gw, gb,
+    hipLaunchKernelGGL(k_rownorm_params, dim3((unsigned)((2 * (int64_t)C + 15) / 16)), dim3(1024), 0, st, part, nb, C, gw, gb,
                        wdtype);
     DIG3D_CHECK_LAUNCH();
   }

@@ -2123,13 +2123,16 @@ def graph_norm(x, weight, bias, mean_scale, gptr, B, eps=1e-5, padded=False):
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # csrc/half16.h
 
 
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _on_device(dev, name, *args):
     """The C entry ``name`` on the current stream of device number ``dev``, whatever the current device is."""
-    if torch.cuda.current_device() == dev:
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    if _current_device() == dev:
+        call(name, *args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            call(name, *args, _raw_stream(dev))
 
 
 def _once(backward):
@@ -2180,47 +2183,43 @@ class _LayerNorm(Function):
         dt, dev = _DTYPES[x.dtype], x.get_device()
         p = weight if weight is not None else bias
         wd = dt if p is None else _DTYPES[p.dtype]
-        ld = _pitch(x)
         y = torch.empty((R, C), dtype=x.dtype, device=x.device)
+        stat, m, m2 = None, None, None
         if any(ctx.needs_input_grad):
             stat = torch.empty(2 * R, dtype=torch.float32, device=x.device)
             m = stat.data_ptr()
-            _on_device(dev, 'dig3d_rownorm_fwd', dt, x.data_ptr(), ld, R, C, ptr(weight), ptr(bias), wd, eps, y.data_ptr(), m, m + 4 * R)
-            ctx.meta = (wd, None if p is None else p.dtype, _all_leaf((weight, bias)))
+            m2 = m + 4 * R
+            ctx.meta = (R, C, dt, dev, wd, None if p is None else p.dtype, _hip.query('dig3d_rownorm_bwd_blocks', R, C, dt),
+                        _all_leaf((weight, bias)))
             ctx.save_for_backward(x, weight, stat)
-        else:
-            _on_device(dev, 'dig3d_rownorm_fwd', dt, x.data_ptr(), ld, R, C, ptr(weight), ptr(bias), wd, eps, y.data_ptr(), None, None)
+        _on_device(dev, 'dig3d_rownorm_fwd', dt, x.data_ptr(), _pitch(x), R, C, ptr(weight), ptr(bias), wd, eps, y.data_ptr(), m, m2)
         return y
 
     @staticmethod
     @_once
     def backward(ctx, gy):
         x, weight, stat = ctx.saved_tensors
-        wd, pd, leaf = ctx.meta
-        R, C = x.shape
-        dt = _DTYPES[x.dtype]
-        nx, nw, nb = ctx.needs_input_grad[:3]
-        gy = gy.contiguous()
+        R, C, dt, dev, wd, pd, blocks, leaf = ctx.meta
+        nx, nw, nb, _ = ctx.needs_input_grad
+        if not gy.is_contiguous():
+            gy = gy.contiguous()
         gx = torch.empty_like(gy) if nx else None
         gw = gb = part = later = None
-        blocks = _hip.query('dig3d_rownorm_bwd_blocks', R, C, dt)
+        if R == 0:
+            zero = lambda need: torch.zeros(C, dtype=pd, device=x.device) if need else None
+            return gx, zero(nw), zero(nb), None
         if nw or nb:
-            if R == 0:
-                gw = torch.zeros(C, dtype=pd, device=x.device) if nw else None
-                gb = torch.zeros(C, dtype=pd, device=x.device) if nb else None
-                return gx, gw, gb, None
             part = torch.empty(blocks * 2 * C, dtype=torch.float32, device=x.device)
-            if pd == torch.float32 and _deferred is not None and leaf:
+            if _deferred is not None and pd == torch.float32 and leaf:
                 # the workgroups' partials join the deferred reductions of the pass
                 later = torch.empty(2 * C, dtype=pd, device=x.device)
                 _reduce_later(part, blocks, 2 * C, later, leaf)
             else:
                 gw = torch.empty(C, dtype=pd, device=x.device) if nw else None
                 gb = torch.empty(C, dtype=pd, device=x.device) if nb else None
-        if R:
-            m = stat.data_ptr()
-            _on_device(x.get_device(), 'dig3d_rownorm_bwd', dt, gy.data_ptr(), x.data_ptr(), _pitch(x), R, C, ptr(weight), wd, m, m + 4 * R, ptr(gx), ptr(part),
-                       blocks, ptr(gw), ptr(gb))
+        m = stat.data_ptr()
+        _on_device(dev, 'dig3d_rownorm_bwd', dt, gy.data_ptr(), x.data_ptr(), _pitch(x), R, C, ptr(weight), wd, m, m + 4 * R, ptr(gx), ptr(part),
+                   blocks, ptr(gw), ptr(gb))
         if later is not None:
             gw, gb = (later[:C] if nw else None), (later[C:] if nb else None)
         return gx, gw, gb, None
