@@ -137,13 +137,16 @@ struct HdLoad {
       }
     }
   }
-  // base: the operand plane's first element.  The load is written out so that the compiler's own waits do not count it: it
-  // has no register result, and the kernel waits for it by count (vmcnt) before the barrier that hands the stage over.
-  // s_nop: the wait states between a scalar register's writer (M0, or a base that came through a vector instruction) and
-  // its reader, which the compiler does not see here.
-  __device__ __forceinline__ void issue(const HdOperand& o, const short* __restrict__ base, int own0, int k0, uint32_t lds,
-                                        int wave, int lane) const {
-    const char* at = hd_uniform((const char*)(base + (TR ? (int64_t)k0 * o.ld : (int64_t)own0 * o.ld + k0)));
+  // first element of the tile at k step 0 of a plane, and the distance between k steps (bytes)
+  static __device__ __forceinline__ const char* start(const HdOperand& o, int64_t plane, int own0) {
+    return (const char*)(o.p + plane + (TR ? 0 : (int64_t)own0 * o.ld));
+  }
+  static __device__ __forceinline__ int64_t advance(const HdOperand& o) { return TR ? 2 * HD_BK * o.ld : 2 * HD_BK; }
+  // The load is written out so that the compiler's own waits do not count it: it has no register result, and the kernel
+  // waits for it (vmcnt) before the barrier that hands the stage over.  s_nop: the wait states between a scalar register's
+  // writer (M0, or a base that came through a vector instruction) and its reader, which the compiler does not see here.
+  __device__ __forceinline__ void issue(const HdOperand& o, const char* base, int k0, uint32_t lds, int wave, int lane) const {
+    const char* at = hd_uniform(base);
 #pragma unroll
     for (int q = 0; q < NL; ++q) {
       const int blk = q * NW + wave;
@@ -152,7 +155,8 @@ struct HdLoad {
         const int k = blk * RPL + lane / CH;
         v -= 2u * (uint32_t)max(0, k - (o.rows - 1 - k0)) * (uint32_t)o.ld;
       }
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + blk * 1024), "v"(v), "s"(at)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds + blk * 1024)), "v"(v),
+                   "s"(at)
                    : "memory");
     }
   }
@@ -189,111 +193,20 @@ __device__ __forceinline__ void hd_store4(void* out, int64_t at, f32x4 v, int n)
   }
 }
 
-// out[j, i] = sum_k Q[j, k] P[i, k] on tiles of BI x BJ, WI x WJ waves; the lanes of a matrix result hold 4 consecutive i of
-// one j, so rows of the output are written in pieces of 4.
-template <class T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
-__global__ void __launch_bounds__(WI* WJ * 64) k_head_gemm(HdArgs a) {
+// a barrier for what passed through LDS; loads and stores of global memory stay in flight
+__device__ __forceinline__ void hd_lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xc07f);      // LDS reads and writes done; vmcnt at its maximum
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// what a finished tile of products becomes (see HdArgs)
+template <class T, int BI, int BJ, int WI, int WJ, int EPI>
+__device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / WI / 16][BJ / WJ / 16], int i0, int j0, int ti, int wi,
+                                            int wj, int tid, float* sh) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
-  constexpr int SZ = hd_tile_shorts<BI>() + hd_tile_shorts<BJ>();
-  __shared__ __attribute__((aligned(1024))) short sm[2 * SZ];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // tile of this workgroup: an XCD takes a contiguous range of tiles, ordered in bands of 4 tiles along j so that the
-  // tiles in flight on one L2 share operand panels along both indices
-  const int n = a.ti * a.tj, per = gridDim.x >> 3;
-  const int id = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
-  if (id >= n) return;
-  const int band = id / (4 * a.ti), j0b = band * 4, bw = min(4, a.tj - j0b), rem = id - band * 4 * a.ti;
-  const int tj = j0b + rem % bw, ti = rem / bw;
-  const int i0 = ti * BI, j0 = tj * BJ;
-  const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
-
-  f32x4 acc[MI][MJ];
-#pragma unroll
-  for (int x = 0; x < MI; ++x)
-#pragma unroll
-    for (int y = 0; y < MJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const int total = a.ktiles * a.nseg;
-  const int t0 = (int)((int64_t)total * blockIdx.z / a.splits), t1 = (int)((int64_t)total * (blockIdx.z + 1) / a.splits);
-
-  // only W is read along k where it lies, with rows beyond its last (PT && !QT); e and the copied x are whole k steps
-  using LP = HdLoad<BI, PT, PT && !QT, NW>;
-  using LQ = HdLoad<BJ, QT, false, NW>;
-  LP lp;
-  LQ lq;
-  lp.init(a.P, i0, wave, lane);
-  lq.init(a.Q, j0, wave, lane);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) short*)sm;
-  auto load = [&](int t, int stage) {
-    const int seg = t / a.ktiles, k0 = (t - seg * a.ktiles) * HD_BK;    // planes (h, h), (h, l), (l, h)
-    lp.issue(a.P, a.P.p + (seg == 2 ? a.P.plane : 0), i0, k0, lds0 + stage * (SZ * 2), wave, lane);
-    lq.issue(a.Q, a.Q.p + (seg == 1 ? a.Q.plane : 0), j0, k0, lds0 + stage * (SZ * 2) + hd_tile_shorts<BI>() * 2, wave, lane);
-  };
-  // Two stages.  A k step is four phases (two halves of k, two of the wave's i); the operands of a phase are read while the
-  // phase before it multiplies.  The barrier that ends a step stands before its last phase, whose operands are in registers
-  // by then: the loads of step t + 2 and the first reads of step t + 1 are issued under that phase's products.
-  constexpr int HX = MI / 2, NLD = LP::NL + LQ::NL;
-  s16x8 fp[2][HX], fq[2][MJ];
-  auto read_p = [&](int stage, int ph) {
-#pragma unroll
-    for (int x = 0; x < HX; ++x) fp[ph & 1][x] = hd_frag<BI, PT>(sm + stage * SZ, wi + ((ph & 1) * HX + x) * 16, ph >> 1, lane);
-  };
-  auto read_q = [&](int stage, int kk) {
-#pragma unroll
-    for (int y = 0; y < MJ; ++y) fq[kk][y] = hd_frag<BJ, QT>(sm + stage * SZ + hd_tile_shorts<BI>(), wj + y * 16, kk, lane);
-  };
-  auto mul = [&](int ph) {
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int x = 0; x < HX; ++x)
-#pragma unroll
-      for (int y = 0; y < MJ; ++y) acc[(ph & 1) * HX + x][y] = hd_mfma<T>(fp[ph & 1][x], fq[ph >> 1][y], acc[(ph & 1) * HX + x][y]);
-    __builtin_amdgcn_s_setprio(0);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  // all loads of this wave have landed, its LDS reads are done, and every other wave's
-  auto meet = [&]() {
-    __builtin_amdgcn_s_waitcnt(7 << 4);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-  };
-  // Every step issues its loads: beyond the last step they fetch that one again, into a stage that is read no more, so that
-  // the count of loads in flight is the same everywhere
-  auto step = [&](int t, int cur) {
-    read_p(cur, 1);
-    mul(0);
-    read_q(cur, 1);
-    read_p(cur, 2);
-    mul(1);
-    read_p(cur, 3);
-    mul(2);
-    meet();                                // step t + 1 has arrived; step t has been read by all
-    load(min(t + 2, t1 - 1), cur);
-    read_q(cur ^ 1, 0);
-    read_p(cur ^ 1, 0);
-    mul(3);
-  };
-  if (t0 < t1) {
-    load(t0, 0);
-    load(min(t0 + 1, t1 - 1), 1);
-    constexpr int left = NLD;
-    __builtin_amdgcn_s_waitcnt((left & 15) | ((left >> 4) << 14) | (7 << 4) | (15 << 8));
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-    read_q(0, 0);
-    read_p(0, 0);
-    int t = t0;
-    for (; t + 2 <= t1; t += 2) {
-      step(t, 0);
-      step(t + 1, 1);
-    }
-    if (t < t1) step(t, 0);
-  }
-  __builtin_amdgcn_s_waitcnt(0);           // what was issued by hand has landed
-  __syncthreads();                         // nothing is in flight into LDS when it is used again, or given back
-
+  const int lane = tid & 63, wave = tid >> 6;
   const int q4 = 4 * (lane >> 4), l15 = lane & 15;
   if constexpr (EPI == EPI_OUT) {
     const float s = a.out ? hd_factor<T>(a.scal, a.other) : 1.f;
@@ -319,55 +232,74 @@ __global__ void __launch_bounds__(WI* WJ * 64) k_head_gemm(HdArgs a) {
       }
     }
   } else {
-    const float dsc = a.nseg > 1 ? a.inv_tau / (a.scal[SC_X] * a.scal[SC_W]) : a.inv_tau;   // powers of two, and 1 / tau
-    // z = (product + bias) / tau
+    // z = u acc: the product in units of 1 / tau (the scales are powers of two); with a bias, acc becomes z and u one.
+    // The exponentials take z minus a maximum or lse first and the base-2 factor after it: the difference is exact where
+    // it matters.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane
+    // are 128 times whatever one costs.
+    float u = a.nseg > 1 ? a.inv_tau / (a.scal[SC_X] * a.scal[SC_W]) : a.inv_tau;
+    if (a.bias) {
 #pragma unroll
-    for (int x = 0; x < MI; ++x) {
-      float b[4];
+      for (int x = 0; x < MI; ++x)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = i0 + wi + x * 16 + q4 + r;
-        b[r] = a.bias && i < a.ni ? load_as(a.bias, a.dt, a.v0 + i) * a.inv_tau : 0.f;
-      }
+        for (int r = 0; r < 4; ++r) {
+          const int i = i0 + wi + x * 16 + q4 + r;
+          const float b = i < a.ni ? load_as(a.bias, a.dt, a.v0 + i) * a.inv_tau : 0.f;
 #pragma unroll
-      for (int y = 0; y < MJ; ++y)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[x][y][r] = __fmaf_rn(acc[x][y][r], dsc, b[r]);
+          for (int y = 0; y < MJ; ++y) acc[x][y][r] = __fmaf_rn(acc[x][y][r], u, b);
+        }
+      u = 1.f;
     }
+    const bool edge = i0 + BI > a.ni;                            // of the workgroup
+    const int first = i0 + wi + q4, last = a.ni - first;         // this lane's results are classes first + 16 x + r
+    auto target_at = [&](int j) -> int {                         // the place of row j's target among them, or -1
+      if (!a.target || j >= a.nj) return -1;
+      const int64_t t = a.target[j] - a.v0;
+      return t >= first && t < a.ni && t < first + 16 * MI ? (int)t - first : -1;
+    };
     if constexpr (EPI == EPI_STATS) {
       // (max, sum of exp) over this tile's classes without the target, per row; a row's classes lie in the 4 lane groups of
-      // WI waves
-      float* sh = (float*)sm;             // [WI][BJ][2]
+      // WI waves.  sh: [WI][BJ][2]
 #pragma unroll
       for (int y = 0; y < MJ; ++y) {
         const int jl = wj + y * 16 + l15, j = j0 + jl;
-        int64_t tg = -1;
-        if (a.target && j < a.nj) tg = a.target[j] - a.v0;
+        if (edge) {
+#pragma unroll
+          for (int x = 0; x < MI; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[x][y][r] = x * 16 + r >= last ? -INFINITY : acc[x][y][r];
+        }
+        const int tl = target_at(j);
+        if (__any(tl >= 0)) {
+          float z = 0.f;
+#pragma unroll
+          for (int x = 0; x < MI; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              z = tl == x * 16 + r ? acc[x][y][r] : z;
+              acc[x][y][r] = tl == x * 16 + r ? -INFINITY : acc[x][y][r];
+            }
+          if (tl >= 0 && (tl & 15) < 4) a.zt[j] = z * u;
+        }
         float m = -INFINITY, s = 0.f;
 #pragma unroll
         for (int x = 0; x < MI; ++x)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = i0 + wi + x * 16 + q4 + r;
-            if (i < a.ni && i == tg) a.zt[j] = acc[x][y][r];
-            if (i >= a.ni || i == tg) acc[x][y][r] = -INFINITY;
-            m = fmaxf(m, acc[x][y][r]);
-          }
+          for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[x][y][r]);
         m = fmaxf(m, __shfl_xor(m, 16, 64));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const float ms = m == -INFINITY ? 0.f : m;
+        const float ms = m == -INFINITY ? 0.f : m, k = u * L2E;
 #pragma unroll
         for (int x = 0; x < MI; ++x)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[x][y][r] - ms) * L2E);
+          for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[x][y][r] - ms) * k);
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
         if (lane < 16) {
-          sh[((wave % WI) * BJ + jl) * 2] = m;
+          sh[((wave % WI) * BJ + jl) * 2] = m * u;
           sh[((wave % WI) * BJ + jl) * 2 + 1] = s;
         }
       }
-      __syncthreads();
+      hd_lds_barrier();
       for (int jl = tid; jl < BJ; jl += NW * 64) {
         const int j = j0 + jl;
         if (j >= a.nj) continue;
@@ -381,47 +313,207 @@ __global__ void __launch_bounds__(WI* WJ * 64) k_head_gemm(HdArgs a) {
         a.part[(int64_t)j * a.part_ld + a.part_c0 + ti] = make_float2(m, s);
       }
     } else {
-      // e = c (exp(z - lse) - [target]); zeros in the padding that the next products read
+      // e = c (exp(z - lse) - [target]); zeros in the padding that the next products read, and in rows without a loss
 #pragma unroll
       for (int y = 0; y < MJ; ++y) {
         const int j = j0 + wj + y * 16 + l15;
-        if (j >= a.rowsE) continue;
         const bool in = j < a.nj;
-        const float lse = in ? a.lse[j] : 0.f, c = in ? a.coef[j] : 0.f;
-        int64_t tg = -1;
-        float et = 0.f;
-        if (a.target && in) {
-          tg = a.target[j] - a.v0;
-          et = c * expm1f(-a.loss[j]);     // p - 1 of the target: what the other classes hold, not a difference near 1
-        }
+        const float keep = __is_same(T, f16_t) ? E_SCALE : 1.f;
+        const float c = in ? a.coef[j] * keep : 0.f;
+        const float lse = c == 0.f ? INFINITY : a.lse[j];        // its row of x is zero: exp(z - inf) = 0
+        const int tl = target_at(j);
+        const bool any = __any(tl >= 0);
+        // p - 1 of the target: what the other classes hold, not a difference near 1
+        const float et = tl >= 0 ? c * expm1f(-a.loss[j]) : 0.f;
+        if (j >= a.rowsE) continue;
+        short* row = a.E + (int64_t)j * a.ldE + first;
 #pragma unroll
         for (int x = 0; x < MI; ++x) {
-          const int i = i0 + wi + x * 16 + q4;
-          if (i >= a.ldE) continue;
           float e[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = c * __builtin_amdgcn_exp2f((acc[x][y][r] - lse) * L2E);
-            e[r] = i + r >= a.ni || c == 0.f ? 0.f : i + r == tg ? et : p;   // a row without a loss gives nothing, whatever it holds
+          for (int r = 0; r < 4; ++r) e[r] = c * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x][y][r], u, -lse) * L2E);
+          if (any) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) e[r] = tl == x * 16 + r ? et : e[r];
+          }
+          if (edge) {
+            if (first + x * 16 >= a.ldE) continue;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) e[r] = x * 16 + r >= last ? 0.f : e[r];
           }
           struct alignas(8) { T t[4]; } h, l;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) h.t[r] = to_t<T>(e[r]);
+          *(decltype(h)*)(row + x * 16) = h;
           if (a.nseg > 1) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float v = e[r] * E_SCALE;
-              h.t[r] = to_t<T>(v);
-              l.t[r] = to_t<T>(v - (float)h.t[r]);
-            }
-            *(decltype(l)*)(a.E + a.planeE + (int64_t)j * a.ldE + i) = l;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) h.t[r] = to_t<T>(__is_same(T, f16_t) ? e[r] * E_SCALE : e[r]);
+            for (int r = 0; r < 4; ++r) l.t[r] = to_t<T>(e[r] - (float)h.t[r]);
+            *(decltype(l)*)(row + a.planeE + x * 16) = l;
           }
-          *(decltype(h)*)(a.E + (int64_t)j * a.ldE + i) = h;
         }
       }
     }
   }
+}
+
+// out[j, i] = sum_k Q[j, k] P[i, k] on tiles of BI x BJ, WI x WJ waves; the lanes of a matrix result hold 4 consecutive i of
+// one j, so rows of the output are written in pieces of 4.
+//
+// A workgroup walks its tiles as one sequence of k steps.  Two stages are in LDS; a step is four phases (two halves of k, two
+// of the wave's i), and the operands of a phase are read while the phase before it multiplies.  The barrier that ends a
+// step stands before its last phase, whose operands are in registers by then: the loads of the step after the next and the
+// first reads of the next one are issued under that phase's products.  The sequence runs on into the next tile, so a
+// tile's first loads are under way during the last steps and the epilogue of the tile before it.  Behind the last tile the
+// loads fetch that tile's first steps again, into stages that are read no more.
+// Measured (bf16, 4096 x 2048 x 65536): see hd_shape.  What bounds it: the latency of loads that miss the L2 (one step of
+// 64 KB in flight per CU) and the clock, which this load holds near 2.0 GHz.
+template <class T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
+__global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdArgs a) {
+  constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16, HX = MI / 2;
+  constexpr int SZ = hd_tile_shorts<BI>() + hd_tile_shorts<BJ>();
+  __shared__ __attribute__((aligned(1024))) short sm[2 * SZ];
+  __shared__ float sh[EPI == EPI_STATS ? WI * BJ * 2 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // An XCD takes a contiguous range of tiles, ordered in bands of 4 tiles along j, so that the tiles in flight on one L2
+  // share operand panels along both indices
+  const int n = a.ti * a.tj, per = (n + 7) >> 3, stride = (int)gridDim.x >> 3;
+  int id = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+  const int end = min(n, (((int)blockIdx.x & 7) + 1) * per);
+  if (id >= end) return;
+  auto place = [&](int t, int& ti, int& tj) __attribute__((always_inline)) {
+    const int band = t / (4 * a.ti), bw = min(4, a.tj - band * 4), rem = t - band * 4 * a.ti;
+    tj = band * 4 + rem % bw;
+    ti = rem / bw;
+  };
+  const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
+  const int total = a.ktiles * a.nseg;
+  const int t0 = (int)((int64_t)total * blockIdx.z / a.splits), t1 = (int)((int64_t)total * (blockIdx.z + 1) / a.splits);
+
+  // only W is read along k where it lies, with rows beyond its last (PT && !QT); e and the copied x are whole k steps
+  using LP = HdLoad<BI, PT, PT && !QT, NW>;
+  using LQ = HdLoad<BJ, QT, false, NW>;
+  LP lp;
+  LQ lq;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) short*)sm;
+  // The next load: its tile, how many of the tile's are left, the product of planes (h h, h l, l h), the step inside that, and
+  // the operands' bases.  Stages alternate by constants in the code, so an odd count of steps gets one more that repeats the
+  // last load and multiplies nothing.
+  const int steps = t1 - t0, pad = steps & 1;
+  const int first_seg = t0 / a.ktiles, first_k = t0 - first_seg * a.ktiles;
+  const int64_t dp = LP::advance(a.P), dq = LQ::advance(a.Q);
+  int lid = id, left, seg, lk, li0, lj0;
+  const char *bp, *bq;
+  auto base = [&]() __attribute__((always_inline)) {
+    bp = LP::start(a.P, seg == 2 ? a.P.plane : 0, li0) + lk * dp;
+    bq = LQ::start(a.Q, seg == 1 ? a.Q.plane : 0, lj0) + lk * dq;
+  };
+  auto aim = [&]() __attribute__((always_inline)) {
+    int ti, tj;
+    place(lid, ti, tj);
+    li0 = ti * BI;
+    lj0 = tj * BJ;
+    lp.init(a.P, li0, wave, lane);
+    lq.init(a.Q, lj0, wave, lane);
+  };
+  auto rewind = [&]() __attribute__((always_inline)) {
+    left = steps + pad;
+    seg = first_seg;
+    lk = first_k;
+    base();
+  };
+  auto issue = [&](int stage) __attribute__((always_inline)) {
+    lp.issue(a.P, bp, lk * HD_BK, lds0 + stage * (SZ * 2), wave, lane);
+    lq.issue(a.Q, bq, lk * HD_BK, lds0 + stage * (SZ * 2) + hd_tile_shorts<BI>() * 2, wave, lane);
+    if (--left == 0) {
+      if (lid + stride < end) {
+        lid += stride;
+        aim();
+      }
+      rewind();
+    } else if (left > pad) {
+      bp += dp;
+      bq += dq;
+      if (++lk == a.ktiles) {
+        lk = 0;
+        ++seg;
+        base();
+      }
+    }
+  };
+  s16x8 fp[2][HX], fq[2][MJ];
+  f32x4 acc[MI][MJ];
+  auto read_p = [&](int stage, int ph) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < HX; ++x) fp[ph & 1][x] = hd_frag<BI, PT>(sm + stage * SZ, wi + ((ph & 1) * HX + x) * 16, ph >> 1, lane);
+  };
+  auto read_q = [&](int stage, int kk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int y = 0; y < MJ; ++y) fq[kk][y] = hd_frag<BJ, QT>(sm + stage * SZ + hd_tile_shorts<BI>(), wj + y * 16, kk, lane);
+  };
+  auto mul = [&](int ph) __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int x = 0; x < HX; ++x)
+#pragma unroll
+      for (int y = 0; y < MJ; ++y) acc[(ph & 1) * HX + x][y] = hd_mfma<T>(fp[ph & 1][x], fq[ph >> 1][y], acc[(ph & 1) * HX + x][y]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // this wave's loads have landed and its LDS reads are done, and every other wave's
+  auto meet = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(7 << 4);
+    hd_lds_barrier();
+  };
+  aim();
+  rewind();
+  issue(0);
+  issue(1);
+  meet();
+  for (; id < end; id += stride) {
+    int ti, tj;
+    place(id, ti, tj);
+#pragma unroll
+    for (int x = 0; x < MI; ++x)
+#pragma unroll
+      for (int y = 0; y < MJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+    read_q(0, 0);
+    read_p(0, 0);
+    for (int t = 0; t < steps; t += 2) {
+      read_p(0, 1);
+      mul(0);
+      read_q(0, 1);
+      read_p(0, 2);
+      mul(1);
+      read_p(0, 3);
+      mul(2);
+      meet();                              // the next step has arrived; this one has been read by all
+      issue(0);
+      read_q(1, 0);
+      read_p(1, 0);
+      mul(3);
+      const bool more = t + 1 < steps;     // not of an odd count's last step, whose partner is only waited for
+      if (more) {
+        read_p(1, 1);
+        mul(0);
+        read_q(1, 1);
+        read_p(1, 2);
+        mul(1);
+        read_p(1, 3);
+        mul(2);
+      }
+      meet();
+      issue(1);
+      if (t + 2 < steps) {                 // across the epilogue the registers are the result's
+        read_q(0, 0);
+        read_p(0, 0);
+      }
+      if (more) mul(3);
+    }
+    hd_epilogue<T, BI, BJ, WI, WJ, EPI>(a, acc, ti * BI, tj * BJ, ti, wi, wj, tid, sh);
+  }
+  __builtin_amdgcn_s_waitcnt(0);           // nothing is in flight into LDS when it is given back
+  __builtin_amdgcn_s_barrier();
 }
 
 #include "head_small.h"
@@ -803,30 +895,36 @@ __global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __rest
   }
 }
 
-#define HD_SLICE 256
-// column sums of e over slices of HD_SLICE rows: part[slice][ldE]
+#define HD_SLICE 128
+// column sums of e over slices of HD_SLICE rows: part[slice][ldE].  32 lanes across 256 columns (16 bytes each), 8 row lanes
 template <class T>
 __global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E, int64_t ldE, int64_t planeE, int planes, int rows,
                                                       float* __restrict__ part) {
-  const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4, sl = threadIdx.x >> 6;
-  __shared__ float sh[4][64][4];
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < ldE) {
+  __shared__ float sh[8][32 * 8 + 4];
+  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 256 + cl * 8;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (c < ldE) {                           // a multiple of 64: a lane's 8 columns are all there
     const int r0 = blockIdx.y * HD_SLICE, r1 = min(rows, r0 + HD_SLICE);
-    for (int r = r0 + sl; r < r1; r += 4)
-      for (int p = 0; p < planes; ++p) {
-        const T* e = (const T*)E + p * planeE + (int64_t)r * ldE + c;
+    for (int p = 0; p < planes; ++p) {
+#pragma unroll 4
+      for (int r = r0 + rl; r < r1; r += 8) {
+        struct alignas(16) { T t[8]; } v = *(const decltype(v)*)(E + p * planeE + (int64_t)r * ldE + c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] += (float)e[i];
+        for (int i = 0; i < 8; ++i) s[i] += (float)v.t[i];
       }
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sh[sl][threadIdx.x & 63][i] = s[i];
+  for (int i = 0; i < 8; ++i) sh[rl][cl * 8 + i] = s[i];
   __syncthreads();
-  if (sl == 0 && c < ldE)
+  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (o < ldE) {
+    float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      part[(int64_t)blockIdx.y * ldE + c + i] = (sh[0][threadIdx.x][i] + sh[1][threadIdx.x][i]) + (sh[2][threadIdx.x][i] + sh[3][threadIdx.x][i]);
+    for (int q = 0; q < 8; ++q) v += sh[q][threadIdx.x];
+    part[(int64_t)blockIdx.y * ldE + o] = v;
+  }
 }
 
 // out[at0 + i] = factor * sum_s part[s][i] over `slots` partials, in order
@@ -849,10 +947,13 @@ struct HdShape {
 };
 
 // The tile edge and the number of k ranges with the smallest estimated time.  The estimate is fitted to measured launches of
-// the product kernel (bf16; us of one k step of 64 with c tiles on a CU, and us of a tile's first loads and epilogue):
-//   64: 0.5 alone, 1.1 with five on the CU;   128: 0.8 alone, 1.2 with two;   256: 1.9 (one to a CU)
-// e.g. 4096 x 2048 x 65536 (logits): 64 -> 1.9 ms, 128 -> 1.21, 256 -> 1.00;  2048 x 256 x 32768: 103, 83, 74 us;
-// 64 x 1024 x 16384: 11, 17, 35 us;  e W of 1024 x 128 x 65536 in 16 ranges: 51, 56, 113 us.
+// the product kernel (bf16; us of one k step of 64 with c tiles on a CU, and us of a tile's epilogue that its neighbours do
+// not hide):   64: 0.5 alone, 1.1 with five on the CU;   128: 0.8 alone, 1.2 with two;   256: 1.9 (one to a CU)
+// us with tiles of 64 / 128 / 256:
+//   logits' statistics, 4096 x 2048 x 65536: 1956 / 1075 / 950 (1.16 PFLOP/s; a library's plain product of that shape: 904)
+//   2048 x 256 x 32768: 88 / 55 / 48    64 x 1024 x 16384: 11 / 14 / 31    their gradient e, 4096 x 2048 x 65536: - / 1238 / 1052
+//   e W in ranges, 4096 x 2048 x 65536 (2): 2365 / 1212 / 974    1024 x 128 x 65536 (16): 52 / 59 / 118
+//   e^T x, 4096 x 2048 x 65536: 2683 / 1184 / 983    2048 x 256 x 32768: 59 / 41 / 60    16384 x 128 x 1024 (16): 20 / 24 / 44
 // A split product writes its partial results and a second launch adds them (bytes at 4 TB/s and 4 us).
 static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) {
   const int cus = dig3d_num_cus();
@@ -867,7 +968,7 @@ static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) 
       const int c = (int)(c0 < occ ? c0 : occ);
       const int64_t rounds = (items + (int64_t)cus * c - 1) / ((int64_t)cus * c);
       const double step = e == 0 ? 0.35 + 0.15 * c : e == 1 ? 0.42 + 0.38 * c : 1.9;
-      const double fixed = e == 0 ? 2.0 + 0.5 * c : e == 1 ? 3.0 + 1.3 * c : 10.0;
+      const double fixed = e == 0 ? 2.0 + 0.5 * c : e == 1 ? 1.5 + 0.8 * c : 6.0;
       double t = (double)rounds * (fixed + (double)((ksteps + s - 1) / s) * step);
       if (s > 1) t += 4.0 + (double)s * ni * nj * 8 / 4e6;
       if (t < tb) {
@@ -900,8 +1001,16 @@ static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
 
 #define HD_PIECE_BYTES (512ll << 20)   // e of one piece, per plane; a piece also bounds the packed part of W
 
-// Float32 products in place (head_small.h) below this size: SMALL_RULE
-static bool hd_small(int64_t N, int64_t D, int64_t V) { return (double)N * D * V <= 33554432.0; }
+// Float32 products in place (head_small.h) where copies and launches are what the general path costs (GPU us of value and
+// gradients, in place / general):
+//   f32:  32 x 128 x 1195: 39 / 96   512 x 128 x 1195: 65 / 118   2048 x 128 x 1195: 149 / 148   32 x 128 x 32768: 90 / 115
+//         128 x 512 x 1024: 73 / 83   512 x 512 x 256: 89 / 84   8 x 1024 x 1024: 106 / 98   4096 x 128 x 64: 206 / 76
+//   bf16: 32 x 128 x 1195: 42 / 70   512 x 128 x 1195: 67 / 81   32 x 128 x 8192: 51 / 46   8 x 512 x 4096: 75 / 45
+// 16-bit rows that the general path copies (odd widths or addresses) count as f32.
+static bool hd_small(bool copies, int64_t N, int64_t D, int64_t V) {
+  const double work = (double)N * D * V;
+  return N <= 512 && (copies ? D <= 512 && work <= 134217728.0 : D <= 128 && work <= 16777216.0);
+}
 
 // needs: bit 0 gx, bit 1 gw, bit 2 gb; backward = 0: the forward's plan
 static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int backward, int needs) {
@@ -913,7 +1022,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     at += al256(bytes);
     return o;
   };
-  p.small = hd_small(N, D, V);
+  p.small = hd_small(!(dx && dw), N, D, V);
   if (p.small) {
     p.vp = V;
     p.np = 1;
@@ -980,7 +1089,9 @@ static void hd_gemm(const HdArgs& a0, const HdShape& sh, hipStream_t st) {
   a.ti = (a.ni + sh.b - 1) / sh.b;
   a.tj = (a.nj + sh.b - 1) / sh.b;
   a.splits = sh.splits;
-  const dim3 grid((unsigned)dig3d_xcd_grid(a.ti * a.tj), 1, (unsigned)sh.splits);
+  // as many workgroups as run at once; each walks its tiles
+  const int occ = sh.b == 256 ? 1 : sh.b == 128 ? 2 : 5, most = (dig3d_num_cus() * occ / sh.splits + 7) & ~7;
+  const dim3 grid((unsigned)min(dig3d_xcd_grid(a.ti * a.tj), most), 1, (unsigned)sh.splits);
   if (sh.b == 256) hipLaunchKernelGGL((k_head_gemm<T, 256, 256, 2, 4, PT, QT, EPI>), grid, dim3(512), 0, st, a);
   else if (sh.b == 128) hipLaunchKernelGGL((k_head_gemm<T, 128, 128, 2, 2, PT, QT, EPI>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((k_head_gemm<T, 64, 64, 2, 2, PT, QT, EPI>), grid, dim3(256), 0, st, a);
