@@ -10,8 +10,8 @@
 // operands (the second kind by the transposing LDS read), so nothing is transposed in memory.  Its epilogues: the softmax
 // statistics of a tile of logits (forward), the gradient e of a piece of the vocabulary (backward), or the stored product.
 //
-// Types.  bf16 / f16: the inputs as they are, sums in f32; e is rounded once to the same type (2^-9 / 2^-12 of each entry at
-// random sign, below the rounding of the gradients it leads to).  f32: every value is two f16 numbers, v s = h + l with
+// Types.  bf16 / f16: the inputs as they are, sums in f32; e is rounded once to the same type (up to 2^-8 / 2^-11 of each entry,
+// at random sign; with few rows e is two such numbers).  f32: every value is two f16 numbers, v s = h + l with
 // s = 2^k chosen so that the largest |v| of the tensor lies in [2^14, 2^15): 22 bits of every v down to 2^-29 of that
 // largest one, and an absolute error of 2^-40 of it below; three products h h, h l, l h with f32 sums (l l is below 2^-22 of
 // the term).  Three f16 matrix products have 5x the rate of one in f32 on this chip, at the error of an f32 product.
@@ -57,7 +57,7 @@ struct HdArgs {
   HdOperand P, Q;
   int ni, nj;                // extents of the own indices of P and Q
   int ktiles;                // k steps of one product
-  int nseg;                  // 1, or 3 products of planes (h h, h l, l h)
+  int nseg;                  // products of planes (P, Q): 1 (h h), 2 (h h, h l) or 3 (h h, h l, l h)
   int ti, tj;                // tiles along i and j
   int splits;                // the k steps are dealt to gridDim.z workgroups
   // logits epilogues: i = class v0 + i, j = row
@@ -71,10 +71,11 @@ struct HdArgs {
   float2* part;              // EPI_STATS [nj][ti_all]: (max, sum of exp) of the tile
   int part_ld, part_c0;
   float* zt;                 // EPI_STATS: the target's logit
-  const float* lse;          // EPI_GRAD
+  const float *m, *rs;       // EPI_GRAD: softmax = exp(z - m) rs
   const float* loss;
   const float* coef;
-  short* E;                  // EPI_GRAD [planes][rowsE][ldE]
+  int eplanes;               // e as one number, or as two (its rounding and what that left)
+  short* E;                  // EPI_GRAD [eplanes][rowsE][ldE]
   int64_t ldE, planeE;
   int rowsE;
   // EPI_OUT
@@ -233,7 +234,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
     }
   } else {
     // z = u acc: the product in units of 1 / tau (the scales are powers of two); with a bias, acc becomes z and u one.
-    // The exponentials take z minus a maximum or lse first and the base-2 factor after it: the difference is exact where
+    // The exponentials take z minus a maximum first and the base-2 factor after it: the difference is exact where
     // it matters.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane
     // are 128 times whatever one costs.
     float u = a.nseg > 1 ? a.inv_tau / (a.scal[SC_X] * a.scal[SC_W]) : a.inv_tau;
@@ -313,14 +314,15 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         a.part[(int64_t)j * a.part_ld + a.part_c0 + ti] = make_float2(m, s);
       }
     } else {
-      // e = c (exp(z - lse) - [target]); zeros in the padding that the next products read, and in rows without a loss
+      // e = c (exp(z - m) rs - [target]); zeros in the padding that the next products read, and in rows without a loss
 #pragma unroll
       for (int y = 0; y < MJ; ++y) {
         const int j = j0 + wj + y * 16 + l15;
         const bool in = j < a.nj;
         const float keep = __is_same(T, f16_t) ? E_SCALE : 1.f;
         const float c = in ? a.coef[j] * keep : 0.f;
-        const float lse = c == 0.f ? INFINITY : a.lse[j];        // its row of x is zero: exp(z - inf) = 0
+        const float m = c == 0.f ? INFINITY : a.m[j];            // its row of x is zero: exp(z - inf) = 0
+        const float cp = c == 0.f ? 0.f : c * a.rs[j];
         const int tl = target_at(j);
         const bool any = __any(tl >= 0);
         // p - 1 of the target: what the other classes hold, not a difference near 1
@@ -331,7 +333,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         for (int x = 0; x < MI; ++x) {
           float e[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) e[r] = c * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x][y][r], u, -lse) * L2E);
+          for (int r = 0; r < 4; ++r) e[r] = cp * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x][y][r], u, -m) * L2E);
           if (any) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) e[r] = tl == x * 16 + r ? et : e[r];
@@ -345,7 +347,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
 #pragma unroll
           for (int r = 0; r < 4; ++r) h.t[r] = to_t<T>(e[r]);
           *(decltype(h)*)(row + x * 16) = h;
-          if (a.nseg > 1) {
+          if (a.eplanes > 1) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) l.t[r] = to_t<T>(e[r] - (float)h.t[r]);
             *(decltype(l)*)(row + a.planeE + x * 16) = l;
@@ -627,10 +629,11 @@ __device__ __forceinline__ float hd_wave_sum(float v) {
   return v;
 }
 
-// the tiles' statistics of one row joined by a wave (result in lane 0): lse, and with a target the row's loss (0 where the
-// target is `ignore`, NaN where it is no class)
+// the tiles' statistics of one row joined by a wave (result in lane 0): softmax = exp(z - mo) rs, the maximum and the sum
+// apart (their lse, rounded at its own size, would shift every probability of the row); with a target the row's loss, 0
+// where it is `ignore`, NaN where it is no class
 __device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int tiles, int64_t V, bool with_target, int64_t tg,
-                                            int64_t ignore, const float* zt, int lane, float& lse, float& loss) {
+                                            int64_t ignore, const float* zt, int lane, float& mo, float& rs, float& loss) {
   float m = -INFINITY, s = 0.f;
   for (int t = lane; t < tiles; t += 64) m = fmaxf(m, p[t].x);
 #pragma unroll
@@ -638,14 +641,16 @@ __device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int ti
   const float ms = m == -INFINITY ? 0.f : m;
   for (int t = lane; t < tiles; t += 64) s += p[t].y * __builtin_amdgcn_exp2f((p[t].x - ms) * L2E);
   s = hd_wave_sum(s);
-  lse = loss = 0.f;
+  mo = loss = 0.f;
+  rs = 1.f;
   if (!with_target) {
-    lse = ms + logf(s);
+    mo = m;
+    rs = 1.f / s;
     return;
   }
   if (tg == ignore) return;
   if (tg < 0 || tg >= V) {
-    lse = loss = NAN;
+    mo = rs = loss = NAN;
     return;
   }
   // s exp(m) over the other classes, z the target's logit.  The loss from the others' share, not from a difference of
@@ -653,22 +658,25 @@ __device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int ti
   const float z = *zt;
   const float M = fmaxf(m, z), Ms = M == -INFINITY ? 0.f : M;
   const float so = s * expf(ms - Ms), st = expf(z - Ms);
-  lse = Ms + logf(so + st);
+  mo = M;
+  rs = 1.f / (so + st);
   loss = z >= m ? log1pf(so) : (Ms - z) + logf(so + st);
 }
 
 // a wave per row
 __global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ part, int tiles, int N, int64_t V,
                                                     const int64_t* __restrict__ target, int64_t ignore,
-                                                    const float* __restrict__ zt, float* __restrict__ lse,
-                                                    float* __restrict__ loss, float* __restrict__ rows_out) {
+                                                    const float* __restrict__ zt, float* __restrict__ mo,
+                                                    float* __restrict__ rs, float* __restrict__ loss,
+                                                    float* __restrict__ rows_out) {
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= N) return;
-  float l, v;
-  hd_join_row(part + n * tiles, tiles, V, target != nullptr, target ? target[n] : 0, ignore, zt + n, lane, l, v);
+  float m, r, v;
+  hd_join_row(part + n * tiles, tiles, V, target != nullptr, target ? target[n] : 0, ignore, zt + n, lane, m, r, v);
   if (lane == 0) {
-    lse[n] = l;
+    mo[n] = m;
+    rs[n] = r;
     if (target) {
       loss[n] = v;
       if (rows_out) rows_out[n] = v;
@@ -711,17 +719,19 @@ __global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ l
 // few rows: the join and the total in one workgroup
 __global__ void __launch_bounds__(1024) k_head_join_total(const float2* __restrict__ part, int tiles, int N, int64_t V,
                                                            const int64_t* __restrict__ target, int64_t ignore,
-                                                           const float* __restrict__ zt, float* __restrict__ lse,
-                                                           float* __restrict__ loss, int mean, float* __restrict__ out,
+                                                           const float* __restrict__ zt, float* __restrict__ mo,
+                                                           float* __restrict__ rs, float* __restrict__ loss, int mean,
+                                                           float* __restrict__ out,
                                                            float* __restrict__ count) {
   __shared__ float sh[32];
   const int lane = threadIdx.x & 63;
   float s = 0.f, c = 0.f;
   for (int n = threadIdx.x >> 6; n < N; n += 16) {
-    float l, v;
-    hd_join_row(part + (int64_t)n * tiles, tiles, V, true, target[n], ignore, zt + n, lane, l, v);
+    float m, r, v;
+    hd_join_row(part + (int64_t)n * tiles, tiles, V, true, target[n], ignore, zt + n, lane, m, r, v);
     if (lane == 0) {
-      lse[n] = l;
+      mo[n] = m;
+      rs[n] = r;
       loss[n] = v;
       s += v;
       c += target[n] != ignore ? 1.f : 0.f;
@@ -740,8 +750,8 @@ template <class T>
 __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, const T* __restrict__ w, const void* __restrict__ bias,
                                                        int dt, int64_t ldx, int64_t ldw, int D, int64_t V,
                                                        const int64_t* __restrict__ index, const void* __restrict__ tl, int tdt, int K,
-                                                       float inv_tau, float tau, const float* __restrict__ lse, float* __restrict__ q,
-                                                       float* __restrict__ z, float* __restrict__ loss, float* __restrict__ live,
+                                                       float inv_tau, float tau, const float* __restrict__ mo, const float* __restrict__ rs,
+                                                       float* __restrict__ q, float* __restrict__ z, float* __restrict__ loss, float* __restrict__ live,
                                                        float* __restrict__ rows_out) {
   constexpr int N8 = VecLen<T>::n;
   extern __shared__ int64_t dyn[];         // index [K], then t / tau [K], then q [K]
@@ -772,7 +782,7 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
   s = (sh[4] + sh[5]) + (sh[6] + sh[7]);
   const bool any = s > 0.f || s != s;      // a NaN among the listed logits is not an empty row
   const float ls = any ? logf(s) : 0.f;
-  const float L = lse[n];
+  const float sm = mo[n], sl = logf(rs[n]);   // the student's log softmax is z - sm + sl
   for (int k = tid; k < K; k += 256) sq[k] = st[k] == -INFINITY ? 0.f : expf(st[k] - ms - ls);
   __syncthreads();
   const T* xr = x + n * ldx;
@@ -811,7 +821,7 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
       float zk = 0.f;
       if (any && t != -INFINITY) {
         zk = v < V ? (bias ? dot + load_as(bias, dt, v) : dot) * inv_tau : NAN;     // no such class: the row says so
-        part += sq[k] * (t - ms - ls - (zk - L));
+        part += sq[k] * (t - ms - ls - (zk - sm + sl));
       }
       z[n * K + k] = zk;
     }
@@ -867,12 +877,12 @@ __global__ void __launch_bounds__(1024) k_head_coef(const float* __restrict__ g,
   if (threadIdx.x == 0) scal[SC_S] = S;
 }
 
-// teacher: the listed classes of this piece get e = c (exp(z_k - lse) - q_k), from the entry's own logit, over what the
+// teacher: the listed classes of this piece get e = c (softmax_k - q_k), from the entry's own logit, over what the
 // product's epilogue wrote there.  Entries of the same class hold the same q and z and write the same value.
 template <class T>
 __global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __restrict__ index, const float* __restrict__ q,
-                                                            const float* __restrict__ z, const float* __restrict__ lse,
-                                                            const float* __restrict__ coef, int64_t N, int K, int64_t v0,
+                                                            const float* __restrict__ z, const float* __restrict__ mo,
+                                                            const float* __restrict__ rs, const float* __restrict__ coef, int64_t N, int K, int64_t v0,
                                                             int64_t nv, int planes, void* __restrict__ E, int64_t ldE,
                                                             int64_t planeE) {
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -881,17 +891,15 @@ __global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __rest
   const float qk = q[u], c = coef[n];
   const int64_t v = index[u];
   if (v < v0 || v >= v0 + nv || c == 0.f || qk < 0.f) return;
-  const float e = c * (__builtin_amdgcn_exp2f((z[u] - lse[n]) * L2E) - qk);
+  const float e = c * (__builtin_amdgcn_exp2f((z[u] - mo[n]) * L2E) * rs[n] - qk);
   T* o = (T*)E + n * ldE + (v - v0);
   if constexpr (sizeof(T) == 4) {
     *o = e;
-  } else if (planes == 2) {
-    const float s = e * E_SCALE;
+  } else {
+    const float s = __is_same(T, f16_t) ? e * E_SCALE : e;
     const T h = to_t<T>(s);
     *o = h;
-    o[planeE] = to_t<T>(s - (float)h);
-  } else {
-    *o = to_t<T>(__is_same(T, f16_t) ? e * E_SCALE : e);
+    if (planes == 2) o[planeE] = to_t<T>(s - (float)h);
   }
 }
 
@@ -986,6 +994,7 @@ static inline int64_t al256(int64_t v) { return (v + 255) & ~255ll; }
 struct HdPlan {
   bool small;                // head_small.h
   int planes, Dp;
+  int eplanes, nseg;         // of e, and products of planes with it
   bool dx, dw;               // x / W are read where they are
   int64_t Np, vp, np, ldE;
   HdShape lg, gx, gw;
@@ -1045,6 +1054,11 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     return p;
   }
   p.planes = dt == DT_F32 ? 2 : 1;
+  // One rounding of e is lost among the roundings of the gradients where many rows add up (2^1/2 of the error of their own);
+  // in a few rows it is a common factor of a whole row of gw.  There W is what the products wait for, and e is two numbers;
+  // also where the second product costs no more than launches do (512 x 512 x 8192: 15 us of 190)
+  p.eplanes = dt == DT_F32 || N <= 128 || (double)N * D * V <= 2147483648.0 ? 2 : 1;
+  p.nseg = dt == DT_F32 ? 3 : p.eplanes;
   p.Dp = (int)up64(D);
   p.dx = dx && !backward;    // the backward masks rows while it copies x (N D elements: nothing beside its products)
   p.dw = dw;
@@ -1068,13 +1082,13 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     p.o_zt = take(N * 4);
   } else {
     p.o_coef = take(N * 4);
-    p.o_E = take(p.Np * p.ldE * 2 * p.planes);
+    p.o_E = take(p.Np * p.ldE * 2 * p.eplanes);
     if (needs & 1) {
-      p.gx = hd_shape(D, N, p.ldE / HD_BK * nseg, 64);
+      p.gx = hd_shape(D, N, p.ldE / HD_BK * p.nseg, 64);
       if (p.np > 1 || p.gx.splits > 1) p.o_gx = take((int64_t)p.gx.splits * N * D * 4);
     }
     if (needs & 2) {
-      p.gw = hd_shape(D, p.vp, p.Np / HD_BK * nseg, 64);
+      p.gw = hd_shape(D, p.vp, p.Np / HD_BK * p.nseg, 64);
       if (p.gw.splits > 1) p.o_gw = take((int64_t)p.gw.splits * p.vp * D * 4);
     }
     if (needs & 4) p.o_col = take((N + HD_SLICE - 1) / HD_SLICE * p.ldE * 4);
@@ -1129,8 +1143,8 @@ struct HdCall {
   int tdt, K;
   float tau;
   int reduction;             // 0 one loss per row, 1 mean, 2 sum
-  // kept from the forward for the backward (float[HD_KEEP + 3 N + 2 N K])
-  float *scal, *amax, *count, *lse, *loss, *live, *q, *z;
+  // kept from the forward for the backward (float[HD_KEEP + 4 N + 2 N K])
+  float *scal, *amax, *count, *m, *rs, *loss, *live, *q, *z;
   hipStream_t st;
 };
 #define HD_KEEP 520
@@ -1139,8 +1153,9 @@ static void hd_keep(HdCall& c, float* keep) {
   c.scal = keep;
   c.amax = keep + SC_COUNT;
   c.count = keep + SC_COUNT + 2 * HD_AMAX;
-  c.lse = keep + HD_KEEP;
-  c.loss = c.lse + c.N;
+  c.m = keep + HD_KEEP;
+  c.rs = c.m + c.N;
+  c.loss = c.rs + c.N;
   c.live = c.loss + c.N;
   c.q = c.live + c.N;
   c.z = c.q + (int64_t)c.N * c.K;
@@ -1164,7 +1179,8 @@ static SmArgs sm_args(const HdCall& c, const HdPlan& p, char* ws) {
   a.part = (float2*)(ws + p.o_part);
   a.tiles = p.tiles_all;
   a.zt = (float*)(ws + p.o_zt);
-  a.lse = c.lse;
+  a.m = c.m;
+  a.rs = c.rs;
   a.loss = c.loss;
   return a;
 }
@@ -1232,13 +1248,13 @@ static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
   // 64 rows: one workgroup joins them in the time of one more launch (2 us each)
   if (c.target && c.reduction && c.N <= 64) {
     hipLaunchKernelGGL(k_head_join_total, dim3(1), dim3(1024), 0, c.st, part, p.tiles_all, c.N, (int64_t)c.V, c.target, c.ignore, zt,
-                       c.lse, c.loss, c.reduction == 1, out, c.count);
+                       c.m, c.rs, c.loss, c.reduction == 1, out, c.count);
     DIG3D_CHECK_LAUNCH();
     return DIG3D_OK;
   }
   float* rows_out = c.reduction ? nullptr : out;
   hipLaunchKernelGGL(k_head_join, dim3((c.N + 3) / 4), dim3(256), 0, c.st, part, p.tiles_all, c.N, (int64_t)c.V, c.target, c.ignore, zt,
-                     c.lse, c.loss, rows_out);
+                     c.m, c.rs, c.loss, rows_out);
   DIG3D_CHECK_LAUNCH();
   if (c.index) {
     const dim3 g((unsigned)c.N), b(256);
@@ -1246,7 +1262,7 @@ static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
     const float it = 1.0f / c.tau;
 #define TC_GO(T)                                                                                                                       \
   hipLaunchKernelGGL((k_head_teacher<T>), g, b, lds, c.st, (const T*)c.x, (const T*)c.w, c.bias, c.dt, c.ldx, c.ldw, c.D, (int64_t)c.V, \
-                     c.index, c.teacher, c.tdt, c.K, it, c.tau, c.lse, c.q, c.z, c.loss, c.live, rows_out)
+                     c.index, c.teacher, c.tdt, c.K, it, c.tau, c.m, c.rs, c.q, c.z, c.loss, c.live, rows_out)
     if (c.dt == DT_F32) TC_GO(float);
     else if (c.dt == DT_BF16) TC_GO(bf16_t);
     else TC_GO(f16_t);
@@ -1265,7 +1281,7 @@ template <class T>
 static int hd_teacher_grad(const HdCall& c, const float* coef, int64_t v0, int64_t nv, int planes, void* E, int64_t ldE,
                            int64_t planeE) {
   hipLaunchKernelGGL((k_head_teacher_grad<T>), dim3((unsigned)(((int64_t)c.N * c.K + 255) / 256)), dim3(256), 0, c.st, c.index, c.q,
-                     c.z, c.lse, coef, (int64_t)c.N, c.K, v0, nv, planes, E, ldE, planeE);
+                     c.z, c.m, c.rs, coef, (int64_t)c.N, c.K, v0, nv, planes, E, ldE, planeE);
   DIG3D_CHECK_LAUNCH();
   return DIG3D_OK;
 }
@@ -1342,9 +1358,11 @@ static int hd_bwd(const HdCall& c, const HdPlan& p, const float* g, void* gx, vo
     a.v0 = v0;
     a.V = c.V;
     a.target = c.target;
-    a.lse = c.lse;
+    a.m = c.m;
+    a.rs = c.rs;
     a.loss = c.loss;
     a.coef = coef;
+    a.eplanes = p.eplanes;
     a.E = E;
     a.ldE = p.ldE;
     a.planeE = eplane;
@@ -1352,12 +1370,12 @@ static int hd_bwd(const HdCall& c, const HdPlan& p, const float* g, void* gx, vo
     hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, c.st);
     DIG3D_CHECK_LAUNCH();
     if (c.index) {
-      const int rc = hd_teacher_grad<T>(c, coef, v0, nv, p.planes, E, p.ldE, eplane);
+      const int rc = hd_teacher_grad<T>(c, coef, v0, nv, p.eplanes, E, p.ldE, eplane);
       if (rc != DIG3D_OK) return rc;
     }
     HdArgs o;
     memset(&o, 0, sizeof o);
-    o.nseg = a.nseg;
+    o.nseg = p.nseg;
     o.scal = c.scal;
     o.dt = c.dt;
     if (gx) {                              // gx[n, d] += sum_v e[n, v] W[v, d]
@@ -1399,7 +1417,7 @@ static int hd_bwd(const HdCall& c, const HdPlan& p, const float* g, void* gx, vo
       float* part = (float*)(ws + p.o_col);
       const int slices = (c.N + HD_SLICE - 1) / HD_SLICE;
       hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)((p.ldE + 255) / 256), (unsigned)slices), dim3(256), 0, c.st, E, p.ldE,
-                         eplane, p.planes, c.N, part);
+                         eplane, p.eplanes, c.N, part);
       DIG3D_CHECK_LAUNCH();
       hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(nv, 256)), dim3(256), 0, c.st, part, slices, p.ldE, (int64_t)nv, c.scal, -1, gb,
                          c.dt, v0);

@@ -120,7 +120,7 @@ struct SmArgs {
   float2* part;              // [N][tiles]
   int tiles;
   float* zt;
-  const float *lse, *loss, *g, *count;
+  const float *m, *rs, *loss, *g, *count;
   int per_row;
   float* coef;               // [2][N], written by the e kernel: does the row have a loss; the gradient that reaches its logits
   float* E;                  // [N][ldE]
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(256) k_head_small_logits(SmArgs a) {
         a.coef[j] = alive;
         a.coef[a.N + j] = c;
       }
-      const float lse = a.lse[j];
+      const float m = a.m[j], cp = c * a.rs[j];
       const int64_t tg = a.target ? a.target[j] : -1;
       const float et = a.target ? c * expm1f(-a.loss[j]) : 0.f;
 #pragma unroll
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256) k_head_small_logits(SmArgs a) {
         for (int r = 0; r < 4; ++r) {
           const int i = ib + x * 16 + r;
           if (i >= a.V) continue;
-          const float p = c * __builtin_amdgcn_exp2f((acc[x][y][r] - lse) * L2E);
+          const float p = cp * __builtin_amdgcn_exp2f((acc[x][y][r] - m) * L2E);
           a.E[(int64_t)j * a.ldE + i] = alive == 0.f ? 0.f : i == tg ? et : p;
         }
     }

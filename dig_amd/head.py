@@ -36,7 +36,7 @@ class _HeadLoss(Function):
             ctx.meta = None
             ctx.save_for_backward(x, w, bias)
             return out.zero_()
-        keep = torch.empty(520 + N * (3 + 2 * (0 if index is None else index.size(1))), **f32)
+        keep = torch.empty(520 + N * (4 + 2 * (0 if index is None else index.size(1))), **f32)
         _call('dig3d_head_fwd', x.get_device(), 0, 0, x, w, bias, target, index, teacher, keep, tau, ignore_index, reduction, out.data_ptr())
         ctx.meta = (tau, ignore_index, reduction)
         ctx.save_for_backward(x, w, bias, target, index, teacher, keep)
@@ -64,7 +64,7 @@ def _check_head(name, x, weight, bias, reduction):
     if reduction not in _REDUCTIONS:
         raise ValueError(f'{name}: reduction is one of {tuple(_REDUCTIONS)}, got {reduction!r}')
     x2 = ops._check_rows(name, x)
-    if not weight.is_cuda or weight.device != x2.device:
+    if weight.get_device() != x2.get_device():
         raise _hip.Dig3dError(f'{name}: weight is on {weight.device}, the rows on {x2.device}')
     if weight.dim() != 2 or weight.size(1) != x2.size(1) or weight.size(0) < 1 or weight.dtype != x2.dtype:
         raise RuntimeError(f'{name}: expected weight [V, {x2.size(1)}] of {x2.dtype} with V >= 1, got {tuple(weight.shape)} {weight.dtype}')
@@ -75,7 +75,7 @@ def _check_head(name, x, weight, bias, reduction):
 
 
 def _check_index(name, what, t, shape, x):
-    if not t.is_cuda or t.device != x.device:
+    if t.get_device() != x.get_device():
         raise _hip.Dig3dError(f'{name}: {what} is on {t.device}, the rows on {x.device}')
     if t.dtype != torch.int64 or tuple(t.shape) != tuple(shape):
         raise RuntimeError(f'{name}: expected {what} {list(shape)} of torch.int64, got {tuple(t.shape)} {t.dtype}')
@@ -113,7 +113,7 @@ def linear_distillation(x, weight, teacher_index, teacher_logits, bias=None, tem
         raise RuntimeError(f'{name}: expected teacher_index [..., K] with 1 <= K <= {_TOP_MAX} for rows {tuple(x.shape)}, got {tuple(teacher_index.shape)}')
     K = teacher_index.size(-1)
     _check_index(name, 'teacher_index', teacher_index, tuple(x.shape[:-1]) + (K,), x2)
-    if teacher_logits.shape != teacher_index.shape or teacher_logits.dtype not in ops._DTYPES or teacher_logits.device != x2.device:
+    if teacher_logits.shape != teacher_index.shape or teacher_logits.dtype not in ops._DTYPES or teacher_logits.get_device() != x2.get_device():
         raise RuntimeError(f'{name}: expected teacher_logits {list(teacher_index.shape)} of float32, bfloat16 or float16 on {x2.device}, got '
                            f'{tuple(teacher_logits.shape)} {teacher_logits.dtype} on {teacher_logits.device}')
     index = teacher_index.reshape(-1, K).contiguous()

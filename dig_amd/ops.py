@@ -2128,11 +2128,13 @@ _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cud
 
 def _on_device(dev, name, *args):
     """The C entry ``name`` on the current stream of device number ``dev``, whatever the current device is."""
-    if _current_device() == dev:
+    if _current_device() == dev and name in _hip._fns:
+        rc = _hip._fns[name](*args, _raw_stream(dev))       # _hip.call without its second argument list
+        if rc == 0:
+            return
+        raise _hip.Dig3dError(f'{name} failed with code {rc}')
+    with torch.cuda.device(dev):
         call(name, *args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            call(name, *args, _raw_stream(dev))
 
 
 def _once(backward):
@@ -2167,7 +2169,7 @@ def _pitch(x):
 
 
 def _check_vector(name, what, p, n, x, dtypes):
-    if not p.is_cuda or p.device != x.device:
+    if p.get_device() != x.get_device():
         raise _hip.Dig3dError(f'{name}: {what} is on {p.device}, the rows on {x.device}')
     if p.dtype not in dtypes or p.dim() != 1 or p.size(0) != n:
         raise RuntimeError(f'{name}: expected {what} [{n}] of {" or ".join(str(d) for d in dtypes)}, got {tuple(p.shape)} {p.dtype}')
