@@ -521,11 +521,24 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
 #include "head_small.h"
 
 // ---- kernels around the products ---------------------------------------------------------------------------------------------------------
-// partial max |v| over the finite entries of x (blocks [0, HD_AMAX)) and W (the rest): amax[2 HD_AMAX]
+// does row n have a loss: its target is not `ignore`, or its teacher lists a class.  Called by whole waves
+__device__ __forceinline__ bool hd_live(int64_t n, const int64_t* target, int64_t ignore, const int64_t* index, const void* tl, int tdt,
+                                        int K, int lane) {
+  if (target) return target[n] != ignore;
+  bool any = false;
+  for (int k = lane; k < K; k += 64) any |= index[n * K + k] >= 0 && load_as(tl, tdt, n * K + k) != -INFINITY;
+  return __any(any);
+}
+
+// partial max |v| over the finite entries of x's rows that have a loss (blocks [0, HD_AMAX); what the others hold, the
+// lowest value of a mask say, must not set the scale) and of W (the rest): amax[2 HD_AMAX]
 #define HD_AMAX 256
 __global__ void __launch_bounds__(256) k_head_amax(const float* __restrict__ x, int64_t ldx, int64_t R, const float* __restrict__ w,
-                                                    int64_t ldw, int64_t V, int D, float* __restrict__ amax) {
+                                                    int64_t ldw, int64_t V, int D, const int64_t* __restrict__ target, int64_t ignore,
+                                                    const int64_t* __restrict__ index, const void* __restrict__ tl, int tdt, int K,
+                                                    float* __restrict__ amax) {
   __shared__ float sh[4];
+  const int lane = threadIdx.x & 63;
   const bool second = blockIdx.x >= HD_AMAX;
   const float* p = second ? w : x;
   const int64_t ld = second ? ldw : ldx, rows = second ? V : R;
@@ -535,20 +548,23 @@ __global__ void __launch_bounds__(256) k_head_amax(const float* __restrict__ x, 
     v = fabsf(v);
     m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
   };
-  if (ld == D && D % 4 == 0 && ((uintptr_t)p & 15) == 0) {
+  if (second && ld == D && D % 4 == 0 && ((uintptr_t)p & 15) == 0) {
     const float4* q = (const float4*)p;
     const int64_t n = rows * D / 4;
+#pragma unroll 4
     for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n; i += HD_AMAX * 256) {
       const float4 v = q[i];
       see(v.x); see(v.y); see(v.z); see(v.w);
     }
   } else {
-    for (int64_t r = b * 4 + (threadIdx.x >> 6); r < rows; r += HD_AMAX * 4)
-      for (int d = threadIdx.x & 63; d < D; d += 64) see(p[r * ld + d]);
+    for (int64_t r = b * 4 + (threadIdx.x >> 6); r < rows; r += HD_AMAX * 4) {
+      if (!second && !hd_live(r, target, ignore, index, tl, tdt, K, lane)) continue;
+      for (int d = lane; d < D; d += 64) see(p[r * ld + d]);
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  if (lane == 0) sh[threadIdx.x >> 6] = m;
   __syncthreads();
   if (threadIdx.x == 0) amax[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
 }
@@ -1190,7 +1206,7 @@ template <class T>
 static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
   if (c.dt == DT_F32) {
     hipLaunchKernelGGL(k_head_amax, dim3(2 * HD_AMAX), dim3(256), 0, c.st, (const float*)c.x, c.ldx, (int64_t)c.N, (const float*)c.w,
-                       c.ldw, (int64_t)c.V, c.D, c.amax);
+                       c.ldw, (int64_t)c.V, c.D, c.target, c.ignore, c.index, c.teacher, c.tdt, c.K, c.amax);
     DIG3D_CHECK_LAUNCH();
   }
   HdArgs a;
