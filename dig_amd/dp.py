@@ -39,6 +39,26 @@ def init_from_env(backend=None):
     return rank(), world_size()
 
 
+def _through_host(t):
+    """gloo moves host memory: its collectives on device tensors have hung where ranks shared a GPU, so a device tensor goes
+    through a host copy there (synchronous both ways).  RCCL takes it as it is."""
+    return t.is_cuda and dist.get_backend() == 'gloo'
+
+
+def _all_reduce_sum(t):
+    h = t.cpu() if _through_host(t) else t
+    dist.all_reduce(h, op=dist.ReduceOp.SUM)
+    if h is not t:
+        t.copy_(h)
+
+
+def _broadcast(t, src):
+    h = t.cpu() if _through_host(t) else t
+    dist.broadcast(h, src)
+    if h is not t:
+        t.copy_(h)
+
+
 class GradBucket:
     """One flat float32 buffer for the single gradient all-reduce of a step.
 
@@ -60,18 +80,26 @@ class GradBucket:
         """all-reduce a gradient buffer that is ALREADY flat and pre-scaled (dig_amd/graphed.py produces it inside
         the HIP graph): the whole data-parallel exchange of a step is this one collective."""
         if is_dist():
-            dist.all_reduce(flat, op=dist.ReduceOp.SUM)
+            _all_reduce_sum(flat)
 
     def allreduce_flat_start(self, flat):
         """the same collective, asynchronous: enqueued behind the work already on the current stream (the replay) and
         running beside whatever the caller enqueues next (the next batch's graph build); ``allreduce_flat_finish`` makes
         the current stream wait for it before the optimizer reads the buffer."""
-        self._work = dist.all_reduce(flat, op=dist.ReduceOp.SUM, async_op=True) if is_dist() else None
+        self._work = self._staged = None
+        if is_dist():
+            h = flat.cpu() if _through_host(flat) else flat
+            self._staged = None if h is flat else (flat, h)
+            self._work = dist.all_reduce(h, op=dist.ReduceOp.SUM, async_op=True)
 
     def allreduce_flat_finish(self):
         work, self._work = getattr(self, '_work', None), None
         if work is not None:
             work.wait()
+            if self._staged is not None:
+                flat, h = self._staged
+                self._staged = None
+                flat.copy_(h)
 
     def allreduce(self, scale=None):
         """sum over ranks of (scale x local gradient).  ``scale`` = B_local / B_global is this rank's share of the
@@ -85,7 +113,7 @@ class GradBucket:
             scale = 1.0 / world_size()
         if scale != 1.0:
             self.flat.mul_(scale)
-        dist.all_reduce(self.flat, op=dist.ReduceOp.SUM)
+        _all_reduce_sum(self.flat)
         off = 0
         for p in self.params:
             p.grad = self.flat[off:off + p.numel()].view_as(p)
@@ -200,18 +228,18 @@ def broadcast_parameters(model, optimizer=None, src=0):
         for group in optimizer.param_groups:
             fl = group.get('_flat')
             if fl is not None:
-                dist.broadcast(fl['param'], src)
+                _broadcast(fl['param'], src)
                 done.update(id(p) for p in fl['ps'])
     for p in model.parameters():
         if id(p) not in done:
-            dist.broadcast(p.data, src)
+            _broadcast(p.data, src)
     for b in model.buffers():
-        dist.broadcast(b.data, src)
+        _broadcast(b.data, src)
 
 
 def allreduce_scalar_sum(x, device):
     if not is_dist():
         return x
     t = torch.tensor([x], dtype=torch.float64, device=device)
-    dist.all_reduce(t, op=dist.ReduceOp.SUM)
+    _all_reduce_sum(t)
     return t.item()
