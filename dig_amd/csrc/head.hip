@@ -112,7 +112,8 @@ __device__ __forceinline__ const char* hd_uniform(const char* p) {
 }
 
 // lane l of load `q` of a wave fetches 16 bytes to LDS offset 1024 q + 16 l of its tile.
-// not TR: LDS row r holds 8 chunks of 8 k; chunk s of it is source chunk s ^ (r & 7) (reads of 16 rows hit all banks)
+// not TR: LDS row r holds 8 chunks of 8 k; chunk s of it is source chunk s ^ f(r), f(r) = (r & 3) | (r >> 3 & 1) << 2: the 16
+//         rows of either kind of read below (hd_frag) spread over the banks
 // TR:     LDS row k holds B / 8 chunks; chunk s of it is source chunk s ^ (2 g(k) mod B / 8), g(k) = (k & 3) | (k >> 3 & 3) << 2
 // The lane's byte offsets from the tile's first element are formed once (32 bits: 256 rows of at most HD_MAX_PITCH elements);
 // a k step moves the uniform base.
@@ -128,7 +129,7 @@ struct HdLoad {
       const int blk = q * NW + wave;
       if constexpr (!TR) {
         const int r = blk * 8 + (lane >> 3);
-        const int ch = (lane & 7) ^ (r & 7);
+        const int ch = (lane & 7) ^ ((r & 3) | (((r >> 3) & 1) << 2));
         off[q] = 2u * ((uint32_t)(min(own0 + r, o.rows - 1) - own0) * (uint32_t)o.ld + ch * 8);
       } else {
         const int k = blk * RPL + lane / CH;
@@ -167,8 +168,8 @@ struct HdLoad {
 template <int B, bool TR>
 __device__ __forceinline__ s16x8 hd_frag(const short* lds, int o0, int kk, int lane) {
   if constexpr (!TR) {
-    const int r = o0 + (lane & 15);
-    return *(const s16x8*)(lds + r * HD_BK + (((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 8));
+    const int r = o0 + (lane & 15), f = (lane & 3) | (((lane >> 3) & 1) << 2);
+    return *(const s16x8*)(lds + r * HD_BK + (((kk * 4 + (lane >> 4)) ^ f) * 8));
   } else {
     constexpr int CH = B / 8;
     const int k = kk * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2);
@@ -180,15 +181,23 @@ __device__ __forceinline__ s16x8 hd_frag(const short* lds, int o0, int kk, int l
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
+// The logits' products take P's rows in another order: operand x of a wave holds rows hd_row(x) + 8 (m >> 2) + (m & 3), m < 16,
+// so that a lane's results of operands 2 t and 2 t + 1 are 8 consecutive classes of one row: e is stored 16 bytes at a time
+__device__ __forceinline__ constexpr int hd_row(int x) { return (x >> 1) * 32 + (x & 1) * 4; }
+__device__ __forceinline__ s16x8 hd_frag_pairs(const short* lds, int o0, int x, int kk, int lane) {
+  const int m = lane & 15, r = o0 + hd_row(x) + 8 * (m >> 2) + (m & 3);
+  return *(const s16x8*)(lds + r * HD_BK + (((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 8));
+}
 
+// n <= 4 consecutive results of a row, from any element address
 template <class T>
 __device__ __forceinline__ void hd_store4(void* out, int64_t at, f32x4 v, int n) {
   T* o = (T*)out + at;
-  if (n == 4 && ((uintptr_t)o & (4 * sizeof(T) - 1)) == 0) {
-    struct alignas(4 * sizeof(T)) { T t[4]; } u;
+  if (n == 4) {
+    RowVec<T, 4> u;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) u.t[r] = to_t<T>(v[r]);
-    *(decltype(u)*)o = u;
+    for (int r = 0; r < 4; ++r) u.v[r] = to_t<T>(v[r]);
+    *(RowVec<T, 4>*)o = u;
   } else {
     for (int r = 0; r < n; ++r) o[r] = to_t<T>(v[r]);
   }
@@ -227,8 +236,12 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
           else if (a.dt == DT_BF16) hd_store4<bf16_t>(a.out, (int64_t)j * a.ldo + i, v, left);
           else hd_store4<f16_t>(a.out, (int64_t)j * a.ldo + i, v, left);
         } else {
-          float* o = a.acc + ((int64_t)blockIdx.z * a.nj + j) * a.ni + i;
-          for (int r = 0; r < left; ++r) o[r] = a.add ? o[r] + v[r] : v[r];
+          const int64_t at = ((int64_t)blockIdx.z * a.nj + j) * a.ni + i;
+          if (a.add) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += r < left ? a.acc[at + r] : 0.f;
+          }
+          hd_store4<float>(a.acc, at, v, left);
         }
       }
     }
@@ -243,7 +256,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
       for (int x = 0; x < MI; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = i0 + wi + x * 16 + q4 + r;
+          const int i = i0 + wi + hd_row(x) + 2 * q4 + r;
           const float b = i < a.ni ? load_as(a.bias, a.dt, a.v0 + i) * a.inv_tau : 0.f;
 #pragma unroll
           for (int y = 0; y < MJ; ++y) acc[x][y][r] = __fmaf_rn(acc[x][y][r], u, b);
@@ -251,7 +264,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
       u = 1.f;
     }
     const bool edge = i0 + BI > a.ni;                            // of the workgroup
-    const int first = i0 + wi + q4, last = a.ni - first;         // this lane's results are classes first + 16 x + r
+    const int first = i0 + wi + 2 * q4, last = a.ni - first;     // this lane's results are classes first + hd_row(x) + r
     auto target_at = [&](int j) -> int {                         // the place of row j's target among them, or -1
       if (!a.target || j >= a.nj) return -1;
       const int64_t t = a.target[j] - a.v0;
@@ -267,7 +280,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
 #pragma unroll
           for (int x = 0; x < MI; ++x)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[x][y][r] = x * 16 + r >= last ? -INFINITY : acc[x][y][r];
+            for (int r = 0; r < 4; ++r) acc[x][y][r] = hd_row(x) + r >= last ? -INFINITY : acc[x][y][r];
         }
         const int tl = target_at(j);
         if (__any(tl >= 0)) {
@@ -276,10 +289,10 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
           for (int x = 0; x < MI; ++x)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              z = tl == x * 16 + r ? acc[x][y][r] : z;
-              acc[x][y][r] = tl == x * 16 + r ? -INFINITY : acc[x][y][r];
+              z = tl == hd_row(x) + r ? acc[x][y][r] : z;
+              acc[x][y][r] = tl == hd_row(x) + r ? -INFINITY : acc[x][y][r];
             }
-          if (tl >= 0 && (tl & 15) < 4) a.zt[j] = z * u;
+          if (tl >= 0 && (tl & 31) < 8) a.zt[j] = z * u;
         }
         float m = -INFINITY, s = 0.f;
 #pragma unroll
@@ -330,27 +343,28 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         if (j >= a.rowsE) continue;
         short* row = a.E + (int64_t)j * a.ldE + first;
 #pragma unroll
-        for (int x = 0; x < MI; ++x) {
-          float e[4];
+        for (int x = 0; x < MI; x += 2) {
+          float e[8];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) e[r] = cp * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x][y][r], u, -m) * L2E);
+          for (int r = 0; r < 8; ++r)
+            e[r] = cp * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x + (r >> 2)][y][r & 3], u, -m) * L2E);
           if (any) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) e[r] = tl == x * 16 + r ? et : e[r];
+            for (int r = 0; r < 8; ++r) e[r] = tl == hd_row(x) + r ? et : e[r];
           }
           if (edge) {
-            if (first + x * 16 >= a.ldE) continue;
+            if (first + hd_row(x) >= a.ldE) continue;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) e[r] = x * 16 + r >= last ? 0.f : e[r];
+            for (int r = 0; r < 8; ++r) e[r] = hd_row(x) + r >= last ? 0.f : e[r];
           }
-          struct alignas(8) { T t[4]; } h, l;
+          struct alignas(16) { T t[8]; } h, l;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) h.t[r] = to_t<T>(e[r]);
-          *(decltype(h)*)(row + x * 16) = h;
+          for (int r = 0; r < 8; ++r) h.t[r] = to_t<T>(e[r]);
+          *(decltype(h)*)(row + hd_row(x)) = h;
           if (a.eplanes > 1) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) l.t[r] = to_t<T>(e[r] - (float)h.t[r]);
-            *(decltype(l)*)(row + a.planeE + x * 16) = l;
+            for (int r = 0; r < 8; ++r) l.t[r] = to_t<T>(e[r] - (float)h.t[r]);
+            *(decltype(l)*)(row + a.planeE + hd_row(x)) = l;
           }
         }
       }
@@ -446,7 +460,10 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
   f32x4 acc[MI][MJ];
   auto read_p = [&](int stage, int ph) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < HX; ++x) fp[ph & 1][x] = hd_frag<BI, PT>(sm + stage * SZ, wi + ((ph & 1) * HX + x) * 16, ph >> 1, lane);
+    for (int x = 0; x < HX; ++x) {
+      if constexpr (EPI == EPI_OUT) fp[ph & 1][x] = hd_frag<BI, PT>(sm + stage * SZ, wi + ((ph & 1) * HX + x) * 16, ph >> 1, lane);
+      else fp[ph & 1][x] = hd_frag_pairs(sm + stage * SZ, wi, (ph & 1) * HX + x, ph >> 1, lane);
+    }
   };
   auto read_q = [&](int stage, int kk) __attribute__((always_inline)) {
 #pragma unroll
@@ -974,10 +991,10 @@ struct HdShape {
 // the product kernel (bf16; us of one k step of 64 with c tiles on a CU, and us of a tile's epilogue that its neighbours do
 // not hide):   64: 0.5 alone, 1.1 with five on the CU;   128: 0.8 alone, 1.2 with two;   256: 1.9 (one to a CU)
 // us with tiles of 64 / 128 / 256:
-//   logits' statistics, 4096 x 2048 x 65536: 1956 / 1075 / 950 (1.16 PFLOP/s; a library's plain product of that shape: 904)
-//   2048 x 256 x 32768: 88 / 55 / 48    64 x 1024 x 16384: 11 / 14 / 31    their gradient e, 4096 x 2048 x 65536: - / 1238 / 1052
-//   e W in ranges, 4096 x 2048 x 65536 (2): 2365 / 1212 / 974    1024 x 128 x 65536 (16): 52 / 59 / 118
-//   e^T x, 4096 x 2048 x 65536: 2683 / 1184 / 983    2048 x 256 x 32768: 59 / 41 / 60    16384 x 128 x 1024 (16): 20 / 24 / 44
+//   logits' statistics, 4096 x 2048 x 65536: 1956 / 1075 / 892 (1.23 PFLOP/s; a library's plain product of that shape: 904)
+//   2048 x 256 x 32768: 88 / 55 / 48    64 x 1024 x 16384: 11 / 14 / 31    their gradient e, 4096 x 2048 x 65536: - / 1238 / 967
+//   e W in ranges, 4096 x 2048 x 65536 (2): 2365 / 1212 / 925 (library: 892)    1024 x 128 x 65536 (16): 52 / 59 / 118
+//   e^T x, 4096 x 2048 x 65536: 2683 / 1184 / 905 (library: 1000)    2048 x 256 x 32768: 59 / 41 / 60
 // A split product writes its partial results and a second launch adds them (bytes at 4 TB/s and 4 us).
 static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) {
   const int cus = dig3d_num_cus();
