@@ -1099,7 +1099,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
   int64_t most = V;
   if (backward) most = min(most, HD_PIECE_BYTES / (p.Np * 2));
   if (!p.dw) most = min(most, HD_PIECE_BYTES / ((int64_t)p.Dp * 2 * p.planes));
-  most = max((int64_t)256, most & ~255ll);
+  if (most < V) most = max((int64_t)256, most & ~255ll);
   p.np = (V + most - 1) / most;
   p.vp = p.np == 1 ? V : ((V + p.np - 1) / p.np + 255) & ~255ll;
   p.np = (V + p.vp - 1) / p.vp;
