@@ -21,7 +21,6 @@
 
 #define HD_BK 64           // the k step of the product kernel
 #define L2E 1.44269504088896340736f
-#define LN2 0.69314718055994530942f
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -250,7 +249,8 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
     // The exponentials take z minus a maximum first and the base-2 factor after it: the difference is exact where
     // it matters.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane
     // are 128 times whatever one costs.
-    float u = a.nseg > 1 ? a.inv_tau / (a.scal[SC_X] * a.scal[SC_W]) : a.inv_tau;
+    float u = a.inv_tau;
+    if (a.nseg > 1) u = fminf(fmaxf(u / (a.scal[SC_X] * a.scal[SC_W]), 1.175494351e-38f), 3.402823466e38f);   // 0 or infinity times what may be either
     if (a.bias) {
 #pragma unroll
       for (int x = 0; x < MI; ++x)
@@ -586,13 +586,12 @@ __global__ void __launch_bounds__(256) k_head_amax(const float* __restrict__ x, 
   if (threadIdx.x == 0) amax[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
 }
 
-// 2^k with 2^k m in [2^14, 2^15); 1 for an all-zero tensor.  k is kept in the range where 2^k and 2^-k are normal.
+// 2^k with 2^k m in [2^14, 2^15); 1 for an all-zero tensor.  -113 <= k <= 100: 2^k and 2^-k are normal numbers.
 __device__ __forceinline__ float hd_scale(float m) {
   if (!(m > 0.f)) return 1.f;
   int e;
   frexpf(m, &e);
-  const int k = min(max(15 - e, -100), 100);
-  return ldexpf(1.f, k);
+  return ldexpf(1.f, min(15 - e, 100));
 }
 
 // out [planes][orows][ocols] <- rows [0, R) of src (type dt, pitch ld, D columns), zeros elsewhere; `coef`: a row with
@@ -664,7 +663,7 @@ __device__ __forceinline__ float hd_wave_sum(float v) {
 
 // the tiles' statistics of one row joined by a wave (result in lane 0): softmax = exp(z - mo) rs, the maximum and the sum
 // apart (their lse, rounded at its own size, would shift every probability of the row); with a target the row's loss, 0
-// where it is `ignore`, NaN where it is no class
+// where it is `ignore`, NaN where it is no class or where no class has a finite logit
 __device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int tiles, int64_t V, bool with_target, int64_t tg,
                                             int64_t ignore, const float* zt, int lane, float& mo, float& rs, float& loss) {
   float m = -INFINITY, s = 0.f;
@@ -694,6 +693,7 @@ __device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int ti
   mo = M;
   rs = 1.f / (so + st);
   loss = z >= m ? log1pf(so) : (Ms - z) + logf(so + st);
+  if (!(so + st > 0.f)) loss = NAN;        // no class is left, or one is infinite: 0 / 0 and infinity / infinity
 }
 
 // a wave per row
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ pa
 }
 
 // out = sum or mean of the rows' losses, count = how many rows have one (at least 1): a fixed tree of additions over the
-// 1024 threads of one workgroup
+// 1024 threads of a workgroup
 __device__ __forceinline__ void hd_total(float s, float c, int mean, float* out, float* count, float* sh) {
   s = hd_wave_sum(s);
   c = hd_wave_sum(c);
@@ -733,21 +733,29 @@ __device__ __forceinline__ void hd_total(float s, float c, int mean, float* out,
       s += sh[w];
       c += sh[16 + w];
     }
+    if (!count) {                          // one of several partial sums
+      out[0] = s;
+      out[1] = c;
+      return;
+    }
     c = fmaxf(c, 1.f);
     *out = mean ? s / c : s;
     *count = c;
   }
 }
+// HD_TOTAL rows a workgroup; with more than one of them the sums (mid) are joined by a launch more.  `pairs`: N of those sums
+#define HD_TOTAL 8192
 __global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ loss, const int64_t* __restrict__ target,
-                                                      int64_t ignore, const float* __restrict__ live, int N, int mean,
-                                                      float* __restrict__ out, float* __restrict__ count) {
+                                                      int64_t ignore, const float* __restrict__ live, const float2* __restrict__ pairs,
+                                                      int N, int mean, float* __restrict__ out, float* __restrict__ count) {
   __shared__ float sh[32];
   float s = 0.f, c = 0.f;
-  for (int n = threadIdx.x; n < N; n += 1024) {
-    s += loss[n];
-    c += target ? (target[n] != ignore ? 1.f : 0.f) : live[n];
+  const int end = min(N, (int)(blockIdx.x + 1) * HD_TOTAL);
+  for (int n = blockIdx.x * HD_TOTAL + threadIdx.x; n < end; n += 1024) {
+    s += pairs ? pairs[n].x : loss[n];
+    c += pairs ? pairs[n].y : target ? (target[n] != ignore ? 1.f : 0.f) : live[n];
   }
-  hd_total(s, c, mean, out, count, sh);
+  hd_total(s, c, mean, out + (count ? 0 : 2 * blockIdx.x), count, sh);
 }
 // few rows: the join and the total in one workgroup
 __global__ void __launch_bounds__(1024) k_head_join_total(const float2* __restrict__ part, int tiles, int N, int64_t V,
@@ -777,7 +785,8 @@ __global__ void __launch_bounds__(1024) k_head_join_total(const float2* __restri
 
 // teacher: a workgroup per row.  q [N, K]: the softmax over the row's listed classes of t / tau, summed over the entries of
 // the same class, -1 for an absent entry (negative index, or logit -inf); z [N, K]: the student's own logits / tau there;
-// loss[n]; live[n] = 1, 0 without entries, NaN with an index that is no class.  A wave forms four logits at a time: the
+// loss[n]; live[n] = 1, 0 without entries, NaN with an index that is no class.  (t - max) / tau is kept finite, so that a
+// listed logit of the type's lowest value is not an absent entry at any tau.  A wave forms four logits at a time: the
 // row of x and four rows of W in 16-byte pieces (N K D elements of W are gathered: bound by the caches).
 template <class T>
 __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, const T* __restrict__ w, const void* __restrict__ bias,
@@ -787,7 +796,7 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
                                                        float* __restrict__ q, float* __restrict__ z, float* __restrict__ loss, float* __restrict__ live,
                                                        float* __restrict__ rows_out) {
   constexpr int N8 = VecLen<T>::n;
-  extern __shared__ int64_t dyn[];         // index [K], then t / tau [K], then q [K]
+  extern __shared__ int64_t dyn[];         // index [K] (-1: absent), then t, then (t - max) / tau [K], then q [K]
   float* st = (float*)(dyn + K);
   float* sq = st + K;
   __shared__ float sh[8];
@@ -796,8 +805,8 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
   float m = -INFINITY;
   for (int k = tid; k < K; k += 256) {
     const int64_t v = index[n * K + k];
-    const float t = v < 0 ? -INFINITY : load_as(tl, tdt, n * K + k) * inv_tau;
-    dyn[k] = v;
+    const float t = v < 0 ? -INFINITY : load_as(tl, tdt, n * K + k);
+    dyn[k] = t == -INFINITY ? -1 : v;
     st[k] = t;
     m = fmaxf(m, t);
   }
@@ -808,7 +817,12 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
   m = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
   const float ms = m == -INFINITY ? 0.f : m;
   float s = 0.f;
-  for (int k = tid; k < K; k += 256) s += expf(st[k] - ms);
+  for (int k = tid; k < K; k += 256) {
+    float d = (st[k] - ms) * inv_tau;
+    d = d < -3.402823466e38f ? -3.402823466e38f : d;             // a NaN stays one
+    st[k] = d;
+    if (dyn[k] >= 0) s += expf(d);
+  }
   s = hd_wave_sum(s);
   if (lane == 0) sh[4 + wave] = s;
   __syncthreads();
@@ -816,7 +830,7 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
   const bool any = s > 0.f || s != s;      // a NaN among the listed logits is not an empty row
   const float ls = any ? logf(s) : 0.f;
   const float sm = mo[n], sl = logf(rs[n]);   // the student's log softmax is z - sm + sl
-  for (int k = tid; k < K; k += 256) sq[k] = st[k] == -INFINITY ? 0.f : expf(st[k] - ms - ls);
+  for (int k = tid; k < K; k += 256) sq[k] = dyn[k] < 0 ? 0.f : expf(st[k] - ls);
   __syncthreads();
   const T* xr = x + n * ldx;
   float part = 0.f;
@@ -850,11 +864,10 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
       const int k = k0 + e;
       if (lane != 0 || k >= K) continue;
       const int64_t v = dyn[k];
-      const float t = st[k];
       float zk = 0.f;
-      if (any && t != -INFINITY) {
+      if (any && v >= 0) {
         zk = v < V ? (bias ? dot + load_as(bias, dt, v) : dot) * inv_tau : NAN;     // no such class: the row says so
-        part += sq[k] * (t - ms - ls - (zk - sm + sl));
+        if (sq[k] != 0.f || v >= V) part += sq[k] * (st[k] - ls - (zk - sm + sl));   // 0 log 0 = 0, also where p is 0
       }
       z[n * K + k] = zk;
     }
@@ -864,7 +877,7 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
     float sum = 0.f;
     const int64_t v = dyn[k];
     for (int e = 0; e < K; ++e) sum += dyn[e] == v ? sq[e] : 0.f;
-    q[n * K + k] = st[k] == -INFINITY ? -1.f : sum;
+    q[n * K + k] = v < 0 ? -1.f : sum;
   }
   __syncthreads();
   if (tid == 0) {
@@ -875,28 +888,49 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
   }
 }
 
+__device__ __forceinline__ bool hd_has(int n, const int64_t* target, int64_t ignore, const float* live) {
+  return target ? target[n] != ignore : live[n] != 0.f;
+}
+__device__ __forceinline__ float hd_finite_max(float m, float v) {
+  v = fabsf(v);
+  return v <= 3.402823466e38f ? fmaxf(m, v) : m;
+}
+// the maximum over a workgroup of 1024, in every thread
+__device__ __forceinline__ float hd_block_max(float m, float* sh) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) m = fmaxf(m, sh[w]);
+  return m;
+}
+// gm[block] = the largest finite |g f| of HD_TOTAL rows' losses
+__global__ void __launch_bounds__(1024) k_head_gmax(const float* __restrict__ g, float f, const int64_t* __restrict__ target,
+                                                     int64_t ignore, const float* __restrict__ live, int N, float* __restrict__ gm) {
+  __shared__ float sh[16];
+  float m = 0.f;
+  const int end = min(N, (int)(blockIdx.x + 1) * HD_TOTAL);
+  for (int n = blockIdx.x * HD_TOTAL + threadIdx.x; n < end; n += 1024)
+    if (hd_has(n, target, ignore, live)) m = hd_finite_max(m, g[n] * f);
+  m = hd_block_max(m, sh);
+  if (threadIdx.x == 0) gm[blockIdx.x] = m;
+}
+
 // coef[n] (|.| <= 1, 0 for a row without a loss) and the scalar S with coef[n] S = the gradient of row n's logits' loss:
-// reductions: coef = 1 or 0, S = g f / count;  none: S = a power of two over max |g f|.  f: tau for the teacher's loss.
-__global__ void __launch_bounds__(1024) k_head_coef(const float* __restrict__ g, int per_row, const float* __restrict__ count,
-                                                     float f, const int64_t* __restrict__ target, int64_t ignore,
-                                                     const float* __restrict__ live, int N, float* __restrict__ coef,
-                                                     float* __restrict__ scal) {
+// reductions: coef = 1 or 0, S = g f / count;  none: S = a power of two over max |g f| = max gm.  f: tau for the teacher's loss.
+// HD_TOTAL rows a workgroup.
+__global__ void __launch_bounds__(1024) k_head_coef(const float* __restrict__ g, const float* __restrict__ gm, int ngm,
+                                                     const float* __restrict__ count, float f, const int64_t* __restrict__ target,
+                                                     int64_t ignore, const float* __restrict__ live, int N,
+                                                     float* __restrict__ coef, float* __restrict__ scal) {
   __shared__ float sh[16];
   float S = 1.f;
-  auto has = [&](int n) { return target ? target[n] != ignore : live[n] != 0.f; };
-  if (per_row) {
+  if (gm) {
     float m = 0.f;
-    for (int n = threadIdx.x; n < N; n += 1024)
-      if (has(n)) {
-        const float v = fabsf(g[n] * f);
-        m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
-      }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = 0.f;
-    for (int w = 0; w < 16; ++w) m = fmaxf(m, sh[w]);
+    for (int i = threadIdx.x; i < ngm; i += 1024) m = fmaxf(m, gm[i]);
+    m = hd_block_max(m, sh);
     if (m > 0.f) {
       int e;
       frexpf(m, &e);
@@ -906,8 +940,10 @@ __global__ void __launch_bounds__(1024) k_head_coef(const float* __restrict__ g,
     S = g[0] * f / (count ? *count : 1.f);
   }
   // live is NaN for a row that lists a class that does not exist: its gradient says so too
-  for (int n = threadIdx.x; n < N; n += 1024) coef[n] = has(n) ? (per_row ? g[n] * f / S : 1.f) * (live ? live[n] : 1.f) : 0.f;
-  if (threadIdx.x == 0) scal[SC_S] = S;
+  const int end = min(N, (int)(blockIdx.x + 1) * HD_TOTAL);
+  for (int n = blockIdx.x * HD_TOTAL + threadIdx.x; n < end; n += 1024)
+    coef[n] = hd_has(n, target, ignore, live) ? (gm ? g[n] * f / S : 1.f) * (live ? live[n] : 1.f) : 0.f;
+  if (blockIdx.x == 0 && threadIdx.x == 0) scal[SC_S] = S;
 }
 
 // teacher: the listed classes of this piece get e = c (softmax_k - q_k), from the entry's own logit, over what the
@@ -943,10 +979,10 @@ __global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E
                                                       float* __restrict__ part) {
   __shared__ float sh[8][32 * 8 + 4];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 256 + cl * 8;
+  const int64_t c = (int64_t)blockIdx.y * 256 + cl * 8;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (c < ldE) {                           // a multiple of 64: a lane's 8 columns are all there
-    const int r0 = blockIdx.y * HD_SLICE, r1 = min(rows, r0 + HD_SLICE);
+    const int r0 = blockIdx.x * HD_SLICE, r1 = min(rows, r0 + HD_SLICE);
     for (int p = 0; p < planes; ++p) {
 #pragma unroll 4
       for (int r = r0 + rl; r < r1; r += 8) {
@@ -959,12 +995,12 @@ __global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E
 #pragma unroll
   for (int i = 0; i < 8; ++i) sh[rl][cl * 8 + i] = s[i];
   __syncthreads();
-  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t o = (int64_t)blockIdx.y * 256 + threadIdx.x;
   if (o < ldE) {
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) v += sh[q][threadIdx.x];
-    part[(int64_t)blockIdx.y * ldE + o] = v;
+    part[(int64_t)blockIdx.x * ldE + o] = v;
   }
 }
 
@@ -1033,7 +1069,7 @@ struct HdPlan {
   HdShape lg, gx, gw;
   int tiles_all;
   // byte offsets into the workspace
-  int64_t o_x, o_w, o_part, o_zt, o_coef, o_E, o_gx, o_gw, o_col, total;
+  int64_t o_x, o_w, o_part, o_zt, o_coef, o_scal, o_E, o_gx, o_gw, o_col, total;
 };
 
 // 16-bit rows are used in place when their pitch keeps 16-byte loads aligned and D is whole k steps
@@ -1115,6 +1151,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     p.o_zt = take(N * 4);
   } else {
     p.o_coef = take(N * 4);
+    p.o_scal = take(SC_COUNT * 4 + (N + HD_TOTAL - 1) / HD_TOTAL * 4);
     p.o_E = take(p.Np * p.ldE * 2 * p.eplanes);
     if (needs & 1) {
       p.gx = hd_shape(D, N, p.ldE / HD_BK * p.nseg, 64);
@@ -1156,9 +1193,9 @@ static void hd_pack(const void* src, int dt, int64_t ld, int64_t R, int D, const
 }
 
 static bool hd_bad(int dt, int N, int D, int V, int64_t ldx, int64_t ldw) {
-  // tile counts and row offsets of the small index type stay far inside 32 bits
+  // tile counts and the launches' threads (256 a row) stay inside 32 bits
   return dt < 0 || dt > 2 || N <= 0 || D <= 0 || V <= 0 || ldx < D || ldw < D ||
-         ((int64_t)N + 63) / 64 * (((int64_t)V + 63) / 64) > (1ll << 30) || N > (1 << 28) || V > (1 << 28) || D > (1 << 20);
+         ((int64_t)N + 63) / 64 * (((int64_t)V + 63) / 64) > (1ll << 30) || N >= (1 << 24) || V > (1 << 28) || D > (1 << 20);
 }
 
 static const short* at_bytes(const void* p, int64_t o) { return (const short*)((const char*)p + o); }
@@ -1303,9 +1340,16 @@ static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
     DIG3D_CHECK_LAUNCH();
   }
   if (c.reduction) {
-    hipLaunchKernelGGL(k_head_total, dim3(1), dim3(1024), 0, c.st, c.loss, c.target, c.ignore, c.live, c.N, c.reduction == 1, out,
-                       c.count);
+    const int blocks = (c.N + HD_TOTAL - 1) / HD_TOTAL;
+    float* mid = (float*)part;             // the tiles' statistics have been joined
+    hipLaunchKernelGGL(k_head_total, dim3(blocks), dim3(1024), 0, c.st, c.loss, c.target, c.ignore, c.live, (const float2*)nullptr, c.N,
+                       c.reduction == 1, blocks > 1 ? mid : out, blocks > 1 ? (float*)nullptr : c.count);
     DIG3D_CHECK_LAUNCH();
+    if (blocks > 1) {
+      hipLaunchKernelGGL(k_head_total, dim3(1), dim3(1024), 0, c.st, (const float*)nullptr, (const int64_t*)nullptr, (int64_t)0,
+                         (const float*)nullptr, (const float2*)mid, blocks, c.reduction == 1, out, c.count);
+      DIG3D_CHECK_LAUNCH();
+    }
   }
   return DIG3D_OK;
 }
@@ -1352,10 +1396,18 @@ static int hd_bwd_small(const HdCall& c, const HdPlan& p, const float* g, void* 
 }
 
 template <class T>
-static int hd_bwd(const HdCall& c, const HdPlan& p, const float* g, void* gx, void* gw, void* gb, char* ws) {
+static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw, void* gb, char* ws) {
+  c.scal = (float*)(ws + p.o_scal);        // what the forward kept is read only: several backward passes may use it
   float* coef = (float*)(ws + p.o_coef);
-  hipLaunchKernelGGL(k_head_coef, dim3(1), dim3(1024), 0, c.st, g, c.reduction == 0, c.reduction == 1 ? c.count : (const float*)nullptr,
-                     c.index ? c.tau : 1.f, c.target, c.ignore, c.index ? c.live : (const float*)nullptr, c.N, coef, c.scal);
+  const int blocks = (c.N + HD_TOTAL - 1) / HD_TOTAL;
+  const float f = c.index ? c.tau : 1.f, *live = c.index ? c.live : nullptr;
+  float* gm = c.reduction == 0 ? (float*)(ws + p.o_scal) + SC_COUNT : nullptr;
+  if (gm) {
+    hipLaunchKernelGGL(k_head_gmax, dim3(blocks), dim3(1024), 0, c.st, g, f, c.target, c.ignore, live, c.N, gm);
+    DIG3D_CHECK_LAUNCH();
+  }
+  hipLaunchKernelGGL(k_head_coef, dim3(blocks), dim3(1024), 0, c.st, g, gm, blocks, c.reduction == 1 ? c.count : (const float*)nullptr,
+                     f, c.target, c.ignore, live, c.N, coef, c.scal);
   DIG3D_CHECK_LAUNCH();
   const int64_t xplane = p.Np * p.Dp;
   const bool planes2 = p.planes == 2;
@@ -1449,7 +1501,7 @@ static int hd_bwd(const HdCall& c, const HdPlan& p, const float* g, void* gx, vo
     if (gb) {
       float* part = (float*)(ws + p.o_col);
       const int slices = (c.N + HD_SLICE - 1) / HD_SLICE;
-      hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)((p.ldE + 255) / 256), (unsigned)slices), dim3(256), 0, c.st, E, p.ldE,
+      hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)slices, (unsigned)((p.ldE + 255) / 256)), dim3(256), 0, c.st, E, p.ldE,
                          eplane, p.eplanes, c.N, part);
       DIG3D_CHECK_LAUNCH();
       hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(nv, 256)), dim3(256), 0, c.st, part, slices, p.ldE, (int64_t)nv, c.scal, -1, gb,
@@ -1472,7 +1524,7 @@ static bool hd_call(HdCall& c, int dtype, const void* x, int64_t ldx, const void
                     int N, int D, int V, int reduction, float* keep, void* stream) {
   if (hd_bad(dtype, N, D, V, ldx, ldw) || !x || !w || !keep || reduction < 0 || reduction > 2 || !(tau > 0.f)) return false;
   if ((!target) == (!index) || (target && (K != 0 || tau != 1.f))) return false;
-  if (index && (!teacher || tdtype < 0 || tdtype > 2 || K <= 0 || K > TC_MAX)) return false;
+  if (index && (!teacher || tdtype < 0 || tdtype > 2 || K <= 0 || K > TC_MAX || (int64_t)N * K > (1ll << 31))) return false;
   c = {dtype, x, w, bias, ldx, ldw, N, D, V, target, ignore, index, teacher, tdtype, K, tau, reduction};
   c.st = (hipStream_t)stream;
   hd_keep(c, keep);
@@ -1503,10 +1555,11 @@ int dig3d_head_fwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t
 
 int dig3d_head_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const int64_t* target,
                    int64_t ignore_index, const int64_t* index, const void* teacher, int tdtype, int K, float tau, int N, int D, int V,
-                   int reduction, float* keep, const float* g, void* gx, void* gw, void* gb, void* ws, int ws_kib, void* stream) {
+                   int reduction, const float* keep, const float* g, void* gx, void* gw, void* gb, void* ws, int ws_kib, void* stream) {
   DIG3D_ENTER();
   HdCall c;
-  if (!hd_call(c, dtype, x, ldx, w, ldw, bias, target, ignore_index, index, teacher, tdtype, K, tau, N, D, V, reduction, keep, stream) || !g)
+  if (!hd_call(c, dtype, x, ldx, w, ldw, bias, target, ignore_index, index, teacher, tdtype, K, tau, N, D, V, reduction,
+               const_cast<float*>(keep), stream) || !g)
     return DIG3D_ERR_ARG;
   const int needs = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
   if (!needs) return DIG3D_OK;

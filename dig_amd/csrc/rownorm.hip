@@ -418,7 +418,7 @@ static void rn_bwd(const void* gy, const void* x, int64_t ldx, int R, int C, con
 extern "C" {
 
 int dig3d_rownorm_bwd_blocks(int R, int C, int dtype) {
-  if (R <= 0 || C <= 0 || dtype < 0 || dtype > 2) return 0;
+  if (R <= 0 || C <= 0 || C >= (1 << 25) || dtype < 0 || dtype > 2) return 0;
   int tpr, nv;
   rn_pick(C, dtype == DT_F32 ? 4 : 8, tpr, nv);
   const int64_t per = rn_groups_per_block(tpr);
@@ -430,7 +430,7 @@ int dig3d_rownorm_bwd_blocks(int R, int C, int dtype) {
 int dig3d_rownorm_fwd(int dtype, const void* x, int64_t ldx, int R, int C, const void* w, const void* b, int wdtype, float eps,
                       void* y, float* mean, float* rstd, void* stream) {
   DIG3D_ENTER();
-  if (R < 0 || C <= 0 || ldx < C || dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2) return DIG3D_ERR_ARG;
+  if (R < 0 || C <= 0 || C >= (1 << 25) || ldx < C || dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2) return DIG3D_ERR_ARG;
   if (R == 0) return DIG3D_OK;
   if (!x || !y || (!mean) != (!rstd)) return DIG3D_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;
@@ -444,7 +444,7 @@ int dig3d_rownorm_fwd(int dtype, const void* x, int64_t ldx, int R, int C, const
 int dig3d_rownorm_bwd(int dtype, const void* gy, const void* x, int64_t ldx, int R, int C, const void* w, int wdtype,
                       const float* mean, const float* rstd, void* gx, float* part, int nb, void* gw, void* gb, void* stream) {
   DIG3D_ENTER();
-  if (R <= 0 || C <= 0 || ldx < C || dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2) return DIG3D_ERR_ARG;
+  if (R <= 0 || C <= 0 || C >= (1 << 25) || ldx < C || dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2) return DIG3D_ERR_ARG;
   if (!gy || !x || !mean || !rstd || nb != dig3d_rownorm_bwd_blocks(R, C, dtype) || ((gw || gb) && !part))
     return DIG3D_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;

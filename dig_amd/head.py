@@ -17,7 +17,7 @@ def _call(name, dev, backward, needs, x, w, bias, target, index, teacher, keep, 
     operands = (dt, x.data_ptr(), ops._pitch(x), w.data_ptr(), ops._pitch(w))
     kib = _hip.query('dig3d_head_ws_kib', *operands, N, D, V, backward, needs)
     if kib < 0:
-        raise _hip.Dig3dError(f'class head of {N} rows x {D} x {V} classes is beyond the supported sizes')
+        raise _hip.Dig3dError(f'class head of {N} rows x {D} x {V} classes is beyond the supported sizes (2^24 rows, 2^20 channels, 2^28 classes)')
     ws = torch.empty(max(kib, 1) * 1024, dtype=torch.uint8, device=x.device)
     K, tdt = (0, 0) if index is None else (index.size(1), ops._DTYPES[teacher.dtype])
     ops._on_device(dev, name, *operands, ptr(bias), ptr(target), ignore_index, ptr(index), ptr(teacher), tdt, K, tau, N, D, V, reduction,
@@ -93,7 +93,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     x2, weight, bias = _check_head('linear_cross_entropy', x, weight, bias, reduction)
     _check_index('linear_cross_entropy', 'target', target, x.shape[:-1], x2)
     loss = _HeadLoss.apply(x2, weight, bias, target.reshape(-1).contiguous(), None, None, 1.0, int(ignore_index), _REDUCTIONS[reduction])
-    return loss.reshape(target.shape) if reduction == 'none' else loss
+    return loss if reduction != 'none' or x.dim() == 2 else loss.reshape(target.shape)
 
 
 def linear_distillation(x, weight, teacher_index, teacher_logits, bias=None, temperature=1.0, reduction='mean'):
@@ -107,11 +107,13 @@ def linear_distillation(x, weight, teacher_index, teacher_logits, bias=None, tem
     gradient.  Types, reductions and gradients as ``linear_cross_entropy``; teacher_logits float32, bfloat16 or float16."""
     name = 'linear_distillation'
     x2, weight, bias = _check_head(name, x, weight, bias, reduction)
-    if not (isinstance(temperature, (int, float)) and 0.0 < float(temperature) < float('inf')):
-        raise ValueError(f'{name}: temperature is a positive number, got {temperature!r}')
+    if not (isinstance(temperature, (int, float)) and 1e-6 <= float(temperature) <= 1e6):
+        raise ValueError(f'{name}: temperature is a number from 1e-6 to 1e6, got {temperature!r}')
     if teacher_index.dim() != x.dim() or not 1 <= teacher_index.size(-1) <= _TOP_MAX:
         raise RuntimeError(f'{name}: expected teacher_index [..., K] with 1 <= K <= {_TOP_MAX} for rows {tuple(x.shape)}, got {tuple(teacher_index.shape)}')
     K = teacher_index.size(-1)
+    if x2.size(0) * K > 1 << 31:
+        raise RuntimeError(f'{name}: {x2.size(0)} rows of {K} entries are beyond 2^31 entries in one call')
     _check_index(name, 'teacher_index', teacher_index, tuple(x.shape[:-1]) + (K,), x2)
     if teacher_logits.shape != teacher_index.shape or teacher_logits.dtype not in ops._DTYPES or teacher_logits.get_device() != x2.get_device():
         raise RuntimeError(f'{name}: expected teacher_logits {list(teacher_index.shape)} of float32, bfloat16 or float16 on {x2.device}, got '
@@ -119,4 +121,4 @@ def linear_distillation(x, weight, teacher_index, teacher_logits, bias=None, tem
     index = teacher_index.reshape(-1, K).contiguous()
     teacher = teacher_logits.detach().reshape(-1, K).contiguous()
     loss = _HeadLoss.apply(x2, weight, bias, None, index, teacher, float(temperature), 0, _REDUCTIONS[reduction])
-    return loss.reshape(x.shape[:-1]) if reduction == 'none' else loss
+    return loss if reduction != 'none' or x.dim() == 2 else loss.reshape(x.shape[:-1])

@@ -2123,7 +2123,8 @@ def graph_norm(x, weight, bias, mean_scale, gptr, B, eps=1e-5, padded=False):
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # csrc/half16.h
 
 
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+# (a torch without devices has neither; the ops refuse its tensors before they ask)
+_raw_stream, _current_device = getattr(torch._C, '_cuda_getCurrentRawStream', None), getattr(torch._C, '_cuda_getDevice', None)
 
 
 def _on_device(dev, name, *args):
@@ -2237,8 +2238,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         weight = _check_vector('layer_norm', 'weight', weight, C, x2, (x2.dtype, torch.float32))
     if bias is not None:
         bias = _check_vector('layer_norm', 'bias', bias, C, x2, (x2.dtype, torch.float32) if weight is None else (weight.dtype,))
-    if x2.size(0) >= 1 << 31 or C >= 1 << 30:
-        raise RuntimeError(f'layer_norm: {tuple(x.shape)} is beyond 2^31 rows or 2^30 channels')
+    if x2.size(0) >= 1 << 31 or C >= 1 << 25:
+        raise RuntimeError(f'layer_norm: {tuple(x.shape)} is beyond 2^31 rows or 2^25 channels')
     y = _LayerNorm.apply(x2, weight, bias, float(eps))
     return y if x.dim() == 2 else y.reshape(x.shape)
 

@@ -758,3 +758,88 @@ def test_refusals_on_the_device():
     with pytest.raises(RuntimeError):
         torch.autograd.grad(gx.sum(), xr)
     assert issubclass(_hip.Dig3dError, RuntimeError)
+
+
+# ------------------------------------------------------------------------------------------------ the ends of the ranges
+@pytest.mark.parametrize('N,V', [(40, 300), (600, 900)])
+def test_tensors_whose_product_is_below_the_types_range(N, V):
+    """x and w of 1e-25: every logit is 0 in float32, the loss log V to the rounding of a sum and a logarithm; the gradients
+    are those of softmax = 1 / V (e off by 8 u and its two halves, the operands by 2^-22 and 2^-39 of the largest)"""
+    from dig_amd import ops
+    g = gen(80)
+    x, w = (randn(g, N, 64) * 1e-25).requires_grad_(), (randn(g, V, 64) * 1e-25).requires_grad_()
+    target = torch.randint(0, V, (N,), device=DEV, generator=g)
+    rows = ops.linear_cross_entropy(x, w, target, reduction='none')
+    close(rows, torch.full((N,), math.log(V), dtype=torch.float64, device=DEV), 64 * U * math.log(V), 'rows')
+    gx, gw = torch.autograd.grad(rows.sum(), (x, w))
+    e = torch.full((N, V), 1.0 / V, dtype=torch.float64, device=DEV)
+    e[torch.arange(N, device=DEV), target] -= 1.0
+    xd, wd = x.detach().double(), w.detach().double()
+    for got, want, size, n, top in ((gx, e @ wd, e.abs() @ wd.abs(), V, wd.abs().max()), (gw, e.t() @ xd, e.abs().t() @ xd.abs(), N, xd.abs().max())):
+        close(got, want, ((3 * n + 80) * U + 6 * 2.0 ** -22) * size + 2.0 ** -38 * n * top, 'gradient')
+
+
+@pytest.mark.parametrize('N,V', [(40, 300), (600, 900)])
+@pytest.mark.parametrize('t', list(TYPES))
+def test_no_class_left_and_infinite_logits_are_nan(N, V, t):
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, 64, V, TYPES[t], True, 81)
+    none = torch.full_like(b, float('-inf')).requires_grad_()
+    rows = ops.linear_cross_entropy(x, w, target, none, reduction='none')
+    assert torch.isnan(rows).all() and torch.isnan(torch.autograd.grad(rows.sum(), x)[0]).all()
+    for v in (0, int(target[0])):                  # beside a row's target, and as one
+        up = b.detach().clone()
+        up[v] = float('inf')
+        assert torch.isnan(ops.linear_cross_entropy(x, w, target, up, reduction='none')).all()
+
+
+def test_listed_logits_of_the_lowest_value_stay_entries():
+    """at tau = 1/2 the lowest value over tau is beyond the type; alone in a row such entries share it equally, beside others
+    they hold nothing, also where the head itself gives their class nothing"""
+    from dig_amd import ops
+    x, w, b, index, teacher, g = teacher_case(20, 64, 50, 4, torch.float32, True, 82, False)
+    index[0] = torch.tensor([3, 9, 11, 40], device=DEV)
+    index[1] = index[0]
+    low, even = teacher.clone(), teacher.clone()
+    low[0], even[0] = torch.finfo(torch.float32).min, 0.0
+    low[1, 3] = torch.finfo(torch.float32).min
+    even[1, 3] = float('-inf')
+    a = ops.linear_distillation(x, w, index, low, b, temperature=0.5, reduction='none')
+    c = ops.linear_distillation(x, w, index, even, b, temperature=0.5, reduction='none')
+    assert torch.equal(a, c) and torch.isfinite(a).all()
+    bd = b.detach().clone()
+    bd[40] = float('-inf')
+    a = ops.linear_distillation(x[1:2], w, index[1:2], low[1:2], bd, temperature=0.5, reduction='none')
+    q = torch.softmax(teacher[1, :3].double() / 0.5, 0)
+    lp = torch.log_softmax(head64(x.detach()[1:2], w.detach(), bd, 0.5), 1)[0]
+    want = 0.25 * (q * (q.log() - lp[index[1, :3]])).sum()
+    assert abs(float(a[0]) - float(want)) <= 2000 * U * (1 + abs(float(want)) + 20)
+
+
+@pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
+@pytest.mark.parametrize('t', ['f32', 'bf16'])
+def test_more_rows_than_one_workgroup_adds(t, reduction):
+    one_classes(20000, 24, 40, TYPES[t], True, reduction, 0.2)
+
+
+@pytest.mark.parametrize('N,D,V', [(40, 64, 300), (600, 128, 2000)])
+def test_a_backward_leaves_what_the_forward_kept(N, D, V):
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, torch.float32, True, 83)
+    rows = ops.linear_cross_entropy(x, w, target, b, reduction='none')
+    keep = [p for p in rows.grad_fn.saved_tensors if p is not None]
+    before = [p.clone().view(torch.uint8) for p in keep]
+    a = torch.autograd.grad(rows, (x, w, b), torch.full((N,), 3.0, device=DEV), retain_graph=True)
+    torch.autograd.grad(rows, (x, w, b), torch.full((N,), 1e-3, device=DEV), retain_graph=True)
+    assert all(torch.equal(p, q.view(torch.uint8)) for p, q in zip(before, keep))
+    c = torch.autograd.grad(rows, (x, w, b), torch.full((N,), 3.0, device=DEV))
+    assert all(torch.equal(p, q) for p, q in zip(a, c))
+
+
+def test_temperatures_out_of_range_are_refused():
+    from dig_amd import ops
+    x, w = torch.randn(4, 64, device=DEV), torch.randn(10, 64, device=DEV)
+    idx, tl = torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.zeros(4, 2, device=DEV)
+    for tau in (1e-7, 1e7, -1.0, float('inf')):
+        with pytest.raises(ValueError):
+            ops.linear_distillation(x, w, idx, tl, temperature=tau)

@@ -22,6 +22,7 @@ def test_row_norm_partials():
     assert q(608, 128, 0) == 76                    # 32 lanes a row, 8 rows a workgroup
     assert q(608, 128, 1) == 38                    # 16 lanes a row
     assert 1 <= q(10 ** 6, 1024, 1) <= 4096
+    assert q(5, 1 << 25, 0) == 0 and q(5, (1 << 25) - 1, 0) >= 1
 
 
 def test_head_workspace():
@@ -31,6 +32,9 @@ def test_head_workspace():
         assert q(*bad, 0, 0) < 0
     assert q(0, 4, 64, 10, 0, 0, ld=63) < 0                                   # a pitch below the width
     assert q(1, 1 << 20, 64, 1 << 27, 0, 0) < 0                               # more tiles than the kernels index
+    assert q(1, 1 << 24, 64, 10, 0, 0) < 0 <= q(1, (1 << 24) - 1, 64, 10, 0, 0)
+    # a vocabulary of any size that fits one piece is one piece: e's planes alone would differ by 512 MiB otherwise
+    assert q(1, 4096, 1024, 65536, 1, 0) - q(1, 4096, 1024, 65535, 1, 0) < 1024
     # 16-bit rows of whole k steps are read in place; odd widths, odd pitches and odd addresses are copied
     direct = q(1, 64, 128, 40960, 0, 0)
     assert direct < q(1, 64, 127, 40960, 0, 0) and direct < q(1, 64, 128, 40960, 0, 0, ptr=2) and direct < q(1, 64, 128, 40960, 0, 0, ld=129)
