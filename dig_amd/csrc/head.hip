@@ -246,8 +246,8 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
     }
   } else {
     // z = u acc: the product in units of 1 / tau (the scales are powers of two); with a bias, acc becomes z and u one.
-    // The exponentials take z minus a maximum first and the base-2 factor after it: the difference is exact where
-    // it matters.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane
+    // exp(z - m) = 2^(z k - m k) in one fused step, off by the rounding of the product m k alone, which is the same factor in
+    // all of a row and is taken out of its sum.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane
     // are 128 times whatever one costs.
     float u = a.inv_tau;
     if (a.nseg > 1) u = fminf(fmaxf(u / (a.scal[SC_X] * a.scal[SC_W]), 1.175494351e-38f), 3.402823466e38f);   // 0 or infinity times what may be either
@@ -301,13 +301,14 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
           for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[x][y][r]);
         m = fmaxf(m, __shfl_xor(m, 16, 64));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const float ms = m == -INFINITY ? 0.f : m, k = u * L2E;
+        const float ms = m == -INFINITY ? 0.f : m, k = u * L2E, mk = ms * k;
 #pragma unroll
         for (int x = 0; x < MI; ++x)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[x][y][r] - ms) * k);
+          for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(__fmaf_rn(acc[x][y][r], k, -mk));
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
+        s *= __builtin_amdgcn_exp2f(-__fmaf_rn(ms, k, -mk));
         if (lane < 16) {
           sh[((wave % WI) * BJ + jl) * 2] = m * u;
           sh[((wave % WI) * BJ + jl) * 2 + 1] = s;
@@ -328,14 +329,20 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
       }
     } else {
       // e = c (exp(z - m) rs - [target]); zeros in the padding that the next products read, and in rows without a loss
+      const float k = u * L2E;
 #pragma unroll
       for (int y = 0; y < MJ; ++y) {
         const int j = j0 + wj + y * 16 + l15;
         const bool in = j < a.nj;
         const float keep = __is_same(T, f16_t) ? E_SCALE : 1.f;
         const float c = in ? a.coef[j] * keep : 0.f;
-        const float m = c == 0.f ? INFINITY : a.m[j];            // its row of x is zero: exp(z - inf) = 0
-        const float cp = c == 0.f ? 0.f : c * a.rs[j];
+        // exp(z - m) with m = r u + (what the quotient left): 2^(acc k - r k), and what r k left, as in the statistics
+        float mk = INFINITY, cp = 0.f;                           // no loss: its row of x is zero, exp(z - inf) = 0
+        if (c != 0.f) {
+          const float m = a.m[j], r = m / u;
+          mk = r * k;
+          cp = c * a.rs[j] * __builtin_amdgcn_exp2f(-__fmaf_rn(r, k, -mk) - __fmaf_rn(-r, u, m) * L2E);
+        }
         const int tl = target_at(j);
         const bool any = __any(tl >= 0);
         // p - 1 of the target: what the other classes hold, not a difference near 1
@@ -347,7 +354,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
           float e[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            e[r] = cp * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x + (r >> 2)][y][r & 3], u, -m) * L2E);
+            e[r] = cp * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x + (r >> 2)][y][r & 3], k, -mk));
           if (any) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) e[r] = tl == hd_row(x) + r ? et : e[r];
@@ -411,17 +418,18 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
   LP lp;
   LQ lq;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) short*)sm;
-  // The next load: its tile, how many of the tile's are left, the product of planes (h h, h l, l h), the step inside that, and
-  // the operands' bases.  Stages alternate by constants in the code, so an odd count of steps gets one more that repeats the
-  // last load and multiplies nothing.
+  // The next load: its tile, how many of the tile's are left, the step of k and in it the product of planes (h h, h l, l h: a
+  // step's planes are read again while the L2 has them), and the operands' bases.  Stages alternate by constants in the code,
+  // so an odd count of steps gets one more that repeats the last load and multiplies nothing.
   const int steps = t1 - t0, pad = steps & 1;
-  const int first_seg = t0 / a.ktiles, first_k = t0 - first_seg * a.ktiles;
-  const int64_t dp = LP::advance(a.P), dq = LQ::advance(a.Q);
+  const int first_k = t0 / a.nseg, first_seg = t0 - first_k * a.nseg;
+  const int64_t pp = 2 * a.P.plane, pq = 2 * a.Q.plane;
+  const int64_t dp = LP::advance(a.P) - (a.nseg == 3 ? pp : 0), dq = LQ::advance(a.Q) - (a.nseg == 2 ? pq : 0);
   int lid = id, left, seg, lk, li0, lj0;
   const char *bp, *bq;
   auto base = [&]() __attribute__((always_inline)) {
-    bp = LP::start(a.P, seg == 2 ? a.P.plane : 0, li0) + lk * dp;
-    bq = LQ::start(a.Q, seg == 1 ? a.Q.plane : 0, lj0) + lk * dq;
+    bp = LP::start(a.P, seg == 2 ? a.P.plane : 0, li0) + lk * LP::advance(a.P);
+    bq = LQ::start(a.Q, seg == 1 ? a.Q.plane : 0, lj0) + lk * LQ::advance(a.Q);
   };
   auto aim = [&]() __attribute__((always_inline)) {
     int ti, tj;
@@ -447,12 +455,16 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
       }
       rewind();
     } else if (left > pad) {
-      bp += dp;
-      bq += dq;
-      if (++lk == a.ktiles) {
-        lk = 0;
-        ++seg;
-        base();
+      if (++seg == a.nseg) {
+        seg = 0;
+        ++lk;
+        bp += dp;
+        bq += dq;
+      } else if (seg == 1) {
+        bq += pq;
+      } else {
+        bp += pp;
+        bq -= pq;
       }
     }
   };
@@ -565,14 +577,15 @@ __global__ void __launch_bounds__(256) k_head_amax(const float* __restrict__ x, 
     v = fabsf(v);
     m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
   };
-  if (second && ld == D && D % 4 == 0 && ((uintptr_t)p & 15) == 0) {
-    const float4* q = (const float4*)p;
-    const int64_t n = rows * D / 4;
+  if (second && ld == D) {
+    const int64_t n = rows * D, n4 = n >> 2;
+    const RowVec<float, 4>* q = (const RowVec<float, 4>*)p;
 #pragma unroll 4
-    for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n; i += HD_AMAX * 256) {
-      const float4 v = q[i];
-      see(v.x); see(v.y); see(v.z); see(v.w);
+    for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n4; i += HD_AMAX * 256) {
+      const RowVec<float, 4> v = q[i];
+      see(v.v[0]); see(v.v[1]); see(v.v[2]); see(v.v[3]);
     }
+    if (b == 0 && (int64_t)threadIdx.x < (n & 3)) see(p[n - 1 - threadIdx.x]);
   } else {
     for (int64_t r = b * 4 + (threadIdx.x >> 6); r < rows; r += HD_AMAX * 4) {
       if (!second && !hd_live(r, target, ignore, index, tl, tdt, K, lane)) continue;
