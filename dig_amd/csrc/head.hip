@@ -1097,9 +1097,15 @@ static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
 //   f32:  32 x 128 x 1195: 39 / 96   512 x 128 x 1195: 65 / 118   2048 x 128 x 1195: 149 / 148   32 x 128 x 32768: 90 / 115
 //         128 x 512 x 1024: 73 / 83   512 x 512 x 256: 89 / 84   8 x 1024 x 1024: 106 / 98   4096 x 128 x 64: 206 / 76
 //   bf16: 32 x 128 x 1195: 42 / 70   512 x 128 x 1195: 67 / 81   32 x 128 x 8192: 51 / 46   8 x 512 x 4096: 75 / 45
-// 16-bit rows that the general path copies (odd widths or addresses) count as f32.
-static bool hd_small(bool copies, int64_t N, int64_t D, int64_t V) {
+// 16-bit rows that the general path copies (odd widths or addresses) count as f32 there.  And where few float32 rows meet a
+// W that the general path would read four times (its scale, its planes twice) before the first product is done (losses
+// alone, in place / general, and with gradients):
+//   1 x 1024 x 1024: 50 / 43, 105 / 96   1 x 1024 x 8192: 51 / 57, 131 / 140   16 x 2048 x 32768: 115 / 265, 421 / 635
+//   64 x 1024 x 32768: 78 / 127, 272 / 356   256 x 1024 x 32768: 188 / 137, 742 / 446
+// (16-bit rows, copied: 16 x 2047 x 32768: 134 / 87, 536 / 341).  A wave joins a row's V / 64 statistics: up to 2^20 classes.
+static bool hd_small(bool f32, bool copies, int64_t N, int64_t D, int64_t V) {
   const double work = (double)N * D * V;
+  if (f32 && N <= 64 && V >= 4096 && V <= 1048576) return true;
   return N <= 512 && (copies ? D <= 512 && work <= 134217728.0 : D <= 128 && work <= 16777216.0);
 }
 
@@ -1113,7 +1119,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     at += al256(bytes);
     return o;
   };
-  p.small = hd_small(!(dx && dw), N, D, V);
+  p.small = hd_small(dt == DT_F32, !(dx && dw), N, D, V);
   if (p.small) {
     p.vp = V;
     p.np = 1;

@@ -843,3 +843,10 @@ def test_temperatures_out_of_range_are_refused():
     for tau in (1e-7, 1e7, -1.0, float('inf')):
         with pytest.raises(ValueError):
             ops.linear_distillation(x, w, idx, tl, temperature=tau)
+
+
+@pytest.mark.parametrize('N,D,V', [(1, 1024, 4096), (16, 515, 5001), (64, 96, 20000)])
+def test_few_float32_rows_of_many_classes(N, D, V):
+    """sizes that float32 takes in place and 16-bit rows do not"""
+    one_classes(N, D, V, torch.float32, True, 'none', 0.2)
+    one_teacher(N, D, V, 12, torch.float32, False, 'mean', True, 2.0)
