@@ -58,7 +58,7 @@ struct HdArgs {
   int ktiles;                // k steps of one product
   int nseg;                  // products of planes (P, Q): 1 (h h), 2 (h h, h l) or 3 (h h, h l, l h)
   int ti, tj;                // tiles along i and j
-  int splits;                // the k steps are dealt to gridDim.z workgroups
+  int splits, wgs;           // ranges of the k steps, and workgroups to each
   // logits epilogues: i = class v0 + i, j = row
   const void* bias;
   int dt;                    // type of bias / of the stored output
@@ -212,8 +212,8 @@ __device__ __forceinline__ void hd_lds_barrier() {
 
 // what a finished tile of products becomes (see HdArgs)
 template <class T, int BI, int BJ, int WI, int WJ, int EPI>
-__device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / WI / 16][BJ / WJ / 16], int i0, int j0, int ti, int wi,
-                                            int wj, int tid, float* sh) {
+__device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / WI / 16][BJ / WJ / 16], int z, int i0, int j0, int ti,
+                                            int wi, int wj, int tid, float* sh) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
   const int lane = tid & 63, wave = tid >> 6;
   const int q4 = 4 * (lane >> 4), l15 = lane & 15;
@@ -235,7 +235,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
           else if (a.dt == DT_BF16) hd_store4<bf16_t>(a.out, (int64_t)j * a.ldo + i, v, left);
           else hd_store4<f16_t>(a.out, (int64_t)j * a.ldo + i, v, left);
         } else {
-          const int64_t at = ((int64_t)blockIdx.z * a.nj + j) * a.ni + i;
+          const int64_t at = ((int64_t)z * a.nj + j) * a.ni + i;
           if (a.add) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] += r < left ? a.acc[at + r] : 0.f;
@@ -398,10 +398,21 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
   __shared__ float sh[EPI == EPI_STATS ? WI * BJ * 2 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // An XCD takes a contiguous range of tiles, ordered in bands of 4 tiles along j, so that the tiles in flight on one L2
-  // share operand panels along both indices
-  const int n = a.ti * a.tj, per = (n + 7) >> 3, stride = (int)gridDim.x >> 3;
-  int id = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
-  const int end = min(n, (((int)blockIdx.x & 7) + 1) * per);
+  // share operand panels along both indices; of split products it takes whole ranges of k, all of whose tiles share panels
+  const int n = a.ti * a.tj, xcd = (int)blockIdx.x & 7, slot = (int)blockIdx.x >> 3;
+  int id, end, stride, z = 0;
+  if (a.splits == 1) {
+    const int per = (n + 7) >> 3;
+    id = xcd * per + slot;
+    end = min(n, (xcd + 1) * per);
+    stride = (int)gridDim.x >> 3;
+  } else {
+    const int w = xcd * ((int)gridDim.x >> 3) + slot;
+    z = w / a.wgs;
+    id = z < a.splits ? w - z * a.wgs : n;
+    end = n;
+    stride = a.wgs;
+  }
   if (id >= end) return;
   auto place = [&](int t, int& ti, int& tj) __attribute__((always_inline)) {
     const int band = t / (4 * a.ti), bw = min(4, a.tj - band * 4), rem = t - band * 4 * a.ti;
@@ -410,7 +421,7 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
   };
   const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
   const int total = a.ktiles * a.nseg;
-  const int t0 = (int)((int64_t)total * blockIdx.z / a.splits), t1 = (int)((int64_t)total * (blockIdx.z + 1) / a.splits);
+  const int t0 = (int)((int64_t)total * z / a.splits), t1 = (int)((int64_t)total * (z + 1) / a.splits);
 
   // only W is read along k where it lies, with rows beyond its last (PT && !QT); e and the copied x are whole k steps
   using LP = HdLoad<BI, PT, PT && !QT, NW>;
@@ -541,7 +552,7 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
       }
       if (more) mul(3);
     }
-    hd_epilogue<T, BI, BJ, WI, WJ, EPI>(a, acc, ti * BI, tj * BJ, ti, wi, wj, tid, sh);
+    hd_epilogue<T, BI, BJ, WI, WJ, EPI>(a, acc, z, ti * BI, tj * BJ, ti, wi, wj, tid, sh);
   }
   __builtin_amdgcn_s_waitcnt(0);           // nothing is in flight into LDS when it is given back
   __builtin_amdgcn_s_barrier();
@@ -1017,17 +1028,36 @@ __global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E
   }
 }
 
-// out[at0 + i] = factor * sum_s part[s][i] over `slots` partials, in order
-template <class T>
+// out[at0 + i] = factor * sum_s part[s][i] over `slots` partials: in order, or where there are many of few results (see
+// hd_sum) by 16 lanes of 16 results, each lane every 16th partial, and the lanes in order
+template <class T, bool MANY>
 __global__ void __launch_bounds__(256) k_head_sum(const float* __restrict__ part, int slots, int64_t stride, int64_t n,
                                                    const float* __restrict__ scal, int other, void* __restrict__ out, int dt,
                                                    int64_t at0) {
   const float f = scal ? hd_factor<T>(scal, other) : 1.f;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float s = part[i];
+  if constexpr (MANY) {
+    __shared__ float sh[16][17];
+    const int col = threadIdx.x & 15, sl = threadIdx.x >> 4;
+    const int64_t i = (int64_t)blockIdx.x * 16 + col;
+    float s = 0.f;
+    if (i < n) {
 #pragma unroll 8
-    for (int k = 1; k < slots; ++k) s += part[(int64_t)k * stride + i];
+      for (int k = sl; k < slots; k += 16) s += part[(int64_t)k * stride + i];
+    }
+    sh[sl][col] = s;
+    __syncthreads();
+    if (sl != 0 || i >= n) return;
+    s = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) s += sh[q][col];
     store_as(out, dt, at0 + i, s * f);
+  } else {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+      float s = part[i];
+#pragma unroll 8
+      for (int k = 1; k < slots; ++k) s += part[(int64_t)k * stride + i];
+      store_as(out, dt, at0 + i, s * f);
+    }
   }
 }
 
@@ -1052,8 +1082,11 @@ static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) 
   for (int e = 0; e < 3; ++e) {
     const int edge = 64 << e, occ = e == 0 ? 5 : e == 1 ? 2 : 1;
     const int64_t tiles = ((ni + edge - 1) / edge) * ((nj + edge - 1) / edge);
-    for (int s = 1; s <= max_splits; s *= 2) {
-      if (s > 1 && (ksteps / s < 4 || (double)s * ni * nj * 4 > 512e6)) break;
+    // powers of two, and the counts that fill the chip once or twice
+    for (int q = 0; q < 9; ++q) {
+      const int64_t fill = (int64_t)cus * occ * (q - 6) / tiles;
+      const int s = q < 7 ? 1 << q : (int)(fill < max_splits ? fill : max_splits);
+      if (s < 1 || s > max_splits || (s > 1 && (ksteps / s < 4 || (double)s * ni * nj * 4 > 512e6))) continue;
       const int64_t items = tiles * s, c0 = (items + cus - 1) / cus;
       const int c = (int)(c0 < occ ? c0 : occ);
       const int64_t rounds = (items + (int64_t)cus * c - 1) / ((int64_t)cus * c);
@@ -1134,7 +1167,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
       p.gx = {64, 1};
       if (needs & 1) {       // about two workgroups per CU, at least four k steps each
         const int64_t tiles = ((D + 63) / 64) * ((N + 63) / 64), steps = (V + SM_BK - 1) / SM_BK;
-        while (p.gx.splits < 32 && tiles * p.gx.splits < 2 * dig3d_num_cus() && steps / (2 * p.gx.splits) >= 2) p.gx.splits *= 2;
+        while (p.gx.splits < 512 && tiles * p.gx.splits < 2 * dig3d_num_cus() && steps / (2 * p.gx.splits) >= 2) p.gx.splits *= 2;
         if (p.gx.splits > 1) p.o_gx = take(p.gx.splits * N * D * 4);
       }
     }
@@ -1159,6 +1192,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
   p.vp = p.np == 1 ? V : ((V + p.np - 1) / p.np + 255) & ~255ll;
   p.np = (V + p.vp - 1) / p.vp;
   p.ldE = up64(p.vp);
+  if (p.ldE % 1024 == 0) p.ldE += 64;      // rows of e a multiple of 2 KB apart fall on few channels of the caches
   const int nseg = p.planes == 2 ? 3 : 1;
   p.lg = hd_shape(p.vp, N, (int64_t)p.Dp / HD_BK * nseg, 1);
   if (!p.dx) p.o_x = take(p.Np * p.Dp * 2 * p.planes);
@@ -1173,7 +1207,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     p.o_scal = take(SC_COUNT * 4 + (N + HD_TOTAL - 1) / HD_TOTAL * 4);
     p.o_E = take(p.Np * p.ldE * 2 * p.eplanes);
     if (needs & 1) {
-      p.gx = hd_shape(D, N, p.ldE / HD_BK * p.nseg, 64);
+      p.gx = hd_shape(D, N, up64(p.vp) / HD_BK * p.nseg, 64);
       if (p.np > 1 || p.gx.splits > 1) p.o_gx = take((int64_t)p.gx.splits * N * D * 4);
     }
     if (needs & 2) {
@@ -1193,8 +1227,9 @@ static void hd_gemm(const HdArgs& a0, const HdShape& sh, hipStream_t st) {
   a.tj = (a.nj + sh.b - 1) / sh.b;
   a.splits = sh.splits;
   // as many workgroups as run at once; each walks its tiles
-  const int occ = sh.b == 256 ? 1 : sh.b == 128 ? 2 : 5, most = (dig3d_num_cus() * occ / sh.splits + 7) & ~7;
-  const dim3 grid((unsigned)min(dig3d_xcd_grid(a.ti * a.tj), most), 1, (unsigned)sh.splits);
+  const int most = dig3d_num_cus() * (sh.b == 256 ? 1 : sh.b == 128 ? 2 : 5);
+  a.wgs = min(a.ti * a.tj, max(1, most / sh.splits));
+  const dim3 grid((unsigned)(sh.splits == 1 ? min(dig3d_xcd_grid(a.ti * a.tj), (most + 7) & ~7) : (a.wgs * sh.splits + 7) & ~7));
   if (sh.b == 256) hipLaunchKernelGGL((k_head_gemm<T, 256, 256, 2, 4, PT, QT, EPI>), grid, dim3(512), 0, st, a);
   else if (sh.b == 128) hipLaunchKernelGGL((k_head_gemm<T, 128, 128, 2, 2, PT, QT, EPI>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((k_head_gemm<T, 64, 64, 2, 2, PT, QT, EPI>), grid, dim3(256), 0, st, a);
@@ -1203,6 +1238,18 @@ static void hd_gemm(const HdArgs& a0, const HdShape& sh, hipStream_t st) {
 static inline unsigned hd_grid(int64_t items, int per) {
   const int64_t b = (items + per - 1) / per, cap = 16ll * dig3d_num_cus();
   return (unsigned)(b < 1 ? 1 : b < cap ? b : cap);
+}
+
+// the sum of partial results.  us in order / by 16 lanes:  2140 results of 64 partials 6.0 / 4.0, 32768 of 16: 5.4 / 4.8; 574 of 32
+// in order 4.1, of 512 by 16 lanes 4.0
+template <class T>
+static void hd_sum(const float* part, int slots, int64_t stride, int64_t n, const float* scal, int other, void* out, int dt, int64_t at0,
+                   hipStream_t st) {
+  if (slots >= 16 && n <= 65536)
+    hipLaunchKernelGGL((k_head_sum<T, true>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, slots, stride, n, scal, other, out, dt,
+                       at0);
+  else
+    hipLaunchKernelGGL((k_head_sum<T, false>), dim3(hd_grid(n, 256)), dim3(256), 0, st, part, slots, stride, n, scal, other, out, dt, at0);
 }
 
 static void hd_pack(const void* src, int dt, int64_t ld, int64_t R, int D, const float* coef, const float* amax, int slot,
@@ -1407,8 +1454,7 @@ static int hd_bwd_small(const HdCall& c, const HdPlan& p, const float* g, void* 
   DIG3D_CHECK_LAUNCH();
   if (a.slots) {
     const int64_t n = (int64_t)c.N * c.D;
-    hipLaunchKernelGGL((k_head_sum<bf16_t>), dim3(hd_grid(n, 256)), dim3(256), 0, c.st, a.slots, p.gx.splits, n, n, (const float*)nullptr, -1,
-                       gx, c.dt, (int64_t)0);
+    hd_sum<bf16_t>(a.slots, p.gx.splits, n, n, nullptr, -1, gx, c.dt, 0, c.st);
     DIG3D_CHECK_LAUNCH();
   }
   return DIG3D_OK;
@@ -1512,8 +1558,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
       DIG3D_CHECK_LAUNCH();
       if (slots) {
         const int64_t n = (int64_t)nv * c.D;
-        hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(n, 256)), dim3(256), 0, c.st, (const float*)(ws + p.o_gw), p.gw.splits, n, n,
-                           c.scal, o.other, gw, c.dt, v0 * c.D);
+        hd_sum<T>((const float*)(ws + p.o_gw), p.gw.splits, n, n, c.scal, o.other, gw, c.dt, v0 * c.D, c.st);
         DIG3D_CHECK_LAUNCH();
       }
     }
@@ -1523,15 +1568,13 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
       hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)slices, (unsigned)((p.ldE + 255) / 256)), dim3(256), 0, c.st, E, p.ldE,
                          eplane, p.eplanes, c.N, part);
       DIG3D_CHECK_LAUNCH();
-      hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(nv, 256)), dim3(256), 0, c.st, part, slices, p.ldE, (int64_t)nv, c.scal, -1, gb,
-                         c.dt, v0);
+      hd_sum<T>(part, slices, p.ldE, nv, c.scal, -1, gb, c.dt, v0, c.st);
       DIG3D_CHECK_LAUNCH();
     }
   }
   if (gx_slots) {
     const int64_t n = (int64_t)c.N * c.D;
-    hipLaunchKernelGGL((k_head_sum<T>), dim3(hd_grid(n, 256)), dim3(256), 0, c.st, (const float*)(ws + p.o_gx), p.gx.splits, n, n, c.scal,
-                       planes2 ? SC_W : -1, gx, c.dt, (int64_t)0);
+    hd_sum<T>((const float*)(ws + p.o_gx), p.gx.splits, n, n, c.scal, planes2 ? SC_W : -1, gx, c.dt, 0, c.st);
     DIG3D_CHECK_LAUNCH();
   }
   return DIG3D_OK;
