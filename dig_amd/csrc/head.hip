@@ -3,6 +3,7 @@
 //   classes:  loss_n = lse(z_n) - z_n[y_n]                                     e_n = c_n (softmax(z_n) - onehot(y_n))
 //   teacher:  loss_n = tau^2 sum_k q_k (log q_k - log p_n[i_k]), p = softmax(z / tau)   e_n = c_n (p_n - scatter(q_n))
 //   gx = S e W,  gW = S e^T x,  gb = S sum_n e_n          (c_n S: the gradient that reaches row n, |c_n| <= 1)
+// (f16 / f32: e is kept to 2^-40 of the largest |c|, so a row whose gradient is 10^-6 of another's keeps 20 bits of its own)
 //
 // Four products of 2 N V D operations: the logits, the logits again in the backward (the price of not keeping them), e W and
 // e^T x.  Bound: the matrix cores.  All four run on ONE product kernel (k_head_gemm): out[j, i] = sum_k Q[j, k] P[i, k], each
@@ -1069,11 +1070,12 @@ struct HdShape {
 // The tile edge and the number of k ranges with the smallest estimated time.  The estimate is fitted to measured launches of
 // the product kernel (bf16; us of one k step of 64 with c tiles on a CU, and us of a tile's epilogue that its neighbours do
 // not hide):   64: 0.5 alone, 1.1 with five on the CU;   128: 0.8 alone, 1.2 with two;   256: 1.9 (one to a CU)
-// us with tiles of 64 / 128 / 256:
-//   logits' statistics, 4096 x 2048 x 65536: 1956 / 1075 / 892 (1.23 PFLOP/s; a library's plain product of that shape: 904)
-//   2048 x 256 x 32768: 88 / 55 / 48    64 x 1024 x 16384: 11 / 14 / 31    their gradient e, 4096 x 2048 x 65536: - / 1238 / 967
-//   e W in ranges, 4096 x 2048 x 65536 (2): 2365 / 1212 / 925 (library: 892)    1024 x 128 x 65536 (16): 52 / 59 / 118
-//   e^T x, 4096 x 2048 x 65536: 2683 / 1184 / 905 (library: 1000)    2048 x 256 x 32768: 59 / 41 / 60
+// us with tiles of 64 / 128 / 256 (and k ranges):
+//   logits' statistics, 4096 x 2048 x 65536: 1985 / 1076 / 945 (1.16 PFLOP/s; on another card 892, a library's plain product: 904)
+//   8192 x 128 x 65536: 424 / 287 / 231    2048 x 256 x 32768: 82 / 55 / 45    64 x 1024 x 16384: 12 / 15 / 29
+//   their gradient e, 4096 x 2048 x 65536: 2372 / 1219 / 1014    2048 x 256 x 32768: 94 / 67 / 55
+//   e W, 4096 x 2048 x 65536: 2325 (1) / 1063 (1) / 946 (2)    2048 x 256 x 32768: 57 (16) / 39 (16) / 43 (32)
+//   1024 x 128 x 65536: 34 (32) / 32 (32) / 40 (64)    e^T x, 4096 x 2048 x 65536: 2452 / 1214 / 989    2048 x 256 x 32768: 56 / 41 / 61
 // A split product writes its partial results and a second launch adds them (bytes at 4 TB/s and 4 us).
 static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) {
   const int cus = dig3d_num_cus();
@@ -1123,7 +1125,10 @@ static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
   return dt != DT_F32 && D % HD_BK == 0 && ld % 8 == 0 && ld <= HD_MAX_PITCH && ((uintptr_t)p & 15) == 0;
 }
 
-#define HD_PIECE_BYTES (512ll << 20)   // e of one piece, per plane; a piece also bounds the packed part of W
+// e of one piece, per plane; a piece also bounds the packed part of W.  ms with gradients by pieces of 64 / 128 / 256 / 512 MiB:
+// 4096 x 2048 x 131072 bf16 7.71 / 7.40 / 7.43 / 7.32   8192 x 128 x 65536 bf16 1.65 / 1.30 / 1.37 / 1.38   8192 x 256 x 32768 f32
+// 2.06 / 2.04 / 2.03 / 1.98   1741 x 114 x 118479 f32 1.52 / 1.41 / 1.33 / 1.34: the last-level cache returns nothing for it
+#define HD_PIECE_BYTES (512ll << 20)
 
 // Float32 products in place (head_small.h) where copies and launches are what the general path costs (GPU us of value and
 // gradients, in place / general):

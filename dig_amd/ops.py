@@ -5,6 +5,9 @@ autograd glue.  Mirrors the third-party call signatures the reference uses (SURV
     scatter(src, index, dim, out, dim_size, reduce)         torch_scatter
     scatter_min(src, index, dim, out, dim_size)             torch_scatter
 
+and, without a counterpart there, the operators of a trained output head: ``layer_norm``, ``linear_cross_entropy`` and
+``linear_distillation`` (dig_amd/head.py).
+
 Everything here launches HIP kernels on the current torch stream; there is no CPU code path.
 """
 import ctypes
