@@ -92,6 +92,8 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     gradients have the type of their inputs and the same bits every time."""
     x2, weight, bias = _check_head('linear_cross_entropy', x, weight, bias, reduction)
     _check_index('linear_cross_entropy', 'target', target, x.shape[:-1], x2)
+    if not -1 << 63 <= int(ignore_index) < 1 << 63:
+        raise ValueError(f'linear_cross_entropy: ignore_index is an int64, got {ignore_index}')
     loss = _HeadLoss.apply(x2, weight, bias, target.reshape(-1).contiguous(), None, None, 1.0, int(ignore_index), _REDUCTIONS[reduction])
     return loss if reduction != 'none' or x.dim() == 2 else loss.reshape(target.shape)
 

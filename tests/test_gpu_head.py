@@ -813,7 +813,7 @@ def test_listed_logits_of_the_lowest_value_stay_entries():
     q = torch.softmax(teacher[1, :3].double() / 0.5, 0)
     lp = torch.log_softmax(head64(x.detach()[1:2], w.detach(), bd, 0.5), 1)[0]
     want = 0.25 * (q * (q.log() - lp[index[1, :3]])).sum()
-    assert abs(float(a[0]) - float(want)) <= 2000 * U * (1 + abs(float(want)) + 20)
+    assert abs(float(a.detach()[0]) - float(want)) <= 2000 * U * (1 + abs(float(want)) + 20)
 
 
 @pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
@@ -850,3 +850,51 @@ def test_few_float32_rows_of_many_classes(N, D, V):
     """sizes that float32 takes in place and 16-bit rows do not"""
     one_classes(N, D, V, torch.float32, True, 'none', 0.2)
     one_teacher(N, D, V, 12, torch.float32, False, 'mean', True, 2.0)
+
+
+def test_offsets_beyond_32_bits():
+    """more than 2^31 elements of W, and of the rows of a layer norm: what lies behind them is what it is alone"""
+    from dig_amd import ops
+    g = gen(90)
+    N, D, V = 4, 2048, 1_100_000
+    w = torch.empty(V, D, device=DEV, dtype=torch.bfloat16)
+    for i in range(0, V, 100_000):
+        w[i:i + 100_000] = (randn(g, 100_000, D) / math.sqrt(D)).to(torch.bfloat16)
+    x = randn(g, N, D).to(torch.bfloat16).requires_grad_()
+    w.requires_grad_()
+    target = torch.tensor([0, V - 1, V - 70_000, 1_048_577], device=DEV)
+    rows = ops.linear_cross_entropy(x, w, target, reduction='none')
+    gx, gw = torch.autograd.grad(rows.sum(), (x, w))
+    xd, wd = x.detach().double(), w.detach()
+    z = torch.cat([xd @ wd[i:i + 100_000].double().t() for i in range(0, V, 100_000)], 1)
+    lse = torch.logsumexp(z, 1)
+    want = lse - z.gather(1, target[:, None])[:, 0]
+    # (D + 8) u of the terms in a logit, 8 u of every exponential, 40 levels of additions, twice (the sum and the target)
+    size = (xd.abs() @ wd[target].double().abs().t()).amax()
+    tol = 2 * ((D + 8) * U * float(size) + 100 * U)
+    close(rows, want, tol * (1 + want.abs()), 'rows')
+    e = torch.exp(z - lse[:, None])
+    e[torch.arange(N, device=DEV), target] -= 1
+    # two bf16 numbers of e: 2^-16 of an entry; the result's half step; V additions in ranges of at most 2^15 terms a chain
+    ref, mag = torch.zeros(N, D, dtype=torch.float64, device=DEV), torch.zeros(N, D, dtype=torch.float64, device=DEV)
+    for i in range(0, V, 100_000):
+        ref += e[:, i:i + 100_000] @ wd[i:i + 100_000].double()
+        mag += e[:, i:i + 100_000].abs() @ wd[i:i + 100_000].double().abs()
+    close(gx, ref, half(torch.bfloat16) * ref.abs() * 1.01 + (2.0 ** -16 + 4 * tol + 2.0 ** 15 * U) * mag, 'gx')
+    for i in (0, 1_048_570, V - 8):
+        part = e[:, i:i + 8].t() @ xd
+        close(gw[i:i + 8], part, half(torch.bfloat16) * part.abs() * 1.01 + (2.0 ** -16 + 4 * tol) * (e[:, i:i + 8].abs().t() @ xd.abs()) + 1e-30, 'gw')
+    del w, gw, z, wd, e
+    R, C = 2_200_000, 1000
+    rows = torch.empty(R, C, device=DEV, dtype=torch.bfloat16)
+    rows[:5], rows[-5:] = randn(g, 5, C).to(torch.bfloat16), randn(g, 5, C).to(torch.bfloat16)
+    rows[5:-5] = 1.0
+    y = ops.layer_norm(rows)
+    assert torch.equal(y[-5:], ops.layer_norm(rows[-5:].clone())) and torch.equal(y[:5], ops.layer_norm(rows[:5].clone())) and not y[5:-5].any()
+
+
+def test_an_ignore_index_beyond_the_type_is_refused():
+    from dig_amd import ops
+    with pytest.raises(ValueError):
+        ops.linear_cross_entropy(torch.randn(4, 64, device=DEV), torch.randn(10, 64, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV),
+                                 ignore_index=1 << 64)
