@@ -40,7 +40,8 @@ __device__ __forceinline__ f32x4 hd_mfma<f16_t>(s16x8 a, s16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// One operand: `planes` matrices of `rows` rows with pitch `ld` (elements, a multiple of 8; base 16-byte aligned).
+// One operand: a matrix of `rows` rows with pitch `ld` (elements, a multiple of 8; base 16-byte aligned); a value of two numbers
+// has its second one `plane` elements behind the first, in the same row.
 //   not TR: row = the operand's own index, columns = k (k extent a multiple of HD_BK inside the pitch)
 //   TR:     row = k, columns = the operand's own index (`cols` of them are readable, a multiple of 8)
 // Rows beyond the last are read as the last one: for the own index their results are not used, for k the other operand
@@ -57,7 +58,7 @@ struct HdArgs {
   HdOperand P, Q;
   int ni, nj;                // extents of the own indices of P and Q
   int ktiles;                // k steps of one product
-  int nseg;                  // products of planes (P, Q): 1 (h h), 2 (h h, h l) or 3 (h h, h l, l h)
+  int nseg;                  // not PAIR: Q as one number, or as two (h h, h l)
   int ti, tj;                // tiles along i and j
   int splits, wgs;           // ranges of the k steps, and workgroups to each
   // logits epilogues: i = class v0 + i, j = row
@@ -75,8 +76,8 @@ struct HdArgs {
   const float* loss;
   const float* coef;
   int eplanes;               // e as one number, or as two (its rounding and what that left)
-  short* E;                  // EPI_GRAD [eplanes][rowsE][ldE]
-  int64_t ldE, planeE;
+  short* E;                  // EPI_GRAD [rowsE][eplanes][colsE]
+  int64_t colsE;
   int rowsE;
   // EPI_OUT
   float* acc;                // f32 partial slots [splits][nj][ni], written or added to
@@ -117,9 +118,12 @@ __device__ __forceinline__ const char* hd_uniform(const char* p) {
 // TR:     LDS row k holds B / 8 chunks; chunk s of it is source chunk s ^ (2 g(k) mod B / 8), g(k) = (k & 3) | (k >> 3 & 3) << 2
 // The lane's byte offsets from the tile's first element are formed once (32 bits: 256 rows of at most HD_MAX_PITCH elements);
 // a k step moves the uniform base.
+// PAIR: a step is 32 deep in k and both numbers of a value are staged: the first in the first 4 chunks (not TR) or 32 rows (TR)
+// of the tile, the second behind it.
 #define HD_MAX_PITCH (1 << 22)
-template <int B, bool TR, bool CLAMP, int NW>
+template <int B, bool TR, bool CLAMP, int NW, bool PAIR>
 struct HdLoad {
+  static constexpr int DEEP = PAIR ? 32 : HD_BK;
   static constexpr int NL = B * HD_BK * 2 / 1024 / NW;
   static constexpr int CH = B / 8, RPL = TR ? 64 / CH : 8;      // TR: chunks per row, rows per load
   uint32_t off[NL];
@@ -130,20 +134,21 @@ struct HdLoad {
       if constexpr (!TR) {
         const int r = blk * 8 + (lane >> 3);
         const int ch = (lane & 7) ^ ((r & 3) | (((r >> 3) & 1) << 2));
-        off[q] = 2u * ((uint32_t)(min(own0 + r, o.rows - 1) - own0) * (uint32_t)o.ld + ch * 8);
+        off[q] = 2u * ((uint32_t)(min(own0 + r, o.rows - 1) - own0) * (uint32_t)o.ld +
+                       (PAIR ? (ch & 3) * 8 + (ch >> 2) * (uint32_t)o.plane : ch * 8));
       } else {
         const int k = blk * RPL + lane / CH;
         const int g = (k & 3) | (((k >> 3) & 3) << 2);
         const int ch = (lane % CH) ^ ((2 * g) & (CH - 1));
-        off[q] = 2u * ((uint32_t)k * (uint32_t)o.ld + min(own0 + ch * 8, o.cols - 8));
+        off[q] = 2u * ((uint32_t)(k % DEEP) * (uint32_t)o.ld + (k / DEEP) * (uint32_t)o.plane + min(own0 + ch * 8, o.cols - 8));
       }
     }
   }
-  // first element of the tile at k step 0 of a plane, and the distance between k steps (bytes)
-  static __device__ __forceinline__ const char* start(const HdOperand& o, int64_t plane, int own0) {
-    return (const char*)(o.p + plane + (TR ? 0 : (int64_t)own0 * o.ld));
+  // first element of the tile at k step 0, and the distance between k steps (bytes)
+  static __device__ __forceinline__ const char* start(const HdOperand& o, int own0) {
+    return (const char*)(o.p + (TR ? 0 : (int64_t)own0 * o.ld));
   }
-  static __device__ __forceinline__ int64_t advance(const HdOperand& o) { return TR ? 2 * HD_BK * o.ld : 2 * HD_BK; }
+  static __device__ __forceinline__ int64_t advance(const HdOperand& o) { return TR ? 2 * DEEP * o.ld : 2 * DEEP; }
   // The load is written out so that the compiler's own waits do not count it: it has no register result, and the kernel
   // waits for it (vmcnt) before the barrier that hands the stage over.  s_nop: the wait states between a scalar register's
   // writer (M0, or a base that came through a vector instruction) and its reader, which the compiler does not see here.
@@ -154,7 +159,7 @@ struct HdLoad {
       const int blk = q * NW + wave;
       uint32_t v = off[q];
       if constexpr (CLAMP) {               // rows of k beyond the last: the last one again
-        const int k = blk * RPL + lane / CH;
+        const int k = (blk * RPL + lane / CH) % DEEP;
         v -= 2u * (uint32_t)max(0, k - (o.rows - 1 - k0)) * (uint32_t)o.ld;
       }
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds + blk * 1024)), "v"(v),
@@ -164,29 +169,35 @@ struct HdLoad {
   }
 };
 
-// the matrix operand of 16 own indices from o0 and k half kk of a staged tile
-template <int B, bool TR>
-__device__ __forceinline__ s16x8 hd_frag(const short* lds, int o0, int kk, int lane) {
-  if constexpr (!TR) {
-    const int r = o0 + (lane & 15), f = (lane & 3) | (((lane >> 3) & 1) << 2);
-    return *(const s16x8*)(lds + r * HD_BK + (((kk * 4 + (lane >> 4)) ^ f) * 8));
-  } else {
-    constexpr int CH = B / 8;
-    const int k = kk * 32 + 8 * (lane >> 4) + ((lane & 15) >> 2);
-    const int ch = ((o0 >> 3) + ((lane & 3) >> 1)) ^ ((2 * (lane >> 2)) & (CH - 1));
-    const short* a = lds + k * B + ch * 8 + (lane & 1) * 4;
-    typedef __attribute__((address_space(3))) s16x4* lp;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(short*)a);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(short*)(a + 4 * B));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-}
-// The logits' products take P's rows in another order: operand x of a wave holds rows hd_row(x) + 8 (m >> 2) + (m & 3), m < 16,
+// Reading a staged tile (swizzled as above) as matrix operands of 16 own indices each.  hd_at: the lane's LDS address for operand
+// 0 of a wave whose own indices start at o0 (a multiple of 32, 8 times a power of two above the operands' range).  hd_frag:
+// operand x of half kk (of k, or PAIR: the kk'th numbers) from it; x and kk are constants, so it is that address with a few
+// bits flipped and an offset in the instruction.
+// `pairs`: the logits' products take P's rows in another order, operand x holds rows hd_row(x) + 8 (m >> 2) + (m & 3), m < 16,
 // so that a lane's results of operands 2 t and 2 t + 1 are 8 consecutive classes of one row: e is stored 16 bytes at a time
 __device__ __forceinline__ constexpr int hd_row(int x) { return (x >> 1) * 32 + (x & 1) * 4; }
-__device__ __forceinline__ s16x8 hd_frag_pairs(const short* lds, int o0, int x, int kk, int lane) {
-  const int m = lane & 15, r = o0 + hd_row(x) + 8 * (m >> 2) + (m & 3);
-  return *(const s16x8*)(lds + r * HD_BK + (((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 8));
+template <int B, bool TR, bool pairs>
+__device__ __forceinline__ uint32_t hd_at(uint32_t tile, int o0, int lane) {
+  const int m = lane & 15;
+  if constexpr (TR) {
+    const int k = 8 * (lane >> 4) + (m >> 2);
+    return tile + k * B * 2 + ((((o0 >> 3) | ((lane & 3) >> 1)) ^ ((2 * (lane >> 2)) & (B / 8 - 1))) << 4) + (lane & 1) * 8;
+  } else {
+    const int r = o0 + (pairs ? 8 * (m >> 2) + (m & 3) : m), f = pairs ? m & 7 : (m & 3) | (((m >> 3) & 1) << 2);
+    return tile + r * HD_BK * 2 + (((lane >> 4) ^ f) << 4);
+  }
+}
+template <int B, bool TR, bool pairs>
+__device__ __forceinline__ s16x8 hd_frag(uint32_t at, int x, int kk) {
+  if constexpr (TR) {
+    typedef __attribute__((address_space(3))) s16x4* lp;
+    const uint32_t a = (at ^ (x << 5)) + kk * 32 * B * 2;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)a);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(a + 4 * B * 2));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+    return *(const __attribute__((address_space(3))) s16x8*)((at ^ (kk << 6)) + (pairs ? hd_row(x) : x * 16) * HD_BK * 2);
+  }
 }
 
 // n <= 4 consecutive results of a row, from any element address
@@ -212,7 +223,7 @@ __device__ __forceinline__ void hd_lds_barrier() {
 }
 
 // what a finished tile of products becomes (see HdArgs)
-template <class T, int BI, int BJ, int WI, int WJ, int EPI>
+template <class T, int BI, int BJ, int WI, int WJ, int EPI, bool PAIR>
 __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / WI / 16][BJ / WJ / 16], int z, int i0, int j0, int ti,
                                             int wi, int wj, int tid, float* sh) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
@@ -251,7 +262,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
     // all of a row and is taken out of its sum.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane
     // are 128 times whatever one costs.
     float u = a.inv_tau;
-    if (a.nseg > 1) u = fminf(fmaxf(u / (a.scal[SC_X] * a.scal[SC_W]), 1.175494351e-38f), 3.402823466e38f);   // 0 or infinity times what may be either
+    if constexpr (PAIR) u = fminf(fmaxf(u / (a.scal[SC_X] * a.scal[SC_W]), 1.175494351e-38f), 3.402823466e38f);   // 0 or infinity times what may be either
     if (a.bias) {
 #pragma unroll
       for (int x = 0; x < MI; ++x)
@@ -349,7 +360,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         // p - 1 of the target: what the other classes hold, not a difference near 1
         const float et = tl >= 0 ? c * expm1f(-a.loss[j]) : 0.f;
         if (j >= a.rowsE) continue;
-        short* row = a.E + (int64_t)j * a.ldE + first;
+        short* row = a.E + (int64_t)j * a.eplanes * a.colsE + first;
 #pragma unroll
         for (int x = 0; x < MI; x += 2) {
           float e[8];
@@ -361,7 +372,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
             for (int r = 0; r < 8; ++r) e[r] = tl == hd_row(x) + r ? et : e[r];
           }
           if (edge) {
-            if (first + hd_row(x) >= a.ldE) continue;
+            if (first + hd_row(x) >= a.colsE) continue;
 #pragma unroll
             for (int r = 0; r < 8; ++r) e[r] = hd_row(x) + r >= last ? 0.f : e[r];
           }
@@ -372,7 +383,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
           if (a.eplanes > 1) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) l.t[r] = to_t<T>(e[r] - (float)h.t[r]);
-            *(decltype(l)*)(row + a.planeE + hd_row(x)) = l;
+            *(decltype(l)*)(row + a.colsE + hd_row(x)) = l;
           }
         }
       }
@@ -384,14 +395,15 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
 // one j, so rows of the output are written in pieces of 4.
 //
 // A workgroup walks its tiles as one sequence of k steps.  Two stages are in LDS; a step is four phases (two halves of k, two
-// of the wave's i), and the operands of a phase are read while the phase before it multiplies.  The barrier that ends a
+// of the wave's i), or six where the values are pairs (three products, two halves of i): what is loaded and read from LDS for
+// four multiplies for six there.  The operands of a phase are read while the phase before it multiplies.  The barrier that ends a
 // step stands before its last phase, whose operands are in registers by then: the loads of the step after the next and the
 // first reads of the next one are issued under that phase's products.  The sequence runs on into the next tile, so a
 // tile's first loads are under way during the last steps and the epilogue of the tile before it.  Behind the last tile the
 // loads fetch that tile's first steps again, into stages that are read no more.
 // Measured (bf16, 4096 x 2048 x 65536): see hd_shape.  What bounds it: the latency of loads that miss the L2 (one step of
 // 64 KB in flight per CU) and the clock, which this load holds near 2.0 GHz.
-template <class T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI>
+template <class T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI, bool PAIR>
 __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdArgs a) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16, HX = MI / 2;
   constexpr int SZ = hd_tile_shorts<BI>() + hd_tile_shorts<BJ>();
@@ -421,27 +433,26 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     ti = rem / bw;
   };
   const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
-  const int total = a.ktiles * a.nseg;
+  const int nseg = PAIR ? 1 : a.nseg, total = a.ktiles * nseg;
   const int t0 = (int)((int64_t)total * z / a.splits), t1 = (int)((int64_t)total * (z + 1) / a.splits);
 
   // only W is read along k where it lies, with rows beyond its last (PT && !QT); e and the copied x are whole k steps
-  using LP = HdLoad<BI, PT, PT && !QT, NW>;
-  using LQ = HdLoad<BJ, QT, false, NW>;
+  using LP = HdLoad<BI, PT, PT && !QT, NW, PAIR>;
+  using LQ = HdLoad<BJ, QT, false, NW, PAIR>;
   LP lp;
   LQ lq;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) short*)sm;
-  // The next load: its tile, how many of the tile's are left, the step of k and in it the product of planes (h h, h l, l h: a
-  // step's planes are read again while the L2 has them), and the operands' bases.  Stages alternate by constants in the code,
-  // so an odd count of steps gets one more that repeats the last load and multiplies nothing.
+  // The next load: its tile, how many of the tile's are left, the step of k and in it the number of Q's values (a step is read
+  // again while the L2 has it), and the operands' bases.  Stages alternate by constants in the code, so an odd count of
+  // steps gets one more that repeats the last load and multiplies nothing.
   const int steps = t1 - t0, pad = steps & 1;
-  const int first_k = t0 / a.nseg, first_seg = t0 - first_k * a.nseg;
-  const int64_t pp = 2 * a.P.plane, pq = 2 * a.Q.plane;
-  const int64_t dp = LP::advance(a.P) - (a.nseg == 3 ? pp : 0), dq = LQ::advance(a.Q) - (a.nseg == 2 ? pq : 0);
+  const int first_k = t0 / nseg, first_seg = t0 - first_k * nseg;
+  const int64_t pq = 2 * a.Q.plane, dp = LP::advance(a.P), dq = LQ::advance(a.Q) - (nseg == 2 ? pq : 0);
   int lid = id, left, seg, lk, li0, lj0;
   const char *bp, *bq;
   auto base = [&]() __attribute__((always_inline)) {
-    bp = LP::start(a.P, seg == 2 ? a.P.plane : 0, li0) + lk * LP::advance(a.P);
-    bq = LQ::start(a.Q, seg == 1 ? a.Q.plane : 0, lj0) + lk * LQ::advance(a.Q);
+    bp = LP::start(a.P, li0) + lk * dp;
+    bq = LQ::start(a.Q, lj0) + lk * LQ::advance(a.Q) + (seg == 1 ? pq : 0);
   };
   auto aim = [&]() __attribute__((always_inline)) {
     int ti, tj;
@@ -458,8 +469,8 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     base();
   };
   auto issue = [&](int stage) __attribute__((always_inline)) {
-    lp.issue(a.P, bp, lk * HD_BK, lds0 + stage * (SZ * 2), wave, lane);
-    lq.issue(a.Q, bq, lk * HD_BK, lds0 + stage * (SZ * 2) + hd_tile_shorts<BI>() * 2, wave, lane);
+    lp.issue(a.P, bp, lk * LP::DEEP, lds0 + stage * (SZ * 2), wave, lane);
+    lq.issue(a.Q, bq, lk * LQ::DEEP, lds0 + stage * (SZ * 2) + hd_tile_shorts<BI>() * 2, wave, lane);
     if (--left == 0) {
       if (lid + stride < end) {
         lid += stride;
@@ -467,41 +478,63 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
       }
       rewind();
     } else if (left > pad) {
-      if (++seg == a.nseg) {
+      if (++seg == nseg) {
         seg = 0;
         ++lk;
         bp += dp;
         bq += dq;
-      } else if (seg == 1) {
-        bq += pq;
       } else {
-        bp += pp;
-        bq -= pq;
+        bq += pq;
       }
     }
   };
   s16x8 fp[2][HX], fq[2][MJ];
   f32x4 acc[MI][MJ];
-  auto read_p = [&](int stage, int ph) __attribute__((always_inline)) {
+  // half `kk` of the tiles' depth (PAIR: the first or second numbers) of half `hx` of the wave's P, and of its Q, into a buffer each
+  // The addresses are formed anew from one register each time: kept per operand and stage they would not fit (the empty asm
+  // keeps the compiler from doing so), and a spilled one is a load that waits for the tiles' loads
+  constexpr bool pairs = EPI != EPI_OUT;
+  const uint32_t ap = hd_at<BI, PT, pairs>(lds0, wi, lane), aq = hd_at<BJ, QT, false>(lds0 + hd_tile_shorts<BI>() * 2, wj, lane);
+  auto read_p = [&](int stage, int kk, int hx) __attribute__((always_inline)) {
+    uint32_t at = ap + stage * (SZ * 2);
+    asm volatile("" : "+v"(at));
 #pragma unroll
-    for (int x = 0; x < HX; ++x) {
-      if constexpr (EPI == EPI_OUT) fp[ph & 1][x] = hd_frag<BI, PT>(sm + stage * SZ, wi + ((ph & 1) * HX + x) * 16, ph >> 1, lane);
-      else fp[ph & 1][x] = hd_frag_pairs(sm + stage * SZ, wi, (ph & 1) * HX + x, ph >> 1, lane);
-    }
+    for (int x = 0; x < HX; ++x) fp[hx][x] = hd_frag<BI, PT, pairs>(at, hx * HX + x, kk);
   };
-  auto read_q = [&](int stage, int kk) __attribute__((always_inline)) {
+  auto read_q = [&](int stage, int kk, int buf) __attribute__((always_inline)) {
+    uint32_t at = aq + stage * (SZ * 2);
+    asm volatile("" : "+v"(at));
 #pragma unroll
-    for (int y = 0; y < MJ; ++y) fq[kk][y] = hd_frag<BJ, QT>(sm + stage * SZ + hd_tile_shorts<BI>(), wj + y * 16, kk, lane);
+    for (int y = 0; y < MJ; ++y) fq[buf][y] = hd_frag<BJ, QT, false>(at, y, kk);
   };
-  auto mul = [&](int ph) __attribute__((always_inline)) {
+  auto mul = [&](int hx, int buf) __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int x = 0; x < HX; ++x)
 #pragma unroll
-      for (int y = 0; y < MJ; ++y) acc[(ph & 1) * HX + x][y] = hd_mfma<T>(fp[ph & 1][x], fq[ph >> 1][y], acc[(ph & 1) * HX + x][y]);
+      for (int y = 0; y < MJ; ++y) acc[hx * HX + x][y] = hd_mfma<T>(fp[hx][x], fq[buf][y], acc[hx * HX + x][y]);
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
+  };
+  // A step's products but for the last group, whose operands are read: on `stage`, whose first half of P and of Q (in buffer
+  // `b`) is in registers.  PAIR: the first and second numbers of P and Q serve three products
+  auto multiply = [&](int stage, int b) __attribute__((always_inline)) {
+    read_p(stage, 0, 1);
+    if constexpr (PAIR) read_q(stage, 1, 1 - b);
+    mul(0, b);
+    if constexpr (PAIR) {
+      mul(1, b);
+      mul(0, 1 - b);
+      read_p(stage, 1, 0);
+      mul(1, 1 - b);
+    } else {
+      read_q(stage, 1, 1 - b);
+      read_p(stage, 1, 0);
+      mul(1, b);
+    }
+    read_p(stage, 1, 1);
+    mul(0, PAIR ? b : 1 - b);
   };
   // this wave's loads have landed and its LDS reads are done, and every other wave's
   auto meet = [&]() __attribute__((always_inline)) {
@@ -520,40 +553,28 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     for (int x = 0; x < MI; ++x)
 #pragma unroll
       for (int y = 0; y < MJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
-    read_q(0, 0);
-    read_p(0, 0);
+    // the buffer of Q that a step's last group leaves free takes the next step's first half
+    constexpr int second = PAIR ? 1 : 0;
+    read_q(0, 0, 0);
+    read_p(0, 0, 0);
     for (int t = 0; t < steps; t += 2) {
-      read_p(0, 1);
-      mul(0);
-      read_q(0, 1);
-      read_p(0, 2);
-      mul(1);
-      read_p(0, 3);
-      mul(2);
+      multiply(0, 0);
       meet();                              // the next step has arrived; this one has been read by all
       issue(0);
-      read_q(1, 0);
-      read_p(1, 0);
-      mul(3);
+      read_q(1, 0, second);
+      read_p(1, 0, 0);
+      mul(1, 1 - second);
       const bool more = t + 1 < steps;     // not of an odd count's last step, whose partner is only waited for
-      if (more) {
-        read_p(1, 1);
-        mul(0);
-        read_q(1, 1);
-        read_p(1, 2);
-        mul(1);
-        read_p(1, 3);
-        mul(2);
-      }
+      if (more) multiply(1, second);
       meet();
       issue(1);
       if (t + 2 < steps) {                 // across the epilogue the registers are the result's
-        read_q(0, 0);
-        read_p(0, 0);
+        read_q(0, 0, 0);
+        read_p(0, 0, 0);
       }
-      if (more) mul(3);
+      if (more) mul(1, 1);
     }
-    hd_epilogue<T, BI, BJ, WI, WJ, EPI>(a, acc, z, ti * BI, tj * BJ, ti, wi, wj, tid, sh);
+    hd_epilogue<T, BI, BJ, WI, WJ, EPI, PAIR>(a, acc, z, ti * BI, tj * BJ, ti, wi, wj, tid, sh);
   }
   __builtin_amdgcn_s_waitcnt(0);           // nothing is in flight into LDS when it is given back
   __builtin_amdgcn_s_barrier();
@@ -619,13 +640,12 @@ __device__ __forceinline__ float hd_scale(float m) {
   return ldexpf(1.f, min(15 - e, 100));
 }
 
-// out [planes][orows][ocols] <- rows [0, R) of src (type dt, pitch ld, D columns), zeros elsewhere; `coef`: a row with
-// coefficient 0 is written as zeros (its contents, whatever they are, take no part in any sum).  f32: two planes, and block
+// out [orows][numbers][ocols] <- rows [0, R) of src (type dt, pitch ld, D columns), zeros elsewhere; `coef`: a row with
+// coefficient 0 is written as zeros (its contents, whatever they are, take no part in any sum).  f32: two numbers, and block
 // 0 leaves the scale in scal[slot].
 __global__ void __launch_bounds__(256) k_head_pack(const void* __restrict__ src, int dt, int64_t ld, int64_t R, int D,
                                                     const float* __restrict__ coef, const float* __restrict__ amax, int slot,
-                                                    float* __restrict__ scal, short* __restrict__ out, int64_t orows, int ocols,
-                                                    int64_t plane) {
+                                                    float* __restrict__ scal, short* __restrict__ out, int64_t orows, int ocols) {
   __shared__ float sh[4];
   float s = 1.f;
   if (dt == DT_F32) {
@@ -638,6 +658,7 @@ __global__ void __launch_bounds__(256) k_head_pack(const void* __restrict__ src,
     if (blockIdx.x == 0 && threadIdx.x == 0) scal[slot] = s;
   }
   const int oc8 = ocols >> 3;
+  const int64_t pitch = dt == DT_F32 ? 2 * (int64_t)ocols : ocols;
   const int64_t n = orows * oc8;
   for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < n; u += (int64_t)gridDim.x * 256) {
     const int64_t r = u / oc8;
@@ -660,11 +681,11 @@ __global__ void __launch_bounds__(256) k_head_pack(const void* __restrict__ src,
       for (int i = 0; i < 8; ++i) {
         const f16_t hi = (f16_t)f[i];
         const float d = f[i] - (float)hi;
-        const f16_t lo = (f16_t)(fabsf(d) <= 65504.f ? d : 0.f);    // an infinity or NaN is its first plane's alone
+        const f16_t lo = (f16_t)(fabsf(d) <= 65504.f ? d : 0.f);    // an infinity or NaN is the first number's alone
         h[i] = __builtin_bit_cast(short, hi);
         l[i] = __builtin_bit_cast(short, lo);
       }
-      *(s16x8*)(out + plane + r * ocols + c) = l;
+      *(s16x8*)(out + r * pitch + ocols + c) = l;
     } else {
       const short* p = (const short*)src + r * ld + c;
       if (left == 8) {
@@ -676,7 +697,7 @@ __global__ void __launch_bounds__(256) k_head_pack(const void* __restrict__ src,
         for (int i = 0; i < 8; ++i) h[i] = i < left ? p[i] : (short)0;
       }
     }
-    *(s16x8*)(out + r * ocols + c) = h;
+    *(s16x8*)(out + r * pitch + c) = h;
   }
 }
 
@@ -977,8 +998,8 @@ template <class T>
 __global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __restrict__ index, const float* __restrict__ q,
                                                             const float* __restrict__ z, const float* __restrict__ mo,
                                                             const float* __restrict__ rs, const float* __restrict__ coef, int64_t N, int K, int64_t v0,
-                                                            int64_t nv, int planes, void* __restrict__ E, int64_t ldE,
-                                                            int64_t planeE) {
+                                                            int64_t nv, int planes, void* __restrict__ E,
+                                                            int64_t colsE) {
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (u >= N * K) return;
   const int64_t n = u / K;
@@ -986,32 +1007,32 @@ __global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __rest
   const int64_t v = index[u];
   if (v < v0 || v >= v0 + nv || c == 0.f || qk < 0.f) return;
   const float e = c * (__builtin_amdgcn_exp2f((z[u] - mo[n]) * L2E) * rs[n] - qk);
-  T* o = (T*)E + n * ldE + (v - v0);
+  T* o = (T*)E + n * planes * colsE + (v - v0);
   if constexpr (sizeof(T) == 4) {
     *o = e;
   } else {
     const float s = __is_same(T, f16_t) ? e * E_SCALE : e;
     const T h = to_t<T>(s);
     *o = h;
-    if (planes == 2) o[planeE] = to_t<T>(s - (float)h);
+    if (planes == 2) o[colsE] = to_t<T>(s - (float)h);
   }
 }
 
 #define HD_SLICE 128
-// column sums of e over slices of HD_SLICE rows: part[slice][ldE].  32 lanes across 256 columns (16 bytes each), 8 row lanes
+// column sums of e over slices of HD_SLICE rows: part[slice][colsE].  32 lanes across 256 columns (16 bytes each), 8 row lanes
 template <class T>
-__global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E, int64_t ldE, int64_t planeE, int planes, int rows,
+__global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E, int64_t colsE, int planes, int rows,
                                                       float* __restrict__ part) {
   __shared__ float sh[8][32 * 8 + 4];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.y * 256 + cl * 8;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (c < ldE) {                           // a multiple of 64: a lane's 8 columns are all there
+  if (c < colsE) {                           // a multiple of 64: a lane's 8 columns are all there
     const int r0 = blockIdx.x * HD_SLICE, r1 = min(rows, r0 + HD_SLICE);
     for (int p = 0; p < planes; ++p) {
 #pragma unroll 4
       for (int r = r0 + rl; r < r1; r += 8) {
-        struct alignas(16) { T t[8]; } v = *(const decltype(v)*)(E + p * planeE + (int64_t)r * ldE + c);
+        struct alignas(16) { T t[8]; } v = *(const decltype(v)*)(E + ((int64_t)r * planes + p) * colsE + c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i] += (float)v.t[i];
       }
@@ -1021,11 +1042,11 @@ __global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E
   for (int i = 0; i < 8; ++i) sh[rl][cl * 8 + i] = s[i];
   __syncthreads();
   const int64_t o = (int64_t)blockIdx.y * 256 + threadIdx.x;
-  if (o < ldE) {
+  if (o < colsE) {
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) v += sh[q][threadIdx.x];
-    part[(int64_t)blockIdx.x * ldE + o] = v;
+    part[(int64_t)blockIdx.x * colsE + o] = v;
   }
 }
 
@@ -1076,8 +1097,10 @@ struct HdShape {
 //   their gradient e, 4096 x 2048 x 65536: 2372 / 1219 / 1014    2048 x 256 x 32768: 94 / 67 / 55
 //   e W, 4096 x 2048 x 65536: 2325 (1) / 1063 (1) / 946 (2)    2048 x 256 x 32768: 57 (16) / 39 (16) / 43 (32)
 //   1024 x 128 x 65536: 34 (32) / 32 (32) / 40 (64)    e^T x, 4096 x 2048 x 65536: 2452 / 1214 / 989    2048 x 256 x 32768: 56 / 41 / 61
+// Pairs, a step of 32 with three products: 1.2 times a step's time (4096 x 1024 x 32000, tiles of 256: 609 to 709 us where products
+// one after the other took 730; 2048 x 256 x 32768, e^T x on 128: 122 -> 105).
 // A split product writes its partial results and a second launch adds them (bytes at 4 TB/s and 4 us).
-static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) {
+static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, bool pair, int max_splits) {
   const int cus = dig3d_num_cus();
   HdShape best = {64, 1};
   double tb = 1e30;
@@ -1092,7 +1115,7 @@ static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, int max_splits) 
       const int64_t items = tiles * s, c0 = (items + cus - 1) / cus;
       const int c = (int)(c0 < occ ? c0 : occ);
       const int64_t rounds = (items + (int64_t)cus * c - 1) / ((int64_t)cus * c);
-      const double step = e == 0 ? 0.35 + 0.15 * c : e == 1 ? 0.42 + 0.38 * c : 1.9;
+      const double step = (pair ? 1.2 : 1.0) * (e == 0 ? 0.35 + 0.15 * c : e == 1 ? 0.42 + 0.38 * c : 1.9);
       const double fixed = e == 0 ? 2.0 + 0.5 * c : e == 1 ? 1.5 + 0.8 * c : 6.0;
       double t = (double)rounds * (fixed + (double)((ksteps + s - 1) / s) * step);
       if (s > 1) t += 4.0 + (double)s * ni * nj * 8 / 4e6;
@@ -1110,8 +1133,8 @@ static inline int64_t al256(int64_t v) { return (v + 255) & ~255ll; }
 
 struct HdPlan {
   bool small;                // head_small.h
-  int planes, Dp;
-  int eplanes, nseg;         // of e, and products of planes with it
+  int Dp, eplanes;           // eplanes: numbers of an entry of e
+  bool pair;                 // float32: every value is two numbers
   bool dx, dw;               // x / W are read where they are
   int64_t Np, vp, np, ldE;
   HdShape lg, gx, gw;
@@ -1147,6 +1170,9 @@ static bool hd_small(bool f32, bool copies, int64_t N, int64_t D, int64_t V) {
   return N <= 512 && (copies ? D <= 512 && work <= 134217728.0 : D <= 128 && work <= 16777216.0);
 }
 
+// k steps of a product over `k` values, one operand of `q` numbers each
+static int64_t hd_steps(const HdPlan& p, int64_t k, int q) { return p.pair ? (k + 31) / 32 : (k + 63) / 64 * q; }
+
 // needs: bit 0 gx, bit 1 gw, bit 2 gb; backward = 0: the forward's plan
 static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int backward, int needs) {
   HdPlan p;
@@ -1179,29 +1205,28 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     p.total = at;
     return p;
   }
-  p.planes = dt == DT_F32 ? 2 : 1;
+  p.pair = dt == DT_F32;
+  const int planes = p.pair ? 2 : 1;
   // One rounding of e is lost among the roundings of the gradients where many rows add up (2^1/2 of the error of their own);
   // in a few rows it is a common factor of a whole row of gw.  There W is what the products wait for, and e is two numbers;
   // also where the second product costs no more than launches do (512 x 512 x 8192: 15 us of 190)
   p.eplanes = dt == DT_F32 || N <= 128 || (double)N * D * V <= 2147483648.0 ? 2 : 1;
-  p.nseg = dt == DT_F32 ? 3 : p.eplanes;
   p.Dp = (int)up64(D);
   p.dx = dx && !backward;    // the backward masks rows while it copies x (N D elements: nothing beside its products)
   p.dw = dw;
   p.Np = up64(N);
   int64_t most = V;
-  if (backward) most = min(most, HD_PIECE_BYTES / (p.Np * 2));
-  if (!p.dw) most = min(most, HD_PIECE_BYTES / ((int64_t)p.Dp * 2 * p.planes));
+  if (backward) most = min(most, min(HD_PIECE_BYTES / (p.Np * 2), (int64_t)HD_MAX_PITCH / 2 - 1024));
+  if (!p.dw) most = min(most, HD_PIECE_BYTES / ((int64_t)p.Dp * 2 * planes));
   if (most < V) most = max((int64_t)256, most & ~255ll);
   p.np = (V + most - 1) / most;
   p.vp = p.np == 1 ? V : ((V + p.np - 1) / p.np + 255) & ~255ll;
   p.np = (V + p.vp - 1) / p.vp;
   p.ldE = up64(p.vp);
-  if (p.ldE % 1024 == 0) p.ldE += 64;      // rows of e a multiple of 2 KB apart fall on few channels of the caches
-  const int nseg = p.planes == 2 ? 3 : 1;
-  p.lg = hd_shape(p.vp, N, (int64_t)p.Dp / HD_BK * nseg, 1);
-  if (!p.dx) p.o_x = take(p.Np * p.Dp * 2 * p.planes);
-  if (!p.dw) p.o_w = take(min(p.vp, V) * p.Dp * 2 * p.planes);
+  if (p.ldE * p.eplanes % 1024 == 0) p.ldE += 64;      // rows of e a multiple of 2 KB apart fall on few channels of the caches
+  p.lg = hd_shape(p.vp, N, hd_steps(p, p.Dp, 1), p.pair, 1);
+  if (!p.dx) p.o_x = take(p.Np * p.Dp * 2 * planes);
+  if (!p.dw) p.o_w = take(min(p.vp, V) * p.Dp * 2 * planes);
   if (!backward) {
     p.tiles_all = 0;
     for (int64_t v0 = 0; v0 < V; v0 += p.vp) p.tiles_all += (int)((min(p.vp, V - v0) + p.lg.b - 1) / p.lg.b);
@@ -1212,11 +1237,11 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     p.o_scal = take(SC_COUNT * 4 + (N + HD_TOTAL - 1) / HD_TOTAL * 4);
     p.o_E = take(p.Np * p.ldE * 2 * p.eplanes);
     if (needs & 1) {
-      p.gx = hd_shape(D, N, up64(p.vp) / HD_BK * p.nseg, 64);
+      p.gx = hd_shape(D, N, hd_steps(p, p.vp, p.eplanes), p.pair, 64);
       if (p.np > 1 || p.gx.splits > 1) p.o_gx = take((int64_t)p.gx.splits * N * D * 4);
     }
     if (needs & 2) {
-      p.gw = hd_shape(D, p.vp, p.Np / HD_BK * p.nseg, 64);
+      p.gw = hd_shape(D, p.vp, hd_steps(p, N, p.eplanes), p.pair, 64);
       if (p.gw.splits > 1) p.o_gw = take((int64_t)p.gw.splits * p.vp * D * 4);
     }
     if (needs & 4) p.o_col = take((N + HD_SLICE - 1) / HD_SLICE * p.ldE * 4);
@@ -1225,8 +1250,14 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
   return p;
 }
 
+template <class T, bool PT, bool QT, int EPI, bool PAIR>
+static void hd_launch(const HdArgs& a, int b, const dim3& grid, hipStream_t st) {
+  if (b == 256) hipLaunchKernelGGL((k_head_gemm<T, 256, 256, 2, 4, PT, QT, EPI, PAIR>), grid, dim3(512), 0, st, a);
+  else if (b == 128) hipLaunchKernelGGL((k_head_gemm<T, 128, 128, 2, 2, PT, QT, EPI, PAIR>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_head_gemm<T, 64, 64, 2, 2, PT, QT, EPI, PAIR>), grid, dim3(256), 0, st, a);
+}
 template <class T, bool PT, bool QT, int EPI>
-static void hd_gemm(const HdArgs& a0, const HdShape& sh, hipStream_t st) {
+static void hd_gemm(const HdArgs& a0, const HdShape& sh, bool pair, hipStream_t st) {
   HdArgs a = a0;
   a.ti = (a.ni + sh.b - 1) / sh.b;
   a.tj = (a.nj + sh.b - 1) / sh.b;
@@ -1235,9 +1266,10 @@ static void hd_gemm(const HdArgs& a0, const HdShape& sh, hipStream_t st) {
   const int most = dig3d_num_cus() * (sh.b == 256 ? 1 : sh.b == 128 ? 2 : 5);
   a.wgs = min(a.ti * a.tj, max(1, most / sh.splits));
   const dim3 grid((unsigned)(sh.splits == 1 ? min(dig3d_xcd_grid(a.ti * a.tj), (most + 7) & ~7) : (a.wgs * sh.splits + 7) & ~7));
-  if (sh.b == 256) hipLaunchKernelGGL((k_head_gemm<T, 256, 256, 2, 4, PT, QT, EPI>), grid, dim3(512), 0, st, a);
-  else if (sh.b == 128) hipLaunchKernelGGL((k_head_gemm<T, 128, 128, 2, 2, PT, QT, EPI>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_head_gemm<T, 64, 64, 2, 2, PT, QT, EPI>), grid, dim3(256), 0, st, a);
+  if constexpr (__is_same(T, f16_t)) {
+    if (pair) return hd_launch<T, PT, QT, EPI, true>(a, sh.b, grid, st);
+  }
+  hd_launch<T, PT, QT, EPI, false>(a, sh.b, grid, st);
 }
 
 static inline unsigned hd_grid(int64_t items, int per) {
@@ -1258,9 +1290,9 @@ static void hd_sum(const float* part, int slots, int64_t stride, int64_t n, cons
 }
 
 static void hd_pack(const void* src, int dt, int64_t ld, int64_t R, int D, const float* coef, const float* amax, int slot,
-                    float* scal, short* out, int64_t orows, int ocols, int64_t plane, hipStream_t st) {
+                    float* scal, short* out, int64_t orows, int ocols, hipStream_t st) {
   hipLaunchKernelGGL(k_head_pack, dim3(hd_grid(orows * (ocols >> 3), 256)), dim3(256), 0, st, src, dt, ld, R, D, coef, amax,
-                     slot, scal, out, orows, ocols, plane);
+                     slot, scal, out, orows, ocols);
 }
 
 static bool hd_bad(int dt, int N, int D, int V, int64_t ldx, int64_t ldw) {
@@ -1336,16 +1368,16 @@ static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
   }
   HdArgs a;
   memset(&a, 0, sizeof a);
-  const int64_t xplane = p.Np * p.Dp;
+  const int two = p.pair ? 2 : 1;          // numbers of a value
   if (p.dx) a.Q = {(const short*)c.x, c.ldx, 0, c.N, c.D};
   else {
-    hd_pack(c.x, c.dt, c.ldx, c.N, c.D, nullptr, c.amax, SC_X, c.scal, (short*)(ws + p.o_x), p.Np, p.Dp, xplane, c.st);
+    hd_pack(c.x, c.dt, c.ldx, c.N, c.D, nullptr, c.amax, SC_X, c.scal, (short*)(ws + p.o_x), p.Np, p.Dp, c.st);
     DIG3D_CHECK_LAUNCH();
-    a.Q = {at_bytes(ws, p.o_x), p.Dp, xplane, c.N, p.Dp};
+    a.Q = {at_bytes(ws, p.o_x), (int64_t)p.Dp * two, p.Dp, c.N, p.Dp};
   }
   a.nj = c.N;
-  a.ktiles = p.Dp / HD_BK;
-  a.nseg = p.planes == 2 ? 3 : 1;
+  a.ktiles = (int)hd_steps(p, p.Dp, 1);
+  a.nseg = 1;
   a.bias = c.bias;
   a.dt = c.dt;
   a.scal = c.scal;
@@ -1361,15 +1393,14 @@ static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
     const char* wp = (const char*)c.w + v0 * c.ldw * esz;
     if (p.dw) a.P = {(const short*)wp, c.ldw, 0, nv, c.D};
     else {
-      const int64_t plane = (int64_t)nv * p.Dp;
-      hd_pack(wp, c.dt, c.ldw, nv, c.D, nullptr, c.amax, SC_W, c.scal, (short*)(ws + p.o_w), nv, p.Dp, plane, c.st);
+      hd_pack(wp, c.dt, c.ldw, nv, c.D, nullptr, c.amax, SC_W, c.scal, (short*)(ws + p.o_w), nv, p.Dp, c.st);
       DIG3D_CHECK_LAUNCH();
-      a.P = {at_bytes(ws, p.o_w), p.Dp, plane, nv, p.Dp};
+      a.P = {at_bytes(ws, p.o_w), (int64_t)p.Dp * two, p.Dp, nv, p.Dp};
     }
     a.ni = nv;
     a.v0 = v0;
     a.part_c0 = (int)(v0 / p.lg.b);
-    hd_gemm<T, false, false, EPI_STATS>(a, p.lg, c.st);
+    hd_gemm<T, false, false, EPI_STATS>(a, p.lg, p.pair, c.st);
     DIG3D_CHECK_LAUNCH();
   }
   return DIG3D_OK;
@@ -1426,10 +1457,9 @@ static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
 }
 
 template <class T>
-static int hd_teacher_grad(const HdCall& c, const float* coef, int64_t v0, int64_t nv, int planes, void* E, int64_t ldE,
-                           int64_t planeE) {
+static int hd_teacher_grad(const HdCall& c, const float* coef, int64_t v0, int64_t nv, int planes, void* E, int64_t colsE) {
   hipLaunchKernelGGL((k_head_teacher_grad<T>), dim3((unsigned)(((int64_t)c.N * c.K + 255) / 256)), dim3(256), 0, c.st, c.index, c.q,
-                     c.z, c.m, c.rs, coef, (int64_t)c.N, c.K, v0, nv, planes, E, ldE, planeE);
+                     c.z, c.m, c.rs, coef, (int64_t)c.N, c.K, v0, nv, planes, E, colsE);
   DIG3D_CHECK_LAUNCH();
   return DIG3D_OK;
 }
@@ -1445,7 +1475,7 @@ static int hd_bwd_small(const HdCall& c, const HdPlan& p, const float* g, void* 
   hipLaunchKernelGGL((k_head_small_logits<true>), dim3((unsigned)p.tiles_all, (unsigned)((c.N + 63) / 64)), dim3(256), 0, c.st, a);
   DIG3D_CHECK_LAUNCH();
   if (c.index) {
-    const int rc = hd_teacher_grad<float>(c, a.coef + c.N, 0, c.V, 1, a.E, a.ldE, 0);
+    const int rc = hd_teacher_grad<float>(c, a.coef + c.N, 0, c.V, 1, a.E, a.ldE);
     if (rc != DIG3D_OK) return rc;
   }
   a.gx = gx;
@@ -1479,12 +1509,12 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
   hipLaunchKernelGGL(k_head_coef, dim3(blocks), dim3(1024), 0, c.st, g, gm, blocks, c.reduction == 1 ? c.count : (const float*)nullptr,
                      f, c.target, c.ignore, live, c.N, coef, c.scal);
   DIG3D_CHECK_LAUNCH();
-  const int64_t xplane = p.Np * p.Dp;
-  const bool planes2 = p.planes == 2;
-  hd_pack(c.x, c.dt, c.ldx, c.N, c.D, coef, c.amax, SC_X, c.scal, (short*)(ws + p.o_x), p.Np, p.Dp, xplane, c.st);
+  const int two = p.pair ? 2 : 1;          // numbers of a value
+  hd_pack(c.x, c.dt, c.ldx, c.N, c.D, coef, c.amax, SC_X, c.scal, (short*)(ws + p.o_x), p.Np, p.Dp, c.st);
   DIG3D_CHECK_LAUNCH();
   short* E = (short*)(ws + p.o_E);
-  const int64_t eplane = p.Np * p.ldE;
+  const HdOperand x = {at_bytes(ws, p.o_x), (int64_t)p.Dp * two, p.Dp, (int)p.Np, p.Dp};
+  const HdOperand e = {E, p.ldE * p.eplanes, p.ldE, (int)p.Np, (int)p.ldE};
   const int esz = c.dt == DT_F32 ? 4 : 2;
   const bool gx_slots = gx && (p.np > 1 || p.gx.splits > 1);
   for (int64_t v0 = 0; v0 < c.V; v0 += p.vp) {
@@ -1493,19 +1523,18 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     HdOperand W;
     if (p.dw) W = {(const short*)wsrc, c.ldw, 0, nv, c.D};
     else {
-      const int64_t plane = (int64_t)nv * p.Dp;
-      hd_pack(wsrc, c.dt, c.ldw, nv, c.D, nullptr, c.amax, SC_W, c.scal, (short*)(ws + p.o_w), nv, p.Dp, plane, c.st);
+      hd_pack(wsrc, c.dt, c.ldw, nv, c.D, nullptr, c.amax, SC_W, c.scal, (short*)(ws + p.o_w), nv, p.Dp, c.st);
       DIG3D_CHECK_LAUNCH();
-      W = {at_bytes(ws, p.o_w), p.Dp, plane, nv, p.Dp};
+      W = {at_bytes(ws, p.o_w), (int64_t)p.Dp * two, p.Dp, nv, p.Dp};
     }
     HdArgs a;
     memset(&a, 0, sizeof a);
     a.P = W;
-    a.Q = {at_bytes(ws, p.o_x), p.Dp, xplane, (int)p.Np, p.Dp};
+    a.Q = x;
     a.ni = nv;
     a.nj = c.N;
-    a.ktiles = p.Dp / HD_BK;
-    a.nseg = planes2 ? 3 : 1;
+    a.ktiles = (int)hd_steps(p, p.Dp, 1);
+    a.nseg = 1;
     a.bias = c.bias;
     a.dt = c.dt;
     a.scal = c.scal;
@@ -1519,47 +1548,46 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     a.coef = coef;
     a.eplanes = p.eplanes;
     a.E = E;
-    a.ldE = p.ldE;
-    a.planeE = eplane;
+    a.colsE = p.ldE;
     a.rowsE = (int)p.Np;
-    hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, c.st);
+    hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, p.pair, c.st);
     DIG3D_CHECK_LAUNCH();
     if (c.index) {
-      const int rc = hd_teacher_grad<T>(c, coef, v0, nv, p.eplanes, E, p.ldE, eplane);
+      const int rc = hd_teacher_grad<T>(c, coef, v0, nv, p.eplanes, E, p.ldE);
       if (rc != DIG3D_OK) return rc;
     }
     HdArgs o;
     memset(&o, 0, sizeof o);
-    o.nseg = p.nseg;
+    o.nseg = p.pair ? 1 : p.eplanes;
     o.scal = c.scal;
     o.dt = c.dt;
     if (gx) {                              // gx[n, d] += sum_v e[n, v] W[v, d]
       o.P = W;
-      o.Q = {E, p.ldE, eplane, (int)p.Np, (int)p.ldE};
+      o.Q = e;
       o.ni = c.D;
       o.nj = c.N;
-      o.ktiles = (int)(up64(nv) / HD_BK);  // no step starts beyond W's last row
+      o.ktiles = (int)hd_steps(p, nv, 1);  // no step starts beyond W's last row
       o.acc = gx_slots ? (float*)(ws + p.o_gx) : nullptr;
       o.add = v0 > 0;
       o.out = gx_slots ? nullptr : gx;
       o.ldo = c.D;
-      o.other = planes2 ? SC_W : -1;
-      hd_gemm<T, true, false, EPI_OUT>(o, p.gx, c.st);
+      o.other = p.pair ? SC_W : -1;
+      hd_gemm<T, true, false, EPI_OUT>(o, p.gx, p.pair, c.st);
       DIG3D_CHECK_LAUNCH();
     }
     if (gw) {                              // gw[v, d] = sum_n e[n, v] x[n, d]
       const bool slots = p.gw.splits > 1;
-      o.P = {at_bytes(ws, p.o_x), p.Dp, xplane, (int)p.Np, p.Dp};
-      o.Q = {E, p.ldE, eplane, (int)p.Np, (int)p.ldE};
+      o.P = x;
+      o.Q = e;
       o.ni = c.D;
       o.nj = nv;
-      o.ktiles = (int)(p.Np / HD_BK);
+      o.ktiles = (int)hd_steps(p, c.N, 1);
       o.acc = slots ? (float*)(ws + p.o_gw) : nullptr;
       o.add = 0;
       o.out = slots ? nullptr : (char*)gw + v0 * c.D * esz;
       o.ldo = c.D;
-      o.other = planes2 ? SC_X : -1;
-      hd_gemm<T, true, true, EPI_OUT>(o, p.gw, c.st);
+      o.other = p.pair ? SC_X : -1;
+      hd_gemm<T, true, true, EPI_OUT>(o, p.gw, p.pair, c.st);
       DIG3D_CHECK_LAUNCH();
       if (slots) {
         const int64_t n = (int64_t)nv * c.D;
@@ -1571,7 +1599,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
       float* part = (float*)(ws + p.o_col);
       const int slices = (c.N + HD_SLICE - 1) / HD_SLICE;
       hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)slices, (unsigned)((p.ldE + 255) / 256)), dim3(256), 0, c.st, E, p.ldE,
-                         eplane, p.eplanes, c.N, part);
+                         p.eplanes, c.N, part);
       DIG3D_CHECK_LAUNCH();
       hd_sum<T>(part, slices, p.ldE, nv, c.scal, -1, gb, c.dt, v0, c.st);
       DIG3D_CHECK_LAUNCH();
@@ -1579,7 +1607,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
   }
   if (gx_slots) {
     const int64_t n = (int64_t)c.N * c.D;
-    hd_sum<T>((const float*)(ws + p.o_gx), p.gx.splits, n, n, c.scal, planes2 ? SC_W : -1, gx, c.dt, 0, c.st);
+    hd_sum<T>((const float*)(ws + p.o_gx), p.gx.splits, n, n, c.scal, p.pair ? SC_W : -1, gx, c.dt, 0, c.st);
     DIG3D_CHECK_LAUNCH();
   }
   return DIG3D_OK;
