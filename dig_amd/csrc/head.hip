@@ -640,35 +640,107 @@ __device__ __forceinline__ float hd_scale(float m) {
   return ldexpf(1.f, min(15 - e, 100));
 }
 
-// out [orows][numbers][ocols] <- rows [0, R) of src (type dt, pitch ld, D columns), zeros elsewhere; `coef`: a row with
-// coefficient 0 is written as zeros (its contents, whatever they are, take no part in any sum).  f32: two numbers, and block
-// 0 leaves the scale in scal[slot].
-__global__ void __launch_bounds__(256) k_head_pack(const void* __restrict__ src, int dt, int64_t ld, int64_t R, int D,
-                                                    const float* __restrict__ coef, const float* __restrict__ amax, int slot,
-                                                    float* __restrict__ scal, short* __restrict__ out, int64_t orows, int ocols) {
-  __shared__ float sh[4];
-  float s = 1.f;
-  if (dt == DT_F32) {
-    float m = amax[slot * HD_AMAX + threadIdx.x];
+__device__ __forceinline__ float hd_wave_max(float v) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
-    __syncthreads();
-    s = hd_scale(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])));
-    if (blockIdx.x == 0 && threadIdx.x == 0) scal[slot] = s;
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+// the maximum over a workgroup of NW waves, in every thread
+template <int NW>
+__device__ __forceinline__ float hd_block_max(float m, float* sh) {
+  m = hd_wave_max(m);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) m = fmaxf(m, sh[w]);
+  return m;
+}
+__device__ __forceinline__ float hd_finite_max(float m, float v) {
+  v = fabsf(v);
+  return v <= 3.402823466e38f ? fmaxf(m, v) : m;
+}
+// live is NaN for a row that lists a class that does not exist
+__device__ __forceinline__ bool hd_has(int64_t n, const int64_t* target, int64_t ignore, const float* live) {
+  return target ? target[n] != ignore : live[n] != 0.f;
+}
+
+// What stands before the products, in one launch: the rows' coefficients (backward), and the copies of x and of a piece of W
+// where they are not read in place.
+struct HdPack {
+  const void* src;
+  int dt;
+  int64_t ld, R;
+  int D;
+  short* out;                // [orows][numbers][ocols]
+  int64_t orows;
+  int ocols, slot, blocks;   // slot: SC_X / SC_W
+};
+struct HdPrep {
+  HdPack x, w;
+  int masked;                // rows of x without a loss are copied as zeros
+  const float* amax;
+  float* scal;
+  int coef_blocks;           // HD_COEF rows each
+  const float *g, *gm;       // per_row: the rows' gradients and, beyond HD_COEF rows, their partial maxima
+  int ngm, per_row;
+  const float* count;
+  float f;                   // tau for the teacher's loss, else 1
+  const int64_t* target;
+  int64_t ignore;
+  const float* live;
+  int N;
+  float* coef;
+};
+#define HD_COEF 2048
+
+// coef[n] (|.| <= 1, 0 for a row without a loss) and the scalar S with coef[n] S = the gradient of row n's logits' loss:
+// reductions: coef = 1 or 0, S = g f / count;  none: S = a power of two over max |g f|
+__device__ __forceinline__ void hd_coef(const HdPrep& a, int b, float* sh) {
+  float S = 1.f;
+  if (a.per_row) {
+    float m = 0.f;
+    if (a.gm) {
+      for (int i = threadIdx.x; i < a.ngm; i += 256) m = fmaxf(m, a.gm[i]);
+    } else {
+      for (int n = threadIdx.x; n < a.N; n += 256)
+        if (hd_has(n, a.target, a.ignore, a.live)) m = hd_finite_max(m, a.g[n] * a.f);
+    }
+    m = hd_block_max<4>(m, sh);
+    if (m > 0.f) {
+      int e;
+      frexpf(m, &e);
+      S = ldexpf(1.f, min(max(e, -100), 100));
+    }
+  } else {
+    S = a.g[0] * a.f / (a.count ? *a.count : 1.f);
   }
-  const int oc8 = ocols >> 3;
-  const int64_t pitch = dt == DT_F32 ? 2 * (int64_t)ocols : ocols;
-  const int64_t n = orows * oc8;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < n; u += (int64_t)gridDim.x * 256) {
+  const int end = min(a.N, (b + 1) * HD_COEF);
+  for (int n = b * HD_COEF + threadIdx.x; n < end; n += 256)       // a NaN of live is the gradient's too
+    a.coef[n] = hd_has(n, a.target, a.ignore, a.live) ? (a.per_row ? a.g[n] * a.f / S : 1.f) * (a.live ? a.live[n] : 1.f) : 0.f;
+  if (b == 0 && threadIdx.x == 0) a.scal[SC_S] = S;
+}
+
+// out <- rows [0, R) of src (type dt, pitch ld, D columns), zeros elsewhere and in masked rows (their contents, whatever they
+// are, take no part in any sum).  f32: two numbers, and block 0 leaves the scale in scal[slot].
+__device__ __forceinline__ void hd_pack(const HdPrep& a, const HdPack& j, int b, bool masked, float* sh) {
+  float s = 1.f;
+  if (j.dt == DT_F32) {
+    s = hd_scale(hd_block_max<4>(a.amax[j.slot * HD_AMAX + threadIdx.x], sh));
+    if (b == 0 && threadIdx.x == 0) a.scal[j.slot] = s;
+  }
+  const int oc8 = j.ocols >> 3;
+  const int64_t pitch = j.dt == DT_F32 ? 2 * (int64_t)j.ocols : j.ocols;
+  const int64_t n = j.orows * oc8;
+  for (int64_t u = (int64_t)b * 256 + threadIdx.x; u < n; u += (int64_t)j.blocks * 256) {
     const int64_t r = u / oc8;
     const int c = (int)(u - r * oc8) * 8;
-    const bool live = r < R && (!coef || coef[r] != 0.f);
-    const int left = live ? min(8, D - c) : 0;
+    const bool live = r < j.R && (!masked || hd_has(r, a.target, a.ignore, a.live));
+    const int left = live ? min(8, j.D - c) : 0;
     s16x8 h = {0, 0, 0, 0, 0, 0, 0, 0}, l = h;
-    if (dt == DT_F32) {
+    if (j.dt == DT_F32) {
       float f[8];
-      const float* p = (const float*)src + r * ld + c;
+      const float* p = (const float*)j.src + r * j.ld + c;
       if (left == 8) {
         const RowVec<float, 8> v = *(const RowVec<float, 8>*)p;
 #pragma unroll
@@ -685,9 +757,9 @@ __global__ void __launch_bounds__(256) k_head_pack(const void* __restrict__ src,
         h[i] = __builtin_bit_cast(short, hi);
         l[i] = __builtin_bit_cast(short, lo);
       }
-      *(s16x8*)(out + r * pitch + ocols + c) = l;
+      *(s16x8*)(j.out + r * pitch + j.ocols + c) = l;
     } else {
-      const short* p = (const short*)src + r * ld + c;
+      const short* p = (const short*)j.src + r * j.ld + c;
       if (left == 8) {
         const RowVec<short, 8> v = *(const RowVec<short, 8>*)p;
 #pragma unroll
@@ -697,8 +769,16 @@ __global__ void __launch_bounds__(256) k_head_pack(const void* __restrict__ src,
         for (int i = 0; i < 8; ++i) h[i] = i < left ? p[i] : (short)0;
       }
     }
-    *(s16x8*)(out + r * pitch + c) = h;
+    *(s16x8*)(j.out + r * pitch + c) = h;
   }
+}
+
+__global__ void __launch_bounds__(256) k_head_prep(HdPrep a) {
+  __shared__ float sh[4];
+  const int b = blockIdx.x, bx = b - a.coef_blocks, bw = bx - a.x.blocks;
+  if (bx < 0) hd_coef(a, b, sh);
+  else if (bw < 0) hd_pack(a, a.x, bx, a.masked, sh);
+  else hd_pack(a, a.w, bw, false, sh);
 }
 
 __device__ __forceinline__ float hd_wave_sum(float v) {
@@ -934,24 +1014,6 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
   }
 }
 
-__device__ __forceinline__ bool hd_has(int n, const int64_t* target, int64_t ignore, const float* live) {
-  return target ? target[n] != ignore : live[n] != 0.f;
-}
-__device__ __forceinline__ float hd_finite_max(float m, float v) {
-  v = fabsf(v);
-  return v <= 3.402823466e38f ? fmaxf(m, v) : m;
-}
-// the maximum over a workgroup of 1024, in every thread
-__device__ __forceinline__ float hd_block_max(float m, float* sh) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
-  __syncthreads();
-  m = 0.f;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) m = fmaxf(m, sh[w]);
-  return m;
-}
 // gm[block] = the largest finite |g f| of HD_TOTAL rows' losses
 __global__ void __launch_bounds__(1024) k_head_gmax(const float* __restrict__ g, float f, const int64_t* __restrict__ target,
                                                      int64_t ignore, const float* __restrict__ live, int N, float* __restrict__ gm) {
@@ -960,36 +1022,8 @@ __global__ void __launch_bounds__(1024) k_head_gmax(const float* __restrict__ g,
   const int end = min(N, (int)(blockIdx.x + 1) * HD_TOTAL);
   for (int n = blockIdx.x * HD_TOTAL + threadIdx.x; n < end; n += 1024)
     if (hd_has(n, target, ignore, live)) m = hd_finite_max(m, g[n] * f);
-  m = hd_block_max(m, sh);
+  m = hd_block_max<16>(m, sh);
   if (threadIdx.x == 0) gm[blockIdx.x] = m;
-}
-
-// coef[n] (|.| <= 1, 0 for a row without a loss) and the scalar S with coef[n] S = the gradient of row n's logits' loss:
-// reductions: coef = 1 or 0, S = g f / count;  none: S = a power of two over max |g f| = max gm.  f: tau for the teacher's loss.
-// HD_TOTAL rows a workgroup.
-__global__ void __launch_bounds__(1024) k_head_coef(const float* __restrict__ g, const float* __restrict__ gm, int ngm,
-                                                     const float* __restrict__ count, float f, const int64_t* __restrict__ target,
-                                                     int64_t ignore, const float* __restrict__ live, int N,
-                                                     float* __restrict__ coef, float* __restrict__ scal) {
-  __shared__ float sh[16];
-  float S = 1.f;
-  if (gm) {
-    float m = 0.f;
-    for (int i = threadIdx.x; i < ngm; i += 1024) m = fmaxf(m, gm[i]);
-    m = hd_block_max(m, sh);
-    if (m > 0.f) {
-      int e;
-      frexpf(m, &e);
-      S = ldexpf(1.f, min(max(e, -100), 100));
-    }
-  } else {
-    S = g[0] * f / (count ? *count : 1.f);
-  }
-  // live is NaN for a row that lists a class that does not exist: its gradient says so too
-  const int end = min(N, (int)(blockIdx.x + 1) * HD_TOTAL);
-  for (int n = blockIdx.x * HD_TOTAL + threadIdx.x; n < end; n += 1024)
-    coef[n] = hd_has(n, target, ignore, live) ? (gm ? g[n] * f / S : 1.f) * (live ? live[n] : 1.f) : 0.f;
-  if (blockIdx.x == 0 && threadIdx.x == 0) scal[SC_S] = S;
 }
 
 // teacher: the listed classes of this piece get e = c (softmax_k - q_k), from the entry's own logit, over what the
@@ -1050,35 +1084,50 @@ __global__ void __launch_bounds__(256) k_head_colsum(const short* __restrict__ E
   }
 }
 
-// out[at0 + i] = factor * sum_s part[s][i] over `slots` partials: in order, or where there are many of few results (see
-// hd_sum) by 16 lanes of 16 results, each lane every 16th partial, and the lanes in order
-template <class T, bool MANY>
-__global__ void __launch_bounds__(256) k_head_sum(const float* __restrict__ part, int slots, int64_t stride, int64_t n,
-                                                   const float* __restrict__ scal, int other, void* __restrict__ out, int dt,
-                                                   int64_t at0) {
-  const float f = scal ? hd_factor<T>(scal, other) : 1.f;
-  if constexpr (MANY) {
-    __shared__ float sh[16][17];
+// out[at0 + i] = factor * sum_s part[s][i] over `slots` partials: in order, or `many` (see hd_sums) by 16 lanes of 16 results, each
+// lane every 16th partial, and the lanes in order.  Up to three such sums in one launch.
+struct HdSum {
+  const float* part;
+  int slots;
+  int64_t stride, n;
+  int other;                 // its factor (hd_factor)
+  void* out;
+  int64_t at0;
+  int many, blocks;
+};
+struct HdSums {
+  HdSum j[3];
+  int dt;
+  const float* scal;         // null: factors of 1
+};
+template <class T>
+__global__ void __launch_bounds__(256) k_head_sum(HdSums a) {
+  __shared__ float sh[16][17];
+  int b = blockIdx.x, k = 0;
+  while (k < 2 && b >= a.j[k].blocks) b -= a.j[k++].blocks;
+  const HdSum& j = a.j[k];
+  const float f = a.scal ? hd_factor<T>(a.scal, j.other) : 1.f;
+  if (j.many) {
     const int col = threadIdx.x & 15, sl = threadIdx.x >> 4;
-    const int64_t i = (int64_t)blockIdx.x * 16 + col;
+    const int64_t i = (int64_t)b * 16 + col;
     float s = 0.f;
-    if (i < n) {
+    if (i < j.n) {
 #pragma unroll 8
-      for (int k = sl; k < slots; k += 16) s += part[(int64_t)k * stride + i];
+      for (int q = sl; q < j.slots; q += 16) s += j.part[(int64_t)q * j.stride + i];
     }
     sh[sl][col] = s;
     __syncthreads();
-    if (sl != 0 || i >= n) return;
+    if (sl != 0 || i >= j.n) return;
     s = 0.f;
 #pragma unroll
     for (int q = 0; q < 16; ++q) s += sh[q][col];
-    store_as(out, dt, at0 + i, s * f);
+    store_as(j.out, a.dt, j.at0 + i, s * f);
   } else {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-      float s = part[i];
+    for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < j.n; i += (int64_t)j.blocks * 256) {
+      float s = j.part[i];
 #pragma unroll 8
-      for (int k = 1; k < slots; ++k) s += part[(int64_t)k * stride + i];
-      store_as(out, dt, at0 + i, s * f);
+      for (int q = 1; q < j.slots; ++q) s += j.part[(int64_t)q * j.stride + i];
+      store_as(j.out, a.dt, j.at0 + i, s * f);
     }
   }
 }
@@ -1277,22 +1326,32 @@ static inline unsigned hd_grid(int64_t items, int per) {
   return (unsigned)(b < 1 ? 1 : b < cap ? b : cap);
 }
 
-// the sum of partial results.  us in order / by 16 lanes:  2140 results of 64 partials 6.0 / 4.0, 32768 of 16: 5.4 / 4.8; 574 of 32
-// in order 4.1, of 512 by 16 lanes 4.0
+// one of a launch's sums.  us in order / by 16 lanes:  2140 results of 64 partials 6.0 / 4.0, 32768 of 16: 5.4 / 4.8; 574 of 32 in
+// order 4.1, of 512 by 16 lanes 4.0
+static void hd_add_sum(HdSums& a, const float* part, int slots, int64_t stride, int64_t n, int other, void* out, int64_t at0) {
+  int k = 0;
+  while (a.j[k].blocks) ++k;
+  const bool many = slots >= 16 && n <= 65536;
+  a.j[k] = {part, slots, stride, n, other, out, at0, many, many ? (int)((n + 15) / 16) : (int)hd_grid(n, 256)};
+}
 template <class T>
-static void hd_sum(const float* part, int slots, int64_t stride, int64_t n, const float* scal, int other, void* out, int dt, int64_t at0,
-                   hipStream_t st) {
-  if (slots >= 16 && n <= 65536)
-    hipLaunchKernelGGL((k_head_sum<T, true>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, part, slots, stride, n, scal, other, out, dt,
-                       at0);
-  else
-    hipLaunchKernelGGL((k_head_sum<T, false>), dim3(hd_grid(n, 256)), dim3(256), 0, st, part, slots, stride, n, scal, other, out, dt, at0);
+static int hd_sums(const HdSums& a, hipStream_t st) {
+  const int blocks = a.j[0].blocks + a.j[1].blocks + a.j[2].blocks;
+  if (!blocks) return DIG3D_OK;
+  hipLaunchKernelGGL((k_head_sum<T>), dim3(blocks), dim3(256), 0, st, a);
+  DIG3D_CHECK_LAUNCH();
+  return DIG3D_OK;
 }
 
-static void hd_pack(const void* src, int dt, int64_t ld, int64_t R, int D, const float* coef, const float* amax, int slot,
-                    float* scal, short* out, int64_t orows, int ocols, hipStream_t st) {
-  hipLaunchKernelGGL(k_head_pack, dim3(hd_grid(orows * (ocols >> 3), 256)), dim3(256), 0, st, src, dt, ld, R, D, coef, amax,
-                     slot, scal, out, orows, ocols);
+static HdPack hd_pack_job(const void* src, int dt, int64_t ld, int64_t R, int D, void* out, int64_t orows, int ocols, int slot) {
+  return {src, dt, ld, R, D, (short*)out, orows, ocols, slot, (int)hd_grid(orows * (ocols >> 3), 256)};
+}
+static int hd_prep(const HdPrep& a, hipStream_t st) {
+  const int blocks = a.coef_blocks + a.x.blocks + a.w.blocks;
+  if (!blocks) return DIG3D_OK;
+  hipLaunchKernelGGL(k_head_prep, dim3(blocks), dim3(256), 0, st, a);
+  DIG3D_CHECK_LAUNCH();
+  return DIG3D_OK;
 }
 
 static bool hd_bad(int dt, int N, int D, int V, int64_t ldx, int64_t ldw) {
@@ -1368,11 +1427,14 @@ static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
   }
   HdArgs a;
   memset(&a, 0, sizeof a);
+  HdPrep prep;
+  memset(&prep, 0, sizeof prep);
+  prep.amax = c.amax;
+  prep.scal = c.scal;
   const int two = p.pair ? 2 : 1;          // numbers of a value
   if (p.dx) a.Q = {(const short*)c.x, c.ldx, 0, c.N, c.D};
   else {
-    hd_pack(c.x, c.dt, c.ldx, c.N, c.D, nullptr, c.amax, SC_X, c.scal, (short*)(ws + p.o_x), p.Np, p.Dp, c.st);
-    DIG3D_CHECK_LAUNCH();
+    prep.x = hd_pack_job(c.x, c.dt, c.ldx, c.N, c.D, ws + p.o_x, p.Np, p.Dp, SC_X);
     a.Q = {at_bytes(ws, p.o_x), (int64_t)p.Dp * two, p.Dp, c.N, p.Dp};
   }
   a.nj = c.N;
@@ -1393,10 +1455,12 @@ static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
     const char* wp = (const char*)c.w + v0 * c.ldw * esz;
     if (p.dw) a.P = {(const short*)wp, c.ldw, 0, nv, c.D};
     else {
-      hd_pack(wp, c.dt, c.ldw, nv, c.D, nullptr, c.amax, SC_W, c.scal, (short*)(ws + p.o_w), nv, p.Dp, c.st);
-      DIG3D_CHECK_LAUNCH();
+      prep.w = hd_pack_job(wp, c.dt, c.ldw, nv, c.D, ws + p.o_w, nv, p.Dp, SC_W);
       a.P = {at_bytes(ws, p.o_w), (int64_t)p.Dp * two, p.Dp, nv, p.Dp};
     }
+    const int rc = hd_prep(prep, c.st);
+    if (rc != DIG3D_OK) return rc;
+    prep.x.blocks = 0;                     // once
     a.ni = nv;
     a.v0 = v0;
     a.part_c0 = (int)(v0 / p.lg.b);
@@ -1489,8 +1553,11 @@ static int hd_bwd_small(const HdCall& c, const HdPlan& p, const float* g, void* 
   DIG3D_CHECK_LAUNCH();
   if (a.slots) {
     const int64_t n = (int64_t)c.N * c.D;
-    hd_sum<bf16_t>(a.slots, p.gx.splits, n, n, nullptr, -1, gx, c.dt, 0, c.st);
-    DIG3D_CHECK_LAUNCH();
+    HdSums sums;
+    memset(&sums, 0, sizeof sums);
+    sums.dt = c.dt;
+    hd_add_sum(sums, a.slots, p.gx.splits, n, n, -1, gx, 0);
+    return hd_sums<bf16_t>(sums, c.st);
   }
   return DIG3D_OK;
 }
@@ -1498,20 +1565,30 @@ static int hd_bwd_small(const HdCall& c, const HdPlan& p, const float* g, void* 
 template <class T>
 static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw, void* gb, char* ws) {
   c.scal = (float*)(ws + p.o_scal);        // what the forward kept is read only: several backward passes may use it
-  float* coef = (float*)(ws + p.o_coef);
-  const int blocks = (c.N + HD_TOTAL - 1) / HD_TOTAL;
-  const float f = c.index ? c.tau : 1.f, *live = c.index ? c.live : nullptr;
-  float* gm = c.reduction == 0 ? (float*)(ws + p.o_scal) + SC_COUNT : nullptr;
-  if (gm) {
-    hipLaunchKernelGGL(k_head_gmax, dim3(blocks), dim3(1024), 0, c.st, g, f, c.target, c.ignore, live, c.N, gm);
+  const int two = p.pair ? 2 : 1;          // numbers of a value
+  HdPrep prep;
+  memset(&prep, 0, sizeof prep);
+  prep.x = hd_pack_job(c.x, c.dt, c.ldx, c.N, c.D, ws + p.o_x, p.Np, p.Dp, SC_X);
+  prep.masked = 1;
+  prep.amax = c.amax;
+  prep.scal = c.scal;
+  prep.coef_blocks = (c.N + HD_COEF - 1) / HD_COEF;
+  prep.g = g;
+  prep.per_row = c.reduction == 0;
+  prep.count = c.reduction == 1 ? c.count : nullptr;
+  prep.f = c.index ? c.tau : 1.f;
+  prep.target = c.target;
+  prep.ignore = c.ignore;
+  prep.live = c.index ? c.live : nullptr;
+  prep.N = c.N;
+  prep.coef = (float*)(ws + p.o_coef);
+  if (prep.per_row && prep.coef_blocks > 1) {
+    float* gm = c.scal + SC_COUNT;
+    prep.gm = gm;
+    prep.ngm = (c.N + HD_TOTAL - 1) / HD_TOTAL;
+    hipLaunchKernelGGL(k_head_gmax, dim3(prep.ngm), dim3(1024), 0, c.st, g, prep.f, c.target, c.ignore, prep.live, c.N, gm);
     DIG3D_CHECK_LAUNCH();
   }
-  hipLaunchKernelGGL(k_head_coef, dim3(blocks), dim3(1024), 0, c.st, g, gm, blocks, c.reduction == 1 ? c.count : (const float*)nullptr,
-                     f, c.target, c.ignore, live, c.N, coef, c.scal);
-  DIG3D_CHECK_LAUNCH();
-  const int two = p.pair ? 2 : 1;          // numbers of a value
-  hd_pack(c.x, c.dt, c.ldx, c.N, c.D, coef, c.amax, SC_X, c.scal, (short*)(ws + p.o_x), p.Np, p.Dp, c.st);
-  DIG3D_CHECK_LAUNCH();
   short* E = (short*)(ws + p.o_E);
   const HdOperand x = {at_bytes(ws, p.o_x), (int64_t)p.Dp * two, p.Dp, (int)p.Np, p.Dp};
   const HdOperand e = {E, p.ldE * p.eplanes, p.ldE, (int)p.Np, (int)p.ldE};
@@ -1523,10 +1600,16 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     HdOperand W;
     if (p.dw) W = {(const short*)wsrc, c.ldw, 0, nv, c.D};
     else {
-      hd_pack(wsrc, c.dt, c.ldw, nv, c.D, nullptr, c.amax, SC_W, c.scal, (short*)(ws + p.o_w), nv, p.Dp, c.st);
-      DIG3D_CHECK_LAUNCH();
+      prep.w = hd_pack_job(wsrc, c.dt, c.ldw, nv, c.D, ws + p.o_w, nv, p.Dp, SC_W);
       W = {at_bytes(ws, p.o_w), (int64_t)p.Dp * two, p.Dp, nv, p.Dp};
     }
+    const int rc = hd_prep(prep, c.st);
+    if (rc != DIG3D_OK) return rc;
+    prep.x.blocks = prep.coef_blocks = 0;  // once
+    HdSums sums;
+    memset(&sums, 0, sizeof sums);
+    sums.dt = c.dt;
+    sums.scal = c.scal;
     HdArgs a;
     memset(&a, 0, sizeof a);
     a.P = W;
@@ -1545,7 +1628,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     a.m = c.m;
     a.rs = c.rs;
     a.loss = c.loss;
-    a.coef = coef;
+    a.coef = prep.coef;
     a.eplanes = p.eplanes;
     a.E = E;
     a.colsE = p.ldE;
@@ -1553,7 +1636,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, p.pair, c.st);
     DIG3D_CHECK_LAUNCH();
     if (c.index) {
-      const int rc = hd_teacher_grad<T>(c, coef, v0, nv, p.eplanes, E, p.ldE);
+      const int rc = hd_teacher_grad<T>(c, prep.coef, v0, nv, p.eplanes, E, p.ldE);
       if (rc != DIG3D_OK) return rc;
     }
     HdArgs o;
@@ -1589,11 +1672,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
       o.other = p.pair ? SC_X : -1;
       hd_gemm<T, true, true, EPI_OUT>(o, p.gw, p.pair, c.st);
       DIG3D_CHECK_LAUNCH();
-      if (slots) {
-        const int64_t n = (int64_t)nv * c.D;
-        hd_sum<T>((const float*)(ws + p.o_gw), p.gw.splits, n, n, c.scal, o.other, gw, c.dt, v0 * c.D, c.st);
-        DIG3D_CHECK_LAUNCH();
-      }
+      if (slots) hd_add_sum(sums, (const float*)(ws + p.o_gw), p.gw.splits, (int64_t)nv * c.D, (int64_t)nv * c.D, o.other, gw, v0 * c.D);
     }
     if (gb) {
       float* part = (float*)(ws + p.o_col);
@@ -1601,14 +1680,12 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
       hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)slices, (unsigned)((p.ldE + 255) / 256)), dim3(256), 0, c.st, E, p.ldE,
                          p.eplanes, c.N, part);
       DIG3D_CHECK_LAUNCH();
-      hd_sum<T>(part, slices, p.ldE, nv, c.scal, -1, gb, c.dt, v0, c.st);
-      DIG3D_CHECK_LAUNCH();
+      hd_add_sum(sums, part, slices, p.ldE, nv, -1, gb, v0);
     }
-  }
-  if (gx_slots) {
-    const int64_t n = (int64_t)c.N * c.D;
-    hd_sum<T>((const float*)(ws + p.o_gx), p.gx.splits, n, n, c.scal, p.pair ? SC_W : -1, gx, c.dt, 0, c.st);
-    DIG3D_CHECK_LAUNCH();
+    if (gx_slots && v0 + p.vp >= c.V)
+      hd_add_sum(sums, (const float*)(ws + p.o_gx), p.gx.splits, (int64_t)c.N * c.D, (int64_t)c.N * c.D, p.pair ? SC_W : -1, gx, 0);
+    const int rs = hd_sums<T>(sums, c.st);
+    if (rs != DIG3D_OK) return rs;
   }
   return DIG3D_OK;
 }
