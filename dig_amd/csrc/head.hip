@@ -491,19 +491,20 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
   s16x8 fp[2][HX], fq[2][MJ];
   f32x4 acc[MI][MJ];
   // half `kk` of the tiles' depth (PAIR: the first or second numbers) of half `hx` of the wave's P, and of its Q, into a buffer each
-  // The addresses are formed anew from one register each time: kept per operand and stage they would not fit (the empty asm
-  // keeps the compiler from doing so), and a spilled one is a load that waits for the tiles' loads
+  // PAIR: the addresses are formed anew from one register each time.  Kept per operand and stage they would not fit beside both
+  // numbers' operands (the empty asm keeps the compiler from doing so), and a spilled one is a load that waits for the tiles'
+  // loads: 4096 x 1024 x 32000 at 1000 us instead of 640 a product.  Single numbers have the registers, and lose 3 % without them.
   constexpr bool pairs = EPI != EPI_OUT;
   const uint32_t ap = hd_at<BI, PT, pairs>(lds0, wi, lane), aq = hd_at<BJ, QT, false>(lds0 + hd_tile_shorts<BI>() * 2, wj, lane);
   auto read_p = [&](int stage, int kk, int hx) __attribute__((always_inline)) {
     uint32_t at = ap + stage * (SZ * 2);
-    asm volatile("" : "+v"(at));
+    if constexpr (PAIR) asm volatile("" : "+v"(at));
 #pragma unroll
     for (int x = 0; x < HX; ++x) fp[hx][x] = hd_frag<BI, PT, pairs>(at, hx * HX + x, kk);
   };
   auto read_q = [&](int stage, int kk, int buf) __attribute__((always_inline)) {
     uint32_t at = aq + stage * (SZ * 2);
-    asm volatile("" : "+v"(at));
+    if constexpr (PAIR) asm volatile("" : "+v"(at));
 #pragma unroll
     for (int y = 0; y < MJ; ++y) fq[buf][y] = hd_frag<BJ, QT, false>(at, y, kk);
   };
