@@ -1203,21 +1203,26 @@ static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
 // 2.06 / 2.04 / 2.03 / 1.98   1741 x 114 x 118479 f32 1.52 / 1.41 / 1.33 / 1.34: the last-level cache returns nothing for it
 #define HD_PIECE_BYTES (512ll << 20)
 
-// Float32 products in place (head_small.h) where copies and launches are what the general path costs (GPU us of value and
-// gradients, in place / general):
-//   f32:  32 x 128 x 1195: 39 / 96   512 x 128 x 1195: 65 / 118   2048 x 128 x 1195: 149 / 148   32 x 128 x 32768: 90 / 115
-//         128 x 512 x 1024: 73 / 83   512 x 512 x 256: 89 / 84   8 x 1024 x 1024: 106 / 98   4096 x 128 x 64: 206 / 76
-//   bf16: 32 x 128 x 1195: 42 / 70   512 x 128 x 1195: 67 / 81   32 x 128 x 8192: 51 / 46   8 x 512 x 4096: 75 / 45
-// 16-bit rows that the general path copies (odd widths or addresses) count as f32 there.  And where few float32 rows meet a
-// W that the general path would read four times (its scale, its planes twice) before the first product is done (losses
-// alone, in place / general, and with gradients):
-//   1 x 1024 x 1024: 50 / 43, 105 / 96   1 x 1024 x 8192: 51 / 57, 131 / 140   16 x 2048 x 32768: 115 / 265, 421 / 635
-//   64 x 1024 x 32768: 78 / 127, 272 / 356   256 x 1024 x 32768: 188 / 137, 742 / 446
-// (16-bit rows, copied: 16 x 2047 x 32768: 134 / 87, 536 / 341).  A wave joins a row's V / 64 statistics: up to 2^20 classes.
+// Float32 products in place (head_small.h) where copies and launches are what the general path costs, or where few float32 rows meet
+// a W that it would read three times (its scale, its copy) before the first product is done.  GPU us in place / general, with
+// gradients (losses alone).  A training call is five launches in place and eight to eleven otherwise, which a host that
+// launches them one by one pays with some 15 us: the border is where the GPU loses that much.
+//   f32: 128 x 128 x 1195: 41 / 54 (20 / 24)   512 x 128 x 1195: 64 / 58 (19 / 25)   1024 x 128 x 1195: 98 / 64   512 x 128 x 4096: 77 / 72 (21 / 27)
+//        256 x 128 x 16384: 99 / 87 (29 / 34)   64 x 256 x 1024: 50 / 56 (25 / 28)   64 x 256 x 32768: 116 / 117 (42 / 56)
+//        128 x 512 x 1024: 73 / 64   256 x 512 x 1024: 82 / 67   8 x 1024 x 1024: 103 / 70   64 x 512 x 16384: 116 / 116 (41 / 52)
+//        1 x 1024 x 8192: 130 / 108 (52 / 46)   16 x 1024 x 16384: 156 / 155 (52 / 62)   64 x 2048 x 32768: 523 / 610 (128 / 258)
+//   16-bit rows read in place by both: 32 x 128 x 1195: 38 / 39   128 x 64 x 300: 37 / 42   32 x 128 x 8192: 44 / 40   512 x 128 x 256: 60 / 44
+//   16-bit rows that the general path copies (odd widths or addresses): 32 x 127 x 8192: 46 / 47   14 x 40 x 67126: 67 / 83
+//        64 x 127 x 32768: 95 / 84   128 x 127 x 4096: 57 / 49   16 x 255 x 8192: 56 / 52   10 x 214 x 105058: 225 / 165   512 x 127 x 1195: 84 / 53   128 x 511 x 1024: 87 / 55
+// A wave joins a row's V / 64 statistics: up to 2^20 classes.
 static bool hd_small(bool f32, bool copies, int64_t N, int64_t D, int64_t V) {
   const double work = (double)N * D * V;
-  if (f32 && N <= 64 && V >= 4096 && V <= 1048576) return true;
-  return N <= 512 && (copies ? D <= 512 && work <= 134217728.0 : D <= 128 && work <= 16777216.0);
+  if (V > 1048576) return false;
+  if (f32)
+    return (N <= 512 && D <= 128 && work <= 268435456.0) || (N <= 128 && D <= 512 && work <= 134217728.0) ||
+           (N <= 64 && (D <= 256 || V >= 16384));
+  if (N > 128 || D > (copies ? 256 : 128)) return false;
+  return work <= (!copies || D > 128 ? 33554432.0 : N <= 64 ? 268435456.0 : 67108864.0);
 }
 
 // k steps of a product over `k` values, one operand of `q` numbers each

@@ -845,9 +845,9 @@ def test_temperatures_out_of_range_are_refused():
             ops.linear_distillation(x, w, idx, tl, temperature=tau)
 
 
-@pytest.mark.parametrize('N,D,V', [(1, 1024, 4096), (16, 515, 5001), (64, 96, 20000)])
+@pytest.mark.parametrize('N,D,V', [(1, 1024, 4096), (16, 515, 5001), (16, 515, 17001), (64, 96, 20000), (200, 100, 3000)])
 def test_few_float32_rows_of_many_classes(N, D, V):
-    """sizes that float32 takes in place and 16-bit rows do not"""
+    """sizes around those that float32 takes in place and 16-bit rows do not"""
     one_classes(N, D, V, torch.float32, True, 'none', 0.2)
     one_teacher(N, D, V, 12, torch.float32, False, 'mean', True, 2.0)
 

@@ -38,7 +38,7 @@ def test_head_workspace():
     # 16-bit rows of whole k steps are read in place; odd widths, odd pitches and odd addresses are copied
     direct = q(1, 64, 128, 40960, 0, 0)
     assert direct < q(1, 64, 127, 40960, 0, 0) and direct < q(1, 64, 128, 40960, 0, 0, ptr=2) and direct < q(1, 64, 128, 40960, 0, 0, ld=129)
-    assert q(1, 64, 128, 4096, 0, 0) == q(1, 64, 128, 4096, 0, 0, ptr=2)      # small products read anything in place
+    assert q(1, 32, 128, 1024, 0, 0) == q(1, 32, 128, 1024, 0, 0, ptr=2)      # small products read anything in place
     # the backward's workspace is bounded in the vocabulary: e in pieces of at most 512 MiB per plane
     big, bigger = q(1, 4096, 1024, 1 << 17, 1, 7), q(1, 4096, 1024, 1 << 20, 1, 7)
     assert bigger <= big + (64 << 10) and bigger < (1 << 21)
