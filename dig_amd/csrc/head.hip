@@ -833,14 +833,12 @@ __global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ pa
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= N) return;
   float m, r, v;
-  hd_join_row(part + n * tiles, tiles, V, target != nullptr, target ? target[n] : 0, ignore, zt + n, lane, m, r, v);
+  hd_join_row(part + n * tiles, tiles, V, true, target[n], ignore, zt + n, lane, m, r, v);
   if (lane == 0) {
     mo[n] = m;
     rs[n] = r;
-    if (target) {
-      loss[n] = v;
-      if (rows_out) rows_out[n] = v;
-    }
+    loss[n] = v;
+    if (rows_out) rows_out[n] = v;
   }
 }
 
@@ -910,7 +908,7 @@ __global__ void __launch_bounds__(1024) k_head_join_total(const float2* __restri
 
 #define TC_MAX 2048          // a teacher's entries per row (16 bytes of LDS each)
 
-// teacher: a workgroup per row.  q [N, K]: the softmax over the row's listed classes of t / tau, summed over the entries of
+// teacher: a workgroup per row, whose statistics its first wave joins beside the teacher's softmax.  q [N, K]: the softmax over the row's listed classes of t / tau, summed over the entries of
 // the same class, -1 for an absent entry (negative index, or logit -inf); z [N, K]: the student's own logits / tau there;
 // loss[n]; live[n] = 1, 0 without entries, NaN with an index that is no class.  (t - max) / tau is kept finite, so that a
 // listed logit of the type's lowest value is not an absent entry at any tau.  A wave forms four logits at a time: the
@@ -919,16 +917,25 @@ template <class T>
 __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, const T* __restrict__ w, const void* __restrict__ bias,
                                                        int dt, int64_t ldx, int64_t ldw, int D, int64_t V,
                                                        const int64_t* __restrict__ index, const void* __restrict__ tl, int tdt, int K,
-                                                       float inv_tau, float tau, const float* __restrict__ mo, const float* __restrict__ rs,
+                                                       float inv_tau, float tau, const float2* __restrict__ stats, int tiles,
+                                                       float* __restrict__ mo, float* __restrict__ rs,
                                                        float* __restrict__ q, float* __restrict__ z, float* __restrict__ loss, float* __restrict__ live,
                                                        float* __restrict__ rows_out) {
   constexpr int N8 = VecLen<T>::n;
   extern __shared__ int64_t dyn[];         // index [K] (-1: absent), then t, then (t - max) / tau [K], then q [K]
   float* st = (float*)(dyn + K);
   float* sq = st + K;
-  __shared__ float sh[8];
+  __shared__ float sh[8], own[2];
   const int64_t n = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (wave == 0) {
+    float jm, jr, jl;
+    hd_join_row(stats + n * tiles, tiles, V, false, 0, 0, nullptr, lane, jm, jr, jl);
+    if (lane == 0) {
+      mo[n] = own[0] = jm;
+      rs[n] = own[1] = jr;
+    }
+  }
   float m = -INFINITY;
   for (int k = tid; k < K; k += 256) {
     const int64_t v = index[n * K + k];
@@ -956,7 +963,7 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
   s = (sh[4] + sh[5]) + (sh[6] + sh[7]);
   const bool any = s > 0.f || s != s;      // a NaN among the listed logits is not an empty row
   const float ls = any ? logf(s) : 0.f;
-  const float sm = mo[n], sl = logf(rs[n]);   // the student's log softmax is z - sm + sl
+  const float sm = own[0], sl = logf(own[1]);   // the student's log softmax is z - sm + sl
   for (int k = tid; k < K; k += 256) sq[k] = dyn[k] < 0 ? 0.f : expf(st[k] - ls);
   __syncthreads();
   const T* xr = x + n * ldx;
@@ -1495,16 +1502,17 @@ static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
     return DIG3D_OK;
   }
   float* rows_out = c.reduction ? nullptr : out;
-  hipLaunchKernelGGL(k_head_join, dim3((c.N + 3) / 4), dim3(256), 0, c.st, part, p.tiles_all, c.N, (int64_t)c.V, c.target, c.ignore, zt,
-                     c.m, c.rs, c.loss, rows_out);
-  DIG3D_CHECK_LAUNCH();
-  if (c.index) {
+  if (!c.index) {
+    hipLaunchKernelGGL(k_head_join, dim3((c.N + 3) / 4), dim3(256), 0, c.st, part, p.tiles_all, c.N, (int64_t)c.V, c.target, c.ignore, zt,
+                       c.m, c.rs, c.loss, rows_out);
+    DIG3D_CHECK_LAUNCH();
+  } else {
     const dim3 g((unsigned)c.N), b(256);
     const size_t lds = (size_t)c.K * 16;
     const float it = 1.0f / c.tau;
 #define TC_GO(T)                                                                                                                       \
   hipLaunchKernelGGL((k_head_teacher<T>), g, b, lds, c.st, (const T*)c.x, (const T*)c.w, c.bias, c.dt, c.ldx, c.ldw, c.D, (int64_t)c.V, \
-                     c.index, c.teacher, c.tdt, c.K, it, c.tau, c.m, c.rs, c.q, c.z, c.loss, c.live, rows_out)
+                     c.index, c.teacher, c.tdt, c.K, it, c.tau, part, p.tiles_all, c.m, c.rs, c.q, c.z, c.loss, c.live, rows_out)
     if (c.dt == DT_F32) TC_GO(float);
     else if (c.dt == DT_BF16) TC_GO(bf16_t);
     else TC_GO(f16_t);
