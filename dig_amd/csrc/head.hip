@@ -584,63 +584,6 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
 #include "head_small.h"
 
 // ---- kernels around the products ---------------------------------------------------------------------------------------------------------
-// does row n have a loss: its target is not `ignore`, or its teacher lists a class.  Called by whole waves
-__device__ __forceinline__ bool hd_live(int64_t n, const int64_t* target, int64_t ignore, const int64_t* index, const void* tl, int tdt,
-                                        int K, int lane) {
-  if (target) return target[n] != ignore;
-  bool any = false;
-  for (int k = lane; k < K; k += 64) any |= index[n * K + k] >= 0 && load_as(tl, tdt, n * K + k) != -INFINITY;
-  return __any(any);
-}
-
-// partial max |v| over the finite entries of x's rows that have a loss (blocks [0, HD_AMAX); what the others hold, the
-// lowest value of a mask say, must not set the scale) and of W (the rest): amax[2 HD_AMAX]
-#define HD_AMAX 256
-__global__ void __launch_bounds__(256) k_head_amax(const float* __restrict__ x, int64_t ldx, int64_t R, const float* __restrict__ w,
-                                                    int64_t ldw, int64_t V, int D, const int64_t* __restrict__ target, int64_t ignore,
-                                                    const int64_t* __restrict__ index, const void* __restrict__ tl, int tdt, int K,
-                                                    float* __restrict__ amax) {
-  __shared__ float sh[4];
-  const int lane = threadIdx.x & 63;
-  const bool second = blockIdx.x >= HD_AMAX;
-  const float* p = second ? w : x;
-  const int64_t ld = second ? ldw : ldx, rows = second ? V : R;
-  const int b = second ? blockIdx.x - HD_AMAX : blockIdx.x;
-  float m = 0.f;
-  auto see = [&](float v) {
-    v = fabsf(v);
-    m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
-  };
-  if (second && ld == D) {
-    const int64_t n = rows * D, n4 = n >> 2;
-    const RowVec<float, 4>* q = (const RowVec<float, 4>*)p;
-#pragma unroll 4
-    for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n4; i += HD_AMAX * 256) {
-      const RowVec<float, 4> v = q[i];
-      see(v.v[0]); see(v.v[1]); see(v.v[2]); see(v.v[3]);
-    }
-    if (b == 0 && (int64_t)threadIdx.x < (n & 3)) see(p[n - 1 - threadIdx.x]);
-  } else {
-    for (int64_t r = b * 4 + (threadIdx.x >> 6); r < rows; r += HD_AMAX * 4) {
-      if (!second && !hd_live(r, target, ignore, index, tl, tdt, K, lane)) continue;
-      for (int d = lane; d < D; d += 64) see(p[r * ld + d]);
-    }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (lane == 0) sh[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) amax[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-}
-
-// 2^k with 2^k m in [2^14, 2^15); 1 for an all-zero tensor.  -113 <= k <= 100: 2^k and 2^-k are normal numbers.
-__device__ __forceinline__ float hd_scale(float m) {
-  if (!(m > 0.f)) return 1.f;
-  int e;
-  frexpf(m, &e);
-  return ldexpf(1.f, min(15 - e, 100));
-}
-
 __device__ __forceinline__ float hd_wave_max(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
@@ -657,6 +600,85 @@ __device__ __forceinline__ float hd_block_max(float m, float* sh) {
   for (int w = 0; w < NW; ++w) m = fmaxf(m, sh[w]);
   return m;
 }
+// does row n's teacher list a class.  Called by whole waves
+__device__ __forceinline__ bool hd_listed(int64_t n, const int64_t* index, const void* tl, int tdt, int K, int lane) {
+  bool any = false;
+  for (int k = lane; k < K; k += 64) any |= index[n * K + k] >= 0 && load_as(tl, tdt, n * K + k) != -INFINITY;
+  return __any(any);
+}
+
+// partial max |v| over the finite entries of x's rows that have a loss (blocks [0, HD_AMAX); what the others hold, the
+// lowest value of a mask say, must not set the scale) and of W (the rest): amax[2 HD_AMAX]
+#define HD_AMAX 256
+__global__ void __launch_bounds__(512) k_head_amax(const float* __restrict__ x, int64_t ldx, int64_t R, const float* __restrict__ w,
+                                                    int64_t ldw, int64_t V, int D, const int64_t* __restrict__ target, int64_t ignore,
+                                                    const int64_t* __restrict__ index, const void* __restrict__ tl, int tdt, int K,
+                                                    float* __restrict__ amax) {
+  __shared__ float sh[8];
+  const int lane = threadIdx.x & 63;
+  const bool second = blockIdx.x >= HD_AMAX;
+  const float* p = second ? w : x;
+  const int64_t ld = second ? ldw : ldx, rows = second ? V : R;
+  const int b = second ? blockIdx.x - HD_AMAX : blockIdx.x;
+  float m = 0.f;
+  auto see = [&](float v) {
+    v = fabsf(v);
+    m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
+  };
+  if (second && ld == D) {
+    const int64_t n = rows * D, n4 = n >> 2;
+    const RowVec<float, 4>* q = (const RowVec<float, 4>*)p;
+#pragma unroll 4
+    for (int64_t i = (int64_t)b * 512 + threadIdx.x; i < n4; i += HD_AMAX * 512) {
+      const RowVec<float, 4> v = q[i];
+      see(v.v[0]); see(v.v[1]); see(v.v[2]); see(v.v[3]);
+    }
+    if (b == 0 && (int64_t)threadIdx.x < (n & 3)) see(p[n - 1 - threadIdx.x]);
+  } else {
+    // a wave takes up to 64 rows at a time, fewer where that would leave waves idle, looks which of them have a loss, then
+    // its lanes read 4 entries each of as many rows as they hold
+    const int most = (int)min((int64_t)64, (rows + HD_AMAX * 8 - 1) / (HD_AMAX * 8));
+    int lpr = 1;
+    while (lpr < 64 && lpr * 4 < D) lpr *= 2;
+    const int rpi = 64 / lpr, mine = lane / lpr, d0 = lane % lpr * 4;
+    for (int64_t r0 = (int64_t)(b * 8 + (threadIdx.x >> 6)) * most; r0 < rows; r0 += (int64_t)HD_AMAX * 8 * most) {
+      const int n = (int)min((int64_t)most, rows - r0);
+      uint64_t live = ~0ull;
+      if (!second && target) {
+        live = __ballot(lane < n && target[r0 + lane] != ignore);
+      } else if (!second) {
+        live = 0;
+#pragma unroll 4
+        for (int r = 0; r < n; ++r) live |= (uint64_t)hd_listed(r0 + r, index, tl, tdt, K, lane) << r;
+      }
+#pragma unroll 4
+      for (int q = 0; q < n; q += rpi) {
+        const int r = q + mine;
+        if (r >= n || !(live >> r & 1)) continue;
+        const float* row = p + (r0 + r) * ld;
+        for (int d = d0; d < D; d += lpr * 4) {
+          if (d + 4 <= D) {
+            const RowVec<float, 4> v = *(const RowVec<float, 4>*)(row + d);
+            see(v.v[0]); see(v.v[1]); see(v.v[2]); see(v.v[3]);
+          } else {
+            for (int i = d; i < D; ++i) see(row[i]);
+          }
+        }
+      }
+    }
+  }
+  m = hd_block_max<8>(m, sh);
+  if (threadIdx.x == 0) amax[blockIdx.x] = m;
+}
+
+// 2^k with 2^k m in [2^14, 2^15); 1 for an all-zero tensor.  -113 <= k <= 100: 2^k and 2^-k are normal numbers.
+__device__ __forceinline__ float hd_scale(float m) {
+  if (!(m > 0.f)) return 1.f;
+  int e;
+  frexpf(m, &e);
+  return ldexpf(1.f, min(15 - e, 100));
+}
+
 __device__ __forceinline__ float hd_finite_max(float m, float v) {
   v = fabsf(v);
   return v <= 3.402823466e38f ? fmaxf(m, v) : m;
@@ -788,18 +810,20 @@ __device__ __forceinline__ float hd_wave_sum(float v) {
   return v;
 }
 
-// the tiles' statistics of one row joined by a wave (result in lane 0): softmax = exp(z - mo) rs, the maximum and the sum
+// the tiles' statistics of one row joined by G lanes (result in their first, `lane` 0): softmax = exp(z - mo) rs, the maximum and the sum
 // apart (their lse, rounded at its own size, would shift every probability of the row); with a target the row's loss, 0
 // where it is `ignore`, NaN where it is no class or where no class has a finite logit
+template <int G>
 __device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int tiles, int64_t V, bool with_target, int64_t tg,
                                             int64_t ignore, const float* zt, int lane, float& mo, float& rs, float& loss) {
   float m = -INFINITY, s = 0.f;
-  for (int t = lane; t < tiles; t += 64) m = fmaxf(m, p[t].x);
+  for (int t = lane; t < tiles; t += G) m = fmaxf(m, p[t].x);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const float ms = m == -INFINITY ? 0.f : m;
-  for (int t = lane; t < tiles; t += 64) s += p[t].y * __builtin_amdgcn_exp2f((p[t].x - ms) * L2E);
-  s = hd_wave_sum(s);
+  for (int t = lane; t < tiles; t += G) s += p[t].y * __builtin_amdgcn_exp2f((p[t].x - ms) * L2E);
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   mo = loss = 0.f;
   rs = 1.f;
   if (!with_target) {
@@ -823,17 +847,18 @@ __device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int ti
   if (!(so + st > 0.f)) loss = NAN;        // no class is left, or one is infinite: 0 / 0 and infinity / infinity
 }
 
-// a wave per row
+// G lanes per row
+template <int G>
 __global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ part, int tiles, int N, int64_t V,
                                                     const int64_t* __restrict__ target, int64_t ignore,
                                                     const float* __restrict__ zt, float* __restrict__ mo,
                                                     float* __restrict__ rs, float* __restrict__ loss,
                                                     float* __restrict__ rows_out) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= N) return;
+  const int lane = threadIdx.x % G;
+  const int64_t n = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  if (n >= N) return;                      // G lanes together
   float m, r, v;
-  hd_join_row(part + n * tiles, tiles, V, true, target[n], ignore, zt + n, lane, m, r, v);
+  hd_join_row<G>(part + n * tiles, tiles, V, true, target[n], ignore, zt + n, lane, m, r, v);
   if (lane == 0) {
     mo[n] = m;
     rs[n] = r;
@@ -894,7 +919,7 @@ __global__ void __launch_bounds__(1024) k_head_join_total(const float2* __restri
   float s = 0.f, c = 0.f;
   for (int n = threadIdx.x >> 6; n < N; n += 16) {
     float m, r, v;
-    hd_join_row(part + (int64_t)n * tiles, tiles, V, true, target[n], ignore, zt + n, lane, m, r, v);
+    hd_join_row<64>(part + (int64_t)n * tiles, tiles, V, true, target[n], ignore, zt + n, lane, m, r, v);
     if (lane == 0) {
       mo[n] = m;
       rs[n] = r;
@@ -930,7 +955,7 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (wave == 0) {
     float jm, jr, jl;
-    hd_join_row(stats + n * tiles, tiles, V, false, 0, 0, nullptr, lane, jm, jr, jl);
+    hd_join_row<64>(stats + n * tiles, tiles, V, false, 0, 0, nullptr, lane, jm, jr, jl);
     if (lane == 0) {
       mo[n] = own[0] = jm;
       rs[n] = own[1] = jr;
@@ -1434,7 +1459,7 @@ static SmArgs sm_args(const HdCall& c, const HdPlan& p, char* ws) {
 template <class T>
 static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
   if (c.dt == DT_F32) {
-    hipLaunchKernelGGL(k_head_amax, dim3(2 * HD_AMAX), dim3(256), 0, c.st, (const float*)c.x, c.ldx, (int64_t)c.N, (const float*)c.w,
+    hipLaunchKernelGGL(k_head_amax, dim3(2 * HD_AMAX), dim3(512), 0, c.st, (const float*)c.x, c.ldx, (int64_t)c.N, (const float*)c.w,
                        c.ldw, (int64_t)c.V, c.D, c.target, c.ignore, c.index, c.teacher, c.tdt, c.K, c.amax);
     DIG3D_CHECK_LAUNCH();
   }
@@ -1503,8 +1528,14 @@ static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
   }
   float* rows_out = c.reduction ? nullptr : out;
   if (!c.index) {
-    hipLaunchKernelGGL(k_head_join, dim3((c.N + 3) / 4), dim3(256), 0, c.st, part, p.tiles_all, c.N, (int64_t)c.V, c.target, c.ignore, zt,
-                       c.m, c.rs, c.loss, rows_out);
+    // as many lanes as tiles, several rows of few classes a wave (1000000 x 64 x 16: 24 us, a wave each 284)
+#define JOIN_GO(G)                                                                                                                          \
+  hipLaunchKernelGGL((k_head_join<G>), dim3((unsigned)(((int64_t)c.N * G + 255) / 256)), dim3(256), 0, c.st, part, p.tiles_all, c.N,         \
+                     (int64_t)c.V, c.target, c.ignore, zt, c.m, c.rs, c.loss, rows_out)
+    if (p.tiles_all <= 4) JOIN_GO(4);
+    else if (p.tiles_all <= 16) JOIN_GO(16);
+    else JOIN_GO(64);
+#undef JOIN_GO
     DIG3D_CHECK_LAUNCH();
   } else {
     const dim3 g((unsigned)c.N), b(256);

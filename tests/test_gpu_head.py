@@ -898,3 +898,19 @@ def test_an_ignore_index_beyond_the_type_is_refused():
     with pytest.raises(ValueError):
         ops.linear_cross_entropy(torch.randn(4, 64, device=DEV), torch.randn(10, 64, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV),
                                  ignore_index=1 << 64)
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16'])
+def test_many_rows_of_a_teacher_with_few_classes(t):
+    one_teacher(9000, 24, 40, 6, TYPES[t], True, 'mean', True, 2.0)
+
+
+def test_many_ignored_rows_of_huge_values_leave_the_scale_alone():
+    """float32, several rows a wave: the ignored ones hold the type's largest value and do not set the scale of the others"""
+    x, w, b, target, g = classes_case(9000, 24, 40, torch.float32, True, 95)
+    target[torch.rand(9000, device=DEV, generator=g) < 0.5] = -100
+    clean = run_classes(x, w, b, target, 'mean', torch.tensor(1.0, device=DEV))
+    y = x.detach().clone()
+    y[target == -100] = torch.finfo(torch.float32).max
+    got = run_classes(y.requires_grad_(), w, b, target, 'mean', torch.tensor(1.0, device=DEV))
+    assert all(torch.equal(clean[k], got[k]) for k in clean)
