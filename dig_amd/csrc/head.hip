@@ -1324,11 +1324,11 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     p.o_scal = take(SC_COUNT * 4 + (N + HD_TOTAL - 1) / HD_TOTAL * 4);
     p.o_E = take(p.Np * p.ldE * 2 * p.eplanes);
     if (needs & 1) {
-      p.gx = hd_shape(D, N, hd_steps(p, p.vp, p.eplanes), p.pair, 64);
+      p.gx = hd_shape(D, N, hd_steps(p, p.vp, p.eplanes), p.pair, 512);
       if (p.np > 1 || p.gx.splits > 1) p.o_gx = take((int64_t)p.gx.splits * N * D * 4);
     }
     if (needs & 2) {
-      p.gw = hd_shape(D, p.vp, hd_steps(p, N, p.eplanes), p.pair, 64);
+      p.gw = hd_shape(D, p.vp, hd_steps(p, N, p.eplanes), p.pair, 512);
       if (p.gw.splits > 1) p.o_gw = take((int64_t)p.gw.splits * p.vp * D * 4);
     }
     if (needs & 4) p.o_col = take((N + HD_SLICE - 1) / HD_SLICE * p.ldE * 4);
