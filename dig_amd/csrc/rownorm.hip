@@ -336,8 +336,8 @@ __global__ void __launch_bounds__(1024) k_rownorm_params(const float* __restrict
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-// the smallest group whose registers hold the row: two vectors per thread at most, one at 1024 threads (the backward keeps
-// five values of each element: four vectors of eight spilled)
+// the smallest group whose registers hold the row (the backward keeps five values of each element: 16 elements a thread are the
+// most that 1024 threads hold)
 static inline void rn_pick(int C, int n, int& tpr, int& nv) {
   const int v = (C + n - 1) / n;
   if (v <= 8) { tpr = 8; nv = 1; }
@@ -348,6 +348,8 @@ static inline void rn_pick(int C, int n, int& tpr, int& nv) {
   else if (v <= 256) { tpr = 256; nv = 1; }
   else if (v <= 512) { tpr = 256; nv = 2; }
   else if (v <= 1024) { tpr = 1024; nv = 1; }
+  else if (v <= 2048) { tpr = 1024; nv = 2; }
+  else if (v <= 4096 && n == 4) { tpr = 1024; nv = 4; }
   else { tpr = 0; nv = 0; }
 }
 
@@ -359,6 +361,8 @@ static inline void rn_pick(int C, int n, int& tpr, int& nv) {
 //   32768 x 4096 bf16 (256 threads, 2):    2: 3.1 / 3.3   3: 4.5 / 4.5   4: 5.0 / 3.2
 //   32768 x 2048 f32 (256 threads, 2):     2: 4.6 / 5.7   3: 5.8 / 5.4   4: 5.3 / 5.1
 //   16384 x 8192 bf16 (1024 threads):      1: 3.6 / 4.2   2: 5.0 / 4.1   4: 4.7 / 3.7
+// (1024 threads, 16 elements each: 8192 x 8192 f32 4.8 / 4.6 where a row that is read again reaches 2.4 / 1.7; 4096 x 12288 bf16
+// 3.3 / 2.5 and 1.3 / 0.6)
 static inline int rn_per_cu(int tpr, int nv, bool f32, bool backward) {
   if (tpr <= 64 && tpr) return backward && f32 ? 3 : 4;
   if (tpr == 256 && nv == 1) return backward ? (f32 ? 3 : 5) : 6;
@@ -394,7 +398,8 @@ static void rn_fwd(const void* x, int64_t ldx, int R, int C, const void* w, cons
   if (tpr == TP && nv == NVV)                                                                                  \
     return rn_launch_fwd<T, TP, NVV>(x, ldx, R, C, w, b, wdt, eps, y, mean, rstd, grid, st);
   RN_CASE(8, 1) RN_CASE(16, 1) RN_CASE(32, 1) RN_CASE(64, 1) RN_CASE(64, 2)
-  RN_CASE(256, 1) RN_CASE(256, 2) RN_CASE(1024, 1)
+  RN_CASE(256, 1) RN_CASE(256, 2) RN_CASE(1024, 1) RN_CASE(1024, 2)
+  if constexpr (sizeof(T) == 4) { RN_CASE(1024, 4) }
 #undef RN_CASE
   hipLaunchKernelGGL((k_rownorm_fwd_long<T>), dim3(grid), dim3(1024), 0, st, (const T*)x, ldx, R, C, w, b, wdt, eps, (T*)y,
                      mean, rstd);
@@ -409,7 +414,8 @@ static void rn_bwd(const void* gy, const void* x, int64_t ldx, int R, int C, con
   if (tpr == TP && nv == NVV)                                                                                  \
     return rn_launch_bwd<T, TP, NVV>(gy, x, ldx, R, C, w, wdt, mean, rstd, gx, part, grid, st);
   RN_CASE(8, 1) RN_CASE(16, 1) RN_CASE(32, 1) RN_CASE(64, 1) RN_CASE(64, 2)
-  RN_CASE(256, 1) RN_CASE(256, 2) RN_CASE(1024, 1)
+  RN_CASE(256, 1) RN_CASE(256, 2) RN_CASE(1024, 1) RN_CASE(1024, 2)
+  if constexpr (sizeof(T) == 4) { RN_CASE(1024, 4) }
 #undef RN_CASE
   hipLaunchKernelGGL((k_rownorm_bwd_long<T>), dim3(grid), dim3(1024), 0, st, (const T*)gy, (const T*)x, ldx, R, C, w, wdt,
                      mean, rstd, (T*)gx, part);

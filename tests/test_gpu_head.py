@@ -914,3 +914,16 @@ def test_many_ignored_rows_of_huge_values_leave_the_scale_alone():
     y[target == -100] = torch.finfo(torch.float32).max
     got = run_classes(y.requires_grad_(), w, b, target, 'mean', torch.tensor(1.0, device=DEV))
     assert all(torch.equal(clean[k], got[k]) for k in clean)
+
+
+@pytest.mark.parametrize('t', list(TYPES))
+@pytest.mark.parametrize('R,C', [(600, 5000), (3, 12289), (5, 16384), (530, 8193)])
+def test_layer_norm_of_long_rows(R, C, t):
+    from dig_amd import ops
+    g = gen(R + C)
+    x = (randn(g, R, C) + 0.5).to(TYPES[t]).requires_grad_()
+    w, b = (1 + 0.2 * randn(g, C)).to(TYPES[t]).requires_grad_(), (0.1 * randn(g, C)).to(TYPES[t]).requires_grad_()
+    gy = randn(g, R, C).to(TYPES[t])
+    y = ops.layer_norm(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), gy)
+    check_norm(x.detach(), w.detach(), b.detach(), 1e-5, gy, y.detach(), gx, gw, gb)
