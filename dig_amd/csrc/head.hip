@@ -931,74 +931,84 @@ __global__ void __launch_bounds__(1024) k_head_join_total(const float2* __restri
   hd_total(s, c, mean, out, count, sh);
 }
 
-#define TC_MAX 2048          // a teacher's entries per row (16 bytes of LDS each)
+#define TC_MAX 2048          // a teacher's entries per row (12 bytes of LDS each)
 
-// teacher: a workgroup per row, whose statistics its first wave joins beside the teacher's softmax.  q [N, K]: the softmax over the row's listed classes of t / tau, summed over the entries of
-// the same class, -1 for an absent entry (negative index, or logit -inf); z [N, K]: the student's own logits / tau there;
-// loss[n]; live[n] = 1, 0 without entries, NaN with an index that is no class.  (t - max) / tau is kept finite, so that a
-// listed logit of the type's lowest value is not an absent entry at any tau.  A wave forms four logits at a time: the
-// row of x and four rows of W in 16-byte pieces (N K D elements of W are gathered: bound by the caches).
-template <class T>
+// sum / maximum over the WPR waves of a row, in every one of its threads (`sh`: its WPR floats)
+template <int WPR, bool MAX>
+__device__ __forceinline__ float hd_row_reduce(float v, float* sh, int wave, int lane) {
+  v = MAX ? hd_wave_max(v) : hd_wave_sum(v);
+  if constexpr (WPR == 1) return __shfl(v, 0, 64);
+  if (lane == 0) sh[wave] = v;
+  __syncthreads();
+  v = sh[0];
+#pragma unroll
+  for (int w = 1; w < WPR; ++w) v = MAX ? fmaxf(v, sh[w]) : v + sh[w];
+  __syncthreads();
+  return v;
+}
+
+// teacher: WPR waves per row, the first of which joins the row's statistics.  q [N, K]: the softmax over the row's listed
+// classes of t / tau, summed over the entries of the same class, -1 for an absent entry (negative index, or logit -inf);
+// z [N, K]: the student's own logits / tau there; loss[n]; live[n] = 1, 0 without entries, NaN with an index that is no
+// class.  (t - max) / tau is kept finite, so that a listed logit of the type's lowest value is not an absent entry at any
+// tau.  A wave forms four logits at a time: the row of x and four rows of W in 16-byte pieces (N K D elements of W are
+// gathered: bound by the caches).
+template <class T, int WPR>
 __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, const T* __restrict__ w, const void* __restrict__ bias,
                                                        int dt, int64_t ldx, int64_t ldw, int D, int64_t V,
                                                        const int64_t* __restrict__ index, const void* __restrict__ tl, int tdt, int K,
-                                                       float inv_tau, float tau, const float2* __restrict__ stats, int tiles,
-                                                       float* __restrict__ mo, float* __restrict__ rs,
-                                                       float* __restrict__ q, float* __restrict__ z, float* __restrict__ loss, float* __restrict__ live,
+                                                       float inv_tau, float tau, const float2* __restrict__ stats, int tiles, int N,
+                                                       float* __restrict__ mo, float* __restrict__ rs, float* __restrict__ q,
+                                                       float* __restrict__ z, float* __restrict__ loss, float* __restrict__ live,
                                                        float* __restrict__ rows_out) {
-  constexpr int N8 = VecLen<T>::n;
-  extern __shared__ int64_t dyn[];         // index [K] (-1: absent), then t, then (t - max) / tau [K], then q [K]
-  float* st = (float*)(dyn + K);
-  float* sq = st + K;
-  __shared__ float sh[8], own[2];
-  const int64_t n = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int N8 = VecLen<T>::n, RPB = 4 / WPR, TPR = 64 * WPR;
+  extern __shared__ float dyn[];           // per row: t, then (t - max) / tau [K], q [K], index [K] (-1: absent, V: no class)
+  __shared__ float shared[4], own[RPB][2];
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % WPR, slot = (threadIdx.x >> 6) / WPR, tid = wave * 64 + lane;
+  const int64_t n = (int64_t)blockIdx.x * RPB + slot;
+  if (WPR == 1 && n >= N) return;          // one wave to a row: nothing to meet at
+  float *st = dyn + slot * 3 * K, *sq = st + K, *sh = shared + slot * WPR;
+  int* si = (int*)(sq + K);
   if (wave == 0) {
     float jm, jr, jl;
     hd_join_row<64>(stats + n * tiles, tiles, V, false, 0, 0, nullptr, lane, jm, jr, jl);
     if (lane == 0) {
-      mo[n] = own[0] = jm;
-      rs[n] = own[1] = jr;
+      mo[n] = own[slot][0] = jm;
+      rs[n] = own[slot][1] = jr;
     }
   }
   float m = -INFINITY;
-  for (int k = tid; k < K; k += 256) {
+  for (int k = tid; k < K; k += TPR) {
     const int64_t v = index[n * K + k];
     const float t = v < 0 ? -INFINITY : load_as(tl, tdt, n * K + k);
-    dyn[k] = t == -INFINITY ? -1 : v;
+    si[k] = t == -INFINITY ? -1 : (int)(v < V ? v : V);
     st[k] = t;
     m = fmaxf(m, t);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (lane == 0) sh[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+  m = hd_row_reduce<WPR, true>(m, sh, wave, lane);
   const float ms = m == -INFINITY ? 0.f : m;
   float s = 0.f;
-  for (int k = tid; k < K; k += 256) {
+  for (int k = tid; k < K; k += TPR) {
     float d = (st[k] - ms) * inv_tau;
     d = d < -3.402823466e38f ? -3.402823466e38f : d;             // a NaN stays one
     st[k] = d;
-    if (dyn[k] >= 0) s += expf(d);
+    if (si[k] >= 0) s += expf(d);
   }
-  s = hd_wave_sum(s);
-  if (lane == 0) sh[4 + wave] = s;
-  __syncthreads();
-  s = (sh[4] + sh[5]) + (sh[6] + sh[7]);
+  s = hd_row_reduce<WPR, false>(s, sh, wave, lane);
   const bool any = s > 0.f || s != s;      // a NaN among the listed logits is not an empty row
   const float ls = any ? logf(s) : 0.f;
-  const float sm = own[0], sl = logf(own[1]);   // the student's log softmax is z - sm + sl
-  for (int k = tid; k < K; k += 256) sq[k] = dyn[k] < 0 ? 0.f : expf(st[k] - ls);
-  __syncthreads();
+  for (int k = tid; k < K; k += TPR) sq[k] = si[k] < 0 ? 0.f : expf(st[k] - ls);
+  if constexpr (WPR > 1) __syncthreads();
+  else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const float sm = own[slot][0], sl = logf(own[slot][1]);         // the student's log softmax is z - sm + sl
   const T* xr = x + n * ldx;
   float part = 0.f;
-  for (int k0 = wave * 4; k0 < K; k0 += 16) {
+  for (int k0 = wave * 4; k0 < K; k0 += 4 * WPR) {
     const T* row[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int64_t v = k0 + e < K ? dyn[k0 + e] : 0;
-      row[e] = w + (v >= 0 && v < V ? v : 0) * ldw;              // what is not there reads class 0, and is not used
+      const int v = k0 + e < K ? si[k0 + e] : 0;
+      row[e] = w + (int64_t)(v >= 0 && v < V ? v : 0) * ldw;     // what is not there reads class 0, and is not used
     }
     float d[4] = {0.f, 0.f, 0.f, 0.f};
     for (int c = lane * N8; c < D; c += 64 * N8) {
@@ -1022,7 +1032,7 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
       const float dot = hd_wave_sum(d[e]);
       const int k = k0 + e;
       if (lane != 0 || k >= K) continue;
-      const int64_t v = dyn[k];
+      const int v = si[k];
       float zk = 0.f;
       if (any && v >= 0) {
         zk = v < V ? (bias ? dot + load_as(bias, dt, v) : dot) * inv_tau : NAN;     // no such class: the row says so
@@ -1031,16 +1041,25 @@ __global__ void __launch_bounds__(256) k_head_teacher(const T* __restrict__ x, c
       z[n * K + k] = zk;
     }
   }
-  if (lane == 0) sh[wave] = part;
-  for (int k = tid; k < K; k += 256) {     // entries of the same class add up
-    float sum = 0.f;
-    const int64_t v = dyn[k];
-    for (int e = 0; e < K; ++e) sum += dyn[e] == v ? sq[e] : 0.f;
-    q[n * K + k] = v < 0 ? -1.f : sum;
+  // entries of the same class add up: 4 entries a thread at a time against every other (4096 rows of 2048: 5.7 ms, one at a time 8.1)
+  for (int k0 = tid; k0 < K; k0 += 4 * TPR) {
+    int v[4];
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = k0 + j * TPR < K ? si[k0 + j * TPR] : -1;
+    for (int e = 0; e < K; ++e) {
+      const int o = si[e];
+      const float w1 = sq[e];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += o == v[j] ? w1 : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (k0 + j * TPR < K) q[n * K + k0 + j * TPR] = v[j] < 0 ? -1.f : sum[j];
   }
-  __syncthreads();
+  part = hd_row_reduce<WPR, false>(lane == 0 ? part : 0.f, sh, wave, lane);
   if (tid == 0) {
-    const float v = tau * tau * ((sh[0] + sh[1]) + (sh[2] + sh[3]));
+    const float v = tau * tau * part;
     loss[n] = any ? v : 0.f;
     live[n] = !any ? 0.f : v == v ? 1.f : v;
     if (rows_out) rows_out[n] = any ? v : 0.f;
@@ -1538,15 +1557,20 @@ static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
 #undef JOIN_GO
     DIG3D_CHECK_LAUNCH();
   } else {
-    const dim3 g((unsigned)c.N), b(256);
-    const size_t lds = (size_t)c.K * 16;
+    // One wave to a row where there are many rows and the rows of W are short, four otherwise.  us of the forward, one / four:
+    // 5000 x 256 x 1000 float32 with 8, 16, 64 entries 49 / 62, 53 / 65, 81 / 94; 4096 x 1024 x 32000 with 64: 896 / 866;
+    // 64 x 128 x 1195 with 16: 28 / 22
+    const int wpr = c.K <= 4 || (c.K <= 64 && c.N >= 2048 && c.D <= 512) ? 1 : 4, rpb = 4 / wpr;
+    const dim3 g((unsigned)((c.N + rpb - 1) / rpb)), b(256);
+    const size_t lds = (size_t)c.K * 12 * rpb;
     const float it = 1.0f / c.tau;
-#define TC_GO(T)                                                                                                                       \
-  hipLaunchKernelGGL((k_head_teacher<T>), g, b, lds, c.st, (const T*)c.x, (const T*)c.w, c.bias, c.dt, c.ldx, c.ldw, c.D, (int64_t)c.V, \
-                     c.index, c.teacher, c.tdt, c.K, it, c.tau, part, p.tiles_all, c.m, c.rs, c.q, c.z, c.loss, c.live, rows_out)
-    if (c.dt == DT_F32) TC_GO(float);
-    else if (c.dt == DT_BF16) TC_GO(bf16_t);
-    else TC_GO(f16_t);
+#define TC_GO(T, WPR)                                                                                                                   \
+  hipLaunchKernelGGL((k_head_teacher<T, WPR>), g, b, lds, c.st, (const T*)c.x, (const T*)c.w, c.bias, c.dt, c.ldx, c.ldw, c.D,           \
+                     (int64_t)c.V, c.index, c.teacher, c.tdt, c.K, it, c.tau, part, p.tiles_all, c.N, c.m, c.rs, c.q, c.z, c.loss,      \
+                     c.live, rows_out)
+    if (c.dt == DT_F32) { if (wpr == 1) TC_GO(float, 1); else TC_GO(float, 4); }
+    else if (c.dt == DT_BF16) { if (wpr == 1) TC_GO(bf16_t, 1); else TC_GO(bf16_t, 4); }
+    else { if (wpr == 1) TC_GO(f16_t, 1); else TC_GO(f16_t, 4); }
 #undef TC_GO
     DIG3D_CHECK_LAUNCH();
   }

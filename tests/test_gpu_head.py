@@ -927,3 +927,12 @@ def test_layer_norm_of_long_rows(R, C, t):
     y = ops.layer_norm(x, w, b)
     gx, gw, gb = torch.autograd.grad(y, (x, w, b), gy)
     check_norm(x.detach(), w.detach(), b.detach(), 1e-5, gy, y.detach(), gx, gw, gb)
+
+
+@pytest.mark.parametrize('t', list(TYPES))
+@pytest.mark.parametrize('N,D,V,K', [(5, 40, 30, 3), (2100, 72, 90, 33), (2050, 600, 70, 20), (2049, 64, 300, 64), (70, 128, 900, 300)])
+def test_teacher_rows_of_one_wave_and_of_four(N, D, V, K, t):
+    def change(index, teacher):
+        index[0, -1] = index[0, 0]                 # a class listed twice, by the first and the last entry
+        index[1, :] = -1
+    one_teacher(N, D, V, K, TYPES[t], True, 'none', True, 2.0, change=change)
