@@ -88,8 +88,8 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
 
     -> float32: the mean over the rows whose target is not ``ignore_index`` (0 if there are none), their sum, or with
     ``reduction='none'`` one loss per row (0 for an ignored one).  Ignored rows take no part in any gradient, whatever they
-    hold.  A target outside [0, V) gives NaN, in the loss and the gradients, and so does a row without a finite logit.  Differentiable once, in x, weight and bias; the
-    gradients have the type of their inputs and the same bits every time."""
+    hold.  A target outside [0, V) gives NaN, in the loss and the gradients, and so does a row without a finite logit.
+    Differentiable once, in x, weight and bias; the gradients have the type of their inputs and the same bits every time."""
     x2, weight, bias = _check_head('linear_cross_entropy', x, weight, bias, reduction)
     _check_index('linear_cross_entropy', 'target', target, x.shape[:-1], x2)
     if not -1 << 63 <= int(ignore_index) < 1 << 63:
@@ -100,9 +100,9 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
 
 def linear_distillation(x, weight, teacher_index, teacher_logits, bias=None, temperature=1.0, reduction='mean'):
     """Distillation of the head ``x @ weight.T + bias`` from a teacher's K largest logits: per row
-    ``temperature**2 * KL(q || p)`` (temperature from 1e-6 to 1e6) with q the softmax of ``teacher_logits`` [..., K] / temperature over the listed classes
-    ``teacher_index`` [..., K] (int64) and p the head's softmax over ALL classes at the same temperature, the head's logits never
-    kept.
+    ``temperature**2 * KL(q || p)`` (temperature from 1e-6 to 1e6) with q the softmax of ``teacher_logits`` [..., K] /
+    temperature over the listed classes ``teacher_index`` [..., K] (int64) and p the head's softmax over ALL classes at the same
+    temperature, the head's logits never kept.
 
     An entry with a negative index or the logit -inf is absent, whatever else it holds; a row without entries has the loss 0, no
     gradient, and is not counted by the mean.  Equal indices of a row add up.  An index >= V gives NaN.  The teacher takes no

@@ -744,7 +744,7 @@ int dig3d_wide_dd(int G, int nl, int M, int K0, const void* const* H0, const voi
 /* ---------------------------------------------------------------------------------------------------
  * Layer norm over the C channels of a row (rownorm.hip).  No reference counterpart (its models normalise per graph,
  * method/comenet/comenet.py:160): y = w (x - mean) rstd + b, the variance centred, statistics in f32.
- * dtype of x / y / gy / gx and wdtype of w / b / gw / gb: 0 f32, 1 bf16, 2 f16; w, b may be NULL.  x: R rows of pitch ldx
+ * dtype of x / y / gy / gx and wdtype of w / b / gw / gb: 0 f32, 1 bf16, 2 f16; w, b may be NULL; C < 2^25.  x: R rows of pitch ldx
  * >= C elements, any alignment of the element type; y, gy, gx: pitch C.  mean / rstd [R]: kept for the backward (both NULL:
  * not wanted).  Backward: gx, and gw / gb [C] from part = float[nb * 2 * C], nb = dig3d_rownorm_bwd_blocks(R, C, dtype);
  * gx, gw, gb may be NULL; gw == gb == NULL with a part: the caller sums its nb rows (dig3d_reduce_many).
