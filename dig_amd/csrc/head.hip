@@ -90,6 +90,8 @@ struct HdArgs {
 // device scalars: the power-of-two scales of x and W (f32 inputs) and the common factor S of the gradients
 enum { SC_X = 0, SC_W = 1, SC_S = 2, SC_COUNT = 4 };
 
+#define HD_FAR 16777216.0f // 2^24: a float32 product below it is off by less than one
+
 #define E_SCALE 32768.0f   // e in f16 (|e| <= 1) is stored times this: small entries stay normal numbers
 
 // what a product with e is multiplied by: S over the scales of its operands
@@ -259,8 +261,10 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
   } else {
     // z = u acc: the product in units of 1 / tau (the scales are powers of two); with a bias, acc becomes z and u one.
     // exp(z - m) = 2^(z k - m k) in one fused step, off by the rounding of the product m k alone, which is the same factor in
-    // all of a row and is taken out of its sum.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane
-    // are 128 times whatever one costs.
+    // all of a row and is taken out of its sum.  That rounding is below one only for |m k| < HD_FAR: beyond (a tile whose classes are
+    // all masked by a bias of -1e10, or of the type's lowest value) 2^rounding leaves the range, and the difference is formed
+    // first.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane are 128
+    // times whatever one costs.
     float u = a.inv_tau;
     if constexpr (PAIR) u = fminf(fmaxf(u / (a.scal[SC_X] * a.scal[SC_W]), 1.175494351e-38f), 3.402823466e38f);   // 0 or infinity times what may be either
     if (a.bias) {
@@ -314,13 +318,21 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         m = fmaxf(m, __shfl_xor(m, 16, 64));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const float ms = m == -INFINITY ? 0.f : m, k = u * L2E, mk = ms * k;
+        const bool far = !(fabsf(mk) < HD_FAR);                   // the same in a row's four lanes, and no matter of other rows
+        if (far) {
 #pragma unroll
-        for (int x = 0; x < MI; ++x)
+          for (int x = 0; x < MI; ++x)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(__fmaf_rn(acc[x][y][r], k, -mk));
+            for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[x][y][r] - ms) * k);
+        } else {
+#pragma unroll
+          for (int x = 0; x < MI; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(__fmaf_rn(acc[x][y][r], k, -mk));
+        }
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
-        s *= __builtin_amdgcn_exp2f(-__fmaf_rn(ms, k, -mk));
+        if (!far) s *= __builtin_amdgcn_exp2f(-__fmaf_rn(ms, k, -mk));
         if (lane < 16) {
           sh[((wave % WI) * BJ + jl) * 2] = m * u;
           sh[((wave % WI) * BJ + jl) * 2 + 1] = s;
@@ -349,11 +361,23 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         const float keep = __is_same(T, f16_t) ? E_SCALE : 1.f;
         const float c = in ? a.coef[j] * keep : 0.f;
         // exp(z - m) with m = r u + (what the quotient left): 2^(acc k - r k), and what r k left, as in the statistics
-        float mk = INFINITY, cp = 0.f;                           // no loss: its row of x is zero, exp(z - inf) = 0
+        float mk = INFINITY, cp = 0.f, m = 0.f;                  // no loss: its row of x is zero, exp(z - inf) = 0
+        bool far = false;
         if (c != 0.f) {
-          const float m = a.m[j], r = m / u;
+          m = a.m[j];
+          const float r = m / u;
           mk = r * k;
-          cp = c * a.rs[j] * __builtin_amdgcn_exp2f(-__fmaf_rn(r, k, -mk) - __fmaf_rn(-r, u, m) * L2E);
+          far = !(fabsf(mk) < HD_FAR);
+          cp = c * a.rs[j] * (far ? 1.f : __builtin_amdgcn_exp2f(-__fmaf_rn(r, k, -mk) - __fmaf_rn(-r, u, m) * L2E));
+        }
+        float ky = k;
+        if (far) {                                               // the exponents themselves take the products' place
+          ky = 1.f;
+          mk = 0.f;
+#pragma unroll
+          for (int x = 0; x < MI; ++x)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[x][y][q] = __fmaf_rn(acc[x][y][q], u, -m) * L2E;
         }
         const int tl = target_at(j);
         const bool any = __any(tl >= 0);
@@ -366,7 +390,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
           float e[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            e[r] = cp * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x + (r >> 2)][y][r & 3], k, -mk));
+            e[r] = cp * __builtin_amdgcn_exp2f(__fmaf_rn(acc[x + (r >> 2)][y][r & 3], ky, -mk));
           if (any) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) e[r] = tl == hd_row(x) + r ? et : e[r];

@@ -1,0 +1,66 @@
+"""GPU: the class losses where their arithmetic comes to its ends — classes masked by the type's lowest value, rows with a single class
+left, rows without a number beside others, and float32 operands whose sizes lie far apart — against float64 formulas.
+
+Tolerances as in test_gpu_head.py: sums of the roundings that are made, derived before any run.  Each case runs at a size that the
+kernels of head_small.h take in place and at one that the general path takes."""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_head import DEV, TYPES, U, check_head, check_teacher, classes_case, close, gen, half, head64, randn, ref_classes, ref_teacher
+
+pytestmark = pytest.mark.gpu
+SMALL, GENERAL = (40, 64, 600), (600, 64, 1100)          # rows, width, classes
+
+
+def teacher_lists(g, N, V, K):
+    return torch.rand(N, V, device=DEV, generator=g).topk(K, 1).indices, 2 * randn(g, N, K)
+
+
+# ------------------------------------------------------------------------------------------------ masked classes
+@pytest.mark.parametrize('t', list(TYPES))
+@pytest.mark.parametrize('N,D,V', [SMALL, GENERAL])
+def test_whole_tiles_of_classes_masked_by_the_lowest_value(N, D, V, t):
+    """300 classes and behind them only masked ones: probability 0, no gradient, the others as if alone"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, TYPES[t], True, 101)
+    target = target % 300
+    index, teacher = teacher_lists(g, N, 300, 5)
+    one = torch.tensor(float(N) if t == 'f16' else 1.0, device=DEV)
+    xd, wd, bd = x.detach(), w.detach()[:300], b.detach()[:300]
+    for value in (torch.finfo(TYPES[t]).min, float('-inf')) + (() if t == 'f16' else (-1e10, -1e30)):
+        low = b.detach().clone()
+        low[300:] = value
+        low.requires_grad_()
+        out = ops.linear_cross_entropy(x, w, target, low)
+        got = dict(zip(('gx', 'gw', 'gb'), torch.autograd.grad(out, (x, w, low), one)), out=out.detach())
+        z, e, rows, loss, scale, div = ref_classes(xd, wd, bd, target, 'mean', one)
+        assert not got['gw'][300:].any() and not got['gb'][300:].any(), value
+        check_head(xd, wd, bd, z, e, rows, 1.0, 1.0, dict(got, gw=got['gw'][:300], gb=got['gb'][:300], div=div), scale, loss)
+        for tau in (1.0, 0.5):             # at 1/2 logits of the lowest value are beyond the type's range
+            out = ops.linear_distillation(x, w, index, teacher, low, temperature=tau)
+            got = dict(zip(('gx', 'gw', 'gb'), torch.autograd.grad(out, (x, w, low), one)), out=out.detach())
+            z, e, rows, size, scale, div = ref_teacher(xd, wd, bd, index, teacher, tau, 'mean', one)
+            assert not got['gw'][300:].any() and not got['gb'][300:].any(), (value, tau)
+            check_teacher(xd, wd, bd, z, e, rows, size, tau, dict(got, gw=got['gw'][:300], gb=got['gb'][:300], div=div), scale, rows.sum() / div,
+                          index, teacher)
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16'])
+@pytest.mark.parametrize('N,D,V', [SMALL, GENERAL])
+def test_every_class_at_the_lowest_value(N, D, V, t):
+    """the bias swallows every product: all logits equal, the loss log V to the rounding of a sum and a logarithm, softmax = 1 / V.
+    gx: V products of e, off by 16 u, and of w; in 16 bits e is rounded to half a step"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, TYPES[t], True, 102)
+    e = torch.full((N, V), 1.0 / V, dtype=torch.float64, device=DEV)
+    e[torch.arange(N, device=DEV), target] -= 1.0
+    wd = w.detach().double()
+    keep = 2.0 ** -22 if t == 'f32' else half(TYPES[t])
+    for value in (torch.finfo(TYPES[t]).min, -1e10):
+        low = torch.full_like(b, value).requires_grad_()
+        rows = ops.linear_cross_entropy(x, w, target, low, reduction='none')
+        close(rows.detach(), torch.full((N,), math.log(V), dtype=torch.float64, device=DEV), 64 * U * math.log(V), 'rows')
+        (gx,) = torch.autograd.grad(rows.sum(), x)
+        close(gx, e @ wd, half(TYPES[t]) * (e @ wd).abs() * 1.01 + (keep + (6 * V + 200) * U) * (e.abs() @ wd.abs()), 'gx')
