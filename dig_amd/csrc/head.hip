@@ -864,7 +864,8 @@ __device__ __forceinline__ void hd_join_row(const float2* __restrict__ p, int ti
   // two near numbers, where the target holds almost everything
   const float z = *zt;
   const float M = fmaxf(m, z), Ms = M == -INFINITY ? 0.f : M;
-  const float so = s * expf(ms - Ms), st = expf(z - Ms);
+  // no other class is left (s = 0, their maximum -inf): their share is 0, not 0 times exp(0 - z), which overflows below z = -88
+  const float so = s == 0.f ? 0.f : s * expf(ms - Ms), st = expf(z - Ms);
   mo = M;
   rs = 1.f / (so + st);
   loss = z >= m ? log1pf(so) : (Ms - z) + logf(so + st);

@@ -64,3 +64,29 @@ def test_every_class_at_the_lowest_value(N, D, V, t):
         close(rows.detach(), torch.full((N,), math.log(V), dtype=torch.float64, device=DEV), 64 * U * math.log(V), 'rows')
         (gx,) = torch.autograd.grad(rows.sum(), x)
         close(gx, e @ wd, half(TYPES[t]) * (e @ wd).abs() * 1.01 + (keep + (6 * V + 200) * U) * (e.abs() @ wd.abs()), 'gx')
+
+
+# ------------------------------------------------------------------------------------------------ one class left
+@pytest.mark.parametrize('t', list(TYPES))
+@pytest.mark.parametrize('N,D,V', [(40, 64, 1), (600, 64, 1), SMALL, GENERAL])
+def test_the_target_is_the_only_class_left(N, D, V, t):
+    """loss 0 and no gradient, whatever the size of its logit"""
+    from dig_amd import ops
+    t = TYPES[t]
+    at = V // 2
+    w = torch.zeros(V, D, device=DEV, dtype=t)
+    w[at, 0] = 1
+    w.requires_grad_()
+    b = torch.full((V,), float('-inf'), device=DEV, dtype=t)
+    b[at] = 0
+    b.requires_grad_()
+    target = torch.full((N,), at, device=DEV)
+    for logit in (0.0, -80.0, -100.0, -1e4, 1e4):
+        x = torch.zeros(N, D, device=DEV, dtype=t)
+        x[:, 0] = logit
+        x.requires_grad_()
+        for red in ('mean', 'none'):
+            out = ops.linear_cross_entropy(x, w, target, b, reduction=red)
+            assert not out.detach().any(), (logit, red, out)
+            for name, gr in zip('xwb', torch.autograd.grad(out.sum(), (x, w, b))):
+                assert not gr.any(), (logit, red, name)
