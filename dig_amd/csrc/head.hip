@@ -892,8 +892,8 @@ __global__ void __launch_bounds__(256) k_head_join(const float2* __restrict__ pa
   }
 }
 
-// out = sum or mean of the rows' losses, count = how many rows have one (at least 1): a fixed tree of additions over the
-// 1024 threads of a workgroup
+// out = sum or mean of the rows' losses, count = how many rows have one (at least 1; one that is NaN is a row like others): a
+// fixed tree of additions over the 1024 threads of a workgroup
 __device__ __forceinline__ void hd_total(float s, float c, int mean, float* out, float* count, float* sh) {
   s = hd_wave_sum(s);
   c = hd_wave_sum(c);
@@ -928,7 +928,7 @@ __global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ l
   const int end = min(N, (int)(blockIdx.x + 1) * HD_TOTAL);
   for (int n = blockIdx.x * HD_TOTAL + threadIdx.x; n < end; n += 1024) {
     s += pairs ? pairs[n].x : loss[n];
-    c += pairs ? pairs[n].y : target ? (target[n] != ignore ? 1.f : 0.f) : live[n];
+    c += pairs ? pairs[n].y : hd_has(n, target, ignore, live) ? 1.f : 0.f;
   }
   hd_total(s, c, mean, out + (count ? 0 : 2 * blockIdx.x), count, sh);
 }

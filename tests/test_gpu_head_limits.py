@@ -90,3 +90,39 @@ def test_the_target_is_the_only_class_left(N, D, V, t):
             assert not out.detach().any(), (logit, red, out)
             for name, gr in zip('xwb', torch.autograd.grad(out.sum(), (x, w, b))):
                 assert not gr.any(), (logit, red, name)
+
+
+# ------------------------------------------------------------------------------------------------ a row without a number
+@pytest.mark.parametrize('N,D,V', [(40, 64, 600), (600, 64, 900)])
+@pytest.mark.parametrize('what', ['index', 'teacher', 'row', 'target'])
+def test_a_row_without_a_number_counts_once(N, D, V, what):
+    """the mean over 32 or 512 rows, one of them NaN: the loss and w's gradient are NaN, the other rows' gradients are those of the
+    sum over the count of rows (a power of two: the same bits)"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, torch.float32, True, 103)
+    n = 32 if N < 512 else 512
+    index, teacher = teacher_lists(g, N, V, 4)
+    index[n:], target[n:] = -1, -100
+    x = x.detach()
+    if what == 'index':
+        index[3, 1] = V
+    elif what == 'teacher':
+        teacher[3, 1] = float('nan')
+    elif what == 'row':
+        x[3, 5] = float('nan')
+    else:
+        target[3] = V
+    x.requires_grad_()
+    losses = []
+    if what != 'target':
+        losses.append(lambda red: ops.linear_distillation(x, w, index, teacher, b, temperature=2.0, reduction=red))
+    if what in ('row', 'target'):
+        losses.append(lambda red: ops.linear_cross_entropy(x, w, target, b, reduction=red))
+    others = [i for i in range(N) if i != 3]
+    for f in losses:
+        mean = f('mean')
+        gm, gw = torch.autograd.grad(mean, (x, w))
+        (gs,) = torch.autograd.grad(f('sum'), x)
+        assert torch.isnan(mean.detach()) and torch.isnan(gw).any() and torch.isnan(gm[3]).all()
+        assert torch.isfinite(gs[others]).all() and gs[others].any()
+        assert torch.equal(gm[others] * n, gs[others])
