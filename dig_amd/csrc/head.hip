@@ -361,9 +361,12 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         const float keep = __is_same(T, f16_t) ? E_SCALE : 1.f;
         const float c = in ? a.coef[j] * keep : 0.f;
         // exp(z - m) with m = r u + (what the quotient left): 2^(acc k - r k), and what r k left, as in the statistics
-        float mk = INFINITY, cp = 0.f, m = 0.f;                  // no loss: its row of x is zero, exp(z - inf) = 0
+        float mk = INFINITY, cp = 0.f, m = 0.f;                  // no loss: exp(0 - inf) = 0, whatever W and the bias hold
         bool far = false;
-        if (c != 0.f) {
+        if (c == 0.f) {
+#pragma unroll
+          for (int x = 0; x < MI; ++x) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
           m = a.m[j];
           const float r = m / u;
           mk = r * k;
@@ -382,7 +385,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         const int tl = target_at(j);
         const bool any = __any(tl >= 0);
         // p - 1 of the target: what the other classes hold, not a difference near 1
-        const float et = tl >= 0 ? c * expm1f(-a.loss[j]) : 0.f;
+        const float et = tl >= 0 && c != 0.f ? c * expm1f(-a.loss[j]) : 0.f;
         if (j >= a.rowsE) continue;
         short* row = a.E + (int64_t)j * a.eplanes * a.colsE + first;
 #pragma unroll

@@ -126,3 +126,49 @@ def test_a_row_without_a_number_counts_once(N, D, V, what):
         assert torch.isnan(mean.detach()) and torch.isnan(gw).any() and torch.isnan(gm[3]).all()
         assert torch.isfinite(gs[others]).all() and gs[others].any()
         assert torch.equal(gm[others] * n, gs[others])
+
+
+# ------------------------------------------------------------------------------------------------ rows without a loss
+@pytest.mark.parametrize('t', list(TYPES))
+@pytest.mark.parametrize('N,D,V', [SMALL, GENERAL])
+def test_ignored_rows_beside_a_class_without_a_number(N, D, V, t):
+    """a class whose bias is NaN or +inf makes every row's loss NaN; a row without a loss has none, and no gradient"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, TYPES[t], True, 104)
+    index, teacher = teacher_lists(g, N, V, 4)
+    for value in (float('nan'), float('inf')):
+        bad = b.detach().clone()
+        bad[V - 2] = value
+        bad.requires_grad_()
+        for every in (False, True):
+            tg, ix = target.clone(), index.clone()
+            if every:
+                tg[:], ix[:] = -100, -1
+            else:
+                tg[::3], ix[::3] = -100, -1
+            for f in (lambda: ops.linear_cross_entropy(x, w, tg, bad), lambda: ops.linear_distillation(x, w, ix, teacher, bad)):
+                out = f()
+                gx, gw, gb = torch.autograd.grad(out, (x, w, bad))
+                assert not gx[::3].any(), (value, every)
+                if every:
+                    assert float(out.detach()) == 0.0 and not gx.any() and not gw.any() and not gb.any()
+                else:
+                    assert torch.isnan(out.detach()) and torch.isnan(gx[1]).all()
+
+
+@pytest.mark.parametrize('t', list(TYPES))
+@pytest.mark.parametrize('N,D,V', [SMALL, GENERAL])
+def test_what_reaches_an_ignored_row_is_not_used(N, D, V, t):
+    """one loss per row: an incoming gradient of NaN or infinity at a row without a loss changes no bit"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, TYPES[t], True, 105)
+    index, teacher = teacher_lists(g, N, V, 4)
+    target[::4], index[::4] = -100, -1
+    up = torch.rand(N, device=DEV, generator=g) + 0.5
+    for f in (lambda: ops.linear_cross_entropy(x, w, target, b, reduction='none'),
+              lambda: ops.linear_distillation(x, w, index, teacher, b, reduction='none')):
+        want = torch.autograd.grad(f(), (x, w, b), up)
+        bad = up.clone()
+        bad[0], bad[4], bad[8] = float('nan'), float('inf'), float('-inf')
+        got = torch.autograd.grad(f(), (x, w, b), bad)
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.isfinite(p).all() for p in want)
