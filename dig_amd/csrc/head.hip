@@ -3,7 +3,7 @@
 //   classes:  loss_n = lse(z_n) - z_n[y_n]                                     e_n = c_n (softmax(z_n) - onehot(y_n))
 //   teacher:  loss_n = tau^2 sum_k q_k (log q_k - log p_n[i_k]), p = softmax(z / tau)   e_n = c_n (p_n - scatter(q_n))
 //   gx = S e W,  gW = S e^T x,  gb = S sum_n e_n          (c_n S: the gradient that reaches row n, |c_n| <= 1)
-// (f16 / f32: e is kept to 2^-40 of the largest |c|, so a row whose gradient is 10^-6 of another's keeps 20 bits of its own)
+// (f16: e is kept to 2^-40 of the largest |c|: 11 bits of every entry down to 2^-29 of it, fewer below)
 //
 // Four products of 2 N V D operations: the logits, the logits again in the backward (the price of not keeping them), e W and
 // e^T x.  Bound: the matrix cores.  All four run on ONE product kernel (k_head_gemm): out[j, i] = sum_k Q[j, k] P[i, k], each
@@ -12,10 +12,12 @@
 // statistics of a tile of logits (forward), the gradient e of a piece of the vocabulary (backward), or the stored product.
 //
 // Types.  bf16 / f16: the inputs as they are, sums in f32; e is rounded once to the same type (up to 2^-8 / 2^-11 of each entry,
-// at random sign; with few rows e is two such numbers).  f32: every value is two f16 numbers, v s = h + l with
-// s = 2^k chosen so that the largest |v| of the tensor lies in [2^14, 2^15): 22 bits of every v down to 2^-29 of that
-// largest one, and an absolute error of 2^-40 of it below; three products h h, h l, l h with f32 sums (l l is below 2^-22 of
-// the term).  Three f16 matrix products have 5x the rate of one in f32 on this chip, at the error of an f32 product.
+// at random sign; with few rows e is two such numbers).  f32: every value, of x, W and e alike, is the sum of three bf16
+// numbers v = h + m + l, exactly down to 2^-110 (8 bits each, the exponent range of f32: no scale, no entry's bits depend on another's), and a
+// product of two is the six products of them that reach 2^-24 of it: h h, h m, m h, m m, h l, l h, with f32 sums.  What is
+// dropped (m l, l m, l l) is at most 2^-23 of the term.  Six bf16 products take two thirds of the time of one in f32 on this
+// chip.  (Two f16 numbers and three products would take half of that again, but their second number runs out of exponents:
+// below 2^-18 of the largest value of its tensor an entry loses bits, and the gradient of an unlikely class has no other entries.)
 #include <string.h>
 
 #include "half16.h"
@@ -40,8 +42,8 @@ __device__ __forceinline__ f32x4 hd_mfma<f16_t>(s16x8 a, s16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// One operand: a matrix of `rows` rows with pitch `ld` (elements, a multiple of 8; base 16-byte aligned); a value of two numbers
-// has its second one `plane` elements behind the first, in the same row.
+// One operand: a matrix of `rows` rows with pitch `ld` (elements, a multiple of 8; base 16-byte aligned); a value of several numbers
+// has each `plane` elements behind the one before, in the same row.
 //   not TR: row = the operand's own index, columns = k (k extent a multiple of HD_BK inside the pitch)
 //   TR:     row = k, columns = the operand's own index (`cols` of them are readable, a multiple of 8)
 // Rows beyond the last are read as the last one: for the own index their results are not used, for k the other operand
@@ -58,16 +60,15 @@ struct HdArgs {
   HdOperand P, Q;
   int ni, nj;                // extents of the own indices of P and Q
   int ktiles;                // k steps of one product
-  int nseg;                  // not PAIR: Q as one number, or as two (h h, h l)
+  int nseg;                  // not F32: Q as one number, or as two (h h, h l)
   int ti, tj;                // tiles along i and j
   int splits, wgs;           // ranges of the k steps, and workgroups to each
   // logits epilogues: i = class v0 + i, j = row
   const void* bias;
   int dt;                    // type of bias / of the stored output
-  const float* scal;         // device scalars of the call (SC_*)
+  const float* S;            // the gradients' common factor
   float inv_tau;
   int64_t v0;                // first class of the piece
-  int64_t V;
   const int64_t* target;     // null: no class is kept apart
   float2* part;              // EPI_STATS [nj][ti_all]: (max, sum of exp) of the tile
   int part_ld, part_c0;
@@ -75,7 +76,7 @@ struct HdArgs {
   const float *m, *rs;       // EPI_GRAD: softmax = exp(z - m) rs
   const float* loss;
   const float* coef;
-  int eplanes;               // e as one number, or as two (its rounding and what that left)
+  int eplanes;               // not F32: e as one number, or as two (its rounding and what that left)
   short* E;                  // EPI_GRAD [rowsE][eplanes][colsE]
   int64_t colsE;
   int rowsE;
@@ -84,21 +85,34 @@ struct HdArgs {
   int add;
   void* out;                 // or the finished result, row pitch ldo
   int64_t ldo;
-  int other;                 // scale of the operand beside e (SC_X / SC_W with f32 inputs, else -1)
 };
-
-// device scalars: the power-of-two scales of x and W (f32 inputs) and the common factor S of the gradients
-enum { SC_X = 0, SC_W = 1, SC_S = 2, SC_COUNT = 4 };
 
 #define HD_FAR 16777216.0f // 2^24: a float32 product below it is off by less than one
 
 #define E_SCALE 32768.0f   // e in f16 (|e| <= 1) is stored times this: small entries stay normal numbers
 
-// what a product with e is multiplied by: S over the scales of its operands
+// what a product with e is multiplied by
 template <class T>
-__device__ __forceinline__ float hd_factor(const float* scal, int other) {
-  const float s = __is_same(T, f16_t) ? scal[SC_S] * (1.f / E_SCALE) : scal[SC_S];
-  return other >= 0 ? s / scal[other] : s;
+__device__ __forceinline__ float hd_factor(const float* S) {
+  return __is_same(T, f16_t) ? *S * (1.f / E_SCALE) : *S;
+}
+
+// three bf16 numbers whose sum is v; the first alone where v is an infinity or NaN
+struct Bf3 {
+  bf16_t h, m, l;
+};
+__device__ __forceinline__ Bf3 hd_split(float v) {
+  Bf3 b;
+  b.h = (bf16_t)v;
+  float r = v - (float)b.h;
+  if (!(fabsf(r) <= 3.402823466e38f)) {    // no finite number, or one that rounds to infinity
+    const bool fin = fabsf(v) <= 3.402823466e38f;
+    b.h = fin ? (bf16_t)copysignf(3.38953139e38f, v) : b.h;
+    r = fin ? v - (float)b.h : 0.f;
+  }
+  b.m = (bf16_t)r;
+  b.l = (bf16_t)(r - (float)b.m);
+  return b;
 }
 
 // LDS of one stage: P tile then Q tile, HD_BK deep
@@ -120,14 +134,15 @@ __device__ __forceinline__ const char* hd_uniform(const char* p) {
 // TR:     LDS row k holds B / 8 chunks; chunk s of it is source chunk s ^ (2 g(k) mod B / 8), g(k) = (k & 3) | (k >> 3 & 3) << 2
 // The lane's byte offsets from the tile's first element are formed once (32 bits: 256 rows of at most HD_MAX_PITCH elements);
 // a k step moves the uniform base.
-// PAIR: a step is 32 deep in k and both numbers of a value are staged: the first in the first 4 chunks (not TR) or 32 rows (TR)
-// of the tile, the second behind it.
+// F32: a step is 32 deep in k and two of the three numbers of a value are staged: the first in the first 4 chunks (not TR) or 32
+// rows (TR) of the tile, behind it the second (stage 0) or the third (stage 1).
 #define HD_MAX_PITCH (1 << 22)
-template <int B, bool TR, bool CLAMP, int NW, bool PAIR>
+template <int B, bool TR, bool CLAMP, int NW, bool F32>
 struct HdLoad {
-  static constexpr int DEEP = PAIR ? 32 : HD_BK;
+  static constexpr int DEEP = F32 ? 32 : HD_BK;
   static constexpr int NL = B * HD_BK * 2 / 1024 / NW;
   static constexpr int CH = B / 8, RPL = TR ? 64 / CH : 8;      // TR: chunks per row, rows per load
+  static_assert(NL % 2 == 0 && NW % 2 == 0, "which lanes and loads fetch the later number: see issue");
   uint32_t off[NL];
   __device__ __forceinline__ void init(const HdOperand& o, int own0, int wave, int lane) {
 #pragma unroll
@@ -137,7 +152,7 @@ struct HdLoad {
         const int r = blk * 8 + (lane >> 3);
         const int ch = (lane & 7) ^ ((r & 3) | (((r >> 3) & 1) << 2));
         off[q] = 2u * ((uint32_t)(min(own0 + r, o.rows - 1) - own0) * (uint32_t)o.ld +
-                       (PAIR ? (ch & 3) * 8 + (ch >> 2) * (uint32_t)o.plane : ch * 8));
+                       (F32 ? (ch & 3) * 8 + (ch >> 2) * (uint32_t)o.plane : ch * 8));
       } else {
         const int k = blk * RPL + lane / CH;
         const int g = (k & 3) | (((k >> 3) & 3) << 2);
@@ -154,18 +169,22 @@ struct HdLoad {
   // The load is written out so that the compiler's own waits do not count it: it has no register result, and the kernel
   // waits for it (vmcnt) before the barrier that hands the stage over.  s_nop: the wait states between a scalar register's
   // writer (M0, or a base that came through a vector instruction) and its reader, which the compiler does not see here.
-  __device__ __forceinline__ void issue(const HdOperand& o, const char* base, int k0, uint32_t lds, int wave, int lane) const {
+  __device__ __forceinline__ void issue(const HdOperand& o, const char* base, int k0, uint32_t lds, int wave, int lane, bool third) const {
+    // F32 with the third number in the second one's place: not TR, the lanes of chunks 4 to 7 (r >> 3 is blk, whose parity is the
+    // wave's); TR, the loads of rows 32 to 63
     const char* at = hd_uniform(base);
+    const char* at2 = F32 && TR && third ? hd_uniform(base + 2 * o.plane) : at;
+    const uint32_t add = F32 && !TR && third && (((lane >> 2) ^ wave) & 1) ? 2u * (uint32_t)o.plane : 0u;
 #pragma unroll
     for (int q = 0; q < NL; ++q) {
       const int blk = q * NW + wave;
-      uint32_t v = off[q];
+      uint32_t v = off[q] + add;
       if constexpr (CLAMP) {               // rows of k beyond the last: the last one again
         const int k = (blk * RPL + lane / CH) % DEEP;
         v -= 2u * (uint32_t)max(0, k - (o.rows - 1 - k0)) * (uint32_t)o.ld;
       }
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds + blk * 1024)), "v"(v),
-                   "s"(at)
+                   "s"(q < NL / 2 ? at : at2)
                    : "memory");
     }
   }
@@ -173,7 +192,7 @@ struct HdLoad {
 
 // Reading a staged tile (swizzled as above) as matrix operands of 16 own indices each.  hd_at: the lane's LDS address for operand
 // 0 of a wave whose own indices start at o0 (a multiple of 32, 8 times a power of two above the operands' range).  hd_frag:
-// operand x of half kk (of k, or PAIR: the kk'th numbers) from it; x and kk are constants, so it is that address with a few
+// operand x of half kk (of k, or F32: the kk'th numbers of the stage) from it; x and kk are constants, so it is that address with a few
 // bits flipped and an offset in the instruction.
 // `pairs`: the logits' products take P's rows in another order, operand x holds rows hd_row(x) + 8 (m >> 2) + (m & 3), m < 16,
 // so that a lane's results of operands 2 t and 2 t + 1 are 8 consecutive classes of one row: e is stored 16 bytes at a time
@@ -225,14 +244,14 @@ __device__ __forceinline__ void hd_lds_barrier() {
 }
 
 // what a finished tile of products becomes (see HdArgs)
-template <class T, int BI, int BJ, int WI, int WJ, int EPI, bool PAIR>
+template <class T, int BI, int BJ, int WI, int WJ, int EPI, bool F32>
 __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / WI / 16][BJ / WJ / 16], int z, int i0, int j0, int ti,
                                             int wi, int wj, int tid, float* sh) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16;
   const int lane = tid & 63, wave = tid >> 6;
   const int q4 = 4 * (lane >> 4), l15 = lane & 15;
   if constexpr (EPI == EPI_OUT) {
-    const float s = a.out ? hd_factor<T>(a.scal, a.other) : 1.f;
+    const float s = a.out ? hd_factor<T>(a.S) : 1.f;
 #pragma unroll
     for (int y = 0; y < MJ; ++y) {
       const int j = j0 + wj + y * 16 + l15;
@@ -259,14 +278,13 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
       }
     }
   } else {
-    // z = u acc: the product in units of 1 / tau (the scales are powers of two); with a bias, acc becomes z and u one.
+    // z = u acc: the product in units of 1 / tau; with a bias, acc becomes z and u one.
     // exp(z - m) = 2^(z k - m k) in one fused step, off by the rounding of the product m k alone, which is the same factor in
     // all of a row and is taken out of its sum.  That rounding is below one only for |m k| < HD_FAR: beyond (a tile whose classes are
     // all masked by a bias of -1e10, or of the type's lowest value) 2^rounding leaves the range, and the difference is formed
     // first.  Classes beyond the last and targets are looked for only where a tile can hold them: 128 results a lane are 128
     // times whatever one costs.
     float u = a.inv_tau;
-    if constexpr (PAIR) u = fminf(fmaxf(u / (a.scal[SC_X] * a.scal[SC_W]), 1.175494351e-38f), 3.402823466e38f);   // 0 or infinity times what may be either
     if (a.bias) {
 #pragma unroll
       for (int x = 0; x < MI; ++x)
@@ -387,7 +405,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
         // p - 1 of the target: what the other classes hold, not a difference near 1
         const float et = tl >= 0 && c != 0.f ? c * expm1f(-a.loss[j]) : 0.f;
         if (j >= a.rowsE) continue;
-        short* row = a.E + (int64_t)j * a.eplanes * a.colsE + first;
+        short* row = a.E + (int64_t)j * (F32 ? 3 : a.eplanes) * a.colsE + first;
 #pragma unroll
         for (int x = 0; x < MI; x += 2) {
           float e[8];
@@ -404,6 +422,20 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
             for (int r = 0; r < 8; ++r) e[r] = hd_row(x) + r >= last ? 0.f : e[r];
           }
           struct alignas(16) { T t[8]; } h, l;
+          if constexpr (F32) {
+            decltype(h) m;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              h.t[r] = to_t<T>(e[r]);                            // |e| <= 1: no infinities to keep apart
+              const float d = e[r] - (float)h.t[r];
+              m.t[r] = to_t<T>(d);
+              l.t[r] = to_t<T>(d - (float)m.t[r]);
+            }
+            *(decltype(h)*)(row + hd_row(x)) = h;
+            *(decltype(h)*)(row + a.colsE + hd_row(x)) = m;
+            *(decltype(h)*)(row + 2 * a.colsE + hd_row(x)) = l;
+            continue;
+          }
 #pragma unroll
           for (int r = 0; r < 8; ++r) h.t[r] = to_t<T>(e[r]);
           *(decltype(h)*)(row + hd_row(x)) = h;
@@ -422,15 +454,15 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
 // one j, so rows of the output are written in pieces of 4.
 //
 // A workgroup walks its tiles as one sequence of k steps.  Two stages are in LDS; a step is four phases (two halves of k, two
-// of the wave's i), or six where the values are pairs (three products, two halves of i): what is loaded and read from LDS for
-// four multiplies for six there.  The operands of a phase are read while the phase before it multiplies.  The barrier that ends a
+// of the wave's i).  F32: 32 of k are two steps, one over the first and second numbers (h h, h m, m h, m m: eight phases), one
+// over the first and third (h l, l h: four), so that what is loaded and read from LDS for four multiplies for six.  The operands of a phase are read while the phase before it multiplies.  The barrier that ends a
 // step stands before its last phase, whose operands are in registers by then: the loads of the step after the next and the
 // first reads of the next one are issued under that phase's products.  The sequence runs on into the next tile, so a
 // tile's first loads are under way during the last steps and the epilogue of the tile before it.  Behind the last tile the
 // loads fetch that tile's first steps again, into stages that are read no more.
 // Measured (bf16, 4096 x 2048 x 65536): see hd_shape.  What bounds it: the latency of loads that miss the L2 (one step of
 // 64 KB in flight per CU) and the clock, which this load holds near 2.0 GHz.
-template <class T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI, bool PAIR>
+template <class T, int BI, int BJ, int WI, int WJ, bool PT, bool QT, int EPI, bool F32>
 __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdArgs a) {
   constexpr int NW = WI * WJ, MI = BI / WI / 16, MJ = BJ / WJ / 16, HX = MI / 2;
   constexpr int SZ = hd_tile_shorts<BI>() + hd_tile_shorts<BJ>();
@@ -460,19 +492,19 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     ti = rem / bw;
   };
   const int wi = (wave % WI) * (BI / WI), wj = (wave / WI) * (BJ / WJ);
-  const int nseg = PAIR ? 1 : a.nseg, total = a.ktiles * nseg;
+  const int nseg = F32 ? 1 : a.nseg, total = a.ktiles * nseg;
   const int t0 = (int)((int64_t)total * z / a.splits), t1 = (int)((int64_t)total * (z + 1) / a.splits);
 
   // only W is read along k where it lies, with rows beyond its last (PT && !QT); e and the copied x are whole k steps
-  using LP = HdLoad<BI, PT, PT && !QT, NW, PAIR>;
-  using LQ = HdLoad<BJ, QT, false, NW, PAIR>;
+  using LP = HdLoad<BI, PT, PT && !QT, NW, F32>;
+  using LQ = HdLoad<BJ, QT, false, NW, F32>;
   LP lp;
   LQ lq;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) short*)sm;
   // The next load: its tile, how many of the tile's are left, the step of k and in it the number of Q's values (a step is read
   // again while the L2 has it), and the operands' bases.  Stages alternate by constants in the code, so an odd count of
-  // steps gets one more that repeats the last load and multiplies nothing.
-  const int steps = t1 - t0, pad = steps & 1;
+  // steps gets one more that repeats the last load and multiplies nothing (F32: two steps to a k, so never).
+  const int steps = F32 ? 2 * (t1 - t0) : t1 - t0, pad = F32 ? 0 : steps & 1;
   const int first_k = t0 / nseg, first_seg = t0 - first_k * nseg;
   const int64_t pq = 2 * a.Q.plane, dp = LP::advance(a.P), dq = LQ::advance(a.Q) - (nseg == 2 ? pq : 0);
   int lid = id, left, seg, lk, li0, lj0;
@@ -496,14 +528,20 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     base();
   };
   auto issue = [&](int stage) __attribute__((always_inline)) {
-    lp.issue(a.P, bp, lk * LP::DEEP, lds0 + stage * (SZ * 2), wave, lane);
-    lq.issue(a.Q, bq, lk * LQ::DEEP, lds0 + stage * (SZ * 2) + hd_tile_shorts<BI>() * 2, wave, lane);
+    lp.issue(a.P, bp, lk * LP::DEEP, lds0 + stage * (SZ * 2), wave, lane, stage == 1);
+    lq.issue(a.Q, bq, lk * LQ::DEEP, lds0 + stage * (SZ * 2) + hd_tile_shorts<BI>() * 2, wave, lane, stage == 1);
     if (--left == 0) {
       if (lid + stride < end) {
         lid += stride;
         aim();
       }
       rewind();
+    } else if constexpr (F32) {
+      if (stage == 1) {
+        ++lk;
+        bp += dp;
+        bq += dq;
+      }
     } else if (left > pad) {
       if (++seg == nseg) {
         seg = 0;
@@ -517,21 +555,21 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
   };
   s16x8 fp[2][HX], fq[2][MJ];
   f32x4 acc[MI][MJ];
-  // half `kk` of the tiles' depth (PAIR: the first or second numbers) of half `hx` of the wave's P, and of its Q, into a buffer each
-  // PAIR: the addresses are formed anew from one register each time.  Kept per operand and stage they would not fit beside both
+  // half `kk` of the tiles' depth (F32: the first or the later numbers) of half `hx` of the wave's P, and of its Q, into a buffer each
+  // F32: the addresses are formed anew from one register each time.  Kept per operand and stage they would not fit beside both
   // numbers' operands (the empty asm keeps the compiler from doing so), and a spilled one is a load that waits for the tiles'
-  // loads: 4096 x 1024 x 32000 at 1000 us instead of 640 a product.  Single numbers have the registers, and lose 3 % without them.
+  // loads (two thirds more time).  Single numbers have the registers, and lose 3 % without them.
   constexpr bool pairs = EPI != EPI_OUT;
   const uint32_t ap = hd_at<BI, PT, pairs>(lds0, wi, lane), aq = hd_at<BJ, QT, false>(lds0 + hd_tile_shorts<BI>() * 2, wj, lane);
   auto read_p = [&](int stage, int kk, int hx) __attribute__((always_inline)) {
     uint32_t at = ap + stage * (SZ * 2);
-    if constexpr (PAIR) asm volatile("" : "+v"(at));
+    if constexpr (F32) asm volatile("" : "+v"(at));
 #pragma unroll
     for (int x = 0; x < HX; ++x) fp[hx][x] = hd_frag<BI, PT, pairs>(at, hx * HX + x, kk);
   };
   auto read_q = [&](int stage, int kk, int buf) __attribute__((always_inline)) {
     uint32_t at = aq + stage * (SZ * 2);
-    if constexpr (PAIR) asm volatile("" : "+v"(at));
+    if constexpr (F32) asm volatile("" : "+v"(at));
 #pragma unroll
     for (int y = 0; y < MJ; ++y) fq[buf][y] = hd_frag<BJ, QT, false>(at, y, kk);
   };
@@ -545,24 +583,38 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // A step's products but for the last group, whose operands are read: on `stage`, whose first half of P and of Q (in buffer
-  // `b`) is in registers.  PAIR: the first and second numbers of P and Q serve three products
-  auto multiply = [&](int stage, int b) __attribute__((always_inline)) {
+  // A step's products but for the last group, mul(1, 1), whose operands are read: on `stage`, whose first half of P and of Q is in
+  // registers (fp[0], fq[0]).
+  auto multiply = [&](int stage) __attribute__((always_inline)) {
     read_p(stage, 0, 1);
-    if constexpr (PAIR) read_q(stage, 1, 1 - b);
-    mul(0, b);
-    if constexpr (PAIR) {
-      mul(1, b);
-      mul(0, 1 - b);
-      read_p(stage, 1, 0);
-      mul(1, 1 - b);
+    if constexpr (F32) {
+      if (stage == 0) {                    // h and m of both
+        read_q(0, 1, 1);
+        mul(0, 0);                         // h h
+        mul(1, 0);
+        mul(0, 1);                         // h m
+        read_p(0, 1, 0);
+        mul(1, 1);
+        read_p(0, 1, 1);
+        mul(0, 0);                         // m h
+        mul(0, 1);                         // m m
+        mul(1, 0);
+      } else {                             // h and l of both, Q's l read first
+        read_q(1, 0, 1);
+        mul(0, 0);                         // h l
+        read_p(1, 1, 0);
+        mul(1, 0);
+        read_p(1, 1, 1);
+        mul(0, 1);                         // l h
+      }
     } else {
-      read_q(stage, 1, 1 - b);
+      mul(0, 0);
+      read_q(stage, 1, 1);
       read_p(stage, 1, 0);
-      mul(1, b);
+      mul(1, 0);
+      read_p(stage, 1, 1);
+      mul(0, 1);
     }
-    read_p(stage, 1, 1);
-    mul(0, PAIR ? b : 1 - b);
   };
   // this wave's loads have landed and its LDS reads are done, and every other wave's
   auto meet = [&]() __attribute__((always_inline)) {
@@ -581,19 +633,19 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     for (int x = 0; x < MI; ++x)
 #pragma unroll
       for (int y = 0; y < MJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // the buffer of Q that a step's last group leaves free takes the next step's first half
-    constexpr int second = PAIR ? 1 : 0;
     read_q(0, 0, 0);
     read_p(0, 0, 0);
     for (int t = 0; t < steps; t += 2) {
-      multiply(0, 0);
+      multiply(0);
       meet();                              // the next step has arrived; this one has been read by all
       issue(0);
-      read_q(1, 0, second);
+      read_q(1, F32 ? 1 : 0, 0);
       read_p(1, 0, 0);
-      mul(1, 1 - second);
-      const bool more = t + 1 < steps;     // not of an odd count's last step, whose partner is only waited for
-      if (more) multiply(1, second);
+      mul(1, 1);
+      // not of an odd count's last step, whose partner is only waited for (F32 has none; without the branch the compiler keeps
+      // both steps' addresses and spills 13 to 31 registers, with it at most 7)
+      const bool more = t + 1 < steps;
+      if (more) multiply(1);
       meet();
       issue(1);
       if (t + 2 < steps) {                 // across the epilogue the registers are the result's
@@ -602,7 +654,7 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
       }
       if (more) mul(1, 1);
     }
-    hd_epilogue<T, BI, BJ, WI, WJ, EPI, PAIR>(a, acc, z, ti * BI, tj * BJ, ti, wi, wj, tid, sh);
+    hd_epilogue<T, BI, BJ, WI, WJ, EPI, F32>(a, acc, z, ti * BI, tj * BJ, ti, wi, wj, tid, sh);
   }
   __builtin_amdgcn_s_waitcnt(0);           // nothing is in flight into LDS when it is given back
   __builtin_amdgcn_s_barrier();
@@ -627,85 +679,6 @@ __device__ __forceinline__ float hd_block_max(float m, float* sh) {
   for (int w = 0; w < NW; ++w) m = fmaxf(m, sh[w]);
   return m;
 }
-// does row n's teacher list a class.  Called by whole waves
-__device__ __forceinline__ bool hd_listed(int64_t n, const int64_t* index, const void* tl, int tdt, int K, int lane) {
-  bool any = false;
-  for (int k = lane; k < K; k += 64) any |= index[n * K + k] >= 0 && load_as(tl, tdt, n * K + k) != -INFINITY;
-  return __any(any);
-}
-
-// partial max |v| over the finite entries of x's rows that have a loss (blocks [0, HD_AMAX); what the others hold, the
-// lowest value of a mask say, must not set the scale) and of W (the rest): amax[2 HD_AMAX]
-#define HD_AMAX 256
-__global__ void __launch_bounds__(512) k_head_amax(const float* __restrict__ x, int64_t ldx, int64_t R, const float* __restrict__ w,
-                                                    int64_t ldw, int64_t V, int D, const int64_t* __restrict__ target, int64_t ignore,
-                                                    const int64_t* __restrict__ index, const void* __restrict__ tl, int tdt, int K,
-                                                    float* __restrict__ amax) {
-  __shared__ float sh[8];
-  const int lane = threadIdx.x & 63;
-  const bool second = blockIdx.x >= HD_AMAX;
-  const float* p = second ? w : x;
-  const int64_t ld = second ? ldw : ldx, rows = second ? V : R;
-  const int b = second ? blockIdx.x - HD_AMAX : blockIdx.x;
-  float m = 0.f;
-  auto see = [&](float v) {
-    v = fabsf(v);
-    m = v <= 3.402823466e38f ? fmaxf(m, v) : m;
-  };
-  if (second && ld == D) {
-    const int64_t n = rows * D, n4 = n >> 2;
-    const RowVec<float, 4>* q = (const RowVec<float, 4>*)p;
-#pragma unroll 4
-    for (int64_t i = (int64_t)b * 512 + threadIdx.x; i < n4; i += HD_AMAX * 512) {
-      const RowVec<float, 4> v = q[i];
-      see(v.v[0]); see(v.v[1]); see(v.v[2]); see(v.v[3]);
-    }
-    if (b == 0 && (int64_t)threadIdx.x < (n & 3)) see(p[n - 1 - threadIdx.x]);
-  } else {
-    // a wave takes up to 64 rows at a time, fewer where that would leave waves idle, looks which of them have a loss, then
-    // its lanes read 4 entries each of as many rows as they hold
-    const int most = (int)min((int64_t)64, (rows + HD_AMAX * 8 - 1) / (HD_AMAX * 8));
-    int lpr = 1;
-    while (lpr < 64 && lpr * 4 < D) lpr *= 2;
-    const int rpi = 64 / lpr, mine = lane / lpr, d0 = lane % lpr * 4;
-    for (int64_t r0 = (int64_t)(b * 8 + (threadIdx.x >> 6)) * most; r0 < rows; r0 += (int64_t)HD_AMAX * 8 * most) {
-      const int n = (int)min((int64_t)most, rows - r0);
-      uint64_t live = ~0ull;
-      if (!second && target) {
-        live = __ballot(lane < n && target[r0 + lane] != ignore);
-      } else if (!second) {
-        live = 0;
-#pragma unroll 4
-        for (int r = 0; r < n; ++r) live |= (uint64_t)hd_listed(r0 + r, index, tl, tdt, K, lane) << r;
-      }
-#pragma unroll 4
-      for (int q = 0; q < n; q += rpi) {
-        const int r = q + mine;
-        if (r >= n || !(live >> r & 1)) continue;
-        const float* row = p + (r0 + r) * ld;
-        for (int d = d0; d < D; d += lpr * 4) {
-          if (d + 4 <= D) {
-            const RowVec<float, 4> v = *(const RowVec<float, 4>*)(row + d);
-            see(v.v[0]); see(v.v[1]); see(v.v[2]); see(v.v[3]);
-          } else {
-            for (int i = d; i < D; ++i) see(row[i]);
-          }
-        }
-      }
-    }
-  }
-  m = hd_block_max<8>(m, sh);
-  if (threadIdx.x == 0) amax[blockIdx.x] = m;
-}
-
-// 2^k with 2^k m in [2^14, 2^15); 1 for an all-zero tensor.  -113 <= k <= 100: 2^k and 2^-k are normal numbers.
-__device__ __forceinline__ float hd_scale(float m) {
-  if (!(m > 0.f)) return 1.f;
-  int e;
-  frexpf(m, &e);
-  return ldexpf(1.f, min(15 - e, 100));
-}
-
 __device__ __forceinline__ float hd_finite_max(float m, float v) {
   v = fabsf(v);
   return v <= 3.402823466e38f ? fmaxf(m, v) : m;
@@ -724,13 +697,12 @@ struct HdPack {
   int D;
   short* out;                // [orows][numbers][ocols]
   int64_t orows;
-  int ocols, slot, blocks;   // slot: SC_X / SC_W
+  int ocols, blocks;
 };
 struct HdPrep {
   HdPack x, w;
   int masked;                // rows of x without a loss are copied as zeros
-  const float* amax;
-  float* scal;
+  float* S;
   int coef_blocks;           // HD_COEF rows each
   const float *g, *gm;       // per_row: the rows' gradients and, beyond HD_COEF rows, their partial maxima
   int ngm, per_row;
@@ -768,46 +740,41 @@ __device__ __forceinline__ void hd_coef(const HdPrep& a, int b, float* sh) {
   const int end = min(a.N, (b + 1) * HD_COEF);
   for (int n = b * HD_COEF + threadIdx.x; n < end; n += 256)       // a NaN of live is the gradient's too
     a.coef[n] = hd_has(n, a.target, a.ignore, a.live) ? (a.per_row ? a.g[n] * a.f / S : 1.f) * (a.live ? a.live[n] : 1.f) : 0.f;
-  if (b == 0 && threadIdx.x == 0) a.scal[SC_S] = S;
+  if (b == 0 && threadIdx.x == 0) *a.S = S;
 }
 
 // out <- rows [0, R) of src (type dt, pitch ld, D columns), zeros elsewhere and in masked rows (their contents, whatever they
-// are, take no part in any sum).  f32: two numbers, and block 0 leaves the scale in scal[slot].
-__device__ __forceinline__ void hd_pack(const HdPrep& a, const HdPack& j, int b, bool masked, float* sh) {
-  float s = 1.f;
-  if (j.dt == DT_F32) {
-    s = hd_scale(hd_block_max<4>(a.amax[j.slot * HD_AMAX + threadIdx.x], sh));
-    if (b == 0 && threadIdx.x == 0) a.scal[j.slot] = s;
-  }
+// are, take no part in any sum).  f32: three numbers.
+__device__ __forceinline__ void hd_pack(const HdPrep& a, const HdPack& j, int b, bool masked) {
   const int oc8 = j.ocols >> 3;
-  const int64_t pitch = j.dt == DT_F32 ? 2 * (int64_t)j.ocols : j.ocols;
+  const int64_t pitch = j.dt == DT_F32 ? 3 * (int64_t)j.ocols : j.ocols;
   const int64_t n = j.orows * oc8;
   for (int64_t u = (int64_t)b * 256 + threadIdx.x; u < n; u += (int64_t)j.blocks * 256) {
     const int64_t r = u / oc8;
     const int c = (int)(u - r * oc8) * 8;
     const bool live = r < j.R && (!masked || hd_has(r, a.target, a.ignore, a.live));
     const int left = live ? min(8, j.D - c) : 0;
-    s16x8 h = {0, 0, 0, 0, 0, 0, 0, 0}, l = h;
+    s16x8 h = {0, 0, 0, 0, 0, 0, 0, 0}, m = h, l = h;
     if (j.dt == DT_F32) {
       float f[8];
       const float* p = (const float*)j.src + r * j.ld + c;
       if (left == 8) {
         const RowVec<float, 8> v = *(const RowVec<float, 8>*)p;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = v.v[i] * s;
+        for (int i = 0; i < 8; ++i) f[i] = v.v[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < left ? p[i] * s : 0.f;
+        for (int i = 0; i < 8; ++i) f[i] = i < left ? p[i] : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const f16_t hi = (f16_t)f[i];
-        const float d = f[i] - (float)hi;
-        const f16_t lo = (f16_t)(fabsf(d) <= 65504.f ? d : 0.f);    // an infinity or NaN is the first number's alone
-        h[i] = __builtin_bit_cast(short, hi);
-        l[i] = __builtin_bit_cast(short, lo);
+        const Bf3 n = hd_split(f[i]);
+        h[i] = __builtin_bit_cast(short, n.h);
+        m[i] = __builtin_bit_cast(short, n.m);
+        l[i] = __builtin_bit_cast(short, n.l);
       }
-      *(s16x8*)(j.out + r * pitch + j.ocols + c) = l;
+      *(s16x8*)(j.out + r * pitch + j.ocols + c) = m;
+      *(s16x8*)(j.out + r * pitch + 2 * j.ocols + c) = l;
     } else {
       const short* p = (const short*)j.src + r * j.ld + c;
       if (left == 8) {
@@ -827,8 +794,8 @@ __global__ void __launch_bounds__(256) k_head_prep(HdPrep a) {
   __shared__ float sh[4];
   const int b = blockIdx.x, bx = b - a.coef_blocks, bw = bx - a.x.blocks;
   if (bx < 0) hd_coef(a, b, sh);
-  else if (bw < 0) hd_pack(a, a.x, bx, a.masked, sh);
-  else hd_pack(a, a.w, bw, false, sh);
+  else if (bw < 0) hd_pack(a, a.x, bx, a.masked);
+  else hd_pack(a, a.w, bw, false);
 }
 
 __device__ __forceinline__ float hd_wave_sum(float v) {
@@ -1125,10 +1092,12 @@ __global__ void __launch_bounds__(256) k_head_teacher_grad(const int64_t* __rest
   if constexpr (sizeof(T) == 4) {
     *o = e;
   } else {
-    const float s = __is_same(T, f16_t) ? e * E_SCALE : e;
-    const T h = to_t<T>(s);
-    *o = h;
-    if (planes == 2) o[colsE] = to_t<T>(s - (float)h);
+    float s = __is_same(T, f16_t) ? e * E_SCALE : e;
+    for (int q = 0; q < planes; ++q) {     // its rounding, and that of what it left
+      const T h = to_t<T>(s);
+      o[q * colsE] = h;
+      s -= (float)h;
+    }
   }
 }
 
@@ -1170,7 +1139,6 @@ struct HdSum {
   const float* part;
   int slots;
   int64_t stride, n;
-  int other;                 // its factor (hd_factor)
   void* out;
   int64_t at0;
   int many, blocks;
@@ -1178,7 +1146,7 @@ struct HdSum {
 struct HdSums {
   HdSum j[3];
   int dt;
-  const float* scal;         // null: factors of 1
+  const float* S;            // the factor's (hd_factor); null: factors of 1
 };
 template <class T>
 __global__ void __launch_bounds__(256) k_head_sum(HdSums a) {
@@ -1186,7 +1154,7 @@ __global__ void __launch_bounds__(256) k_head_sum(HdSums a) {
   int b = blockIdx.x, k = 0;
   while (k < 2 && b >= a.j[k].blocks) b -= a.j[k++].blocks;
   const HdSum& j = a.j[k];
-  const float f = a.scal ? hd_factor<T>(a.scal, j.other) : 1.f;
+  const float f = a.S ? hd_factor<T>(a.S) : 1.f;
   if (j.many) {
     const int col = threadIdx.x & 15, sl = threadIdx.x >> 4;
     const int64_t i = (int64_t)b * 16 + col;
@@ -1226,10 +1194,12 @@ struct HdShape {
 //   their gradient e, 4096 x 2048 x 65536: 2372 / 1219 / 1014    2048 x 256 x 32768: 94 / 67 / 55
 //   e W, 4096 x 2048 x 65536: 2325 (1) / 1063 (1) / 946 (2)    2048 x 256 x 32768: 57 (16) / 39 (16) / 43 (32)
 //   1024 x 128 x 65536: 34 (32) / 32 (32) / 40 (64)    e^T x, 4096 x 2048 x 65536: 2452 / 1214 / 989    2048 x 256 x 32768: 56 / 41 / 61
-// Pairs, a step of 32 with three products: 1.2 times a step's time (4096 x 1024 x 32000, tiles of 256: 609 to 709 us where products
-// one after the other took 730; 2048 x 256 x 32768, e^T x on 128: 122 -> 105).
+// F32, 32 of k with six products: 2.4 times a step's time.  us with tiles of 64 / 128 / 256:
+//   statistics, 4096 x 1024 x 32000: 2985 / 1469 / 1200 (1.34 PFLOP/s of bf16 products, the copies included)   2048 x 256 x 32768:
+//   315 / 205 / 188   1024 x 128 x 65536: 186 / 126 / 117   512 x 512 x 4096: 41 / 48 / 88.  What the estimate takes is within 2 % of
+//   the best of every tile and count of ranges tried, in all three products of seven sizes.
 // A split product writes its partial results and a second launch adds them (bytes at 4 TB/s and 4 us).
-static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, bool pair, int max_splits) {
+static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, bool f32, int max_splits) {
   const int cus = dig3d_num_cus();
   HdShape best = {64, 1};
   double tb = 1e30;
@@ -1244,7 +1214,7 @@ static HdShape hd_shape(int64_t ni, int64_t nj, int64_t ksteps, bool pair, int m
       const int64_t items = tiles * s, c0 = (items + cus - 1) / cus;
       const int c = (int)(c0 < occ ? c0 : occ);
       const int64_t rounds = (items + (int64_t)cus * c - 1) / ((int64_t)cus * c);
-      const double step = (pair ? 1.2 : 1.0) * (e == 0 ? 0.35 + 0.15 * c : e == 1 ? 0.42 + 0.38 * c : 1.9);
+      const double step = (f32 ? 2.4 : 1.0) * (e == 0 ? 0.35 + 0.15 * c : e == 1 ? 0.42 + 0.38 * c : 1.9);
       const double fixed = e == 0 ? 2.0 + 0.5 * c : e == 1 ? 1.5 + 0.8 * c : 6.0;
       double t = (double)rounds * (fixed + (double)((ksteps + s - 1) / s) * step);
       if (s > 1) t += 4.0 + (double)s * ni * nj * 8 / 4e6;
@@ -1263,13 +1233,13 @@ static inline int64_t al256(int64_t v) { return (v + 255) & ~255ll; }
 struct HdPlan {
   bool small;                // head_small.h
   int Dp, eplanes;           // eplanes: numbers of an entry of e
-  bool pair;                 // float32: every value is two numbers
+  bool f32;                  // every value is three numbers
   bool dx, dw;               // x / W are read where they are
   int64_t Np, vp, np, ldE;
   HdShape lg, gx, gw;
   int tiles_all;
   // byte offsets into the workspace
-  int64_t o_x, o_w, o_part, o_zt, o_coef, o_scal, o_E, o_gx, o_gw, o_col, total;
+  int64_t o_x, o_w, o_part, o_zt, o_coef, o_S, o_E, o_gx, o_gw, o_col, total;
 };
 
 // 16-bit rows are used in place when their pitch keeps 16-byte loads aligned and D is whole k steps
@@ -1278,18 +1248,19 @@ static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
 }
 
 // e of one piece, per plane; a piece also bounds the packed part of W.  ms with gradients by pieces of 64 / 128 / 256 / 512 MiB:
-// 4096 x 2048 x 131072 bf16 7.71 / 7.40 / 7.43 / 7.32   8192 x 128 x 65536 bf16 1.65 / 1.30 / 1.37 / 1.38   8192 x 256 x 32768 f32
-// 2.06 / 2.04 / 2.03 / 1.98   1741 x 114 x 118479 f32 1.52 / 1.41 / 1.33 / 1.34: the last-level cache returns nothing for it
+// 4096 x 2048 x 131072 bf16 7.71 / 7.40 / 7.43 / 7.32   8192 x 128 x 65536 bf16 1.65 / 1.30 / 1.37 / 1.38: the last-level cache
+// returns nothing for it.  A piece is 256 classes at least, whatever its rows take.
 #define HD_PIECE_BYTES (512ll << 20)
 
 // Float32 products in place (head_small.h) where copies and launches are what the general path costs, or where few float32 rows meet
-// a W that it would read three times (its scale, its copy) before the first product is done.  GPU us in place / general, with
-// gradients (losses alone).  A training call is five launches in place and eight to eleven otherwise, which a host that
+// a W that it would copy, at one and a half times its size, before the first product.  GPU us in place / general, with
+// gradients (losses alone).  A training call is five launches in place and eight to ten otherwise, which a host that
 // launches them one by one pays with some 15 us: the border is where the GPU loses that much.
-//   f32: 128 x 128 x 1195: 41 / 54 (20 / 24)   512 x 128 x 1195: 64 / 58 (19 / 25)   1024 x 128 x 1195: 98 / 64   512 x 128 x 4096: 77 / 72 (21 / 27)
-//        256 x 128 x 16384: 99 / 87 (29 / 34)   64 x 256 x 1024: 50 / 56 (25 / 28)   64 x 256 x 32768: 116 / 117 (42 / 56)
-//        128 x 512 x 1024: 73 / 64   256 x 512 x 1024: 82 / 67   8 x 1024 x 1024: 103 / 70   64 x 512 x 16384: 116 / 116 (41 / 52)
-//        1 x 1024 x 8192: 130 / 108 (52 / 46)   16 x 1024 x 16384: 156 / 155 (52 / 62)   64 x 2048 x 32768: 523 / 610 (128 / 258)
+//   f32: 32 x 128 x 1195: 38 / 48 (18 / 21)   128 x 128 x 1195: 41 / 51   512 x 128 x 1195: 62 / 57 (18 / 22)   1024 x 128 x 1195: 93 / 65
+//        512 x 128 x 4096: 76 / 68 (21 / 25)   256 x 128 x 16384: 89 / 89 (28 / 33)   200 x 256 x 2048: 66 / 62   64 x 256 x 1024: 50 / 57 (25 / 27)
+//        64 x 256 x 32768: 110 / 131 (42 / 54)   128 x 512 x 1024: 73 / 72 (31 / 30)   128 x 512 x 2048: 81 / 77   256 x 512 x 1024: 83 / 78
+//        8 x 1024 x 1024: 103 / 92 (50 / 39)   64 x 512 x 16384: 112 / 123 (41 / 50)   1 x 1024 x 8192: 127 / 126 (51 / 50)
+//        64 x 1024 x 8192: 144 / 141 (54 / 58)   16 x 1024 x 16384: 152 / 207 (51 / 65)   64 x 2048 x 32768: 469 / 793 (124 / 272)
 //   16-bit rows read in place by both: 32 x 128 x 1195: 38 / 39   128 x 64 x 300: 37 / 42   32 x 128 x 8192: 44 / 40   512 x 128 x 256: 60 / 44
 //   16-bit rows that the general path copies (odd widths or addresses): 32 x 127 x 8192: 46 / 47   14 x 40 x 67126: 67 / 83
 //        64 x 127 x 32768: 95 / 84   128 x 127 x 4096: 57 / 49   16 x 255 x 8192: 56 / 52   10 x 214 x 105058: 225 / 165   512 x 127 x 1195: 84 / 53   128 x 511 x 1024: 87 / 55
@@ -1305,7 +1276,7 @@ static bool hd_small(bool f32, bool copies, int64_t N, int64_t D, int64_t V) {
 }
 
 // k steps of a product over `k` values, one operand of `q` numbers each
-static int64_t hd_steps(const HdPlan& p, int64_t k, int q) { return p.pair ? (k + 31) / 32 : (k + 63) / 64 * q; }
+static int64_t hd_steps(const HdPlan& p, int64_t k, int q) { return p.f32 ? (k + 31) / 32 : (k + 63) / 64 * q; }
 
 // needs: bit 0 gx, bit 1 gw, bit 2 gb; backward = 0: the forward's plan
 static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int backward, int needs) {
@@ -1339,18 +1310,18 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     p.total = at;
     return p;
   }
-  p.pair = dt == DT_F32;
-  const int planes = p.pair ? 2 : 1;
+  p.f32 = dt == DT_F32;
+  const int planes = p.f32 ? 3 : 1;
   // One rounding of e is lost among the roundings of the gradients where many rows add up (2^1/2 of the error of their own);
   // in a few rows it is a common factor of a whole row of gw.  There W is what the products wait for, and e is two numbers;
   // also where the second product costs no more than launches do (512 x 512 x 8192: 15 us of 190)
-  p.eplanes = dt == DT_F32 || N <= 128 || (double)N * D * V <= 2147483648.0 ? 2 : 1;
+  p.eplanes = p.f32 ? 3 : N <= 128 || (double)N * D * V <= 2147483648.0 ? 2 : 1;
   p.Dp = (int)up64(D);
   p.dx = dx && !backward;    // the backward masks rows while it copies x (N D elements: nothing beside its products)
   p.dw = dw;
   p.Np = up64(N);
   int64_t most = V;
-  if (backward) most = min(most, min(HD_PIECE_BYTES / (p.Np * 2), (int64_t)HD_MAX_PITCH / 2 - 1024));
+  if (backward) most = min(most, min(HD_PIECE_BYTES / (p.Np * 2), (int64_t)HD_MAX_PITCH / p.eplanes - 1024));
   if (!p.dw) most = min(most, HD_PIECE_BYTES / ((int64_t)p.Dp * 2 * planes));
   if (most < V) most = max((int64_t)256, most & ~255ll);
   p.np = (V + most - 1) / most;
@@ -1358,7 +1329,7 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
   p.np = (V + p.vp - 1) / p.vp;
   p.ldE = up64(p.vp);
   if (p.ldE * p.eplanes % 1024 == 0) p.ldE += 64;      // rows of e a multiple of 2 KB apart fall on few channels of the caches
-  p.lg = hd_shape(p.vp, N, hd_steps(p, p.Dp, 1), p.pair, 1);
+  p.lg = hd_shape(p.vp, N, hd_steps(p, p.Dp, 1), p.f32, 1);
   if (!p.dx) p.o_x = take(p.Np * p.Dp * 2 * planes);
   if (!p.dw) p.o_w = take(min(p.vp, V) * p.Dp * 2 * planes);
   if (!backward) {
@@ -1368,14 +1339,14 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
     p.o_zt = take(N * 4);
   } else {
     p.o_coef = take(N * 4);
-    p.o_scal = take(SC_COUNT * 4 + (N + HD_TOTAL - 1) / HD_TOTAL * 4);
+    p.o_S = take(4 + (N + HD_TOTAL - 1) / HD_TOTAL * 4);
     p.o_E = take(p.Np * p.ldE * 2 * p.eplanes);
     if (needs & 1) {
-      p.gx = hd_shape(D, N, hd_steps(p, p.vp, p.eplanes), p.pair, 512);
+      p.gx = hd_shape(D, N, hd_steps(p, p.vp, p.eplanes), p.f32, 512);
       if (p.np > 1 || p.gx.splits > 1) p.o_gx = take((int64_t)p.gx.splits * N * D * 4);
     }
     if (needs & 2) {
-      p.gw = hd_shape(D, p.vp, hd_steps(p, N, p.eplanes), p.pair, 512);
+      p.gw = hd_shape(D, p.vp, hd_steps(p, N, p.eplanes), p.f32, 512);
       if (p.gw.splits > 1) p.o_gw = take((int64_t)p.gw.splits * p.vp * D * 4);
     }
     if (needs & 4) p.o_col = take((N + HD_SLICE - 1) / HD_SLICE * p.ldE * 4);
@@ -1384,14 +1355,14 @@ static HdPlan hd_plan(int dt, int64_t N, int D, int64_t V, bool dx, bool dw, int
   return p;
 }
 
-template <class T, bool PT, bool QT, int EPI, bool PAIR>
+template <class T, bool PT, bool QT, int EPI, bool F32>
 static void hd_launch(const HdArgs& a, int b, const dim3& grid, hipStream_t st) {
-  if (b == 256) hipLaunchKernelGGL((k_head_gemm<T, 256, 256, 2, 4, PT, QT, EPI, PAIR>), grid, dim3(512), 0, st, a);
-  else if (b == 128) hipLaunchKernelGGL((k_head_gemm<T, 128, 128, 2, 2, PT, QT, EPI, PAIR>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_head_gemm<T, 64, 64, 2, 2, PT, QT, EPI, PAIR>), grid, dim3(256), 0, st, a);
+  if (b == 256) hipLaunchKernelGGL((k_head_gemm<T, 256, 256, 2, 4, PT, QT, EPI, F32>), grid, dim3(512), 0, st, a);
+  else if (b == 128) hipLaunchKernelGGL((k_head_gemm<T, 128, 128, 2, 2, PT, QT, EPI, F32>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_head_gemm<T, 64, 64, 2, 2, PT, QT, EPI, F32>), grid, dim3(256), 0, st, a);
 }
 template <class T, bool PT, bool QT, int EPI>
-static void hd_gemm(const HdArgs& a0, const HdShape& sh, bool pair, hipStream_t st) {
+static void hd_gemm(const HdArgs& a0, const HdShape& sh, bool f32, hipStream_t st) {
   HdArgs a = a0;
   a.ti = (a.ni + sh.b - 1) / sh.b;
   a.tj = (a.nj + sh.b - 1) / sh.b;
@@ -1400,8 +1371,8 @@ static void hd_gemm(const HdArgs& a0, const HdShape& sh, bool pair, hipStream_t 
   const int most = dig3d_num_cus() * (sh.b == 256 ? 1 : sh.b == 128 ? 2 : 5);
   a.wgs = min(a.ti * a.tj, max(1, most / sh.splits));
   const dim3 grid((unsigned)(sh.splits == 1 ? min(dig3d_xcd_grid(a.ti * a.tj), (most + 7) & ~7) : (a.wgs * sh.splits + 7) & ~7));
-  if constexpr (__is_same(T, f16_t)) {
-    if (pair) return hd_launch<T, PT, QT, EPI, true>(a, sh.b, grid, st);
+  if constexpr (__is_same(T, bf16_t)) {
+    if (f32) return hd_launch<T, PT, QT, EPI, true>(a, sh.b, grid, st);
   }
   hd_launch<T, PT, QT, EPI, false>(a, sh.b, grid, st);
 }
@@ -1413,11 +1384,11 @@ static inline unsigned hd_grid(int64_t items, int per) {
 
 // one of a launch's sums.  us in order / by 16 lanes:  2140 results of 64 partials 6.0 / 4.0, 32768 of 16: 5.4 / 4.8; 574 of 32 in
 // order 4.1, of 512 by 16 lanes 4.0
-static void hd_add_sum(HdSums& a, const float* part, int slots, int64_t stride, int64_t n, int other, void* out, int64_t at0) {
+static void hd_add_sum(HdSums& a, const float* part, int slots, int64_t stride, int64_t n, void* out, int64_t at0) {
   int k = 0;
   while (a.j[k].blocks) ++k;
   const bool many = slots >= 16 && n <= 65536;
-  a.j[k] = {part, slots, stride, n, other, out, at0, many, many ? (int)((n + 15) / 16) : (int)hd_grid(n, 256)};
+  a.j[k] = {part, slots, stride, n, out, at0, many, many ? (int)((n + 15) / 16) : (int)hd_grid(n, 256)};
 }
 template <class T>
 static int hd_sums(const HdSums& a, hipStream_t st) {
@@ -1428,8 +1399,8 @@ static int hd_sums(const HdSums& a, hipStream_t st) {
   return DIG3D_OK;
 }
 
-static HdPack hd_pack_job(const void* src, int dt, int64_t ld, int64_t R, int D, void* out, int64_t orows, int ocols, int slot) {
-  return {src, dt, ld, R, D, (short*)out, orows, ocols, slot, (int)hd_grid(orows * (ocols >> 3), 256)};
+static HdPack hd_pack_job(const void* src, int dt, int64_t ld, int64_t R, int D, void* out, int64_t orows, int ocols) {
+  return {src, dt, ld, R, D, (short*)out, orows, ocols, (int)hd_grid(orows * (ocols >> 3), 256)};
 }
 static int hd_prep(const HdPrep& a, hipStream_t st) {
   const int blocks = a.coef_blocks + a.x.blocks + a.w.blocks;
@@ -1461,15 +1432,13 @@ struct HdCall {
   float tau;
   int reduction;             // 0 one loss per row, 1 mean, 2 sum
   // kept from the forward for the backward (float[HD_KEEP + 4 N + 2 N K])
-  float *scal, *amax, *count, *m, *rs, *loss, *live, *q, *z;
+  float *count, *m, *rs, *loss, *live, *q, *z;
   hipStream_t st;
 };
-#define HD_KEEP 520
+#define HD_KEEP 8
 
 static void hd_keep(HdCall& c, float* keep) {
-  c.scal = keep;
-  c.amax = keep + SC_COUNT;
-  c.count = keep + SC_COUNT + 2 * HD_AMAX;
+  c.count = keep;
   c.m = keep + HD_KEEP;
   c.rs = c.m + c.N;
   c.loss = c.rs + c.N;
@@ -1505,31 +1474,22 @@ static SmArgs sm_args(const HdCall& c, const HdPlan& p, char* ws) {
 // the logits' statistics into a.part / a.zt
 template <class T>
 static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
-  if (c.dt == DT_F32) {
-    hipLaunchKernelGGL(k_head_amax, dim3(2 * HD_AMAX), dim3(512), 0, c.st, (const float*)c.x, c.ldx, (int64_t)c.N, (const float*)c.w,
-                       c.ldw, (int64_t)c.V, c.D, c.target, c.ignore, c.index, c.teacher, c.tdt, c.K, c.amax);
-    DIG3D_CHECK_LAUNCH();
-  }
   HdArgs a;
   memset(&a, 0, sizeof a);
   HdPrep prep;
   memset(&prep, 0, sizeof prep);
-  prep.amax = c.amax;
-  prep.scal = c.scal;
-  const int two = p.pair ? 2 : 1;          // numbers of a value
+  const int nums = p.f32 ? 3 : 1;          // numbers of a value
   if (p.dx) a.Q = {(const short*)c.x, c.ldx, 0, c.N, c.D};
   else {
-    prep.x = hd_pack_job(c.x, c.dt, c.ldx, c.N, c.D, ws + p.o_x, p.Np, p.Dp, SC_X);
-    a.Q = {at_bytes(ws, p.o_x), (int64_t)p.Dp * two, p.Dp, c.N, p.Dp};
+    prep.x = hd_pack_job(c.x, c.dt, c.ldx, c.N, c.D, ws + p.o_x, p.Np, p.Dp);
+    a.Q = {at_bytes(ws, p.o_x), (int64_t)p.Dp * nums, p.Dp, c.N, p.Dp};
   }
   a.nj = c.N;
   a.ktiles = (int)hd_steps(p, p.Dp, 1);
   a.nseg = 1;
   a.bias = c.bias;
   a.dt = c.dt;
-  a.scal = c.scal;
   a.inv_tau = 1.0f / c.tau;
-  a.V = c.V;
   a.target = c.target;
   a.part = (float2*)(ws + p.o_part);
   a.part_ld = p.tiles_all;
@@ -1540,8 +1500,8 @@ static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
     const char* wp = (const char*)c.w + v0 * c.ldw * esz;
     if (p.dw) a.P = {(const short*)wp, c.ldw, 0, nv, c.D};
     else {
-      prep.w = hd_pack_job(wp, c.dt, c.ldw, nv, c.D, ws + p.o_w, nv, p.Dp, SC_W);
-      a.P = {at_bytes(ws, p.o_w), (int64_t)p.Dp * two, p.Dp, nv, p.Dp};
+      prep.w = hd_pack_job(wp, c.dt, c.ldw, nv, c.D, ws + p.o_w, nv, p.Dp);
+      a.P = {at_bytes(ws, p.o_w), (int64_t)p.Dp * nums, p.Dp, nv, p.Dp};
     }
     const int rc = hd_prep(prep, c.st);
     if (rc != DIG3D_OK) return rc;
@@ -1549,7 +1509,7 @@ static int hd_stats(const HdCall& c, const HdPlan& p, char* ws) {
     a.ni = nv;
     a.v0 = v0;
     a.part_c0 = (int)(v0 / p.lg.b);
-    hd_gemm<T, false, false, EPI_STATS>(a, p.lg, p.pair, c.st);
+    hd_gemm<T, false, false, EPI_STATS>(a, p.lg, p.f32, c.st);
     DIG3D_CHECK_LAUNCH();
   }
   return DIG3D_OK;
@@ -1563,7 +1523,7 @@ static int hd_fwd(const HdCall& c, const HdPlan& p, char* ws, float* out) {
                        sm_args(c, p, ws));
     DIG3D_CHECK_LAUNCH();
   } else {
-    const int rc = c.dt == DT_BF16 ? hd_stats<bf16_t>(c, p, ws) : hd_stats<f16_t>(c, p, ws);
+    const int rc = c.dt == DT_F16 ? hd_stats<f16_t>(c, p, ws) : hd_stats<bf16_t>(c, p, ws);
     if (rc != DIG3D_OK) return rc;
   }
   // 64 rows: one workgroup joins them in the time of one more launch (2 us each)
@@ -1653,22 +1613,21 @@ static int hd_bwd_small(const HdCall& c, const HdPlan& p, const float* g, void* 
     HdSums sums;
     memset(&sums, 0, sizeof sums);
     sums.dt = c.dt;
-    hd_add_sum(sums, a.slots, p.gx.splits, n, n, -1, gx, 0);
+    hd_add_sum(sums, a.slots, p.gx.splits, n, n, gx, 0);
     return hd_sums<bf16_t>(sums, c.st);
   }
   return DIG3D_OK;
 }
 
 template <class T>
-static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw, void* gb, char* ws) {
-  c.scal = (float*)(ws + p.o_scal);        // what the forward kept is read only: several backward passes may use it
-  const int two = p.pair ? 2 : 1;          // numbers of a value
+static int hd_bwd(const HdCall& c, const HdPlan& p, const float* g, void* gx, void* gw, void* gb, char* ws) {
+  float* S = (float*)(ws + p.o_S);         // what the forward kept is read only: several backward passes may use it
+  const int nums = p.f32 ? 3 : 1;          // numbers of a value
   HdPrep prep;
   memset(&prep, 0, sizeof prep);
-  prep.x = hd_pack_job(c.x, c.dt, c.ldx, c.N, c.D, ws + p.o_x, p.Np, p.Dp, SC_X);
+  prep.x = hd_pack_job(c.x, c.dt, c.ldx, c.N, c.D, ws + p.o_x, p.Np, p.Dp);
   prep.masked = 1;
-  prep.amax = c.amax;
-  prep.scal = c.scal;
+  prep.S = S;
   prep.coef_blocks = (c.N + HD_COEF - 1) / HD_COEF;
   prep.g = g;
   prep.per_row = c.reduction == 0;
@@ -1680,14 +1639,14 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
   prep.N = c.N;
   prep.coef = (float*)(ws + p.o_coef);
   if (prep.per_row && prep.coef_blocks > 1) {
-    float* gm = c.scal + SC_COUNT;
+    float* gm = S + 1;
     prep.gm = gm;
     prep.ngm = (c.N + HD_TOTAL - 1) / HD_TOTAL;
     hipLaunchKernelGGL(k_head_gmax, dim3(prep.ngm), dim3(1024), 0, c.st, g, prep.f, c.target, c.ignore, prep.live, c.N, gm);
     DIG3D_CHECK_LAUNCH();
   }
   short* E = (short*)(ws + p.o_E);
-  const HdOperand x = {at_bytes(ws, p.o_x), (int64_t)p.Dp * two, p.Dp, (int)p.Np, p.Dp};
+  const HdOperand x = {at_bytes(ws, p.o_x), (int64_t)p.Dp * nums, p.Dp, (int)p.Np, p.Dp};
   const HdOperand e = {E, p.ldE * p.eplanes, p.ldE, (int)p.Np, (int)p.ldE};
   const int esz = c.dt == DT_F32 ? 4 : 2;
   const bool gx_slots = gx && (p.np > 1 || p.gx.splits > 1);
@@ -1697,8 +1656,8 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     HdOperand W;
     if (p.dw) W = {(const short*)wsrc, c.ldw, 0, nv, c.D};
     else {
-      prep.w = hd_pack_job(wsrc, c.dt, c.ldw, nv, c.D, ws + p.o_w, nv, p.Dp, SC_W);
-      W = {at_bytes(ws, p.o_w), (int64_t)p.Dp * two, p.Dp, nv, p.Dp};
+      prep.w = hd_pack_job(wsrc, c.dt, c.ldw, nv, c.D, ws + p.o_w, nv, p.Dp);
+      W = {at_bytes(ws, p.o_w), (int64_t)p.Dp * nums, p.Dp, nv, p.Dp};
     }
     const int rc = hd_prep(prep, c.st);
     if (rc != DIG3D_OK) return rc;
@@ -1706,7 +1665,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     HdSums sums;
     memset(&sums, 0, sizeof sums);
     sums.dt = c.dt;
-    sums.scal = c.scal;
+    sums.S = S;
     HdArgs a;
     memset(&a, 0, sizeof a);
     a.P = W;
@@ -1717,10 +1676,8 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     a.nseg = 1;
     a.bias = c.bias;
     a.dt = c.dt;
-    a.scal = c.scal;
     a.inv_tau = 1.0f / c.tau;
     a.v0 = v0;
-    a.V = c.V;
     a.target = c.target;
     a.m = c.m;
     a.rs = c.rs;
@@ -1730,7 +1687,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     a.E = E;
     a.colsE = p.ldE;
     a.rowsE = (int)p.Np;
-    hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, p.pair, c.st);
+    hd_gemm<T, false, false, EPI_GRAD>(a, p.lg, p.f32, c.st);
     DIG3D_CHECK_LAUNCH();
     if (c.index) {
       const int rc = hd_teacher_grad<T>(c, prep.coef, v0, nv, p.eplanes, E, p.ldE);
@@ -1738,8 +1695,8 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
     }
     HdArgs o;
     memset(&o, 0, sizeof o);
-    o.nseg = p.pair ? 1 : p.eplanes;
-    o.scal = c.scal;
+    o.nseg = p.f32 ? 1 : p.eplanes;
+    o.S = S;
     o.dt = c.dt;
     if (gx) {                              // gx[n, d] += sum_v e[n, v] W[v, d]
       o.P = W;
@@ -1751,8 +1708,7 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
       o.add = v0 > 0;
       o.out = gx_slots ? nullptr : gx;
       o.ldo = c.D;
-      o.other = p.pair ? SC_W : -1;
-      hd_gemm<T, true, false, EPI_OUT>(o, p.gx, p.pair, c.st);
+      hd_gemm<T, true, false, EPI_OUT>(o, p.gx, p.f32, c.st);
       DIG3D_CHECK_LAUNCH();
     }
     if (gw) {                              // gw[v, d] = sum_n e[n, v] x[n, d]
@@ -1766,10 +1722,9 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
       o.add = 0;
       o.out = slots ? nullptr : (char*)gw + v0 * c.D * esz;
       o.ldo = c.D;
-      o.other = p.pair ? SC_X : -1;
-      hd_gemm<T, true, true, EPI_OUT>(o, p.gw, p.pair, c.st);
+      hd_gemm<T, true, true, EPI_OUT>(o, p.gw, p.f32, c.st);
       DIG3D_CHECK_LAUNCH();
-      if (slots) hd_add_sum(sums, (const float*)(ws + p.o_gw), p.gw.splits, (int64_t)nv * c.D, (int64_t)nv * c.D, o.other, gw, v0 * c.D);
+      if (slots) hd_add_sum(sums, (const float*)(ws + p.o_gw), p.gw.splits, (int64_t)nv * c.D, (int64_t)nv * c.D, gw, v0 * c.D);
     }
     if (gb) {
       float* part = (float*)(ws + p.o_col);
@@ -1777,10 +1732,10 @@ static int hd_bwd(HdCall c, const HdPlan& p, const float* g, void* gx, void* gw,
       hipLaunchKernelGGL((k_head_colsum<T>), dim3((unsigned)slices, (unsigned)((p.ldE + 255) / 256)), dim3(256), 0, c.st, E, p.ldE,
                          p.eplanes, c.N, part);
       DIG3D_CHECK_LAUNCH();
-      hd_add_sum(sums, part, slices, p.ldE, nv, -1, gb, v0);
+      hd_add_sum(sums, part, slices, p.ldE, nv, gb, v0);
     }
     if (gx_slots && v0 + p.vp >= c.V)
-      hd_add_sum(sums, (const float*)(ws + p.o_gx), p.gx.splits, (int64_t)c.N * c.D, (int64_t)c.N * c.D, p.pair ? SC_W : -1, gx, 0);
+      hd_add_sum(sums, (const float*)(ws + p.o_gx), p.gx.splits, (int64_t)c.N * c.D, (int64_t)c.N * c.D, gx, 0);
     const int rs = hd_sums<T>(sums, c.st);
     if (rs != DIG3D_OK) return rs;
   }
@@ -1835,7 +1790,7 @@ int dig3d_head_bwd(int dtype, const void* x, int64_t ldx, const void* w, int64_t
   const HdPlan p = hd_plan(dtype, N, D, V, hd_direct(dtype, x, ldx, D), hd_direct(dtype, w, ldw, D), 1, needs);
   if (p.total > (int64_t)ws_kib * 1024 || !ws) return DIG3D_ERR_ARG;
   if (p.small) return hd_bwd_small(c, p, g, gx, gw, gb, (char*)ws);
-  return dtype == DT_BF16 ? hd_bwd<bf16_t>(c, p, g, gx, gw, gb, (char*)ws) : hd_bwd<f16_t>(c, p, g, gx, gw, gb, (char*)ws);
+  return dtype == DT_F16 ? hd_bwd<f16_t>(c, p, g, gx, gw, gb, (char*)ws) : hd_bwd<bf16_t>(c, p, g, gx, gw, gb, (char*)ws);
 }
 
 }  // extern "C"

@@ -36,7 +36,7 @@ class _HeadLoss(Function):
             ctx.meta = None
             ctx.save_for_backward(x, w, bias)
             return out.zero_()
-        keep = torch.empty(520 + N * (4 + 2 * (0 if index is None else index.size(1))), **f32)
+        keep = torch.empty(8 + N * (4 + 2 * (0 if index is None else index.size(1))), **f32)
         _call('dig3d_head_fwd', x.get_device(), 0, 0, x, w, bias, target, index, teacher, keep, tau, ignore_index, reduction, out.data_ptr())
         ctx.meta = (tau, ignore_index, reduction)
         ctx.save_for_backward(x, w, bias, target, index, teacher, keep)

@@ -767,7 +767,7 @@ int dig3d_rownorm_bwd(int dtype, const void* gy, const void* x, int64_t ldx, int
  *                      index or the logit -inf is absent, equal indices add; a row without entries has the loss 0 and does not
  *                      count, one with an index >= V has the loss NaN.
  *   reduction          0: out [N]; 1: the mean over the rows that count (0 without any); 2: the sum
- *   keep               float[520 + 4 N + 2 N K], from the forward to any number of backwards
+ *   keep               float[8 + 4 N + 2 N K], from the forward to any number of backwards
  *   sizes              N < 2^24, D <= 2^20, V <= 2^28, N V / 4096 <= 2^30, N K <= 2^31
  *   g                  the incoming gradient: [N] with reduction 0, else one value
  *   dig3d_head_ws_kib  KiB of workspace of the forward, or of the backward (needs = 1 gx + 2 gw + 4 gb); x and w enter by

@@ -172,3 +172,111 @@ def test_what_reaches_an_ignored_row_is_not_used(N, D, V, t):
         bad[0], bad[4], bad[8] = float('nan'), float('inf'), float('-inf')
         got = torch.autograd.grad(f(), (x, w, b), bad)
         assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.isfinite(p).all() for p in want)
+
+
+# ------------------------------------------------------------------------------------------------ float32 entry by entry
+def check_entries(x, w, b, target, out, gx, gw, gb):
+    """sum over rows, every entry against its own terms, no floor: x and w of 24 bits each (a product keeps 22 at least), sums of
+    6 products a term in float32 of any order; p off by its logit's and its sum's errors; the target's p - 1 by its rest's."""
+    N, D = x.shape
+    V = w.size(0)
+    xd, wd, bd = x.double(), w.double(), b.double()
+    z, e, rows, loss, scale, _ = ref_classes(x, w, b, target, 'sum', torch.ones((), device=DEV))
+    dz = ((6 * D + 64) * U + 2.0 ** -22) * (xd.abs() @ wd.abs().t()) + 4 * U * (z.abs() + bd.abs())
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    p = torch.exp(z - lse)
+    rel = dz + 8 * U * (1 + (z - lse).abs())
+    de = p * (rel + (p * rel).sum(1, keepdim=True) + 40 * U)
+    at = torch.where(scale != 0, target, 0)[:, None]
+    rest = p.scatter(1, at, 0.0)
+    have = rest.sum(1, keepdim=True).clamp(min=1e-300)
+    own = rel.gather(1, at) + (rest * rel).sum(1, keepdim=True) / have + 64 * U
+    de.scatter_(1, at, have * own)
+    live = (scale != 0)[:, None]
+    de, e = torch.where(live, de, 0.0), torch.where(live, e, 0.0)
+    # a loss: of the rest's share, and of the difference of two logits where that is what it is
+    tol = torch.where(live, have * own + dz.gather(1, at) + 8 * U * rows[:, None], 0.0).sum() + N * U * rows.sum()
+    close(out, loss, tol, 'loss')
+    for name, got, want, size, off, n in (('gx', gx, e @ wd, e.abs() @ wd.abs(), de @ wd.abs(), V), ('gw', gw, e.t() @ xd, e.abs().t() @ xd.abs(), de.t() @ xd.abs(), N),
+                                          ('gb', gb, e.sum(0), e.abs().sum(0), de.sum(0), N)):
+        close(got, want, off + (2.0 ** -22 + (6 * n + 64) * U) * size + 1e-36, name)
+
+
+# the rows of gw of classes that no row gives more than 1e-8 .. 1e-30; predictions that are nearly certain; one row, class or column of x
+# or w 1e8 times the others, or 1e-8; what the path of a size holds does not depend on the size
+SPREADS = ['unlikely', 'certain', 'row', 'class', 'column of x', 'column of w', 'small column of w', 'everything']
+
+
+@pytest.mark.parametrize('N,D,V', [SMALL, GENERAL, (300, 257, 2000)])
+@pytest.mark.parametrize('spread', SPREADS)
+def test_float32_entries_far_apart_in_size(N, D, V, spread):
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, torch.float32, True, 106, boost=2.0)
+    x, w, b = x.detach().clone(), w.detach().clone(), b.detach().clone()
+    if spread in ('unlikely', 'everything'):
+        b[V // 2:] -= torch.linspace(18, 69, V - V // 2, device=DEV)         # 1e-8 .. 1e-30
+        target %= V // 2
+    if spread == 'certain':
+        b[7] += 25
+        target[:] = 7
+    if spread in ('row', 'everything'):
+        x[3] *= 1e8
+        target[3] = (x[3:4].double() @ w.double().t()).argmax()              # its own class: the others of its row hold nothing
+    if spread == 'class':
+        w[V - 3] *= 1e8
+        w[V - 3] = -w[V - 3].abs() * x.sign().sum(0).sign()                  # rarely a row's largest
+    if spread == 'column of x':
+        x[:, 2] *= 1e8
+        w[:, 2] *= 1e-8
+    if spread == 'column of w':
+        w[:, 2] *= 1e8
+        x[:, 2] *= 1e-8
+    if spread == 'small column of w':
+        w[:, 2] *= 1e-8
+        x[:, 3] *= 1e-8
+    target[5] = -100
+    leaves = [p.requires_grad_() for p in (x, w, b)]
+    out = ops.linear_cross_entropy(x, w, target, b, reduction='sum')
+    grads = torch.autograd.grad(out, leaves)
+    check_entries(x.detach(), w.detach(), b.detach(), target, out.detach(), *grads)
+
+
+@pytest.mark.parametrize('N,D,V', [SMALL, GENERAL])
+def test_one_huge_row_leaves_the_others_alone(N, D, V):
+    """a live row of 1e30, and one of the type's largest value: every other row's loss and gradient keep their bits"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, torch.float32, True, 107)
+    up = torch.ones(N, device=DEV)
+
+    def rows_of(x):
+        rows = ops.linear_cross_entropy(x, w, target, b, reduction='none')
+        return rows.detach(), torch.autograd.grad(rows, x, up)[0]
+    want, gx = rows_of(x)
+    for value in (1e30, torch.finfo(torch.float32).max):
+        y = x.detach().clone()
+        y[9] = value
+        got, gy = rows_of(y.requires_grad_())
+        others = torch.arange(N, device=DEV) != 9
+        assert torch.equal(got[others], want[others]) and torch.equal(gy[others], gx[others]), value
+
+
+@pytest.mark.parametrize('N,D,V,K', [(40, 64, 600, 6), (600, 64, 1100, 6)])
+def test_distillation_of_unlikely_classes(N, D, V, K):
+    """rows of gw of classes outside the lists that hold 1e-8 .. 1e-30: entry by entry"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, torch.float32, True, 108, boost=2.0)
+    x, w, b = x.detach(), w.detach(), b.detach().clone()
+    H = V // 2
+    b[H:] -= torch.linspace(18, 69, V - H, device=DEV)
+    index, teacher = teacher_lists(g, N, H, K)
+    wg = w.clone().requires_grad_()
+    (gw,) = torch.autograd.grad(ops.linear_distillation(x, wg, index, teacher, b, temperature=1.0, reduction='sum'), wg)
+    z, e, rows, size, scale, div = ref_teacher(x, w, b, index, teacher, 1.0, 'sum', torch.ones((), device=DEV))
+    xd = x.double()
+    dz = ((6 * D + 64) * U + 2.0 ** -22) * (xd.abs() @ w.double().abs().t()) + 4 * U * (z.abs() + b.double().abs())
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    p = torch.exp(z - lse)
+    rel = dz + 8 * U * (1 + (z - lse).abs())
+    de = p * (rel + (p * rel).sum(1, keepdim=True) + 40 * U)
+    want = e[:, H:].t() @ xd
+    close(gw[H:], want, de[:, H:].t() @ xd.abs() + (2.0 ** -22 + (6 * N + 64) * U) * (e[:, H:].t() @ xd.abs()) + 1e-36, 'gw')
