@@ -50,6 +50,7 @@ class _HeadLoss(Function):
         x, w, bias = saved[:3]
         if ctx.meta is None:
             return tuple(torch.zeros_like(t) if n else None for t, n in zip((x, w, bias), needs)) + (None,) * 6
+        saved = [ops._same_rows(x), ops._same_rows(w)] + [t if t is None else t.contiguous() for t in saved[2:]]
         gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
         gw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if needs[1] else None
         gb = torch.empty(bias.shape, dtype=x.dtype, device=x.device) if needs[2] else None

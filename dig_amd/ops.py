@@ -2168,6 +2168,11 @@ def _check_rows(name, x):
     return x if x.stride(1) == 1 and x.stride(0) >= x.size(1) else x.contiguous()
 
 
+def _same_rows(x):
+    """``x`` [R, C] as ``_check_rows`` left it when it was saved: hooks on saved tensors may bring it back at other strides."""
+    return x if x.is_contiguous() or (x.stride(1) == 1 and x.stride(0) >= x.size(1)) else x.contiguous()
+
+
 def _pitch(x):
     return x.stride(0) if x.size(0) > 1 else x.size(1)
 
@@ -2205,6 +2210,7 @@ class _LayerNorm(Function):
     @_once
     def backward(ctx, gy):
         x, weight, stat = ctx.saved_tensors
+        x, weight, stat = _same_rows(x), weight if weight is None else weight.contiguous(), stat.contiguous()
         R, C, dt, dev, wd, pd, blocks, leaf = ctx.meta
         nx, nw, nb, _ = ctx.needs_input_grad
         if not gy.is_contiguous():

@@ -280,3 +280,60 @@ def test_distillation_of_unlikely_classes(N, D, V, K):
     de = p * (rel + (p * rel).sum(1, keepdim=True) + 40 * U)
     want = e[:, H:].t() @ xd
     close(gw[H:], want, de[:, H:].t() @ xd.abs() + (2.0 ** -22 + (6 * N + 64) * U) * (e[:, H:].t() @ xd.abs()) + 1e-36, 'gw')
+
+
+# ------------------------------------------------------------------------------------------------ saved tensors elsewhere
+class _Moved(torch.autograd.graph.saved_tensors_hooks):
+    """what is saved comes back elsewhere: 'offset' rows at another alignment and pitch; 'gaps' everything with a gap behind
+    each element; 'turned' matrices whose columns are contiguous"""
+
+    def __init__(self, how):
+        def unpack(t):
+            if how == 'gaps' and t.dim():
+                return torch.stack((t, t.flip(0)), -1)[..., 0]
+            if t.dim() != 2 or how == 'gaps':
+                return t
+            if how == 'turned':
+                return t.t().contiguous().t()
+            wide = torch.zeros(t.size(0), t.size(1) + 3, dtype=t.dtype, device=t.device)
+            wide[:, 1:1 + t.size(1)] = t
+            return wide[:, 1:1 + t.size(1)]
+        super().__init__(lambda t: t.detach().clone(), unpack)
+
+
+HOW = ['offset', 'gaps', 'turned']
+
+
+@pytest.mark.parametrize('how', HOW)
+def test_saved_norms_that_come_back_elsewhere(how):
+    from dig_amd import ops
+    g = gen(110)
+    x, gy = randn(g, 70, 130).requires_grad_(), randn(g, 70, 130)
+    w, b = (1 + 0.2 * randn(g, 130)).requires_grad_(), randn(g, 130).requires_grad_()
+    want = torch.autograd.grad(ops.layer_norm(x, w, b), (x, w, b), gy)
+    with _Moved(how):
+        y = ops.layer_norm(x, w, b)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, w, b), gy), want))
+
+
+@pytest.mark.parametrize('how', HOW)
+@pytest.mark.parametrize('t', list(TYPES))
+@pytest.mark.parametrize('N,D,V', [(32, 128, 8192), (100, 64, 4000), (40, 64, 600), (600, 128, 900)])
+def test_saved_rows_that_come_back_elsewhere(N, D, V, t, how):
+    """the backward may then copy what the forward read in place, or take other kernels than it: the same bounds"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, TYPES[t], True, 109)
+    index, teacher = teacher_lists(g, N, V, 4)
+    teacher = teacher.to(TYPES[t])
+    one = torch.tensor(float(N) if t == 'f16' else 1.0, device=DEV)
+    xd, wd, bd = x.detach(), w.detach(), b.detach()
+    with _Moved(how):
+        out = ops.linear_cross_entropy(x, w, target, b)
+        got = dict(zip(('gx', 'gw', 'gb'), torch.autograd.grad(out, (x, w, b), one)), out=out.detach())
+    z, e, rows, loss, scale, div = ref_classes(xd, wd, bd, target, 'mean', one)
+    check_head(xd, wd, bd, z, e, rows, 1.0, 1.0, dict(got, div=div), scale, loss)
+    with _Moved(how):
+        out = ops.linear_distillation(x, w, index, teacher, b, temperature=2.0)
+        got = dict(zip(('gx', 'gw', 'gb'), torch.autograd.grad(out, (x, w, b), one)), out=out.detach())
+    z, e, rows, size, scale, div = ref_teacher(xd, wd, bd, index, teacher, 2.0, 'mean', one)
+    check_teacher(xd, wd, bd, z, e, rows, size, 2.0, dict(got, div=div), scale, rows.sum() / div, index, teacher)
