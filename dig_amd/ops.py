@@ -2201,7 +2201,7 @@ class _LayerNorm(Function):
             m = stat.data_ptr()
             m2 = m + 4 * R
             ctx.meta = (R, C, dt, dev, wd, None if p is None else p.dtype, _hip.query('dig3d_rownorm_bwd_blocks', R, C, dt),
-                        _all_leaf((weight, bias)))
+                        _all_leaf((weight, bias)), ptr(weight), ptr(bias))
             ctx.save_for_backward(x, weight, stat)
         _on_device(dev, 'dig3d_rownorm_fwd', dt, x.data_ptr(), _pitch(x), R, C, ptr(weight), ptr(bias), wd, eps, y.data_ptr(), m, m2)
         return y
@@ -2211,29 +2211,29 @@ class _LayerNorm(Function):
     def backward(ctx, gy):
         x, weight, stat = ctx.saved_tensors
         x, weight, stat = _same_rows(x), weight if weight is None else weight.contiguous(), stat.contiguous()
-        R, C, dt, dev, wd, pd, blocks, leaf = ctx.meta
+        R, C, dt, dev, wd, pd, blocks, leaf, wkey, bkey = ctx.meta
         nx, nw, nb, _ = ctx.needs_input_grad
         if not gy.is_contiguous():
             gy = gy.contiguous()
         gx = torch.empty_like(gy) if nx else None
-        gw = gb = part = later = None
+        gw = gb = part = None
+        later = _deferred is not None and pd == torch.float32 and leaf and (nw or nb)
+        if later:
+            # the workgroups' partials join the deferred reductions of the pass, under each parameter's own key: a parameter that
+            # is used more than once has one buffer, and the later uses add to it
+            part = torch.empty(blocks * 2 * C, dtype=pd, device=x.device) if R else torch.zeros(2 * C, dtype=pd, device=x.device)
+            gw = _deferred.add_keyed(wkey, part, max(blocks, 1), C, C, x.device, 2 * C) if nw else None
+            gb = _deferred.add_keyed(bkey, part[C:], max(blocks, 1), C, C, x.device, 2 * C) if nb else None
         if R == 0:
-            zero = lambda need: torch.zeros(C, dtype=pd, device=x.device) if need else None
-            return gx, zero(nw), zero(nb), None
-        if nw or nb:
+            zero = lambda need: torch.zeros(C, dtype=pd, device=x.device) if need and not later else None
+            return gx, zero(nw) if gw is None else gw, zero(nb) if gb is None else gb, None
+        if (nw or nb) and not later:
             part = torch.empty(blocks * 2 * C, dtype=torch.float32, device=x.device)
-            if _deferred is not None and pd == torch.float32 and leaf:
-                # the workgroups' partials join the deferred reductions of the pass
-                later = torch.empty(2 * C, dtype=pd, device=x.device)
-                _reduce_later(part, blocks, 2 * C, later, leaf)
-            else:
-                gw = torch.empty(C, dtype=pd, device=x.device) if nw else None
-                gb = torch.empty(C, dtype=pd, device=x.device) if nb else None
+            gw = torch.empty(C, dtype=pd, device=x.device) if nw else None
+            gb = torch.empty(C, dtype=pd, device=x.device) if nb else None
         m = stat.data_ptr()
         _on_device(dev, 'dig3d_rownorm_bwd', dt, gy.data_ptr(), x.data_ptr(), _pitch(x), R, C, ptr(weight), wd, m, m + 4 * R, ptr(gx), ptr(part),
-                   blocks, ptr(gw), ptr(gb))
-        if later is not None:
-            gw, gb = (later[:C] if nw else None), (later[C:] if nb else None)
+                   blocks, *((None, None) if later else (ptr(gw), ptr(gb))))
         return gx, gw, gb, None
 
 

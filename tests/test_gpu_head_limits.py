@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_head import DEV, TYPES, U, check_head, check_teacher, classes_case, close, gen, half, head64, randn, ref_classes, ref_teacher
+from tests.test_gpu_head import DEV, TYPES, U, check_head, check_teacher, classes_case, close, gen, half, norm64, randn, ref_classes, ref_teacher
 
 pytestmark = pytest.mark.gpu
 SMALL, GENERAL = (40, 64, 600), (600, 64, 1100)          # rows, width, classes
@@ -337,3 +337,31 @@ def test_saved_rows_that_come_back_elsewhere(N, D, V, t, how):
         got = dict(zip(('gx', 'gw', 'gb'), torch.autograd.grad(out, (x, w, b), one)), out=out.detach())
     z, e, rows, size, scale, div = ref_teacher(xd, wd, bd, index, teacher, 2.0, 'mean', one)
     check_teacher(xd, wd, bd, z, e, rows, size, 2.0, dict(got, div=div), scale, rows.sum() / div, index, teacher)
+
+
+# ------------------------------------------------------------------------------------------------ deferred reductions
+def test_a_norm_used_twice_joins_the_deferred_reductions():
+    """one weight under two biases, one bias under two weights, one tensor as both: every use reaches the gradient.  Each use adds
+    300 rows in chains of at most 300 / 64 + 128 and joins the others' in at most 64 steps; h is off as in check_norm"""
+    from dig_amd import ops
+    g = gen(111)
+    x, z = randn(g, 300, 128), randn(g, 300, 128) * 1.5 + 0.3
+    w, v, b, c, p = ((1 + 0.2 * randn(g, 128)).requires_grad_() for _ in range(5))
+    none = torch.empty(0, 128, device=DEV)
+    uses = [(none, w, b), (x, w, b), (z, w, c), (x, v, b), (z, p, p), (z, v, None), (none, None, c)]
+    gys = [randn(g, u[0].size(0), 128) for u in uses]
+    ops.backward(sum((ops.layer_norm(*u) * gy).sum() for u, gy in zip(uses, gys)), [w, v, b, c, p])
+    want = {id(t): [0.0, 0.0] for t in (w, v, b, c, p)}
+    for (rows, weight, bias), gy in zip(uses, gys):
+        if not rows.size(0):
+            continue
+        q = norm64(rows, weight.detach(), None, 1e-5, gy)
+        reach = 64 * U * (q['x'].abs().amax(1, keepdim=True) * q['r'] + q['h'].abs())
+        n = (300 / 64 + 128 + 64) * U
+        parts = [(weight, q['gw'], n * (q['gy'] * q['h']).abs().sum(0) + (q['gy'].abs() * reach).sum(0)), (bias, q['gb'], n * q['gy'].abs().sum(0))]
+        for leaf, value, tol in parts:
+            if leaf is not None:
+                want[id(leaf)][0] = want[id(leaf)][0] + value
+                want[id(leaf)][1] = want[id(leaf)][1] + tol
+    for name, leaf in zip('wvbcp', (w, v, b, c, p)):
+        close(leaf.grad, *want[id(leaf)], name)
