@@ -365,3 +365,33 @@ def test_a_norm_used_twice_joins_the_deferred_reductions():
                 want[id(leaf)][1] = want[id(leaf)][1] + tol
     for name, leaf in zip('wvbcp', (w, v, b, c, p)):
         close(leaf.grad, *want[id(leaf)], name)
+
+
+# ------------------------------------------------------------------------------------------------ a model's own head
+@pytest.mark.parametrize('level', ['aminoacid', 'allatom'])
+def test_a_protein_model_trains_its_class_head_without_logits(level):
+    """ProNet with its last layer taken out gives the rows that layer would have got; the fused loss over that layer's weight gives
+    them, the weight and the bias the gradients of the formula, and the model's own backward goes on from there"""
+    from dig_amd import ops
+    from dig_amd.synthetic import make_protein_batch
+    import dig_amd.threedgraph.method as M
+    torch.manual_seed(0)
+    model = M.ProNet(level=level, num_blocks=2, hidden_channels=64, mid_emb=32, out_channels=384).to(DEV)
+    batch = make_protein_batch(6, 20, 40, 33, device=DEV)
+    target = torch.arange(6, device=DEV) * 61
+    logits = model(batch)
+    head, model.lin_out = model.lin_out, torch.nn.Identity()
+    h = model(batch)
+    assert h.shape == (6, 64) and torch.equal(head(h), logits)
+    rows = h.detach().requires_grad_()
+    leaves = (rows, head.weight, head.bias)
+    out = ops.linear_cross_entropy(rows, head.weight, target, head.bias)
+    got = dict(zip(('gx', 'gw', 'gb'), torch.autograd.grad(out, leaves)), out=out.detach())
+    x, w, b = (p.detach() for p in leaves)
+    one = torch.ones((), device=DEV)
+    z, e, lr, loss, scale, div = ref_classes(x, w, b, target, 'mean', one)
+    check_head(x, w, b, z, e, lr, 1.0, 1.0, dict(got, div=div), scale, loss)
+    params = [p for p in model.parameters()]
+    end = torch.autograd.grad(ops.linear_cross_entropy(h, head.weight, target, head.bias), params, retain_graph=True)
+    step = torch.autograd.grad(h, params, got['gx'])
+    assert all(torch.equal(p, q) for p, q in zip(end, step)) and any(p.any() for p in end)
