@@ -426,7 +426,7 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
             decltype(h) m;
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-              h.t[r] = to_t<T>(e[r]);                            // |e| <= 1: no infinities to keep apart
+              h.t[r] = to_t<T>(e[r]);                            // |e| <= 1, or no finite number in all three
               const float d = e[r] - (float)h.t[r];
               m.t[r] = to_t<T>(d);
               l.t[r] = to_t<T>(d - (float)m.t[r]);
@@ -717,9 +717,9 @@ struct HdPrep {
 #define HD_COEF 2048
 
 // coef[n] (|.| <= 1, 0 for a row without a loss) and the scalar S with coef[n] S = the gradient of row n's logits' loss:
-// reductions: coef = 1 or 0, S = g f / count;  none: S = a power of two over max |g f|
+// reductions: coef = 1 or 0, S = g f / count (no finite number: coef takes it);  none: S = a power of two over max |g f|
 __device__ __forceinline__ void hd_coef(const HdPrep& a, int b, float* sh) {
-  float S = 1.f;
+  float S = 1.f, all = 1.f;
   if (a.per_row) {
     float m = 0.f;
     if (a.gm) {
@@ -736,10 +736,14 @@ __device__ __forceinline__ void hd_coef(const HdPrep& a, int b, float* sh) {
     }
   } else {
     S = a.g[0] * a.f / (a.count ? *a.count : 1.f);
+    if (!(fabsf(S) <= 3.402823466e38f)) {  // the rows', not a factor of everything
+      all = S;
+      S = 1.f;
+    }
   }
   const int end = min(a.N, (b + 1) * HD_COEF);
   for (int n = b * HD_COEF + threadIdx.x; n < end; n += 256)       // a NaN of live is the gradient's too
-    a.coef[n] = hd_has(n, a.target, a.ignore, a.live) ? (a.per_row ? a.g[n] * a.f / S : 1.f) * (a.live ? a.live[n] : 1.f) : 0.f;
+    a.coef[n] = hd_has(n, a.target, a.ignore, a.live) ? (a.per_row ? a.g[n] * a.f / S : all) * (a.live ? a.live[n] : 1.f) : 0.f;
   if (b == 0 && threadIdx.x == 0) *a.S = S;
 }
 

@@ -174,6 +174,22 @@ def test_what_reaches_an_ignored_row_is_not_used(N, D, V, t):
         assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.isfinite(p).all() for p in want)
 
 
+@pytest.mark.parametrize('t', list(TYPES))
+@pytest.mark.parametrize('N,D,V', [SMALL, GENERAL])
+def test_a_gradient_without_a_number_reaches_the_rows_with_a_loss(N, D, V, t):
+    """mean and sum under an incoming gradient of NaN or infinity: none of it in rows without a loss"""
+    from dig_amd import ops
+    x, w, b, target, g = classes_case(N, D, V, TYPES[t], True, 112)
+    index, teacher = teacher_lists(g, N, V, 4)
+    target[::4], index[::4] = -100, -1
+    for red in ('mean', 'sum'):
+        for f in (lambda: ops.linear_cross_entropy(x, w, target, b, reduction=red), lambda: ops.linear_distillation(x, w, index, teacher, b, reduction=red)):
+            for value in (float('nan'), float('inf'), float('-inf')):
+                gx, gw, gb = torch.autograd.grad(f(), (x, w, b), torch.tensor(value, device=DEV))
+                assert not gx[::4].any(), (red, value)
+                assert not torch.isfinite(gx[1]).any() and not torch.isfinite(gb[target[1]])
+
+
 # ------------------------------------------------------------------------------------------------ float32 entry by entry
 def check_entries(x, w, b, target, out, gx, gw, gb):
     """sum over rows, every entry against its own terms, no floor: x and w of 24 bits each (a product keeps 22 at least), sums of
