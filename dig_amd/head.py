@@ -89,8 +89,15 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
 
     -> float32: the mean over the rows whose target is not ``ignore_index`` (0 if there are none), their sum, or with
     ``reduction='none'`` one loss per row (0 for an ignored one).  Ignored rows take no part in any gradient, whatever they
-    hold.  A target outside [0, V) gives NaN, in the loss and the gradients, and so does a row without a finite logit.
-    Differentiable once, in x, weight and bias; the gradients have the type of their inputs and the same bits every time."""
+    hold.  A target outside [0, V) gives NaN, in the loss and the gradients, and so does a row without a finite logit or with an
+    infinite one; such a row counts once in the mean.  A bias of -inf or of the type's lowest value takes its class out.
+    Differentiable once, in x, weight and bias; the gradients have the type of their inputs and the same bits every time.
+
+    Precision: sums, statistics and losses in float32.  float32 rows and weights enter with all 24 bits (products to 2^-23 of a
+    term) at every size.  In 16 bits the gradient of the logits is float32 or two numbers of the type where the products are
+    small (up to 128 rows, or N D V up to 2^31), and beyond is rounded once to the type, half a step of each entry (the
+    gradients are then off by 1.1 to 1.4 times what their own rounding costs); in float16 an entry below 2^-29 of the
+    largest incoming gradient of a row keeps fewer bits."""
     x2, weight, bias = _check_head('linear_cross_entropy', x, weight, bias, reduction)
     _check_index('linear_cross_entropy', 'target', target, x.shape[:-1], x2)
     if not -1 << 63 <= int(ignore_index) < 1 << 63:
@@ -106,8 +113,9 @@ def linear_distillation(x, weight, teacher_index, teacher_logits, bias=None, tem
     temperature, the head's logits never kept.
 
     An entry with a negative index or the logit -inf is absent, whatever else it holds; a row without entries has the loss 0, no
-    gradient, and is not counted by the mean.  Equal indices of a row add up.  An index >= V gives NaN.  The teacher takes no
-    gradient.  K is at most 2048.  Types, reductions and gradients as ``linear_cross_entropy``; teacher_logits float32, bfloat16 or float16."""
+    gradient, and is not counted by the mean.  Equal indices of a row add up.  An index >= V or a NaN among the listed logits gives
+    NaN; such a row counts once in the mean.  The teacher takes no gradient.  K is at most 2048.  Types, reductions, gradients
+    and precision as ``linear_cross_entropy``; teacher_logits float32, bfloat16 or float16."""
     name = 'linear_distillation'
     x2, weight, bias = _check_head(name, x, weight, bias, reduction)
     if not (isinstance(temperature, (int, float)) and 1e-6 <= float(temperature) <= 1e6):
