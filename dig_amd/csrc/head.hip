@@ -633,6 +633,18 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     for (int x = 0; x < MI; ++x)
 #pragma unroll
       for (int y = 0; y < MJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // Tiles of 64 are for few rows, whose losses nothing averages: their sums are added up every eight steps (a chain of 1024 products
+    // is off by 6e-7 of the loss of one row, this by a third of it).  The larger ones have no registers for a second sum.
+    f32x4 sum[BI == 64 ? MI : 1][BI == 64 ? MJ : 1] = {};
+    auto collect = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int x = 0; x < MI; ++x)
+#pragma unroll
+        for (int y = 0; y < MJ; ++y) {
+          sum[x][y] += acc[x][y];
+          acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    };
     read_q(0, 0, 0);
     read_p(0, 0, 0);
     for (int t = 0; t < steps; t += 2) {
@@ -653,6 +665,16 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
         read_p(0, 0, 0);
       }
       if (more) mul(1, 1);
+      if constexpr (BI == 64) {
+        if ((t & 7) == 6) collect();
+      }
+    }
+    if constexpr (BI == 64) {
+      collect();
+#pragma unroll
+      for (int x = 0; x < MI; ++x)
+#pragma unroll
+        for (int y = 0; y < MJ; ++y) acc[x][y] = sum[x][y];
     }
     hd_epilogue<T, BI, BJ, WI, WJ, EPI, F32>(a, acc, z, ti * BI, tj * BJ, ti, wi, wj, tid, sh);
   }

@@ -70,7 +70,8 @@ __device__ __forceinline__ void sm_stage(float* lds, int tid, const float* f) {
 }
 
 // acc[x][y]: out[j, i] = sum over k in [ks, ke) of Q[j, k] P[i, k] for i = i0 + 32 (wave & 1) + 16 x + 4 (lane >> 4) + r,
-// j = j0 + 32 (wave >> 1) + 16 y + (lane & 15)
+// j = j0 + 32 (wave >> 1) + 16 y + (lane & 15).  A k step's sum is formed by itself and then added: in one chain of D / 4 additions
+// the loss of one row of 1024 is off by 1e-6.
 template <bool PT, bool QT>
 __device__ __forceinline__ void sm_product(const SmOperand& P, const SmOperand& Q, int i0, int j0, int ks, int ke, float* lds,
                                            f32x4 (&acc)[2][2]) {
@@ -98,14 +99,19 @@ __device__ __forceinline__ void sm_product(const SmOperand& P, const SmOperand& 
     }
     const float* ap = sp + (lane >> 4) * SM_PITCH + (wave & 1) * 32 + (lane & 15);
     const float* aq = sq + (lane >> 4) * SM_PITCH + (wave >> 1) * 32 + (lane & 15);
+    f32x4 sum[2][2] = {};
 #pragma unroll
     for (int kk = 0; kk < SM_BK; kk += 4) {
       const float p0 = ap[kk * SM_PITCH], p1 = ap[kk * SM_PITCH + 16], q0 = aq[kk * SM_PITCH], q1 = aq[kk * SM_PITCH + 16];
-      acc[0][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(p0, q0, acc[0][0], 0, 0, 0);
-      acc[0][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(p0, q1, acc[0][1], 0, 0, 0);
-      acc[1][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(p1, q0, acc[1][0], 0, 0, 0);
-      acc[1][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(p1, q1, acc[1][1], 0, 0, 0);
+      sum[0][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(p0, q0, sum[0][0], 0, 0, 0);
+      sum[0][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(p0, q1, sum[0][1], 0, 0, 0);
+      sum[1][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(p1, q0, sum[1][0], 0, 0, 0);
+      sum[1][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(p1, q1, sum[1][1], 0, 0, 0);
     }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) acc[x][y] += sum[x][y];
   }
 }
 

@@ -298,6 +298,27 @@ def test_distillation_of_unlikely_classes(N, D, V, K):
     close(gw[H:], want, de[:, H:].t() @ xd.abs() + (2.0 ** -22 + (6 * N + 64) * U) * (e[:, H:].t() @ xd.abs()) + 1e-36, 'gw')
 
 
+# what a sum of D products in the small tiles' order is off by at most, in u of the sum of their sizes: the products of a matrix
+# instruction in any order, the additions of a block of them, the blocks, and 8 for what follows
+CHAINS = {'in place': lambda D: 4 + 8 + D / 32 + 8, '16 bits': lambda D: 32 + 16 + D / 512 + 8, 'three numbers': lambda D: 32 + 24 + D / 128 + 8 + 4}
+
+
+@pytest.mark.parametrize('t,D,V,kind', [('bf16', 65536, 2, '16 bits'), ('f16', 65536, 2, '16 bits'), ('f32', 65536, 2, 'three numbers'),
+                                        ('f32', 4096, 16384, 'in place')])
+def test_long_sums_of_few_rows(t, D, V, kind):
+    """64 rows whose D products are all equal, so that a chain's roundings all go one way; every other class has the logit 0"""
+    from dig_amd import ops
+    g = gen(113)
+    N, at = 64, V - 1
+    a = (1 + torch.rand(N, 1, device=DEV, generator=g)).to(TYPES[t])
+    w = torch.zeros(V, D, device=DEV, dtype=TYPES[t])
+    w[at] = -40 / (1.5 * D)
+    rows = ops.linear_cross_entropy(a.expand(N, D).contiguous(), w, torch.full((N,), at, device=DEV), reduction='none')
+    z = a[:, 0].double() * w[at, 0].double() * D
+    want = torch.log((V - 1) + torch.exp(z)) - z
+    close(rows, want, CHAINS[kind](D) * U * z.abs() + 16 * U * want, 'rows')
+
+
 # ------------------------------------------------------------------------------------------------ saved tensors elsewhere
 class _Moved(torch.autograd.graph.saved_tensors_hooks):
     """what is saved comes back elsewhere: 'offset' rows at another alignment and pitch; 'gaps' everything with a gap behind
