@@ -1279,17 +1279,17 @@ static bool hd_direct(int dt, const void* p, int64_t ld, int D) {
 #define HD_PIECE_BYTES (512ll << 20)
 
 // Float32 products in place (head_small.h) where copies and launches are what the general path costs, or where few float32 rows meet
-// a W that it would copy, at one and a half times its size, before the first product.  GPU us in place / general, with
+// a W that it would copy, at one and a half times its size, before the first product.  us of a replayed graph in place / general, with
 // gradients (losses alone).  A training call is five launches in place and eight to ten otherwise, which a host that
 // launches them one by one pays with some 15 us: the border is where the GPU loses that much.
-//   f32: 32 x 128 x 1195: 38 / 48 (18 / 21)   128 x 128 x 1195: 41 / 51   512 x 128 x 1195: 62 / 57 (18 / 22)   1024 x 128 x 1195: 93 / 65
-//        512 x 128 x 4096: 76 / 68 (21 / 25)   256 x 128 x 16384: 89 / 89 (28 / 33)   200 x 256 x 2048: 66 / 62   64 x 256 x 1024: 50 / 57 (25 / 27)
-//        64 x 256 x 32768: 110 / 131 (42 / 54)   128 x 512 x 1024: 73 / 72 (31 / 30)   128 x 512 x 2048: 81 / 77   256 x 512 x 1024: 83 / 78
-//        8 x 1024 x 1024: 103 / 92 (50 / 39)   64 x 512 x 16384: 112 / 123 (41 / 50)   1 x 1024 x 8192: 127 / 126 (51 / 50)
-//        64 x 1024 x 8192: 144 / 141 (54 / 58)   16 x 1024 x 16384: 152 / 207 (51 / 65)   64 x 2048 x 32768: 469 / 793 (124 / 272)
-//   16-bit rows read in place by both: 32 x 128 x 1195: 38 / 39   128 x 64 x 300: 37 / 42   32 x 128 x 8192: 44 / 40   512 x 128 x 256: 60 / 44
-//   16-bit rows that the general path copies (odd widths or addresses): 32 x 127 x 8192: 46 / 47   14 x 40 x 67126: 67 / 83
-//        64 x 127 x 32768: 95 / 84   128 x 127 x 4096: 57 / 49   16 x 255 x 8192: 56 / 52   10 x 214 x 105058: 225 / 165   512 x 127 x 1195: 84 / 53   128 x 511 x 1024: 87 / 55
+//   f32: 32 x 128 x 1195: 38 / 49 (19 / 22)   128 x 128 x 1195: 42 / 52   512 x 128 x 1195: 65 / 57 (19 / 23)   1024 x 128 x 1195: 98 / 66
+//        512 x 128 x 4096: 80 / 70 (22 / 25)   256 x 128 x 16384: 91 / 89 (28 / 32)   200 x 256 x 2048: 68 / 63   64 x 256 x 1024: 52 / 58 (26 / 27)
+//        64 x 256 x 32768: 112 / 131 (43 / 55)   128 x 512 x 1024: 76 / 73 (32 / 30)   128 x 512 x 2048: 85 / 78   256 x 512 x 1024: 86 / 79
+//        8 x 1024 x 1024: 110 / 93 (54 / 39)   64 x 512 x 16384: 115 / 123 (41 / 51)   1 x 1024 x 8192: 133 / 126 (55 / 50)
+//        64 x 1024 x 8192: 149 / 142 (57 / 58)   16 x 1024 x 16384: 156 / 211 (54 / 65)   64 x 2048 x 32768: 507 / 796 (139 / 271)
+//   16-bit rows read in place by both: 32 x 128 x 1195: 40 / 37   128 x 64 x 300: 38 / 35   32 x 128 x 8192: 43 / 37   512 x 128 x 256: 62 / 38
+//   16-bit rows that the general path copies (odd widths or addresses): 32 x 127 x 8192: 47 / 44   14 x 40 x 67126: 66 / 66
+//        64 x 127 x 32768: 95 / 77   128 x 127 x 4096: 57 / 43   16 x 255 x 8192: 58 / 48   10 x 214 x 105058: 215 / 142
 // A wave joins a row's V / 64 statistics: up to 2^20 classes.
 static bool hd_small(bool f32, bool copies, int64_t N, int64_t D, int64_t V) {
   const double work = (double)N * D * V;
