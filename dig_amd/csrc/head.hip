@@ -13,10 +13,10 @@
 //
 // Types.  bf16 / f16: the inputs as they are, sums in f32; e is rounded once to the same type (up to 2^-8 / 2^-11 of each entry,
 // at random sign; with few rows e is two such numbers).  f32: every value, of x, W and e alike, is the sum of three bf16
-// numbers v = h + m + l, exactly down to 2^-110 (8 bits each, the exponent range of f32: no scale, no entry's bits depend on another's), and a
-// product of two is the six products of them that reach 2^-24 of it: h h, h m, m h, m m, h l, l h, with f32 sums.  What is
-// dropped (m l, l m, l l) is at most 2^-23 of the term.  Six bf16 products take two thirds of the time of one in f32 on this
-// chip.  (Two f16 numbers and three products would take half of that again, but their second number runs out of exponents:
+// numbers v = h + m + l, exactly down to 2^-110 (8 bits each, the exponent range of f32: no scale, no entry's bits depend on
+// another's), and a product of two is the six products of them that reach 2^-24 of it: h h, h m, m h, m m, h l, l h, with f32
+// sums.  What is dropped (m l, l m, l l) is at most 2^-23 of the term.  Six bf16 products take two thirds of the time of one in
+// f32 on this chip.  (Two f16 numbers and three products would take half of that again, but their second number runs out of exponents:
 // below 2^-18 of the largest value of its tensor an entry loses bits, and the gradient of an unlikely class has no other entries.)
 #include <string.h>
 
@@ -455,8 +455,9 @@ __device__ __forceinline__ void hd_epilogue(const HdArgs& a, f32x4 (&acc)[BI / W
 //
 // A workgroup walks its tiles as one sequence of k steps.  Two stages are in LDS; a step is four phases (two halves of k, two
 // of the wave's i).  F32: 32 of k are two steps, one over the first and second numbers (h h, h m, m h, m m: eight phases), one
-// over the first and third (h l, l h: four), so that what is loaded and read from LDS for four multiplies for six.  The operands of a phase are read while the phase before it multiplies.  The barrier that ends a
-// step stands before its last phase, whose operands are in registers by then: the loads of the step after the next and the
+// over the first and third (h l, l h: four), so that what is loaded and read from LDS for four multiplies for six.  The
+// operands of a phase are read while the phase before it multiplies.  The barrier that ends a step stands before its last
+// phase, whose operands are in registers by then: the loads of the step after the next and the
 // first reads of the next one are issued under that phase's products.  The sequence runs on into the next tile, so a
 // tile's first loads are under way during the last steps and the epilogue of the tile before it.  Behind the last tile the
 // loads fetch that tile's first steps again, into stages that are read no more.
@@ -633,8 +634,8 @@ __global__ void __launch_bounds__(WI* WJ * 64, BI == 64 ? 4 : 2) k_head_gemm(HdA
     for (int x = 0; x < MI; ++x)
 #pragma unroll
       for (int y = 0; y < MJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // Tiles of 64 are for few rows, whose losses nothing averages: their sums are added up every eight steps (a chain of 1024 products
-    // is off by 6e-7 of the loss of one row, this by a third of it).  The larger ones have no registers for a second sum.
+    // Tiles of 64 are for few rows, whose losses nothing averages: their sums are added up every eight steps (1 x 1024 x 32768 in
+    // bf16: the loss is off by 1.4e-7 of itself, in one chain by 6e-7).  The larger ones have no registers for a second sum.
     f32x4 sum[BI == 64 ? MI : 1][BI == 64 ? MJ : 1] = {};
     auto collect = [&]() __attribute__((always_inline)) {
 #pragma unroll
